@@ -1,0 +1,560 @@
+"""Performance cases of the operators around the expert path: what a program on
+this library runs before, after and in place of its bf16 experts.
+
+  layer_norm  the norm before an MoE block: forward (with the residual add),
+              and for training forward and backward with the reductions of the
+              weight's and the bias's gradient
+  adamw       the optimizer step over many tensors at once with f32 states, f32
+              weights or bf16 weights with f32 masters; with `clip` the
+              gradients' global norm is taken first and scales them
+  adamw8      the same with states in 8 bits: e4m3 values, one f32 scale per 256
+              elements, nearest or stochastic rounding
+  w4          products with 4-bit weights and group scales, of a dense layer
+              (E = 0) or of the experts of a routed batch
+
+A case is a dict of plain values.  Sizes are those of this repository's
+configurations (d = 512 to 7168, E = 8 to 128) or odd ones between them.
+"""
+from __future__ import annotations
+
+import importlib
+import math
+
+import torch
+
+own = False
+
+_DEV = "cuda"
+_LR, _BETAS, _EPS, _DECAY, _MAX_NORM = 3e-4, (0.9, 0.95), 1e-8, 0.1, 1.0
+_LN_EPS = 1e-5
+_BLOCK = 256                  # elements to a scale of the 8-bit states
+
+
+def _et():
+    return importlib.import_module("peer-review-agents_amd")
+
+
+# --------------------------------------------------------------------------- #
+# the cases
+# --------------------------------------------------------------------------- #
+
+def _ln(T, d, *, dtype="bf16", wdtype="f32", train=False, residual=False, pad=0):
+    return dict(kind="layer_norm", T=T, d=d, dtype=dtype, wdtype=wdtype, train=train, residual=residual, pad=pad)
+
+
+def _opt(kind, layers, d, E, F, *, dtype="f32", gdtype="f32", clip=False, stochastic=False, step=100):
+    return dict(kind=kind, layers=layers, d=d, E=E, F=F, dtype=dtype, gdtype=gdtype, clip=clip, stochastic=stochastic,
+                step=step)
+
+
+def _w4(T, K, N, *, E=0, k=0, group=128, epilogue="none", gather=True, scales="bf16", known=False):
+    return dict(kind="w4", T=T, K=K, N=N, E=E, k=k, group=group, epilogue=epilogue, gather=gather, scales=scales,
+                known=known)
+
+
+def listed():
+    return [
+        # the norm of a decode batch of a few sequences, with the residual add
+        dict(name="norm_decode_8", **_ln(8, 4096, residual=True)),
+        # the norm of a long prompt, forward only
+        dict(name="norm_prompt_16384", **_ln(16384, 2048, wdtype="bf16")),
+        # a ragged f32 batch in training, rows that are a slice of wider ones
+        dict(name="norm_train_ragged_3001", **_ln(3001, 2889, dtype="f32", train=True, pad=7)),
+        # the norm of the headline training step (65536 tokens, d = 4096)
+        dict(name="norm_train_65536", **_ln(65536, 4096, train=True, residual=True)),
+        # many small tensors: norms, routers and narrow experts of twelve layers
+        dict(name="adamw_small_60", **_opt("adamw", 12, 512, 8, 32)),
+        # one layer's experts, bf16 weights with f32 masters, clipped: the largest
+        dict(name="adamw_masters_201m", **_opt("adamw", 1, 2048, 64, 512, dtype="bf16", clip=True)),
+        # 8-bit states on tensors of odd sizes, bf16 gradients
+        dict(name="adamw8_ragged", **_opt("adamw8", 3, 1001, 24, 77, gdtype="bf16")),
+        # 8-bit states, stochastic rounding, on one layer's experts
+        dict(name="adamw8_masters_201m", **_opt("adamw8", 1, 2048, 64, 512, dtype="bf16", clip=True, stochastic=True)),
+        # a dense projection of one token
+        dict(name="w4_dense_1", **_w4(1, 4096, 4096)),
+        # gate/up projection of one token's eight experts out of 128
+        dict(name="w4_gate_up_1", **_w4(1, 4096, 4096, E=128, k=8, epilogue="swiglu")),
+        # down projection of a ragged decode batch on one GPU's share of a wide model's experts
+        dict(name="w4_down_61", **_w4(61, 2048, 7168, E=32, k=8, group=64, epilogue="row_scale", gather=False)),
+        # a larger decode batch: every expert has slots, tens each
+        dict(name="w4_gate_up_509", **_w4(509, 2048, 2816, E=64, k=8, epilogue="swiglu", known=True)),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def _multiple(rng, lo, hi, step):
+    return max(step, step * int(round(_log_int(rng, lo, hi) / step)))
+
+
+def _elements(case):
+    return sum(math.prod(s) for s in _shapes(case))
+
+
+def draw(rng):
+    kind = rng.choice(["layer_norm", "layer_norm", "adamw", "adamw8", "w4", "w4"])
+    if kind == "layer_norm":
+        dtype = rng.choice(["bf16", "bf16", "f32"])
+        T, d = _log_int(rng, 1, 65536), _multiple(rng, 64, 8192, rng.choice([1, 8, 64, 512]))
+        while T * d > (1 << 28) // (2 if dtype == "f32" else 1):
+            T = max(1, T // 2)
+        return _ln(T, d, dtype=dtype, wdtype=rng.choice(["f32", dtype]), train=rng.random() < 0.5,
+                   residual=rng.random() < 0.5, pad=rng.choice([0, 0, 8, 5]))
+    if kind in ("adamw", "adamw8"):
+        case = _opt(kind, rng.choice([1, 2, 3, 6, 12, 24]), _log_int(rng, 64, 4096), rng.choice([1, 4, 8, 24, 64]),
+                    _log_int(rng, 8, 2048), dtype=rng.choice(["f32", "bf16"]), gdtype=rng.choice(["f32", "f32", "bf16"]),
+                    clip=rng.random() < 0.5, stochastic=kind == "adamw8" and rng.random() < 0.5,
+                    step=_log_int(rng, 1, 100000))
+        while _elements(case) > 190_000_000:
+            case["F"] = max(1, case["F"] // 2)
+            case["d"] = max(1, case["d"] * 3 // 4)
+        return case
+    if rng.random() < 0.4:
+        return _w4(_log_int(rng, 1, 64), _multiple(rng, 256, 8192, rng.choice([8, 128, 512])),
+                   _multiple(rng, 256, 8192, rng.choice([8, 64, 512])), group=rng.choice([32, 64, 128, 128]),
+                   scales=rng.choice(["bf16", "f16"]))
+    E = rng.choice([8, 16, 24, 32, 48, 64, 96, 128])
+    epilogue = rng.choice(["none", "swiglu", "row_scale"])
+    T = _log_int(rng, 1, 512)
+    K, N = _multiple(rng, 512, 7168, rng.choice([8, 64, 512])), _multiple(rng, 512, 7168, rng.choice([16, 64, 256]))
+    while E * N * K > 1 << 31:
+        E //= 2
+    return _w4(T, K, N, E=E, k=min(rng.choice([1, 2, 4, 6, 8]), E), group=rng.choice([32, 64, 128, 128]),
+               epilogue=epilogue, gather=rng.random() < 0.6, scales=rng.choice(["bf16", "f16"]), known=T > 64)
+
+
+# --------------------------------------------------------------------------- #
+# what a program has in hand before the call
+# --------------------------------------------------------------------------- #
+
+_TYPES = dict(f32=torch.float32, bf16=torch.bfloat16, f16=torch.float16)
+
+
+def _generator(seed):
+    return torch.Generator(device=_DEV).manual_seed(int(seed) * 1000003 + 29)
+
+
+def _randn(g, *shape, scale=1.0):
+    return torch.randn(*shape, generator=g, device=_DEV).mul_(scale)
+
+
+def _ln_inputs(case, seed):
+    g = _generator(seed)
+    T, d, t, wt = case["T"], case["d"], _TYPES[case["dtype"]], _TYPES[case["wdtype"]]
+    # a few channels of large activations and an offset, as residual streams have
+    channel = torch.exp(_randn(g, d, scale=0.5))
+    offset = _randn(g, d, scale=0.3)
+
+    def rows(scale, shaped=False):
+        wide = torch.empty(T, d + case["pad"], dtype=t, device=_DEV)
+        v = _randn(g, T, d, scale=scale)
+        wide[:, :d] = v * channel + offset if shaped else v
+        return wide[:, :d]
+
+    s = dict(case=case, x=rows(1.0, True), weight=(1 + _randn(g, d, scale=0.2)).to(wt), bias=_randn(g, d, scale=0.1).to(wt))
+    s["residual"] = rows(0.5) if case["residual"] else None
+    if case["train"]:
+        s["dy"] = rows(0.02)
+        s["dsum"] = _randn(g, T, d, scale=0.02).to(t) if case["residual"] else None
+    return s
+
+
+def _shapes(case):
+    """The tensors of one MoE block: norm, router, experts; of every layer."""
+    d, E, F = case["d"], case["E"], case["F"]
+    return [(d,), (d,), (E, d), (E, 2 * F, d), (E, d, F)] * case["layers"]
+
+
+def _opt_inputs(case, seed):
+    """Flat buffers, each tensor a view of them from a multiple of 256 elements
+    on (a program that keeps its weights in one allocation); the gaps are 0."""
+    g = _generator(seed)
+    shapes = _shapes(case)
+    starts, n = [], 0
+    for shape in shapes:
+        starts.append(n)
+        n += -(-math.prod(shape) // _BLOCK) * _BLOCK
+    live = torch.zeros(n, dtype=torch.bool, device=_DEV)
+    for a, shape in zip(starts, shapes):
+        live[a:a + math.prod(shape)] = True
+
+    def flat(scale=1.0, spread=None):
+        v = _randn(g, n, scale=scale)
+        if spread is not None:
+            v *= spread
+        return torch.where(live, v, 0.0)
+
+    def views(t, per=1):
+        if per > 1:
+            return [t[a // per:a // per + -(-math.prod(s) // per)] for a, s in zip(starts, shapes)]
+        return [t[a:a + math.prod(s)].view(s) for a, s in zip(starts, shapes)]
+
+    # gradients of one tensor differ by some factors of ten between its elements
+    size = torch.exp(_randn(g, n, scale=1.5)).mul_(1e-3)
+    s = dict(case=case, flat={}, views={})
+    flats = dict(grads=flat(spread=size).to(_TYPES[case["gdtype"]]))
+    p = flat(0.02)
+    if case["dtype"] == "bf16":
+        flats["masters"], flats["params"] = p, p.to(torch.bfloat16)
+    else:
+        flats["params"] = p
+    m = flat(0.3, size)
+    v = flat(0.2, size).add_(torch.where(live, size, 0.0)).square_()
+    if case["kind"] == "adamw":
+        flats["m"], flats["v"] = m, v
+    else:
+        flats["m"], flats["m_scale"] = _to_e4m3(m)
+        flats["root"], flats["root_scale"] = _to_e4m3(v.sqrt_())
+    for name, t in flats.items():
+        s["flat"][name] = t
+        s["views"][name] = views(t, _BLOCK if name.endswith("_scale") else 1)
+    return s
+
+
+def _w4_inputs(case, seed):
+    """q: two 4-bit values to a byte, the even k in the low half [E, N, K / 2];
+    scales [E, N, groups].  The routed batch: every token on k experts, some of
+    which are more popular; slots ordered by expert, then token."""
+    g = _generator(seed)
+    T, K, N, E, k = case["T"], case["K"], case["N"], case["E"], case["k"]
+    groups = -(-K // case["group"])
+    q = torch.randint(0, 256, (max(E, 1), N, K // 2), generator=g, device=_DEV, dtype=torch.uint8)
+    scales = torch.exp(_randn(g, max(E, 1), N, groups, scale=0.25)).mul_(0.25 / math.sqrt(K)).to(_TYPES[case["scales"]])
+    s = dict(case=case, q=q, scales=scales)
+    if E == 0:
+        s["x"] = _randn(g, T, K).to(torch.bfloat16)
+        return s
+    popular = torch.rand(T, E, generator=g, device=_DEV).log_().div_(torch.exp(_randn(g, E, scale=0.5)))
+    chosen = torch.zeros(T, E, dtype=torch.bool, device=_DEV).scatter_(1, popular.topk(k, dim=1).indices, True)
+    expert, token = chosen.t().nonzero(as_tuple=True)
+    counts = chosen.sum(0)
+    offsets = torch.cat([counts.new_zeros(1), counts.cumsum(0)])
+    s.update(expert=expert, token=token, counts=counts, offsets=offsets)
+    s["gate"] = torch.sigmoid(_randn(g, len(token)))
+    s["x"] = _randn(g, T if case["gather"] else len(token), K).to(torch.bfloat16)
+    # what the plain form needs of the plan: busy experts, and each slot's place
+    s["busy"] = counts.nonzero()[:, 0]
+    s["place"] = torch.searchsorted(s["busy"], expert), torch.arange(len(token), device=_DEV) - offsets[expert]
+    s["most"] = int(counts.max())
+    return s
+
+
+_INPUTS = dict(layer_norm=_ln_inputs, adamw=_opt_inputs, adamw8=_opt_inputs, w4=_w4_inputs)
+
+
+def prepare(case, seed):
+    s = _INPUTS[case["kind"]](case, seed)
+    if own and case["kind"] == "w4":
+        # the weight as the library lays it out, once; the plan as its routing gives it
+        et, E = _et(), case["E"]
+        s["weight"] = et.pack_w4(s.pop("q"), s.pop("scales"), group=case["group"],
+                                 parts=2 if case["epilogue"] == "swiglu" else 1)
+        if E:
+            S, T = len(s["token"]), case["T"]
+            i32 = lambda t: t.to(torch.int32)  # noqa: E731
+            by_token = torch.argsort(s["token"] * E + s["expert"])
+            to = torch.searchsorted(s["token"][by_token].contiguous(), torch.arange(T + 1, device=_DEV))
+            s["plan"] = et.RoutingPlan(i32(s["counts"]), i32(s["offsets"]), i32(to), i32(s["token"]), s["gate"],
+                                       i32(by_token), T, E, S, S if case["known"] else None)
+    return s
+
+
+# --------------------------------------------------------------------------- #
+# one pass
+# --------------------------------------------------------------------------- #
+
+def _ln_plain(s):
+    x, t = s["x"].float(), s["x"].dtype
+    d, w = x.shape[1], s["weight"].float()
+    out = {}
+    if s["residual"] is not None:
+        out["sum"] = (x + s["residual"].float()).to(t)
+        x = out["sum"].float()
+    mean = x.sum(1, keepdim=True) / d
+    c = x - mean
+    rstd = 1.0 / torch.sqrt((c * c).sum(1, keepdim=True) / d + _LN_EPS)
+    xhat = c * rstd
+    out["y"] = (xhat * w + s["bias"].float()).to(t)
+    if s["case"]["train"]:
+        out["mean"], out["rstd"] = mean[:, 0], rstd[:, 0]
+        dy = s["dy"].float()
+        g = dy * w
+        dx = rstd * (g - g.sum(1, keepdim=True) / d - xhat * ((g * xhat).sum(1, keepdim=True) / d))
+        if s["dsum"] is not None:
+            dx = dx + s["dsum"].float()
+        out["dx"], out["dweight"], out["dbias"] = dx.to(t), (dy * xhat).sum(0), dy.sum(0)
+    return out
+
+
+def _ln_own(s):
+    et, train = _et(), s["case"]["train"]
+    r = et.layer_norm(s["x"], s["weight"], s["bias"], eps=_LN_EPS, residual=s["residual"], stats=train)
+    r = list(r) if isinstance(r, tuple) else [r]
+    out = dict(y=r.pop(0))
+    if s["residual"] is not None:
+        out["sum"] = r.pop(0)
+    if train:
+        out["mean"], out["rstd"] = r
+        out["dx"], out["dweight"], out["dbias"] = et.layer_norm_backward(
+            s["dy"], out.get("sum", s["x"]), s["weight"], out["mean"], out["rstd"], dsum=s["dsum"])
+    return out
+
+
+def _f32(v):
+    return float(torch.tensor(v, dtype=torch.float32))
+
+
+def _bias_corrections(step):
+    return 1.0 - _BETAS[0] ** step, math.sqrt(1.0 - _BETAS[1] ** step)
+
+
+def _random_words(seed, n):
+    """32 random bits for each of n elements, from the seed and the index."""
+    low = 0xFFFFFFFF
+    x = (torch.arange(n, device=_DEV, dtype=torch.int64) * 0x9E3779B1 + seed) & low
+    x = ((x ^ (x >> 15)) * 0x6A09E667) & low
+    x = ((x ^ (x >> 13)) * 0xBB67AE85) & low
+    return x ^ (x >> 16)
+
+
+def _to_e4m3(x, words=None):
+    """(e4m3 values, f32 scale of every 256): the largest of a block becomes 448.
+    With random words: rounded away from 0 where the 20 bits that a value of 3
+    fraction bits leaves out, and the word's bits, carry."""
+    blocks = x.view(-1, _BLOCK)
+    most = blocks.abs().amax(1, keepdim=True)
+    most = torch.where(most < 1e-35, 0.0, most)
+    scale = most * _f32(1 / 448)
+    r = blocks.abs() * torch.where(most > 0, torch.full_like(most, 448.0) / most, 0.0)
+    r = r.clamp_(max=448.0)
+    if words is not None:
+        # (below 2^-6 the steps are 2^-9, as they are in [2^-6, 2^-5))
+        small = torch.where(r < 2.0 ** -6, 2.0 ** -6, 0.0)
+        bits = ((r + small).view(torch.int32) + words.view(-1, _BLOCK).to(torch.int32)) & -(1 << 20)
+        r = (bits.view(torch.float32) - small).clamp_(max=448.0)
+    return torch.copysign(r, blocks).view(-1).to(torch.float8_e4m3fn), scale.view(-1)
+
+
+def _from_e4m3(q, scale):
+    return (q.float().view(-1, _BLOCK) * scale[:, None]).view(-1)
+
+
+def _opt_plain(s):
+    f, case = s["flat"], s["case"]
+    b1, b2 = _BETAS
+    c1, c2 = _bias_corrections(case["step"])
+    g = f["grads"].float()
+    out = {}
+    if case["clip"]:
+        out["norm"] = torch.sqrt((g * g).sum())
+        g = g * torch.clamp(_MAX_NORM / (out["norm"] + 1e-6), max=1.0)
+    if case["kind"] == "adamw":
+        f["m"].mul_(b1).add_(g * (1.0 - b1))
+        f["v"].mul_(b2).add_(g * g * (1.0 - b2))
+        m, root = f["m"], torch.sqrt(f["v"])
+    else:
+        m = _from_e4m3(f["m"], f["m_scale"]) * b1 + g * (1.0 - b1)
+        root = _from_e4m3(f["root"], f["root_scale"])
+        root = torch.sqrt(root * root * b2 + g * g * (1.0 - b2))
+    p = f["masters"] if case["dtype"] == "bf16" else f["params"]
+    p.mul_(1.0 - _LR * _DECAY).sub_(m / (root * (1.0 / c2) + _EPS) * (_LR / c1))
+    if case["dtype"] == "bf16":
+        f["params"].copy_(p)
+        out["masters"] = p
+    if case["kind"] == "adamw8":
+        words = _random_words(case["step"], len(m)) if case["stochastic"] else None
+        q, scale = _to_e4m3(m, None if words is None else words >> 16 << 4)
+        f["m"].copy_(q), f["m_scale"].copy_(scale)
+        # a root is never stored as 0: the smallest step at least
+        q, scale = _to_e4m3(root, None if words is None else (words & 0xFFFF) << 4)
+        floor = torch.where(root > 0, 2.0 ** -9, 0.0) * (scale > 0).repeat_interleave(_BLOCK)
+        f["root"].copy_(torch.maximum(q.float(), floor)), f["root_scale"].copy_(scale)
+        out.update(m_scale=f["m_scale"], root=f["root"], root_scale=f["root_scale"])
+    else:
+        out["v"] = f["v"]
+    return dict(out, params=f["params"], m=f["m"])
+
+
+def _opt_own(s):
+    et, f, v, case = _et(), s["flat"], s["views"], s["case"]
+    out, scale = {}, None
+    if case["clip"]:
+        out["norm"], scale = et.grad_norm(v["grads"], max_norm=_MAX_NORM)
+    common = dict(step=case["step"], lr=_LR, betas=_BETAS, eps=_EPS, weight_decay=_DECAY, masters=v.get("masters"),
+                  grad_scale=scale)
+    if case["kind"] == "adamw":
+        et.adamw_step_(v["params"], v["grads"], v["m"], v["v"], **common)
+        out["v"] = f["v"]
+    else:
+        et.adamw8_step_(v["params"], v["grads"], v["m"], v["m_scale"], v["root"], v["root_scale"],
+                        seed=case["step"] if case["stochastic"] else None, **common)
+        out.update(m_scale=f["m_scale"], root=f["root"], root_scale=f["root_scale"])
+    if case["dtype"] == "bf16":
+        out["masters"] = f["masters"]
+    return dict(out, params=f["params"], m=f["m"])
+
+
+def _w4_plain(s):
+    case, x = s["case"], s["x"].float()
+    K, N = case["K"], case["N"]
+    q, scales = s["q"], s["scales"]
+    if case["E"]:
+        q, scales = q[s["busy"]], scales[s["busy"]]
+    w = torch.stack([q & 15, q >> 4], -1).view(len(q), N, K).float() - 8.0
+    w *= scales.float().repeat_interleave(case["group"], 2)[:, :, :K]
+    if case["E"]:
+        rows = torch.zeros(len(q), s["most"], K, device=_DEV)
+        rows[s["place"]] = x[s["token"]] if case["gather"] else x
+        p = torch.bmm(rows, w.transpose(1, 2))[s["place"]]
+    else:
+        p = x @ w[0].t()
+    if case["epilogue"] == "swiglu":
+        gate, up = p[:, :N // 2], p[:, N // 2:]
+        p = gate / (1.0 + torch.exp(-gate)) * up
+    elif case["epilogue"] == "row_scale":
+        p = p * s["gate"][:, None]
+    return p.to(torch.bfloat16)
+
+
+def _w4_own(s):
+    et, case = _et(), s["case"]
+    if not case["E"]:
+        return et.linear_w4(s["x"], s["weight"])
+    return et.expert_gemm_w4(s["x"], s["weight"], s["plan"], gather=case["gather"], epilogue=case["epilogue"],
+                             row_scale=s["gate"] if case["epilogue"] == "row_scale" else None)
+
+
+_PLAIN = dict(layer_norm=_ln_plain, adamw=_opt_plain, adamw8=_opt_plain, w4=_w4_plain)
+_OWN = dict(layer_norm=_ln_own, adamw=_opt_own, adamw8=_opt_own, w4=_w4_own)
+
+
+def run(state):
+    return (_OWN if own else _PLAIN)[state["case"]["kind"]](state)
+
+
+# --------------------------------------------------------------------------- #
+# what a pass cannot do without
+# --------------------------------------------------------------------------- #
+
+def work(case):
+    """Bytes: each input read once and each output written once (weights: those
+    of the experts expected to have slots).  Flops: those of the formulas."""
+    kind = case["kind"]
+    if kind == "layer_norm":
+        es, cells = 4 if case["dtype"] == "f32" else 2, case["T"] * case["d"]
+        passes = 2 + 2 * case["residual"] + (2 + case["residual"]) * case["train"]
+        return dict(bytes=passes * es * cells + 16 * case["d"] + 8 * case["T"] * case["train"],
+                    flops=(8 + 16 * case["train"]) * cells)
+    if kind in ("adamw", "adamw8"):
+        n = _elements(case)
+        each = (4 if case["gdtype"] == "f32" else 2) + 8 + (2 if case["dtype"] == "bf16" else 0)
+        each += 16 if kind == "adamw" else 4 + 16 / _BLOCK
+        return dict(bytes=n * each, flops=(16 + 2 * case["clip"]) * n)
+    T, K, N, E, k = case["T"], case["K"], case["N"], case["E"], case["k"]
+    S, busy = (T * k, E * (1.0 - (1.0 - k / E) ** T)) if E else (T, 1)
+    cols = N // 2 if case["epilogue"] == "swiglu" else N
+    rows = T if case["gather"] or not E else S
+    return dict(bytes=busy * (N * K / 2 + 2 * N * -(-K // case["group"])) + 2 * (rows * K + S * cols) + 8 * S,
+                flops=2 * S * N * K)
+
+
+# --------------------------------------------------------------------------- #
+# the same in 64 bits
+# --------------------------------------------------------------------------- #
+
+def _ln_exact(s):
+    def wide(t):
+        return t.to(torch.float64)
+    w, b, out = wide(s["weight"]), wide(s["bias"]), {}
+    h = wide(s["x"])
+    if s["residual"] is not None:
+        # (the sum is held in the activations' type, and the norm is that of what is held)
+        h = wide((h + wide(s["residual"])).to(s["x"].dtype))
+        out["sum"] = h
+    var, mean = torch.var_mean(h, dim=1, correction=0)
+    rstd = torch.rsqrt(var + _LN_EPS)
+    out["y"] = torch.addcmul(b, (h - mean[:, None]) * rstd[:, None], w)
+    if s["case"]["train"]:
+        out["mean"], out["rstd"] = mean, rstd
+        dy = wide(s["dy"])
+        z = (h - mean[:, None]) * rstd[:, None]
+        out["dweight"], out["dbias"] = torch.einsum("td,td->d", dy, z), dy.sum(0)
+        dz = dy * w
+        along = torch.einsum("td,td->t", dz, z)
+        dx = (dz - dz.mean(1)[:, None] - z * (along / z.shape[1])[:, None]) * rstd[:, None]
+        out["dx"] = dx if s["dsum"] is None else dx + wide(s["dsum"])
+    return out
+
+
+def _grid(x, words, least):
+    """x (float64) on the e4m3 grid under a scale per 256, and the scales."""
+    b = x.view(-1, _BLOCK)
+    scale = b.abs().amax(1, keepdim=True) / 448.0
+    r = torch.where(scale > 0, b.abs() / scale, 0.0)
+    step = torch.exp2(torch.frexp(r.clamp(min=2.0 ** -6)).exponent.double() - 4)
+    if words is None:
+        r = torch.round(r / step) * step
+    else:
+        r = torch.floor(r / step + words.view(-1, _BLOCK).double() / 2.0 ** 16) * step
+    if least:
+        r = torch.where((b > 0) & (r == 0), 2.0 ** -9, r)
+    return (torch.sign(b) * r.clamp(max=448.0)).view(-1), scale.view(-1)
+
+
+def _opt_exact(s):
+    f, case = s["flat"], s["case"]
+    (b1, b2), t = _BETAS, case["step"]
+    g, out = f["grads"].double(), {}
+    if case["clip"]:
+        out["norm"] = g.square().sum().sqrt()
+        g = g * min(1.0, _MAX_NORM / (float(out["norm"]) + 1e-6))
+    if case["kind"] == "adamw":
+        m, v = f["m"].double(), f["v"].double()
+    else:
+        def held(name):
+            return f[name].double().view(-1, _BLOCK) * f[name + "_scale"].double()[:, None]
+        m, v = held("m").view(-1), held("root").view(-1).square()
+    m = torch.lerp(g, m, b1)
+    v = torch.lerp(g.square(), v, b2)
+    p = f["masters" if case["dtype"] == "bf16" else "params"].double()
+    p = p * (1.0 - _LR * _DECAY) - _LR * (m / (1.0 - b1 ** t)) / ((v / (1.0 - b2 ** t)).sqrt() + _EPS)
+    out["params"] = p
+    if case["dtype"] == "bf16":
+        out["masters"] = p
+    if case["kind"] == "adamw":
+        return dict(out, m=m, v=v)
+    words = _random_words(t, len(m)) if case["stochastic"] else None
+    out["m"], out["m_scale"] = _grid(m, None if words is None else words >> 16, False)
+    out["root"], out["root_scale"] = _grid(v.sqrt(), None if words is None else words & 0xFFFF, True)
+    return out
+
+
+def _w4_exact(s):
+    case = s["case"]
+    x = s["x"].double()
+    K, N = case["K"], case["N"]
+    number = torch.arange(K, device=_DEV) // case["group"]
+    if case["E"]:
+        bounds = s["offsets"].tolist()
+        rows = [s["token"][a:b] if case["gather"] else slice(a, b) for a, b in zip(bounds, bounds[1:])]
+    else:
+        rows = [slice(0, case["T"])]
+    done = []
+    for e, at in enumerate(rows):
+        q = s["q"][e].long()
+        w = torch.empty(N, K, dtype=torch.float64, device=_DEV)
+        w[:, 0::2], w[:, 1::2] = (q % 16 - 8).double(), (q // 16 - 8).double()
+        done.append(x[at] @ (w * s["scales"][e].double()[:, number]).t())
+    p = torch.cat(done)
+    if case["epilogue"] == "swiglu":
+        return p[:, :N // 2] * torch.sigmoid(p[:, :N // 2]) * p[:, N // 2:]
+    return p * s["gate"].double()[:, None] if case["epilogue"] == "row_scale" else p
+
+
+_EXACT = dict(layer_norm=_ln_exact, adamw=_opt_exact, adamw8=_opt_exact, w4=_w4_exact)
+
+
+def exact(case, seed):
+    return _EXACT[case["kind"]](_INPUTS[case["kind"]](case, seed))
