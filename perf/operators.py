@@ -241,11 +241,27 @@ def _w4_inputs(case, seed):
     return s
 
 
+def _optimizer(et, s):
+    """The optimizer that a program keeps, its states those of the inputs."""
+    case, f, v = s["case"], s["flat"], s["views"]
+    opt = et.AdamW(v["params"], lr=_LR, betas=_BETAS, eps=_EPS, weight_decay=_DECAY, masters=v.get("masters"),
+                   state="f32" if case["kind"] == "adamw" else "e4m3", stochastic=case["stochastic"])
+    names = (("m", "exp_avg"), ("v", "exp_avg_sq"), ("root", "exp_avg_root"), ("m_scale", "exp_avg_scale"),
+             ("root_scale", "exp_avg_root_scale"))
+    for mine, its in names:
+        if mine in f:
+            opt.flat[its].copy_(f[mine])
+            f[mine] = opt.flat[its]
+    return opt
+
+
 _INPUTS = dict(layer_norm=_ln_inputs, adamw=_opt_inputs, adamw8=_opt_inputs, w4=_w4_inputs)
 
 
 def prepare(case, seed):
     s = _INPUTS[case["kind"]](case, seed)
+    if own and case["kind"] in ("adamw", "adamw8"):
+        s["optimizer"] = _optimizer(_et(), s)
     if own and case["kind"] == "w4":
         # the weight as the library lays it out, once; the plan as its routing gives it
         et, E = _et(), case["E"]
@@ -378,21 +394,13 @@ def _opt_plain(s):
 
 
 def _opt_own(s):
-    et, f, v, case = _et(), s["flat"], s["views"], s["case"]
+    f, case, opt = s["flat"], s["case"], s["optimizer"]
     out, scale = {}, None
     if case["clip"]:
-        out["norm"], scale = et.grad_norm(v["grads"], max_norm=_MAX_NORM)
-    common = dict(step=case["step"], lr=_LR, betas=_BETAS, eps=_EPS, weight_decay=_DECAY, masters=v.get("masters"),
-                  grad_scale=scale)
-    if case["kind"] == "adamw":
-        et.adamw_step_(v["params"], v["grads"], v["m"], v["v"], **common)
-        out["v"] = f["v"]
-    else:
-        et.adamw8_step_(v["params"], v["grads"], v["m"], v["m_scale"], v["root"], v["root_scale"],
-                        seed=case["step"] if case["stochastic"] else None, **common)
-        out.update(m_scale=f["m_scale"], root=f["root"], root_scale=f["root_scale"])
-    if case["dtype"] == "bf16":
-        out["masters"] = f["masters"]
+        out["norm"], scale = _et().grad_norm(s["views"]["grads"], max_norm=_MAX_NORM)
+    opt.steps = case["step"] - 1            # (every pass is the same step)
+    opt.step(s["views"]["grads"], grad_scale=scale)
+    out.update({k: f[k] for k in ("v", "m_scale", "root", "root_scale", "masters") if k in f})
     return dict(out, params=f["params"], m=f["m"])
 
 
