@@ -1,0 +1,116 @@
+/*
+ * etmoe_block.h -- C ABI of the operators that an MoE block needs around the
+ * dispatch path of etmoe.h, in the same library (libetmoe.so): the layer norm
+ * before the block, forward and backward; the optimizer step of its weights
+ * (AdamW over many tensors at once, with states in 32 or in 8 bits, and the
+ * global gradient norm that clips it).
+ *
+ * Conventions are those of etmoe.h: device pointers unless a comment says
+ * otherwise, work enqueued on `stream` (NULL: the legacy default stream), no
+ * allocation, no synchronisation, 0 or a negative ET_ERR_* code with
+ * et_last_error(), argument errors found before anything is enqueued, no
+ * state between calls.  Every entry point can be captured in a HIP graph;
+ * values passed by value are then fixed in it.
+ * No entry point has a counterpart in the reference.
+ */
+#ifndef ETMOE_BLOCK_H
+#define ETMOE_BLOCK_H
+
+#include "etmoe.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define ET_BLOCK_ABI_VERSION 1
+
+int et_block_abi_version(void);
+
+/* ------------------------------------------------------------------------ *
+ * AdamW over many tensors
+ * ------------------------------------------------------------------------ */
+
+/* Elements that share one scale of the 8-bit states. */
+#define ET_ADAMW8_BLOCK 256
+
+/* Bytes of device workspace et_grad_norm needs for `count` tensors of
+ * numel[i] elements (HOST array): one binary64 partial sum for every 16384
+ * elements of a tensor.  0 where count or a numel is negative. */
+size_t et_grad_norm_workspace_bytes(const int64_t* numel, int64_t count);
+
+/*
+ * Global 2-norm of many tensors:
+ *   norm[0]  = sqrt(sum over every element of g^2)
+ *   scale[0] = min(1, max_norm / (norm + 1e-6)); NaN if the norm is not finite
+ * grads, numel and dtypes are HOST arrays of `count` entries: device pointers
+ * (element-aligned), element counts, ET_DTYPE_*.  Squares and sums are binary64 in a
+ * fixed order, norm is rounded once: repeated calls give identical bits.
+ * scale (f32 [1]) may be NULL; max_norm is then not read.  workspace 8-byte
+ * aligned.
+ */
+int et_grad_norm(const void* const* grads, const int64_t* numel, const int32_t* dtypes, int64_t count,
+                 float max_norm, float* norm, float* scale, void* workspace, size_t workspace_bytes,
+                 void* stream);
+
+/* The scalars of one AdamW step (passed by value from the host). */
+typedef struct {
+    float beta1, one_minus_beta1;   /* each rounded from the host's binary64 value */
+    float beta2, one_minus_beta2;
+    float inv_root_bias2;           /* 1 / sqrt(1 - beta2^step) */
+    float eps;
+    float decay;                    /* 1 - lr * weight_decay */
+    float step_size;                /* lr / (1 - beta1^step) */
+} et_adamw_scalars;
+
+/*
+ * One AdamW step, in place, on `count` tensors:
+ *   g = grad * grad_scale
+ *   m = beta1 * m + one_minus_beta1 * g
+ *   v = beta2 * v + one_minus_beta2 * (g * g)
+ *   w = decay * w - step_size * (m / (sqrt(v) * inv_root_bias2 + eps))
+ * in binary32, each operation of m and v rounded in the order written.
+ * params, grads, m, v and masters are HOST arrays of device pointers, numel a
+ * HOST array.  param_dtype F32: w is the parameter and masters is NULL.  BF16:
+ * w is the f32 master, and the parameter is w rounded to bf16.  m and v f32.
+ * grads f32 or bf16 (grad_dtype).  grad_scale (f32 [1] on the device) may be
+ * NULL (1).  Where it is not finite the step is skipped: every buffer keeps
+ * its bits.  Pointers are element-aligned; a tensor whose pointers are all
+ * 16-byte aligned (bf16: 8) moves in wide accesses.  Tensors must not overlap.
+ */
+int et_adamw(void* const* params, const void* const* grads, float* const* m, float* const* v,
+             float* const* masters, const int64_t* numel, int64_t count, int param_dtype, int grad_dtype,
+             et_adamw_scalars scalars, const float* grad_scale, void* stream);
+
+/*
+ * The same step with 8-bit states.  m and u = sqrt(v) are held as OCP e4m3
+ * values, one byte per element, times an f32 scale for every block of
+ * ET_ADAMW8_BLOCK consecutive elements of a tensor (the last may be short;
+ * m_scale and u_scale have ceil(numel / 256) entries):
+ *   m = m8 * m_scale, u = u8 * u_scale, v = u * u
+ *   m, v and w stepped as in et_adamw; u = sqrt(v)
+ *   a = the largest |x| of the block (x = m, u; below 1e-35: 0)
+ *   scale = a * (1 / 448),  r = min(|x| * (448 / a), 448)  (0 where a is 0)
+ *   x8 = r rounded to e4m3, with x's sign
+ * so the largest element of a block is kept to f32.  rounding 0: to nearest,
+ * ties to even.  rounding 1: stochastic, up with the probability of the
+ * fraction left out, from 16 random bits: word(seed, i) of element i (counted
+ * over the call's tensors, each beginning at a multiple of 256), m from its
+ * high half and u from its low one:
+ *   x = i * 0x9E3779B1 + seed;           x = (x ^ x >> 15) * 0x6A09E667
+ *   x = (x ^ x >> 13) * 0xBB67AE85;      word = x ^ x >> 16       (mod 2^32)
+ * A moving average needs it: with 1 - beta2 = 0.001 and steps of 1/8 rounding
+ * to nearest returns every value to where it was.  u > 0 is held as 2^-9 of
+ * the scale at least, so no denominator falls to eps.  A block whose largest
+ * value is not finite gets a NaN scale.  The step's own w uses m and v before
+ * they are rounded.
+ */
+int et_adamw8(void* const* params, const void* const* grads, uint8_t* const* m8, float* const* m_scale,
+              uint8_t* const* u8, float* const* u_scale, float* const* masters, const int64_t* numel,
+              int64_t count, int param_dtype, int grad_dtype, et_adamw_scalars scalars, const float* grad_scale,
+              int rounding, uint32_t seed, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* ETMOE_BLOCK_H */

@@ -2,10 +2,11 @@
 
 Import with ``importlib.import_module("peer-review-agents_amd")`` (the
 directory name is not a Python identifier).  Kernels live in csrc/ and are
-built into libetmoe.so by build.py; the host API is in expert_threshold.py,
-and ops.py registers the path as PyTorch operators (torch.ops.etmoe.*).
+built into libetmoe.so by build.py; the host API is in expert_threshold.py (the
+dispatch path) and optimizer.py (AdamW, the gradient norm), and ops.py registers
+the path as PyTorch operators (torch.ops.etmoe.*).
 """
-from ._lib import ETMoEError, LIB_PATH, header_symbols, lib  # noqa: F401
+from ._lib import BLOCK_HEADER_PATH, ETMoEError, LIB_PATH, header_symbols, lib  # noqa: F401
 from . import ops  # noqa: F401  (registers torch.ops.etmoe.*)
 from .expert_threshold import (  # noqa: F401
     ExpertThresholdRouter,
@@ -33,4 +34,12 @@ from .expert_threshold import (  # noqa: F401
     swiglu_backward,
     threshold_update_,
     threshold_workspace_bytes,
+)
+from .optimizer import (  # noqa: F401
+    ADAMW8_BLOCK,
+    AdamW,
+    adamw8_scales,
+    adamw8_step_,
+    adamw_step_,
+    grad_norm,
 )

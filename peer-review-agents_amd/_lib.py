@@ -17,6 +17,7 @@ import torch  # noqa: F401  (see module docstring: must be loaded before the lib
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libetmoe.so")
 HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "etmoe.h")
+BLOCK_HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "etmoe_block.h")
 
 ET_DTYPE_F32 = 0
 ET_DTYPE_BF16 = 1
@@ -39,6 +40,25 @@ _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _sz = ctypes.c_size_t
 _f = ctypes.c_float
+
+_u32 = ctypes.c_uint32
+
+
+class AdamWScalars(ctypes.Structure):
+    """et_adamw_scalars of include/etmoe_block.h."""
+
+    _fields_ = [(name, _f) for name in ("beta1", "one_minus_beta1", "beta2", "one_minus_beta2", "inv_root_bias2", "eps",
+                                        "decay", "step_size")]
+
+
+# Names of include/etmoe_block.h (lists of tensors are host arrays: _p too).
+_BLOCK_SIGNATURES = {
+    "et_block_abi_version": (_int, []),
+    "et_grad_norm_workspace_bytes": (_sz, [_p, _i64]),
+    "et_grad_norm": (_int, [_p, _p, _p, _i64, _f, _p, _p, _p, _sz, _p]),
+    "et_adamw": (_int, [_p, _p, _p, _p, _p, _p, _i64, _int, _int, AdamWScalars, _p, _p]),
+    "et_adamw8": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _int, _int, AdamWScalars, _p, _int, _u32, _p]),
+}
 
 _SIGNATURES = {
     "et_abi_version": (_int, []),
@@ -87,7 +107,7 @@ _lib = None
 
 
 def header_symbols(path: str = HEADER_PATH) -> list[str]:
-    """Names of the functions declared in include/etmoe.h."""
+    """Names of the functions declared in a header, include/etmoe.h by default."""
     text = open(path).read()
     text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
     return sorted(set(re.findall(r"\b(et_[a-z_0-9]+)\s*\(", text)))
@@ -101,7 +121,7 @@ def lib() -> ctypes.CDLL:
                 f"{LIB_PATH} is not built; run __graft_entry__.build() "
                 "(there is no CPU fallback for this path)")
         L = ctypes.CDLL(LIB_PATH)
-        for name, (res, args) in _SIGNATURES.items():
+        for name, (res, args) in {**_SIGNATURES, **_BLOCK_SIGNATURES}.items():
             fn = getattr(L, name)
             fn.restype = res
             fn.argtypes = args

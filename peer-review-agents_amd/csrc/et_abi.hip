@@ -1,5 +1,6 @@
 // et_abi.hip -- status plumbing of the C ABI (et_last_error, et_abi_version).
 #include "et_common.hpp"
+#include "etmoe_block.h"
 
 namespace et {
 
@@ -24,5 +25,7 @@ int check_launch(const char* what)
 }  // namespace et
 
 extern "C" int et_abi_version(void) { return ET_ABI_VERSION; }
+
+extern "C" int et_block_abi_version(void) { return ET_BLOCK_ABI_VERSION; }
 
 extern "C" const char* et_last_error(void) { return et::g_last_error.c_str(); }

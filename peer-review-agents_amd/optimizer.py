@@ -1,0 +1,352 @@
+"""The optimizer step of the weights around the expert path: AdamW over many
+tensors at once, with states in 32 or in 8 bits, and the global gradient norm
+that clips it.
+
+The gradients of this package's expert projections and router are float32
+(:func:`expert_gemm_weight_grad`, :func:`router_weight_grad`) and their weights
+bfloat16, so a parameter is either a float32 tensor or a bfloat16 one with a
+float32 master that the step works on.  Every function validates its arguments
+in Python and makes one library call for all tensors of a kind (include/
+etmoe_block.h has the formulas); there is no CPU fallback.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Sequence
+
+import torch
+
+from ._lib import ET_DTYPE_BF16, ET_DTYPE_F32, AdamWScalars, lib
+from .expert_threshold import _call, _require, _require_device, _vp
+
+# Elements that share one scale of the 8-bit states.
+ADAMW8_BLOCK = 256
+
+_DTYPES = {torch.float32: ET_DTYPE_F32, torch.bfloat16: ET_DTYPE_BF16}
+
+# A step over many small tensors takes some 20 us on the device, so the checks
+# of a list run as C calls mapped over it: 50 ns for each tensor and check.
+_data_ptr = torch.Tensor.data_ptr
+_numel = torch.Tensor.numel
+_get_device = torch.Tensor.get_device
+_is_contiguous = torch.Tensor.is_contiguous
+_is_tensor = torch.is_tensor
+
+
+def _array(ptrs):
+    return (ctypes.c_void_p * len(ptrs))(*ptrs)
+
+
+def _numel_array(sizes):
+    return (ctypes.c_int64 * len(sizes))(*sizes)
+
+
+def _check_list(ts, name: str, dtypes, device: int, sizes) -> None:
+    """Every tensor of `ts` contiguous, on HIP device `device`, of one of
+    `dtypes` and of as many elements as `sizes` says."""
+    if not isinstance(ts, (list, tuple)):
+        raise TypeError(f"{name} must be a list or a tuple of tensors")
+    if len(ts) != len(sizes):
+        raise ValueError(f"{name} has {len(ts)} tensors, params has {len(sizes)}")
+    if not all(map(_is_tensor, ts)):
+        raise TypeError(f"{name} must hold torch.Tensors")
+    if (list(map(_numel, ts)) == sizes and all(map(_is_contiguous, ts)) and set(map(_get_device, ts)) <= {device}
+            and {t.dtype for t in ts} <= dtypes):
+        return
+    for i, t in enumerate(ts):
+        _require_device(t, f"{name}[{i}]")
+        if t.dtype not in dtypes:
+            raise TypeError(f"{name}[{i}] must be {' or '.join(map(str, dtypes))}, got {t.dtype}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name}[{i}] must be contiguous")
+        if t.numel() != sizes[i]:
+            raise ValueError(f"{name}[{i}] has {t.numel()} elements, expected {sizes[i]}")
+        if t.get_device() != device:
+            raise ValueError(f"{name}[{i}] is on {t.device}, expected cuda:{device}")
+
+
+def _check_params(params) -> tuple:
+    """(device index, sizes) of a checked, non-empty list of parameters."""
+    if not isinstance(params, (list, tuple)):
+        raise TypeError("params must be a list or a tuple of tensors")
+    if not params:
+        raise ValueError("params must hold at least one tensor")
+    _require_device(params[0], "params[0]")
+    sizes = [t.numel() if isinstance(t, torch.Tensor) else -1 for t in params]
+    _check_list(params, "params", _DTYPES.keys(), params[0].get_device(), sizes)
+    return params[0].get_device(), sizes
+
+
+def _check_masters(params, masters, device, sizes) -> None:
+    low = [p.dtype == torch.bfloat16 for p in params]
+    if masters is None:
+        if any(low):
+            raise ValueError("bfloat16 parameters need float32 masters")
+        return
+    if not isinstance(masters, (list, tuple)) or len(masters) != len(params):
+        raise ValueError("masters must be a list of one entry for each parameter")
+    if [m is not None for m in masters] != low:
+        raise ValueError("masters must hold a tensor for every bfloat16 parameter and None for every float32 one")
+    _check_list([m for m in masters if m is not None], "masters", {torch.float32}, device,
+                [n for n, b in zip(sizes, low) if b])
+
+
+def _scalars(step: int, lr: float, betas, eps: float, weight_decay: float) -> AdamWScalars:
+    step = int(step)
+    b1, b2 = (float(b) for b in betas)
+    if step < 1:
+        raise ValueError(f"step must be >= 1, got {step}")
+    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+        raise ValueError(f"betas must be in [0, 1), got {betas}")
+    if not (lr >= 0.0 and eps >= 0.0 and weight_decay >= 0.0 and max(lr, eps, weight_decay) < math.inf):
+        raise ValueError("lr, eps and weight_decay must be finite and >= 0")
+    return AdamWScalars(b1, 1.0 - b1, b2, 1.0 - b2, 1.0 / math.sqrt(1.0 - b2 ** step), eps, 1.0 - lr * weight_decay,
+                        lr / (1.0 - b1 ** step))
+
+
+def _check_scale(grad_scale, dev) -> None:
+    if grad_scale is None:
+        return
+    _require_device(grad_scale, "grad_scale")
+    if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != dev:
+        raise ValueError(f"grad_scale must be one float32 value on {dev}")
+
+
+# --------------------------------------------------------------------------- #
+# gradient norm
+# --------------------------------------------------------------------------- #
+
+def grad_norm(grads: Sequence[torch.Tensor], max_norm: Optional[float] = None, *,
+              workspace: Optional[torch.Tensor] = None):
+    """(norm, scale) of many gradients (f32 or bf16, contiguous): their global
+    2-norm and min(1, max_norm / (norm + 1e-6)), one float32 value each on the
+    device; scale is None without max_norm.  Squares and sums are binary64 in a
+    fixed order.  Where the norm is not finite the scale is NaN, with which
+    :func:`adamw_step_` and :func:`adamw8_step_` leave everything as it is.
+    """
+    if not isinstance(grads, (list, tuple)):
+        raise TypeError("grads must be a list or a tuple of tensors")
+    if not grads:
+        raise ValueError("grads must hold at least one tensor")
+    _require_device(grads[0], "grads[0]")
+    if max_norm is not None and not max_norm > 0.0:
+        raise ValueError(f"max_norm must be > 0, got {max_norm}")
+    dev = grads[0].device
+    sizes = [t.numel() if isinstance(t, torch.Tensor) else -1 for t in grads]
+    _check_list(grads, "grads", _DTYPES.keys(), grads[0].get_device(), sizes)
+    numel = _numel_array(sizes)
+    wsb = int(lib().et_grad_norm_workspace_bytes(numel, len(sizes)))
+    if workspace is None:
+        workspace = torch.empty(max(wsb, 8), dtype=torch.uint8, device=dev)
+    elif workspace.device != dev or workspace.numel() * workspace.element_size() < wsb:
+        raise ValueError(f"workspace must hold {wsb} bytes on {dev}")
+    out = torch.empty(2, dtype=torch.float32, device=dev)
+    norm = out.data_ptr()
+    dtypes = (ctypes.c_int32 * len(sizes))(*[_DTYPES[t.dtype] for t in grads])
+    _call("et_grad_norm", dev, _array(list(map(_data_ptr, grads))), numel, dtypes, len(sizes),
+          0.0 if max_norm is None else float(max_norm), norm, None if max_norm is None else norm + 4, _vp(workspace),
+          workspace.numel() * workspace.element_size())
+    return out[0], None if max_norm is None else out[1]
+
+
+# --------------------------------------------------------------------------- #
+# AdamW
+# --------------------------------------------------------------------------- #
+
+def _kinds(params, grads):
+    """Index lists of the tensors that one library call can take: one parameter
+    and one gradient type each (None where a single call takes all)."""
+    pairs = [(p.dtype, g.dtype) for p, g in zip(params, grads)]
+    if len(set(pairs)) == 1:
+        return [None]
+    return [[i for i, q in enumerate(pairs) if q == pair] for pair in dict.fromkeys(pairs)]
+
+
+def _step(fn: str, dev, params, grads, states, masters, sizes, scalars, grad_scale, *more) -> None:
+    """The library calls of one step, its lists checked."""
+    for at in _kinds(params, grads):
+        def take(ts):
+            return ts if at is None else [ts[i] for i in at]
+        p, g = take(params), take(grads)
+        low = p[0].dtype == torch.bfloat16
+        _call(fn, dev, _array(list(map(_data_ptr, p))), _array(list(map(_data_ptr, g))),
+              *(_array(list(map(_data_ptr, take(s)))) for s in states),
+              _array(list(map(_data_ptr, take(masters)))) if low else None, _numel_array(take(sizes)), len(p),
+              _DTYPES[p[0].dtype], _DTYPES[g[0].dtype], scalars, _vp(grad_scale), *more)
+
+
+def adamw_step_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avg: Sequence[torch.Tensor],
+                exp_avg_sq: Sequence[torch.Tensor], *, step: int, lr: float, betas=(0.9, 0.999), eps: float = 1e-8,
+                weight_decay: float = 0.01, masters: Optional[Sequence[Optional[torch.Tensor]]] = None,
+                grad_scale: Optional[torch.Tensor] = None) -> None:
+    """One AdamW step (decoupled weight decay), in place, over all tensors:
+    with g = grad * grad_scale,
+
+        m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2
+        w = (1 - lr wd) w - lr / (1 - b1^step) * m / (sqrt(v / (1 - b2^step)) + eps)
+
+    in binary32.  A float32 parameter is w itself; a bfloat16 one is w rounded,
+    w being its float32 master (``masters[i]``, None for float32 parameters).
+    exp_avg (m) and exp_avg_sq (v) are float32; grads float32 or bfloat16.
+    ``grad_scale`` is one float32 value on the device (:func:`grad_norm`'s); the
+    step is skipped, every bit kept, where it is not finite.
+    """
+    index, sizes = _check_params(params)
+    dev = params[0].device
+    _check_list(grads, "grads", _DTYPES.keys(), index, sizes)
+    _check_list(exp_avg, "exp_avg", {torch.float32}, index, sizes)
+    _check_list(exp_avg_sq, "exp_avg_sq", {torch.float32}, index, sizes)
+    _check_masters(params, masters, index, sizes)
+    _check_scale(grad_scale, dev)
+    _step("et_adamw", dev, params, grads, (exp_avg, exp_avg_sq), masters, sizes,
+          _scalars(step, lr, betas, eps, weight_decay), grad_scale)
+
+
+def adamw8_scales(numel: int) -> int:
+    """Entries of the scale tensor of an 8-bit state of `numel` elements."""
+    return -(-int(numel) // ADAMW8_BLOCK)
+
+
+def adamw8_step_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avg: Sequence[torch.Tensor],
+                 exp_avg_scale: Sequence[torch.Tensor], exp_avg_root: Sequence[torch.Tensor],
+                 exp_avg_root_scale: Sequence[torch.Tensor], *, step: int, lr: float, betas=(0.9, 0.999),
+                 eps: float = 1e-8, weight_decay: float = 0.01,
+                 masters: Optional[Sequence[Optional[torch.Tensor]]] = None,
+                 grad_scale: Optional[torch.Tensor] = None, seed: Optional[int] = None) -> None:
+    """:func:`adamw_step_` with 8-bit states: exp_avg (m) and exp_avg_root
+    (sqrt(v)) are ``torch.float8_e4m3fn`` of the parameter's element count, and
+    their scales float32 with one entry for every 256 elements; the value held
+    is the e4m3 value times its block's scale.  All zero is the start.
+
+    ``seed`` None rounds the states to nearest; a number (32 bits are used)
+    rounds them stochastically, which a moving average needs to keep moving on
+    so coarse a grid: give another one every step.
+    """
+    index, sizes = _check_params(params)
+    dev = params[0].device
+    blocks = list(map(adamw8_scales, sizes))
+    _check_list(grads, "grads", _DTYPES.keys(), index, sizes)
+    _check_list(exp_avg, "exp_avg", {torch.float8_e4m3fn}, index, sizes)
+    _check_list(exp_avg_root, "exp_avg_root", {torch.float8_e4m3fn}, index, sizes)
+    _check_list(exp_avg_scale, "exp_avg_scale", {torch.float32}, index, blocks)
+    _check_list(exp_avg_root_scale, "exp_avg_root_scale", {torch.float32}, index, blocks)
+    _check_masters(params, masters, index, sizes)
+    _check_scale(grad_scale, dev)
+    _step("et_adamw8", dev, params, grads, (exp_avg, exp_avg_scale, exp_avg_root, exp_avg_root_scale), masters, sizes,
+          _scalars(step, lr, betas, eps, weight_decay), grad_scale, int(seed is not None), (seed or 0) & 0xFFFFFFFF)
+
+
+class AdamW:
+    """AdamW that holds its states, for a fixed list of parameters.
+
+    ``state`` "f32" or "e4m3" (8 bits; ``stochastic`` rounding with the random
+    words of ``seed + step number``, or to nearest).  The states (and the
+    masters of bfloat16 parameters, unless given) are views of one allocation
+    for each kind, ``flat[name]``, each tensor from a multiple of 256 elements
+    on.  ``step(grads)`` takes one gradient for each parameter, or None for one
+    that has none this time.  The parameters' own storage may move between
+    steps (``p.data = ...``) as long as type, shape and device stay.
+    """
+
+    def __init__(self, params: Sequence[torch.Tensor], *, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 0.01, state: str = "f32",
+                 masters: Optional[Sequence[Optional[torch.Tensor]]] = None, stochastic: bool = True, seed: int = 0):
+        self.params = list(params)
+        self._index, self._sizes = _check_params(self.params)
+        self._dtypes = [p.dtype for p in self.params]
+        dev = self.params[0].device
+        _scalars(1, lr, betas, eps, weight_decay)
+        if state not in ("f32", "e4m3"):
+            raise ValueError(f"state must be 'f32' or 'e4m3', got {state!r}")
+        self.lr, self.betas, self.eps, self.weight_decay = lr, betas, eps, weight_decay
+        self.state, self.stochastic, self.seed, self.steps = state, bool(stochastic), int(seed), 0
+        self._starts, n = [], 0
+        for size in self._sizes:
+            self._starts.append(n)
+            n += adamw8_scales(size) * ADAMW8_BLOCK
+        self.flat = {}
+
+        def views(name, dtype, per=1):
+            flat = self.flat[name] = torch.zeros(n // per, dtype=dtype, device=dev)
+            if per > 1:
+                return [flat[a // per:a // per + adamw8_scales(s)] for a, s in zip(self._starts, self._sizes)]
+            return [flat[a:a + s].view(p.shape) for a, s, p in zip(self._starts, self._sizes, self.params)]
+
+        if state == "f32":
+            self.exp_avg, self.exp_avg_sq = (views(k, torch.float32) for k in ("exp_avg", "exp_avg_sq"))
+            self._states = self.exp_avg, self.exp_avg_sq
+        else:
+            self.exp_avg, self.exp_avg_root = (views(k, torch.float8_e4m3fn) for k in ("exp_avg", "exp_avg_root"))
+            self.exp_avg_scale, self.exp_avg_root_scale = (
+                views(k, torch.float32, ADAMW8_BLOCK) for k in ("exp_avg_scale", "exp_avg_root_scale"))
+            self._states = self.exp_avg, self.exp_avg_scale, self.exp_avg_root, self.exp_avg_root_scale
+        if masters is None and torch.bfloat16 in self._dtypes:
+            masters = [v if p.dtype == torch.bfloat16 else None
+                       for v, p in zip(views("masters", torch.float32), self.params)]
+            for v, p in zip(masters, self.params):
+                if v is not None:
+                    v.copy_(p.detach())
+        _check_masters(self.params, masters, self._index, self._sizes)
+        self.masters = None if masters is None else list(masters)
+        # (the states' own buffers never move)
+        self._tables = [_array(list(map(_data_ptr, s))) for s in self._states]
+        self._numel = _numel_array(self._sizes)
+
+    def step(self, grads: Sequence[Optional[torch.Tensor]], *, grad_scale: Optional[torch.Tensor] = None,
+             lr: Optional[float] = None) -> None:
+        """One step; ``lr`` for this step only.  The step number counts the steps
+        that a grad_scale that is not finite made the device skip, too."""
+        params, sizes, states, masters = self.params, self._sizes, self._states, self.masters
+        dev = params[0].device
+        if not isinstance(grads, (list, tuple)):
+            raise TypeError("grads must be a list or a tuple of tensors")
+        if len(grads) != len(params):
+            raise ValueError(f"grads has {len(grads)} tensors, params has {len(params)}")
+        if [p.dtype for p in params] != self._dtypes:
+            raise TypeError("a parameter changed its type")
+        _check_list(params, "params", _DTYPES.keys(), self._index, sizes)
+        whole = all(g is not None for g in grads)
+        if not whole:
+            at = [i for i, g in enumerate(grads) if g is not None]
+            params, grads, sizes = ([ts[i] for i in at] for ts in (params, grads, sizes))
+            states = [[s[i] for i in at] for s in states]
+            masters = None if masters is None else [masters[i] for i in at]
+        _check_list(grads, "grads", _DTYPES.keys(), self._index, sizes)
+        _check_scale(grad_scale, dev)
+        scalars = _scalars(self.steps + 1, self.lr if lr is None else lr, self.betas, self.eps, self.weight_decay)
+        fn, more = "et_adamw", ()
+        if self.state == "e4m3":
+            fn, more = "et_adamw8", (int(self.stochastic), (self.seed + self.steps + 1) & 0xFFFFFFFF)
+        if whole and len(set(self._dtypes)) == 1 and len({g.dtype for g in grads}) == 1:
+            _call(fn, dev, _array(list(map(_data_ptr, params))), _array(list(map(_data_ptr, grads))), *self._tables,
+                  None if masters is None else _array(list(map(_data_ptr, masters))), self._numel, len(params),
+                  _DTYPES[self._dtypes[0]], _DTYPES[grads[0].dtype], scalars, _vp(grad_scale), *more)
+        elif params:
+            _step(fn, dev, params, grads, states, masters, sizes, scalars, grad_scale, *more)
+        self.steps += 1
+
+    def state_dict(self) -> dict:
+        """Copies of the states and masters (flat), and the step number."""
+        held = {k: v.clone() for k, v in self.flat.items()}
+        if self.masters is not None and "masters" not in held:
+            held["masters"] = [None if m is None else m.clone() for m in self.masters]
+        return dict(held, steps=self.steps)
+
+    def load_state_dict(self, held: dict) -> None:
+        """Takes over :meth:`state_dict`'s values; the parameters are the caller's."""
+        names = set(self.flat) | ({"masters"} if self.masters is not None else set()) | {"steps"}
+        if set(held) != names:
+            raise ValueError(f"state has {sorted(held)}, expected {sorted(names)}")
+        for k, v in self.flat.items():
+            if held[k].shape != v.shape or held[k].dtype != v.dtype:
+                raise ValueError(f"{k} must be {v.dtype} of shape {tuple(v.shape)}")
+        if "masters" in held and "masters" not in self.flat:
+            if len(held["masters"]) != len(self.masters):
+                raise ValueError("masters must have one entry for each parameter")
+            for mine, other in zip(self.masters, held["masters"]):
+                if mine is not None:
+                    mine.copy_(other)
+        for k, v in self.flat.items():
+            v.copy_(held[k])
+        self.steps = int(held["steps"])
