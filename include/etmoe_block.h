@@ -27,6 +27,53 @@ extern "C" {
 int et_block_abi_version(void);
 
 /* ------------------------------------------------------------------------ *
+ * Layer norm
+ * ------------------------------------------------------------------------ */
+
+/* Longest row of the layer norm (a row is held in one block's registers). */
+#define ET_MAX_NORM_WIDTH 16384
+
+/*
+ * Layer norm over rows of d elements, with the residual add before it:
+ *   h[t, c]  = x[t, c] + residual[t, c], rounded to `dtype`, written to sum
+ *              (without a residual: h = x, nothing written)
+ *   mean[t]  = sum_c h[t, c] / d
+ *   rstd[t]  = 1 / sqrt(sum_c (h[t, c] - mean[t])^2 / d + eps)
+ *   y[t, c]  = (h[t, c] - mean[t]) * rstd[t] * weight[c] + bias[c]
+ * in binary32 in a fixed order, y rounded once to `dtype`: repeated calls give
+ * identical bits.  x and residual [rows, d] of `dtype` with row strides in
+ * elements (>= d); sum and y dense.  weight and bias [d] of weight_dtype: that
+ * of the rows, or ET_DTYPE_F32.  residual and sum go together, and mean and
+ * rstd (f32 [rows], what the backward needs); each pair may be NULL, and
+ * bias.  Every pointer element-aligned; 1 <= d <= ET_MAX_NORM_WIDTH.  A NaN or
+ * an infinity in a row makes that row's outputs NaN and no other's.  sum may
+ * be x or residual, and y may be x or residual, where those rows are dense.
+ */
+int et_layer_norm_fwd(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                      const void* weight, const void* bias, int64_t rows, int64_t d, int dtype, int weight_dtype,
+                      float eps, void* y, void* sum, float* mean, float* rstd, void* stream);
+
+/* Bytes of device workspace et_layer_norm_bwd needs (partial column sums of
+ * its blocks; 0 for invalid sizes). */
+size_t et_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t d);
+
+/*
+ * Backward of the layer norm, with h its input (x or sum of the forward):
+ *   xhat = (h - mean) * rstd,  g = dy * weight
+ *   dx[t, c]   = rstd[t] * (g - sum_c(g) / d - xhat * sum_c(g * xhat) / d) + dsum[t, c]
+ *   dweight[c] = sum_t dy[t, c] * xhat[t, c],  dbias[c] = sum_t dy[t, c]
+ * in binary32, dx rounded once to `dtype` and dense, dweight and dbias f32 [d].
+ * dy, h and dsum [rows, d] with row strides in elements.  dsum, the gradient
+ * that reaches h past the norm (the residual branch), and dbias may be NULL.
+ * The column sums are over blocks of rows, then over the blocks, in a fixed order.
+ * No rows: dweight and dbias are 0.  workspace 4-byte aligned.
+ */
+int et_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* h, int64_t h_stride, const void* dsum,
+                      int64_t dsum_stride, const void* weight, const float* mean, const float* rstd, int64_t rows,
+                      int64_t d, int dtype, int weight_dtype, void* dx, float* dweight, float* dbias,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ *
  * AdamW over many tensors
  * ------------------------------------------------------------------------ */
 

@@ -3,7 +3,8 @@
 Import with ``importlib.import_module("peer-review-agents_amd")`` (the
 directory name is not a Python identifier).  Kernels live in csrc/ and are
 built into libetmoe.so by build.py; the host API is in expert_threshold.py (the
-dispatch path) and optimizer.py (AdamW, the gradient norm), and ops.py registers
+dispatch path), norm.py (layer norm) and optimizer.py (AdamW, the gradient
+norm), and ops.py registers
 the path as PyTorch operators (torch.ops.etmoe.*).
 """
 from ._lib import BLOCK_HEADER_PATH, ETMoEError, LIB_PATH, header_symbols, lib  # noqa: F401
@@ -34,6 +35,12 @@ from .expert_threshold import (  # noqa: F401
     swiglu_backward,
     threshold_update_,
     threshold_workspace_bytes,
+)
+from .norm import (  # noqa: F401
+    layer_norm,
+    layer_norm_autograd,
+    layer_norm_backward,
+    layer_norm_backward_workspace_bytes,
 )
 from .optimizer import (  # noqa: F401
     ADAMW8_BLOCK,

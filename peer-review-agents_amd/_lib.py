@@ -23,6 +23,7 @@ ET_DTYPE_F32 = 0
 ET_DTYPE_BF16 = 1
 ET_MAX_EXPERTS = 1024
 ET_MAX_ROUTER_EXPERTS = 256
+ET_MAX_NORM_WIDTH = 16384
 ET_GEMM_PLAIN, ET_GEMM_ROW_SCALE, ET_GEMM_SWIGLU = 0, 1, 2
 
 
@@ -54,6 +55,10 @@ class AdamWScalars(ctypes.Structure):
 # Names of include/etmoe_block.h (lists of tensors are host arrays: _p too).
 _BLOCK_SIGNATURES = {
     "et_block_abi_version": (_int, []),
+    "et_layer_norm_fwd": (_int, [_p, _i64, _p, _i64, _p, _p, _i64, _i64, _int, _int, _f, _p, _p, _p, _p, _p]),
+    "et_layer_norm_bwd_workspace_bytes": (_sz, [_i64, _i64]),
+    "et_layer_norm_bwd": (_int, [_p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _i64, _i64, _int, _int, _p, _p, _p, _p, _sz,
+                                 _p]),
     "et_grad_norm_workspace_bytes": (_sz, [_p, _i64]),
     "et_grad_norm": (_int, [_p, _p, _p, _i64, _f, _p, _p, _p, _sz, _p]),
     "et_adamw": (_int, [_p, _p, _p, _p, _p, _p, _i64, _int, _int, AdamWScalars, _p, _p]),

@@ -1,0 +1,505 @@
+// et_layer_norm.hip -- layer norm over rows, with the residual add before it,
+// and its backward with the reductions of the weight's and bias's gradients
+// (gfx950).
+#include <algorithm>
+
+#include "et_common.hpp"
+#include "etmoe_block.h"
+
+namespace et {
+namespace {
+
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+// 16 bytes at an address aligned to the element only: rows may start anywhere
+// (one global_load_dwordx4 all the same; a row that starts at a 16-byte
+// address costs no more than with an aligned type).
+typedef u32x4_t u32x4_any_t __attribute__((aligned(2)));
+typedef float f32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
+
+// An element type: V of them in 16 bytes.
+template <typename X>
+struct Elem {
+    static constexpr int V = 16 / sizeof(X);
+    static __device__ __forceinline__ float get(u32x4_t w, int j)
+    {
+        if constexpr (sizeof(X) == 2) return j & 1 ? bf16hi(w[j >> 1]) : bf16lo(w[j >> 1]);
+        else return u2f(w[j]);
+    }
+    static __device__ __forceinline__ u32x4_t pack(const float (&v)[V])
+    {
+        if constexpr (sizeof(X) == 2)
+            return u32x4_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                           pack_bf16x2(v[6], v[7])};
+        else
+            return u32x4_t{f2u(v[0]), f2u(v[1]), f2u(v[2]), f2u(v[3])};
+    }
+    static __device__ __forceinline__ float to_float(X x)
+    {
+        if constexpr (sizeof(X) == 2) return u2f((uint32_t)x << 16);
+        else return x;
+    }
+    static __device__ __forceinline__ X from_float(float v)
+    {
+        if constexpr (sizeof(X) == 2) return (X)f32_to_bf16_bits(v);
+        else return v;
+    }
+};
+
+// A row dealt to TPR threads: NV whole vectors of V elements each (vector t +
+// TPR i to thread t), and the d % V elements behind them one to a thread.
+template <typename X, int TPR, int NV>
+struct Row {
+    static constexpr int V = Elem<X>::V;
+    u32x4_t v[NV];
+    float tail;
+
+    __device__ __forceinline__ void load(const X* row, int d, int t)
+    {
+        const int nvec = d / V;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            v[i] = u32x4_t{};
+            const int k = t + TPR * i;
+            if (k < nvec) v[i] = *reinterpret_cast<const u32x4_any_t*>(row + (int64_t)k * V);
+        }
+        tail = 0.0f;
+        if (t < d % V) tail = Elem<X>::to_float(row[nvec * V + t]);
+    }
+    // f(vector, its first column, whether the row holds it) and g(tail, its column), in a fixed order
+    template <typename F, typename G>
+    __device__ __forceinline__ void each(int d, int t, F f, G g)
+    {
+        const int nvec = d / V;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int k = t + TPR * i;
+            if (k < nvec) f(v[i], k * V, i);
+        }
+        if (t < d % V) g(tail, nvec * V + t);
+    }
+};
+
+template <typename W, int V>
+__device__ __forceinline__ void load_weights(const W* w, int col, float (&out)[V])
+{
+    if constexpr (sizeof(W) == 2) {
+        static_assert(V == 8, "bf16 weights go with bf16 rows");
+        const u32x4_t u = *reinterpret_cast<const u32x4_any_t*>(w + col);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) out[j] = Elem<W>::get(u, j);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+            const f32x4_any_t u = *reinterpret_cast<const f32x4_any_t*>(w + col + j);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) out[j + i] = u[i];
+        }
+    }
+}
+
+// Sums over the threads of a row: a wave's lanes, then its waves through LDS
+// (the caller's slots; one barrier).  Every thread gets the same bits.
+template <int WPR, int N>
+__device__ __forceinline__ void row_sums(float (&s)[N], float (*slots)[N], int wave)
+{
+#pragma unroll
+    for (int j = 0; j < N; ++j) s[j] = wave_sum_dpp(s[j]);
+    if constexpr (WPR > 1) {
+        if (lane_id() == 0) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) slots[wave][j] = s[j];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            s[j] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WPR; ++w) s[j] += slots[w][j];
+        }
+    }
+}
+
+struct FwdArgs {
+    const void* x;
+    const void* residual;     // or null
+    const void* weight;
+    const void* bias;         // or null
+    void* y;
+    void* sum;                // with a residual
+    float* mean;              // or null
+    float* rstd;
+    int64_t ldx, ldr, T;
+    int d;
+    float eps;
+};
+
+// WPR waves per row; blocks of 256 threads (WPR = 16: 1024).
+template <typename X, typename W, int WPR, int NV>
+__global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void layer_norm_fwd_kernel(FwdArgs a)
+{
+    constexpr int TPR = WPR * kWave, V = Elem<X>::V, kRows = WPR == 16 ? 1 : 4 / WPR;
+    __shared__ float slots[2][WPR == 16 ? 16 : 4][1];
+    const int t = (int)threadIdx.x % TPR, wave = t / kWave;
+    const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
+    if (row >= a.T) return;               // (whole waves; whole blocks where there are barriers)
+    const int d = a.d;
+    Row<X, TPR, NV> r;
+    r.load((const X*)a.x + row * a.ldx, d, t);
+    if (a.residual) {
+        Row<X, TPR, NV> q;
+        q.load((const X*)a.residual + row * a.ldr, d, t);
+        X* const sum = (X*)a.sum + row * d;
+        r.each(
+            d, t,
+            [&](u32x4_t& v, int col, int i) {
+                float s[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) s[j] = Elem<X>::get(v, j) + Elem<X>::get(q.v[i], j);
+                v = Elem<X>::pack(s);
+                *reinterpret_cast<u32x4_any_t*>(sum + col) = v;
+            },
+            [&](float& v, int col) {
+                const X s = Elem<X>::from_float(v + q.tail);
+                sum[col] = s;
+                v = Elem<X>::to_float(s);
+            });
+    }
+    float s[1] = {0.0f};
+    r.each(
+        d, t,
+        [&](u32x4_t& v, int, int) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) s[0] += Elem<X>::get(v, j);
+        },
+        [&](float v, int) { s[0] += v; });
+    row_sums<WPR, 1>(s, slots[0], wave);
+    const float mean = s[0] / (float)d;
+    s[0] = 0.0f;
+    r.each(
+        d, t,
+        [&](u32x4_t& v, int, int) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float c = Elem<X>::get(v, j) - mean;
+                s[0] = __builtin_fmaf(c, c, s[0]);
+            }
+        },
+        [&](float v, int) { s[0] = __builtin_fmaf(v - mean, v - mean, s[0]); });
+    row_sums<WPR, 1>(s, slots[1], wave);
+    const float rstd = 1.0f / __builtin_sqrtf(s[0] / (float)d + a.eps);
+    const W* const w = (const W*)a.weight;
+    const W* const b = (const W*)a.bias;
+    X* const y = (X*)a.y + row * d;
+    r.each(
+        d, t,
+        [&](u32x4_t& v, int col, int) {
+            float wv[V], bv[V] = {}, out[V];
+            load_weights(w, col, wv);
+            if (b) load_weights(b, col, bv);
+#pragma unroll
+            for (int j = 0; j < V; ++j) out[j] = __builtin_fmaf((Elem<X>::get(v, j) - mean) * rstd, wv[j], bv[j]);
+            *reinterpret_cast<u32x4_any_t*>(y + col) = Elem<X>::pack(out);
+        },
+        [&](float v, int col) {
+            y[col] = Elem<X>::from_float(__builtin_fmaf((v - mean) * rstd, Elem<W>::to_float(w[col]),
+                                                        b ? Elem<W>::to_float(b[col]) : 0.0f));
+        });
+    if (a.mean && t == 0) {
+        a.mean[row] = mean;
+        a.rstd[row] = rstd;
+    }
+}
+
+struct BwdArgs {
+    const void* dy;
+    const void* x;
+    const void* dsum;         // or null
+    const void* weight;
+    const float* mean;
+    const float* rstd;
+    void* dx;
+    float* partial;           // [blocks][2][d]: the blocks' sums of dy * xhat and of dy
+    int64_t lddy, ldx, ldds, T;
+    int d;
+};
+
+// A block walks rows blockIdx, blockIdx + gridDim, ... (4 / WPR at a time), its
+// threads keeping their columns' sums for the weight and the bias.
+template <typename X, typename W, int WPR, int NV>
+__global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void layer_norm_bwd_kernel(BwdArgs a)
+{
+    constexpr int TPR = WPR * kWave, V = Elem<X>::V, kRows = WPR == 16 ? 1 : 4 / WPR;
+    __shared__ float slots[2][WPR == 16 ? 16 : 4][2];
+    const int t = (int)threadIdx.x % TPR, wave = t / kWave, sub = (int)threadIdx.x / TPR;
+    const int d = a.d;
+    const W* const w = (const W*)a.weight;
+    float dw[NV][V], db[NV][V], dwt = 0.0f, dbt = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) dw[i][j] = db[i][j] = 0.0f;
+    int turn = 0;
+    for (int64_t row = (int64_t)blockIdx.x * kRows + sub; row < a.T; row += (int64_t)gridDim.x * kRows, turn ^= 1) {
+        Row<X, TPR, NV> x, dy, ds;
+        x.load((const X*)a.x + row * a.ldx, d, t);
+        dy.load((const X*)a.dy + row * a.lddy, d, t);
+        if (a.dsum) ds.load((const X*)a.dsum + row * a.ldds, d, t);
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        float s[2] = {0.0f, 0.0f};
+        x.each(
+            d, t,
+            [&](u32x4_t& v, int col, int i) {
+                float wv[V];
+                load_weights(w, col, wv);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float xh = (Elem<X>::get(v, j) - mean) * rstd, dyv = Elem<X>::get(dy.v[i], j);
+                    const float g = dyv * wv[j];
+                    s[0] += g;
+                    s[1] = __builtin_fmaf(g, xh, s[1]);
+                    dw[i][j] = __builtin_fmaf(dyv, xh, dw[i][j]);
+                    db[i][j] += dyv;
+                }
+            },
+            [&](float v, int col) {
+                const float xh = (v - mean) * rstd, g = dy.tail * Elem<W>::to_float(w[col]);
+                s[0] += g;
+                s[1] = __builtin_fmaf(g, xh, s[1]);
+                dwt = __builtin_fmaf(dy.tail, xh, dwt);
+                dbt += dy.tail;
+            });
+        row_sums<WPR, 2>(s, slots[turn], wave);
+        const float c1 = s[0] / (float)d, c2 = s[1] / (float)d;
+        X* const dx = (X*)a.dx + row * d;
+        x.each(
+            d, t,
+            [&](u32x4_t& v, int col, int i) {
+                float wv[V], out[V];
+                load_weights(w, col, wv);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float xh = (Elem<X>::get(v, j) - mean) * rstd;
+                    const float g = __builtin_fmaf(Elem<X>::get(dy.v[i], j), wv[j], -c1);
+                    out[j] = rstd * __builtin_fmaf(-xh, c2, g) + (a.dsum ? Elem<X>::get(ds.v[i], j) : 0.0f);
+                }
+                *reinterpret_cast<u32x4_any_t*>(dx + col) = Elem<X>::pack(out);
+            },
+            [&](float v, int col) {
+                const float xh = (v - mean) * rstd;
+                const float g = __builtin_fmaf(dy.tail, Elem<W>::to_float(w[col]), -c1);
+                dx[col] = Elem<X>::from_float(rstd * __builtin_fmaf(-xh, c2, g) + (a.dsum ? ds.tail : 0.0f));
+            });
+    }
+    // the block's sums; with several rows at a time their threads' are added first
+    float* const out = a.partial + (int64_t)blockIdx.x * 2 * d;
+    const int nvec = d / V;
+    if constexpr (kRows > 1) {
+        constexpr int kCols = TPR * NV * V;
+        __shared__ float cols[2][kCols + kWave];
+        for (int q = 0; q < kRows; ++q) {
+            if (sub == q) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        const int c = (t + TPR * i) * V + j;
+                        cols[0][c] = q ? cols[0][c] + dw[i][j] : dw[i][j];
+                        cols[1][c] = q ? cols[1][c] + db[i][j] : db[i][j];
+                    }
+                if (t < V) {
+                    cols[0][kCols + t] = q ? cols[0][kCols + t] + dwt : dwt;
+                    cols[1][kCols + t] = q ? cols[1][kCols + t] + dbt : dbt;
+                }
+            }
+            __syncthreads();
+        }
+        for (int c = (int)threadIdx.x; c < d; c += 256) {
+            const int at = c < nvec * V ? c : kCols + c - nvec * V;
+            out[c] = cols[0][at];
+            out[d + c] = cols[1][at];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int k = t + TPR * i;
+            if (k < nvec) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    out[k * V + j] = dw[i][j];
+                    out[d + k * V + j] = db[i][j];
+                }
+            }
+        }
+        if (t < d % V) {
+            out[nvec * V + t] = dwt;
+            out[d + nvec * V + t] = dbt;
+        }
+    }
+}
+
+// Column sums of the blocks' partials, in a fixed order: 64 columns to a
+// block, wave w the partials w, w + 4, ...
+__global__ __launch_bounds__(256) void layer_norm_cols_kernel(const float* partial, int64_t blocks, int d, float* dweight,
+                                                              float* dbias)
+{
+    __shared__ float part[4][kWave];
+    const int lane = lane_id(), wave = (int)threadIdx.x / kWave;
+    const int col = (int)blockIdx.x * kWave + lane;
+    float s = 0.0f;
+    if (col < 2 * d)
+        for (int64_t b = wave; b < blocks; b += 4) s += partial[b * 2 * d + col];
+    part[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && col < 2 * d) {
+        s = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+        if (col < d) dweight[col] = s;
+        else if (dbias) dbias[col - d] = s;
+    }
+}
+
+constexpr int kMaxWidth = ET_MAX_NORM_WIDTH;
+constexpr int64_t kMaxBlocks = 1024;
+
+int64_t bwd_blocks(int64_t T) { return std::max<int64_t>(1, std::min<int64_t>((T + 3) / 4, kMaxBlocks)); }
+
+// Vectors of a row of d elements for each of `threads`.
+int vectors(int64_t d, int V, int threads) { return (int)((d / V + threads - 1) / threads); }
+
+template <typename X, typename W>
+int launch_fwd(const FwdArgs& a, hipStream_t s)
+{
+    constexpr int V = Elem<X>::V;
+    const auto go = [&](auto kernel, int rows, int threads) {
+        kernel<<<dim3((unsigned)((a.T + rows - 1) / rows)), dim3(threads), 0, s>>>(a);
+        return check_launch("layer_norm_fwd_kernel");
+    };
+    const int n1 = vectors(a.d, V, 64), n4 = vectors(a.d, V, 256);
+    if (n1 <= 1) return go(layer_norm_fwd_kernel<X, W, 1, 1>, 4, 256);
+    if (n1 <= 2) return go(layer_norm_fwd_kernel<X, W, 1, 2>, 4, 256);
+    if (n1 <= 4) return go(layer_norm_fwd_kernel<X, W, 1, 4>, 4, 256);
+    if (n4 <= 2) return go(layer_norm_fwd_kernel<X, W, 4, 2>, 1, 256);
+    if (n4 <= 4) return go(layer_norm_fwd_kernel<X, W, 4, 4>, 1, 256);
+    return go(layer_norm_fwd_kernel<X, W, 16, 16 / V>, 1, 1024);
+}
+
+template <typename X, typename W>
+int launch_bwd(const BwdArgs& a, int64_t blocks, hipStream_t s)
+{
+    constexpr int V = Elem<X>::V;
+    const auto go = [&](auto kernel, int threads) {
+        kernel<<<dim3((unsigned)blocks), dim3(threads), 0, s>>>(a);
+        return check_launch("layer_norm_bwd_kernel");
+    };
+    const int n1 = vectors(a.d, V, 64), n4 = vectors(a.d, V, 256), n16 = vectors(a.d, V, 1024);
+    if (n1 <= 1) return go(layer_norm_bwd_kernel<X, W, 1, 1>, 256);
+    if (n1 <= 2) return go(layer_norm_bwd_kernel<X, W, 1, 2>, 256);
+    if (n4 <= 1) return go(layer_norm_bwd_kernel<X, W, 4, 1>, 256);
+    if (n4 <= 2) return go(layer_norm_bwd_kernel<X, W, 4, 2>, 256);
+    if (n16 <= 1) return go(layer_norm_bwd_kernel<X, W, 16, 1>, 1024);
+    if (sizeof(X) == 2 || n16 <= 2) return go(layer_norm_bwd_kernel<X, W, 16, 2>, 1024);
+    if constexpr (sizeof(X) == 4) return go(layer_norm_bwd_kernel<X, W, 16, 4>, 1024);
+}
+
+// Checks that both directions share.
+int check_common(const char* fn, int64_t T, int64_t d, int dtype, int wdtype, int& esize)
+{
+    const std::string f(fn);
+    if (dtype != ET_DTYPE_F32 && dtype != ET_DTYPE_BF16)
+        return fail(ET_ERR_INVALID_ARGUMENT, f + ": dtype must be ET_DTYPE_F32 or ET_DTYPE_BF16");
+    if (wdtype != ET_DTYPE_F32 && wdtype != dtype)
+        return fail(ET_ERR_INVALID_ARGUMENT, f + ": weight_dtype must be ET_DTYPE_F32 or that of the rows");
+    if (T < 0 || T >= (int64_t)1 << 31) return fail(ET_ERR_INVALID_ARGUMENT, f + ": rows must be in [0, 2^31)");
+    if (d < 1 || d > kMaxWidth)
+        return fail(ET_ERR_INVALID_ARGUMENT, f + ": d must be in [1, " + std::to_string(kMaxWidth) + "]");
+    esize = dtype == ET_DTYPE_F32 ? 4 : 2;
+    return ET_OK;
+}
+
+int check_rows(const char* fn, const char* name, const void* p, int64_t ld, int64_t d, int esize)
+{
+    if (!p) return fail(ET_ERR_INVALID_ARGUMENT, std::string(fn) + ": null " + name);
+    if (ld < d) return fail(ET_ERR_INVALID_ARGUMENT, std::string(fn) + ": the row stride of " + name + " is below d");
+    if ((uintptr_t)p % esize) return fail(ET_ERR_INVALID_ARGUMENT, std::string(fn) + ": " + name + " is not aligned");
+    return ET_OK;
+}
+
+}  // namespace
+}  // namespace et
+
+using namespace et;
+
+extern "C" int et_layer_norm_fwd(const void* x, int64_t x_stride, const void* residual, int64_t residual_stride,
+                                 const void* weight, const void* bias, int64_t rows, int64_t d, int dtype,
+                                 int weight_dtype, float eps, void* y, void* sum, float* mean, float* rstd,
+                                 void* stream)
+{
+    const char* fn = "et_layer_norm_fwd";
+    int es = 0;
+    int rc = check_common(fn, rows, d, dtype, weight_dtype, es);
+    if (rc) return rc;
+    if (!(eps >= 0.0f && eps < __builtin_inff())) return fail(ET_ERR_INVALID_ARGUMENT, "et_layer_norm_fwd: eps must be >= 0");
+    if ((mean == nullptr) != (rstd == nullptr))
+        return fail(ET_ERR_INVALID_ARGUMENT, "et_layer_norm_fwd: mean and rstd go together");
+    if ((residual == nullptr) != (sum == nullptr))
+        return fail(ET_ERR_INVALID_ARGUMENT, "et_layer_norm_fwd: residual and sum go together");
+    if (rows == 0) return ET_OK;
+    const int ws = weight_dtype == ET_DTYPE_F32 ? 4 : 2;
+    rc = check_rows(fn, "x", x, x_stride, d, es);
+    if (!rc && residual) rc = check_rows(fn, "residual", residual, residual_stride, d, es);
+    if (!rc && sum) rc = check_rows(fn, "sum", sum, d, d, es);
+    if (!rc) rc = check_rows(fn, "y", y, d, d, es);
+    if (!rc) rc = check_rows(fn, "weight", weight, d, d, ws);
+    if (!rc && bias) rc = check_rows(fn, "bias", bias, d, d, ws);
+    if (!rc && mean) rc = check_rows(fn, "mean", mean, d, d, 4);
+    if (!rc && rstd) rc = check_rows(fn, "rstd", rstd, d, d, 4);
+    if (rc) return rc;
+    const FwdArgs a{x, residual, weight, bias, y, sum, mean, rstd, x_stride, residual_stride, rows, (int)d, eps};
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == ET_DTYPE_F32) return launch_fwd<float, float>(a, s);
+    return weight_dtype == ET_DTYPE_F32 ? launch_fwd<uint16_t, float>(a, s) : launch_fwd<uint16_t, uint16_t>(a, s);
+}
+
+extern "C" size_t et_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t d)
+{
+    if (rows < 0 || d < 1 || d > kMaxWidth) return 0;
+    return (size_t)bwd_blocks(rows) * 2 * (size_t)d * sizeof(float);
+}
+
+extern "C" int et_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* dsum,
+                                 int64_t dsum_stride, const void* weight, const float* mean, const float* rstd,
+                                 int64_t rows, int64_t d, int dtype, int weight_dtype, void* dx, float* dweight,
+                                 float* dbias, void* workspace, size_t workspace_bytes, void* stream)
+{
+    const char* fn = "et_layer_norm_bwd";
+    int es = 0;
+    int rc = check_common(fn, rows, d, dtype, weight_dtype, es);
+    if (rc) return rc;
+    const int ws = weight_dtype == ET_DTYPE_F32 ? 4 : 2;
+    if (rows) {
+        rc = check_rows(fn, "dy", dy, dy_stride, d, es);
+        if (!rc) rc = check_rows(fn, "x", x, x_stride, d, es);
+        if (!rc && dsum) rc = check_rows(fn, "dsum", dsum, dsum_stride, d, es);
+        if (!rc) rc = check_rows(fn, "dx", dx, d, d, es);
+        if (!rc) rc = check_rows(fn, "mean", mean, d, d, 4);
+        if (!rc) rc = check_rows(fn, "rstd", rstd, d, d, 4);
+    }
+    if (!rc) rc = check_rows(fn, "weight", weight, d, d, ws);
+    if (!rc) rc = check_rows(fn, "dweight", dweight, d, d, 4);
+    if (!rc && dbias) rc = check_rows(fn, "dbias", dbias, d, d, 4);
+    if (rc) return rc;
+    const size_t need = et_layer_norm_bwd_workspace_bytes(rows, d);
+    if (!workspace || workspace_bytes < need)
+        return fail(ET_ERR_WORKSPACE_TOO_SMALL, "et_layer_norm_bwd: workspace needs " + std::to_string(need) + " bytes");
+    if ((uintptr_t)workspace % 4) return fail(ET_ERR_INVALID_ARGUMENT, "et_layer_norm_bwd: workspace is not aligned");
+    const int64_t blocks = bwd_blocks(rows);
+    const BwdArgs a{dy, x, dsum, weight, mean, rstd, dx, (float*)workspace, dy_stride, x_stride, dsum_stride, rows, (int)d};
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == ET_DTYPE_F32) rc = launch_bwd<float, float>(a, blocks, s);
+    else rc = weight_dtype == ET_DTYPE_F32 ? launch_bwd<uint16_t, float>(a, blocks, s)
+                                           : launch_bwd<uint16_t, uint16_t>(a, blocks, s);
+    if (rc) return rc;
+    layer_norm_cols_kernel<<<dim3((unsigned)((2 * d + kWave - 1) / kWave)), dim3(256), 0, s>>>((const float*)workspace,
+                                                                                             blocks, (int)d, dweight,
+                                                                                             dbias);
+    return check_launch("layer_norm_cols_kernel");
+}

@@ -1,0 +1,157 @@
+"""Layer norm over rows, with the residual add before it, and its backward: the
+norm in front of an MoE block.  Arguments are checked in Python, each call is
+one library call on torch's current stream (include/etmoe_block.h has the
+formulas); there is no CPU fallback."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from ._lib import ET_DTYPE_F32, ET_MAX_NORM_WIDTH, lib
+from .expert_threshold import _act_dtype, _call, _out_or_new, _require, _require_device, _vp
+
+
+def _require_rows(t, name: str, dtype=None, shape=None, device=None) -> int:
+    """A 2-D tensor of rows: dense ones, any row stride.  Returns the stride."""
+    _require_device(t, name)
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be 2-D [rows, d], got shape {tuple(t.shape)}")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    rows, d = t.shape
+    along, inner = t.stride()
+    if (inner != 1 and d > 1) or (along < d and rows > 1):
+        raise ValueError(f"the rows of {name} must be contiguous and must not overlap, got strides {t.stride()}")
+    return max(along, d)
+
+
+def _check_width(d: int) -> None:
+    if not 1 <= d <= ET_MAX_NORM_WIDTH:
+        raise ValueError(f"d must be in [1, {ET_MAX_NORM_WIDTH}], got {d}")
+
+
+def _require_weight(w, name: str, d: int, dtype, device) -> int:
+    _require_device(w, name)
+    if w.dtype != torch.float32 and w.dtype != dtype:
+        raise TypeError(f"{name} must be float32 or {dtype}, got {w.dtype}")
+    _require(w, name, w.dtype, 1, device)
+    if w.shape[0] != d:
+        raise ValueError(f"{name} has {w.shape[0]} entries, the rows have {d}")
+    return _act_dtype(w, name)
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *, eps: float = 1e-5,
+               residual: Optional[torch.Tensor] = None, stats: bool = False, out: Optional[torch.Tensor] = None,
+               out_sum: Optional[torch.Tensor] = None):
+    """y = (h - mean) * rstd * weight + bias over the rows of h = x (+ residual).
+
+    x [rows, d] f32 or bf16, rows contiguous at any stride; weight and bias [d]
+    of x's type or float32.  With ``residual`` (x's type) the sum is rounded to
+    x's type and returned behind y; with ``stats`` so are mean and rstd (f32
+    [rows]), for :func:`layer_norm_backward`:
+        y | (y, sum) | (y, mean, rstd) | (y, sum, mean, rstd)
+    Binary32 arithmetic, one rounding of y, identical bits on repeated calls.
+    """
+    ldx = _require_rows(x, "x")
+    dt = _act_dtype(x, "x")
+    rows, d = x.shape
+    dev, dtype = x.device, x.dtype
+    _check_width(d)
+    wdt = _require_weight(weight, "weight", d, dtype, dev)
+    if bias is not None and _require_weight(bias, "bias", d, dtype, dev) != wdt:
+        raise TypeError("weight and bias must have the same dtype")
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"eps must be finite and >= 0, got {eps}")
+    ldr = 0
+    if residual is not None:
+        ldr = _require_rows(residual, "residual", dtype, x.shape, dev)
+        out_sum = _out_or_new(out_sum, (rows, d), dtype, dev, "out_sum")
+    elif out_sum is not None:
+        raise ValueError("out_sum needs a residual")
+    y = _out_or_new(out, (rows, d), dtype, dev, "out")
+    if stats:
+        mean, rstd = (torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(2))
+    else:
+        mean = rstd = None
+    _call("et_layer_norm_fwd", dev, _vp(x), ldx, _vp(residual), ldr, _vp(weight), _vp(bias), rows, d, dt, wdt, eps,
+          _vp(y), _vp(out_sum), _vp(mean), _vp(rstd))
+    if residual is None:
+        return (y, mean, rstd) if stats else y
+    return (y, out_sum, mean, rstd) if stats else (y, out_sum)
+
+
+def layer_norm_backward_workspace_bytes(rows: int, d: int) -> int:
+    return int(lib().et_layer_norm_bwd_workspace_bytes(rows, d))
+
+
+def layer_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, mean: torch.Tensor,
+                        rstd: torch.Tensor, *, dsum: Optional[torch.Tensor] = None, need_dbias: bool = True,
+                        out_dx: Optional[torch.Tensor] = None, out_dweight: Optional[torch.Tensor] = None,
+                        out_dbias: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None):
+    """(dx, dweight, dbias) of :func:`layer_norm`, h being its x, or the sum it
+    returned; dx is then the gradient of x and of the residual alike.
+
+    ``dsum`` (h's type) is added to dx: the gradient that reaches the sum past
+    the norm.  dx has h's type, dweight and dbias are f32 [d] (dbias None
+    without ``need_dbias``).
+    """
+    ldh = _require_rows(h, "h")
+    dt = _act_dtype(h, "h")
+    rows, d = h.shape
+    dev, dtype = h.device, h.dtype
+    _check_width(d)
+    lddy = _require_rows(dy, "dy", dtype, h.shape, dev)
+    ldds = 0 if dsum is None else _require_rows(dsum, "dsum", dtype, h.shape, dev)
+    wdt = _require_weight(weight, "weight", d, dtype, dev)
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        _require(t, name, torch.float32, 1, dev)
+        if t.shape[0] != rows:
+            raise ValueError(f"{name} has {t.shape[0]} entries, h has {rows} rows")
+    dx = _out_or_new(out_dx, (rows, d), dtype, dev, "out_dx")
+    dweight = _out_or_new(out_dweight, (d,), torch.float32, dev, "out_dweight")
+    dbias = None
+    if need_dbias or out_dbias is not None:
+        dbias = _out_or_new(out_dbias, (d,), torch.float32, dev, "out_dbias")
+    wsb = layer_norm_backward_workspace_bytes(rows, d)
+    if workspace is None:
+        workspace = torch.empty(wsb, dtype=torch.uint8, device=dev)
+    elif workspace.device != dev or workspace.numel() * workspace.element_size() < wsb:
+        raise ValueError(f"workspace must hold {wsb} bytes on {dev}")
+    _call("et_layer_norm_bwd", dev, _vp(dy), lddy, _vp(h), ldh, _vp(dsum), ldds, _vp(weight), _vp(mean), _vp(rstd),
+          rows, d, dt, wdt, _vp(dx), _vp(dweight), _vp(dbias), _vp(workspace), wsb)
+    return dx, dweight, dbias
+
+
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, residual):
+        r = layer_norm(x, weight, bias, eps=eps, residual=residual, stats=True)
+        y, mean, rstd = r[0], r[-2], r[-1]
+        h = x if residual is None else r[1]
+        ctx.save_for_backward(h, weight, mean, rstd)
+        ctx.has = bias is not None, residual is not None
+        ctx.set_materialize_grads(False)
+        return y if residual is None else (y, h)
+
+    @staticmethod
+    def backward(ctx, dy, dsum=None):
+        h, weight, mean, rstd = ctx.saved_tensors
+        has_bias, has_residual = ctx.has
+        if dy is None:          # only the sum was used
+            return dsum, None, None, None, dsum if has_residual else None
+        dx, dw, db = layer_norm_backward(dy.contiguous(), h, weight, mean, rstd,
+                                         dsum=None if dsum is None else dsum.contiguous(), need_dbias=has_bias)
+        return (dx, dw.to(weight.dtype), db.to(weight.dtype) if has_bias else None, None,
+                dx if has_residual else None)
+
+
+def layer_norm_autograd(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                        eps: float = 1e-5, residual: Optional[torch.Tensor] = None):
+    """:func:`layer_norm` (y, or (y, sum) with a residual) with a backward that
+    runs :func:`layer_norm_backward`."""
+    return _LayerNormFn.apply(x, weight, bias, eps, residual)

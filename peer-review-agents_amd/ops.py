@@ -27,18 +27,24 @@ Every eager kernel calls the C ABI of libetmoe.so through the functions of
                             need_dlogits)                       -> (dYp, dgate, dlogits)
     torch.ops.etmoe.dispatch_backward(dxp, token_offsets, token_slot) -> dX [T, d]
     torch.ops.etmoe.threshold_update_(thr, logits, k_target, momentum) -> stat (thr updated in place)
+    torch.ops.etmoe.layer_norm(x, weight, bias, eps)            -> (Y, mean, rstd)
+    torch.ops.etmoe.add_layer_norm(x, residual, weight, bias, eps) -> (Y, sum, mean, rstd)
+    torch.ops.etmoe.layer_norm_backward(dy, h, weight, mean, rstd, dsum) -> (dX, dweight, dbias)
 
 Gradients: dispatch -> dispatch_backward; combine -> combine_backward, with
 respect to yp, to the router logits (through the gates, which are the
-sigmoid scores at the routed pairs: dlogits) and to slot_gate (dgate).  The
-routing itself is piecewise constant and has no gradient.
+sigmoid scores at the routed pairs: dlogits) and to slot_gate (dgate);
+layer_norm and add_layer_norm -> layer_norm_backward, with respect to the rows,
+the weight and the bias (mean and rstd are not differentiable).  The routing
+itself is piecewise constant and has no gradient.
 """
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
 
 from . import expert_threshold as _et
+from . import norm as _norm
 
 Plan = Tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]
 
@@ -200,3 +206,81 @@ def _combine_grad(ctx, dy):
 
 
 torch.library.register_autograd("etmoe::combine", _combine_grad, setup_context=_combine_setup)
+
+
+# --------------------------------------------------------------------------- #
+# layer norm
+# --------------------------------------------------------------------------- #
+
+@torch.library.custom_op("etmoe::layer_norm", mutates_args=())
+def layer_norm(x: Tensor, weight: Tensor, bias: Optional[Tensor], eps: float) -> Tuple[Tensor, Tensor, Tensor]:
+    """(Y, mean, rstd) of the rows of x."""
+    return _norm.layer_norm(x, weight, bias, eps=eps, stats=True)
+
+
+@layer_norm.register_fake
+def _layer_norm_fake(x, weight, bias, eps):
+    f32 = dict(dtype=torch.float32)
+    return x.new_empty(x.shape), x.new_empty(x.shape[0], **f32), x.new_empty(x.shape[0], **f32)
+
+
+@torch.library.custom_op("etmoe::add_layer_norm", mutates_args=())
+def add_layer_norm(x: Tensor, residual: Tensor, weight: Tensor, bias: Optional[Tensor],
+                   eps: float) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    """(Y, sum, mean, rstd) of the rows of sum = x + residual."""
+    return _norm.layer_norm(x, weight, bias, eps=eps, residual=residual, stats=True)
+
+
+@add_layer_norm.register_fake
+def _add_layer_norm_fake(x, residual, weight, bias, eps):
+    f32 = dict(dtype=torch.float32)
+    return (x.new_empty(x.shape), x.new_empty(x.shape), x.new_empty(x.shape[0], **f32),
+            x.new_empty(x.shape[0], **f32))
+
+
+@torch.library.custom_op("etmoe::layer_norm_backward", mutates_args=())
+def layer_norm_backward(dy: Tensor, h: Tensor, weight: Tensor, mean: Tensor, rstd: Tensor,
+                        dsum: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:
+    """(dX, dweight, dbias), the last two float32; dsum is added to dX."""
+    return _norm.layer_norm_backward(dy, h, weight, mean, rstd, dsum=dsum)
+
+
+@layer_norm_backward.register_fake
+def _layer_norm_backward_fake(dy, h, weight, mean, rstd, dsum):
+    f32 = dict(dtype=torch.float32)
+    return h.new_empty(h.shape), weight.new_empty(weight.shape, **f32), weight.new_empty(weight.shape, **f32)
+
+
+def _norm_grads(ctx, dy, h, dsum):
+    weight, mean, rstd = ctx.saved_tensors[:3]
+    dy = torch.zeros_like(h) if dy is None else dy.contiguous()
+    dx, dw, db = torch.ops.etmoe.layer_norm_backward(dy, h, weight, mean, rstd,
+                                                     None if dsum is None else dsum.contiguous())
+    return dx, dw.to(weight.dtype), db.to(weight.dtype) if ctx.has_bias else None
+
+
+def _layer_norm_setup(ctx, inputs, output):
+    x, weight, bias, _eps = inputs
+    ctx.has_bias = bias is not None
+    ctx.save_for_backward(weight, output[1], output[2], x)
+
+
+def _layer_norm_grad(ctx, dy, _dmean, _drstd):
+    return (*_norm_grads(ctx, dy, ctx.saved_tensors[3], None), None)
+
+
+torch.library.register_autograd("etmoe::layer_norm", _layer_norm_grad, setup_context=_layer_norm_setup)
+
+
+def _add_layer_norm_setup(ctx, inputs, output):
+    _x, _residual, weight, bias, _eps = inputs
+    ctx.has_bias = bias is not None
+    ctx.save_for_backward(weight, output[2], output[3], output[1])
+
+
+def _add_layer_norm_grad(ctx, dy, dsum, _dmean, _drstd):
+    dx, dw, db = _norm_grads(ctx, dy, ctx.saved_tensors[3], dsum)
+    return dx, dx.clone(), dw, db, None
+
+
+torch.library.register_autograd("etmoe::add_layer_norm", _add_layer_norm_grad, setup_context=_add_layer_norm_setup)

@@ -77,3 +77,34 @@ def test_grad_norm_rejects_bad_arguments(et):
     assert call(mx=0.0) == ET_ERR_INVALID_ARGUMENT and "max_norm" in _err(et)
     assert call(wsb=7) == ET_ERR_WORKSPACE_TOO_SMALL and "workspace" in _err(et)
     assert call(ws=ctypes.c_void_p(0x1004)) == ET_ERR_INVALID_ARGUMENT
+
+
+def test_layer_norm_rejects_bad_arguments(et):
+    lib = et.lib()
+    p = ctypes.c_void_p(0x1000)
+
+    def fwd(x=p, ldx=16, r=None, ldr=0, w=p, rows=4, d=16, dt=0, wdt=0, eps=1e-5, y=p, sum=None, mean=None, rstd=None):
+        return lib.et_layer_norm_fwd(x, ldx, r, ldr, w, None, rows, d, dt, wdt, eps, y, sum, mean, rstd, None)
+
+    assert fwd(dt=2) == ET_ERR_INVALID_ARGUMENT and "dtype" in _err(et)
+    assert fwd(wdt=1) == ET_ERR_INVALID_ARGUMENT and "weight_dtype" in _err(et)
+    assert fwd(rows=-1) == ET_ERR_INVALID_ARGUMENT and "rows" in _err(et)
+    assert fwd(d=0) == ET_ERR_INVALID_ARGUMENT and fwd(d=16385, ldx=16385) == ET_ERR_INVALID_ARGUMENT
+    assert fwd(eps=-1.0) == ET_ERR_INVALID_ARGUMENT and fwd(eps=float("nan")) == ET_ERR_INVALID_ARGUMENT
+    assert fwd(x=None) == ET_ERR_INVALID_ARGUMENT and "null x" in _err(et)
+    assert fwd(ldx=15) == ET_ERR_INVALID_ARGUMENT and "stride" in _err(et)
+    assert fwd(x=ctypes.c_void_p(0x1002)) == ET_ERR_INVALID_ARGUMENT and "aligned" in _err(et)
+    assert fwd(r=p, ldr=16) == ET_ERR_INVALID_ARGUMENT and "residual" in _err(et)
+    assert fwd(mean=p) == ET_ERR_INVALID_ARGUMENT and "rstd" in _err(et)
+    assert fwd(rows=0) == 0
+
+    def bwd(dy=p, h=p, ds=None, ldds=16, w=p, mean=p, rows=4, d=16, dt=0, wdt=0, dw=p, ws=p, wsb=1 << 20):
+        return lib.et_layer_norm_bwd(dy, 16, h, 16, ds, ldds, w, mean, p, rows, d, dt, wdt, p, dw, None, ws, wsb, None)
+
+    assert lib.et_layer_norm_bwd_workspace_bytes(0, 16) > 0 and lib.et_layer_norm_bwd_workspace_bytes(4, 0) == 0
+    assert bwd(dy=None) == ET_ERR_INVALID_ARGUMENT and "dy" in _err(et)
+    assert bwd(mean=None) == ET_ERR_INVALID_ARGUMENT and "mean" in _err(et)
+    assert bwd(ds=p, ldds=8) == ET_ERR_INVALID_ARGUMENT and "dsum" in _err(et)
+    assert bwd(dw=None) == ET_ERR_INVALID_ARGUMENT and "dweight" in _err(et)
+    assert bwd(wsb=4) == ET_ERR_WORKSPACE_TOO_SMALL and "workspace" in _err(et)
+    assert bwd(ws=ctypes.c_void_p(0x1002)) == ET_ERR_INVALID_ARGUMENT
