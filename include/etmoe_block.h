@@ -3,7 +3,8 @@
  * dispatch path of etmoe.h, in the same library (libetmoe.so): the layer norm
  * before the block, forward and backward; the optimizer step of its weights
  * (AdamW over many tensors at once, with states in 32 or in 8 bits, and the
- * global gradient norm that clips it).
+ * global gradient norm that clips it); and the experts' and a dense layer's
+ * products with 4-bit weights, for serving a few tokens at a time.
  *
  * Conventions are those of etmoe.h: device pointers unless a comment says
  * otherwise, work enqueued on `stream` (NULL: the legacy default stream), no
@@ -155,6 +156,73 @@ int et_adamw8(void* const* params, const void* const* grads, uint8_t* const* m8,
               uint8_t* const* u8, float* const* u_scale, float* const* masters, const int64_t* numel,
               int64_t count, int param_dtype, int grad_dtype, et_adamw_scalars scalars, const float* grad_scale,
               int rounding, uint32_t seed, void* stream);
+
+/* ------------------------------------------------------------------------ *
+ * Products with 4-bit weights and group scales
+ * ------------------------------------------------------------------------ */
+
+/* types of the group scales */
+#define ET_W4_SCALE_BF16 0
+#define ET_W4_SCALE_F16 1
+
+/*
+ * A 4-bit weight of E experts (1: a dense layer), N rows (output features) and
+ * K columns each:
+ *   w[e, n, k] = (q[e, n, k] - 8) * scale[e, n, k / group],  q in 0..15
+ * group 32, 64 or 128; the last group of a row may be short.  K a multiple of 8 below
+ * 2^22, N*K below 2^31.  q is given as bytes [E, N, K / 2], the even k in the
+ * low half, scales as 16-bit numbers [E, N, ceil(K / group)].
+ *
+ * et_w4_pack lays both out once in the order in which the product reads them:
+ * `packed` of et_w4_packed_bytes bytes and `packed_scales` of
+ * et_w4_packed_scales 16-bit numbers, 16-byte aligned.  parts 2 lays the first and the
+ * second half of the rows out each for itself, as SwiGLU's gate and up rows
+ * need it (N a multiple of 8 for each part); 1 else.  Sizes are 0 for invalid
+ * arguments.
+ */
+size_t et_w4_packed_bytes(int64_t num_experts, int64_t N, int64_t K, int64_t parts);
+size_t et_w4_packed_scales(int64_t num_experts, int64_t N, int64_t K, int64_t group, int64_t parts);
+int et_w4_pack(const void* q, const void* scales, int64_t num_experts, int64_t N, int64_t K, int64_t group,
+               int64_t parts, void* packed, void* packed_scales, void* stream);
+
+/*
+ * 4-bit weights of a weight w [E, N, K] (ET_DTYPE_*), group by group:
+ *   scale = max(largest / 7, -smallest / 8) (0 counts), rounded to scale_type
+ *   q     = 8 + w / scale rounded to nearest, held to 0..15  (8 where scale is 0)
+ * A group with a value (or a scale) that is not finite gets a NaN scale.  q 4-byte
+ * aligned.
+ */
+int et_w4_quantize(const void* w, int dtype, int64_t num_experts, int64_t N, int64_t K, int64_t group,
+                   int scale_type, void* q, void* scales, void* stream);
+
+/*
+ * The weight as bf16 [E, N, K] (16-byte aligned), each value rounded once, of
+ * the experts with slots below slot_capacity; of all with expert_offsets NULL.
+ * The other experts' rows are left as they were.  With it, batches of many
+ * slots per expert run through et_expert_gemm.
+ */
+int et_w4_unpack(const void* packed, const void* packed_scales, int scale_type, const int32_t* expert_offsets,
+                 int64_t num_experts, int64_t N, int64_t K, int64_t group, int64_t parts, int64_t slot_capacity,
+                 void* w, void* stream);
+
+/*
+ * The expert grouped GEMM of et_expert_gemm on 4-bit weights:
+ *   p[s, n] = sum over groups g of scale[e(s), n, g] *
+ *             sum over k in g of a[row(s), k] * (q[e(s), n, k] - 8)
+ * and c[s, :] = the epilogue of p[s, :], rounded once to bf16.  row(s), the modes (gather with
+ * sorted_token, slot-major with NULL), slot_capacity, the epilogues and c are
+ * those of et_expert_gemm; ET_GEMM_SWIGLU needs parts 2.  expert_offsets NULL
+ * (with one expert and sorted_token NULL) is the dense layer: every slot below
+ * slot_capacity.  Binary32 sums in a fixed order: repeated calls give
+ * identical bits.  The inner sum is taken as sum a * (128 + q) from
+ * -136 * sum a on, so a row of a that holds an infinity (or values above
+ * 2^120) gives NaN.  a and c 16-byte aligned.
+ * Implements a 4-bit form of the expert GEMM (no reference counterpart).
+ */
+int et_expert_gemm_w4(const void* a, int64_t a_rows, const int32_t* sorted_token, const void* packed,
+                      const void* packed_scales, int scale_type, const int32_t* expert_offsets,
+                      int64_t num_experts, int64_t K, int64_t N, int64_t group, int64_t parts,
+                      int64_t slot_capacity, int epilogue, const float* row_scale, void* c, void* stream);
 
 #ifdef __cplusplus
 }

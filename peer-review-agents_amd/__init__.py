@@ -3,8 +3,8 @@
 Import with ``importlib.import_module("peer-review-agents_amd")`` (the
 directory name is not a Python identifier).  Kernels live in csrc/ and are
 built into libetmoe.so by build.py; the host API is in expert_threshold.py (the
-dispatch path), norm.py (layer norm) and optimizer.py (AdamW, the gradient
-norm), and ops.py registers
+dispatch path), norm.py (layer norm), optimizer.py (AdamW, the gradient norm)
+and w4.py (products with 4-bit weights), and ops.py registers
 the path as PyTorch operators (torch.ops.etmoe.*).
 """
 from ._lib import BLOCK_HEADER_PATH, ETMoEError, LIB_PATH, header_symbols, lib  # noqa: F401
@@ -49,4 +49,12 @@ from .optimizer import (  # noqa: F401
     adamw8_step_,
     adamw_step_,
     grad_norm,
+)
+from .w4 import (  # noqa: F401
+    W4Weight,
+    expert_gemm_w4,
+    linear_w4,
+    pack_w4,
+    quantize_w4,
+    unpack_w4,
 )

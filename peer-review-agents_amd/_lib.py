@@ -62,6 +62,14 @@ _BLOCK_SIGNATURES = {
     "et_grad_norm_workspace_bytes": (_sz, [_p, _i64]),
     "et_grad_norm": (_int, [_p, _p, _p, _i64, _f, _p, _p, _p, _sz, _p]),
     "et_adamw": (_int, [_p, _p, _p, _p, _p, _p, _i64, _int, _int, AdamWScalars, _p, _p]),
+    "et_w4_packed_bytes": (_sz, [_i64, _i64, _i64, _i64]),
+    "et_w4_packed_scales": (_sz, [_i64, _i64, _i64, _i64, _i64]),
+    "et_w4_pack": (_int, [_p, _p, _i64, _i64, _i64, _i64, _i64, _p, _p, _p]),
+    "et_w4_quantize": (_int, [_p, _int, _i64, _i64, _i64, _i64, _int, _p, _p, _p]),
+    "et_w4_unpack": (_int, [_p, _p, _int, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p]),
+    "et_expert_gemm_w4": (_int, [_p, _i64, _p, _p, _p, _int, _p, _i64, _i64, _i64, _i64, _i64, _i64, _int, _p, _p, _p]),
+    "et_expert_gemm_w4_impl": (_int, [_p, _i64, _p, _p, _p, _int, _p, _i64, _i64, _i64, _i64, _i64, _i64, _int, _p, _p,
+                                      _i64, _p]),
     "et_adamw8": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _int, _int, AdamWScalars, _p, _int, _u32, _p]),
 }
 

@@ -1,0 +1,634 @@
+// et_w4.hip -- products with 4-bit weights and group scales (gfx950): the
+// experts' projections over the routing CSR and a dense layer's, for batches of
+// a few tokens, where the time is that of reading the weights.
+//
+//   p[s, n] = sum_k a[row(s), k] * (q[e(s), n, k] - 8) * scale[e(s), n, k / G]
+//
+// Weights are laid out once, in the order in which waves read them.  A tile is
+// 16 weight rows x 128 k, 1 KiB: lane l of the wave that reads it takes 16
+// bytes, its dword s the 8 values of row l % 16 at k = 32 s + 8 (l / 16) + 0..7,
+// the operand fragment of v_mfma_f32_16x16x32_bf16 as it is.  Value 2 i of a
+// dword is at bit 4 i, value 2 i + 1 at bit 16 + 4 i, so shifting by 4 i and
+// masking gives two of them, and the bits 0x4300 above each make the bf16
+// number 128 + q: 7 instructions for 8 weights, where a conversion through f32
+// takes 12.  The 128 too much (and the 8) go out again through the
+// accumulator: a group's MFMAs begin at -136 * sum(a), which is an MFMA chain
+// of the same activations with a constant operand, shared by the tiles of a
+// wave.  (q - 8) * a is summed exactly as it would be in binary32 but for
+// the size of the partial sums, up to 17 times larger: 4 bits of 24.
+// A group's sum is then scaled and added in binary32.
+//
+// Two tiles (32 rows) of one k range are neighbours, their k ranges follow each
+// other, and their scales lie in the lanes' order: a wave's loads are whole
+// KiBs of consecutive addresses.
+#include <algorithm>
+
+#include "et_gemm_common.hpp"
+#include "etmoe_block.h"
+
+namespace et {
+namespace {
+
+constexpr int kSb = 32;                 // weight rows of a superblock: two tiles
+constexpr int kKt = 128;                // k of a tile
+constexpr int kTileBytes = 1024;
+constexpr uint32_t kMagic = 0x43004300u;    // bf16 128 | q
+constexpr uint32_t kOffset = 0xC308C308u;   // bf16 -136, twice
+
+struct W4Shape {
+    int E, N, K, parts, group;
+    __host__ __device__ int part_rows() const { return N / parts; }
+    __host__ __device__ int part_sbs() const { return (N / parts + kSb - 1) / kSb; }
+    __host__ __device__ int sbs() const { return parts * part_sbs(); }
+    __host__ __device__ int kts() const { return (K + kKt - 1) / kKt; }
+    __host__ __device__ int gpt() const { return kKt / group; }               // groups of a tile
+    __host__ __device__ int64_t expert_bytes() const { return (int64_t)sbs() * kts() * 2 * kTileBytes; }
+    __host__ __device__ int64_t expert_scales() const { return (int64_t)sbs() * kts() * gpt() * kSb; }
+    // the first weight row of superblock b, and how many of its rows there are
+    __host__ __device__ int row0(int b) const { return b / part_sbs() * part_rows() + b % part_sbs() * kSb; }
+    __host__ __device__ int rows(int b) const
+    {
+        const int left = part_rows() - b % part_sbs() * kSb;
+        return left < kSb ? left : kSb;
+    }
+};
+
+// (v >> shift & 0x000F000F) | 0x43004300 in one instruction behind the shift:
+// v_and_or_b32 takes one scalar register and no two literals.
+__device__ __forceinline__ uint32_t unpack2(uint32_t v, int shift, uint32_t mask_s, uint32_t magic_v)
+{
+    return ((v >> shift) & mask_s) | magic_v;
+}
+
+__device__ __forceinline__ float scale16(uint32_t bits16, bool half)
+{
+    return half ? (float)__builtin_bit_cast(_Float16, (uint16_t)bits16) : u2f(bits16 << 16);
+}
+
+// ---------------------------------------------------------------------------
+// laying the weights out, and back
+// ---------------------------------------------------------------------------
+
+// Row of a superblock at place i of its scales: lane row rho's 4 rows of the
+// first tile, then its 4 rows of the second.
+__device__ __forceinline__ int scale_row(int i) { return 16 * (i >> 2 & 1) + 4 * (i >> 3) + (i & 3); }
+
+__global__ __launch_bounds__(256) void w4_pack_kernel(const uint8_t* q, const uint16_t* scales, W4Shape w, uint32_t* packed,
+                                                      uint16_t* packed_scales)
+{
+    const int kts = w.kts(), gpt = w.gpt(), groups = (w.K + w.group - 1) / w.group;
+    // one block: the tiles of one superblock at one k range
+    const int64_t blk = blockIdx.x;
+    const int kt = (int)(blk % kts);
+    const int b = (int)(blk / kts % w.sbs());
+    const int e = (int)(blk / kts / w.sbs());
+    const int row0 = w.row0(b), rows = w.rows(b);
+    for (int i = (int)threadIdx.x; i < 2 * kTileBytes / 4; i += 256) {
+        const int tile = i >> 8, lane = i >> 2 & 63, s = i & 3;
+        const int r = 16 * tile + (lane & 15), k = kt * kKt + 32 * s + 8 * (lane >> 4);
+        uint32_t out = 0x88888888u;
+        if (r < rows && k < w.K) {     // (K a multiple of 8: all of the 8 or none)
+            const uint8_t* src = q + (((int64_t)e * w.N + row0 + r) * w.K + k) / 2;
+            out = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                out |= (uint32_t)(src[j] & 15) << (4 * j);
+                out |= (uint32_t)(src[j] >> 4) << (16 + 4 * j);
+            }
+        }
+        packed[blk * (2 * kTileBytes / 4) + i] = out;
+    }
+    for (int i = (int)threadIdx.x; i < gpt * kSb; i += 256) {
+        const int r = scale_row(i % kSb), g = kt * gpt + i / kSb;
+        packed_scales[blk * gpt * kSb + i] =
+            r < rows && g < groups ? scales[((int64_t)e * w.N + row0 + r) * groups + g] : (uint16_t)0;
+    }
+}
+
+// bf16 [E, N, K] of the experts with slots (all without offsets).
+__global__ __launch_bounds__(256) void w4_unpack_kernel(const uint32_t* packed, const uint16_t* packed_scales, bool half,
+                                                        W4Shape w, const int32_t* expert_offsets, int64_t cap,
+                                                        uint16_t* out)
+{
+    const int kts = w.kts(), gpt = w.gpt();
+    const int64_t blk = blockIdx.x;
+    const int kt = (int)(blk % kts);
+    const int b = (int)(blk / kts % w.sbs());
+    const int e = (int)(blk / kts / w.sbs());
+    if (expert_offsets && min<int64_t>(expert_offsets[e], cap) >= min<int64_t>(expert_offsets[e + 1], cap)) return;
+    const int row0 = w.row0(b), rows = w.rows(b);
+    for (int i = (int)threadIdx.x; i < 2 * kTileBytes / 4; i += 256) {
+        const int tile = i >> 8, lane = i >> 2 & 63, s = i & 3;
+        const int r = 16 * tile + (lane & 15), in = 32 * s + 8 * (lane >> 4), k = kt * kKt + in;
+        if (r >= rows || k >= w.K) continue;
+        const uint32_t v = packed[blk * (2 * kTileBytes / 4) + i];
+        const int at = 8 * ((r & 15) >> 2) + 4 * (r >> 4) + (r & 3);
+        const float sc = scale16(packed_scales[(blk * gpt + in / w.group) * kSb + at], half);
+        u32x4_t o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            o[j] = pack_bf16x2((float)((int)(v >> (4 * j) & 15) - 8) * sc, (float)((int)(v >> (16 + 4 * j) & 15) - 8) * sc);
+        *reinterpret_cast<u32x4_t*>(out + ((int64_t)e * w.N + row0 + r) * w.K + k) = o;
+    }
+}
+
+// Groups of G weights to 4 bits: scale = max(largest / 7, -smallest / 8), so that
+// both ends are reached, rounded to 16 bits; q = 8 + the nearest whole number
+// of scales, held to 0..15.  8 weights to a thread, G / 8 threads to a group.
+template <typename X, int G>
+__global__ __launch_bounds__(256) void w4_quantize_kernel(const X* w, int64_t rows, int K, bool half, uint32_t* q,
+                                                          uint16_t* scales)
+{
+    const int cols = (K + G - 1) / G * (G / 8);     // threads of a row, whole groups
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t row = i / cols;
+    const int k = (int)(i % cols) * 8;
+    const bool in = row < rows && k < K;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        v[j] = 0.0f;
+        if (in) {
+            if constexpr (sizeof(X) == 2) v[j] = u2f((uint32_t)w[row * K + k + j] << 16);
+            else v[j] = w[row * K + k + j];
+        }
+    }
+    float hi = 0.0f, lo = 0.0f;
+    bool nan = false;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        hi = __builtin_fmaxf(hi, v[j]);
+        lo = __builtin_fminf(lo, v[j]);
+        nan |= !(__builtin_fabsf(v[j]) < __builtin_inff());
+    }
+    float s = nan ? __builtin_inff() : __builtin_fmaxf(hi / 7.0f, lo / -8.0f);
+#pragma unroll
+    for (int off = G / 16; off >= 1; off >>= 1) s = __builtin_fmaxf(s, __shfl_xor(s, off, kWave));
+    const uint16_t bits = half ? __builtin_bit_cast(uint16_t, (_Float16)s) : (uint16_t)f32_to_bf16_bits(s);
+    const float sc = scale16(bits, half);
+    uint32_t out = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        // (a group whose scale is not finite, or 0, is all 8: its products are NaN, or 0)
+        const float t = sc > 0.0f && sc < __builtin_inff() ? __builtin_rintf(v[j] / sc) : 0.0f;
+        const int n = (int)__builtin_fminf(__builtin_fmaxf(t, -8.0f), 7.0f) + 8;
+        out |= (uint32_t)n << (4 * j);
+    }
+    if (in) {
+        q[(row * K + k) / 8] = out;
+        if (k % G == 0) scales[row * ((K + G - 1) / G) + k / G] = sc < __builtin_inff() ? bits : (uint16_t)(half ? 0x7E00 : 0x7FC0);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// the product
+// ---------------------------------------------------------------------------
+
+struct W4Args {
+    const uint16_t* a;              // gather: X [a_rows, K]; else [cap, K]
+    const int32_t* sorted_token;    // gather only
+    const unsigned char* packed;
+    const uint16_t* scales;
+    const int32_t* expert_offsets;  // null: one expert, all rows
+    uint16_t* c;                    // [cap, N], or [cap, N / 2] for SwiGLU
+    const float* row_scale;
+    int64_t a_rows, cap;
+    W4Shape w;
+};
+
+struct W4Tile {
+    int64_t s0;     // first slot
+    int rows;       // slots
+    int e;
+    int b;          // first superblock (SwiGLU: of the gate part)
+};
+
+// One block's tile: 16 MT slots x NSB superblocks (SwiGLU: one of the gate
+// part, its twin of the up part), the k range dealt to the block's waves one
+// 128 at a time, their sums joined through LDS in the waves' order.
+template <bool SWIGLU, int MT, int NSB, int GPT, bool HALF, int WAVES>
+__device__ __forceinline__ void w4_tile(const W4Args& g, const W4Tile& t, float* lds)
+{
+    constexpr int NT = 2 * NSB, SPG = 4 / GPT, U = 2;
+    const int lane = lane_id();
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+    const int r16 = lane & 15, rho = lane >> 4;
+    const int K = g.w.K, kts = g.w.kts(), twin = g.w.part_sbs();
+    const unsigned char* const wq = g.packed + t.e * g.w.expert_bytes();
+    const uint16_t* const ws = g.scales + t.e * g.w.expert_scales();
+    const unsigned char* wp[NSB];
+    const uint16_t* sp[NSB];
+#pragma unroll
+    for (int j = 0; j < NSB; ++j) {
+        const int b = min(t.b + (SWIGLU ? j * twin : j), g.w.sbs() - 1);
+        wp[j] = wq + (int64_t)b * kts * 2 * kTileBytes;
+        sp[j] = ws + (int64_t)b * kts * GPT * kSb;
+    }
+    const bool gather = g.sorted_token != nullptr;
+    const __amdgpu_buffer_rsrc_t ares =
+        gather ? __builtin_amdgcn_make_buffer_rsrc((void*)g.a, (short)0, (int)(g.a_rows * K * 2), kBufDword3)
+               : __builtin_amdgcn_make_buffer_rsrc((void*)(g.a + t.s0 * K), (short)0, t.rows * K * 2, kBufDword3);
+    uint32_t ao[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int r = 16 * i + r16;
+        ao[i] = kOOR;
+        if (r < t.rows) {
+            uint32_t at = (uint32_t)r;
+            if (gather) at = (uint32_t)g.sorted_token[t.s0 + r];
+            if (!gather || at < (uint32_t)g.a_rows) ao[i] = (at * (uint32_t)K + 8u * rho) * 2u;
+        }
+    }
+    struct Step {
+        u32x4_t w[NT], s[NSB][GPT], a[MT][4];
+    } ring[U];
+    const auto load = [&](Step& x, int kt) {
+#pragma unroll
+        for (int j = 0; j < NSB; ++j) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                x.w[2 * j + h] = *reinterpret_cast<const u32x4_t*>(wp[j] + (int64_t)kt * 2 * kTileBytes + h * kTileBytes +
+                                                                   16 * lane);
+#pragma unroll
+            for (int q = 0; q < GPT; ++q)
+                x.s[j][q] = *reinterpret_cast<const u32x4_t*>(sp[j] + (kt * GPT + q) * kSb + 8 * rho);
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const bool in = kt * kKt + 32 * s + 8 * rho < K;
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+                x.a[i][s] = __builtin_bit_cast(
+                    u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(ares, (int)(in ? ao[i] : kOOR), kt * kKt * 2 + 64 * s, 0));
+        }
+    };
+    f32x4_t acc[NT][MT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[j][i] = f32x4_t{};
+    const bf16x8_t offset = __builtin_bit_cast(bf16x8_t, u32x4_t{kOffset, kOffset, kOffset, kOffset});
+    uint32_t mask = 0x000F000Fu, magic = kMagic;
+    asm("" : "+s"(mask));
+    asm("" : "+v"(magic));
+    const auto mul = [&](const Step& x) {
+#pragma unroll
+        for (int q = 0; q < GPT; ++q) {
+            f32x4_t base[MT];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                base[i] = f32x4_t{};
+#pragma unroll
+                for (int s = 0; s < SPG; ++s)
+                    base[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        offset, __builtin_bit_cast(bf16x8_t, x.a[i][q * SPG + s]), base[i], 0, 0, 0);
+            }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                // (a tile at a time: the scheduler would else unpack them all first)
+                __builtin_amdgcn_sched_barrier(0);
+                f32x4_t p[MT];
+#pragma unroll
+                for (int i = 0; i < MT; ++i) p[i] = base[i];
+#pragma unroll
+                for (int s = 0; s < SPG; ++s) {
+                    const uint32_t v = x.w[j][q * SPG + s];
+                    u32x4_t f;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) f[k] = unpack2(v, 4 * k, mask, magic);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+                        p[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, f),
+                                                                       __builtin_bit_cast(bf16x8_t, x.a[i][q * SPG + s]),
+                                                                       p[i], 0, 0, 0);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const uint32_t pair = x.s[j / 2][q][2 * (j & 1) + r / 2];
+                    const float sc = scale16(r & 1 ? pair >> 16 : pair & 0xFFFFu, HALF);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) acc[j][i][r] = __builtin_fmaf(sc, p[i][r], acc[j][i][r]);
+                }
+            }
+        }
+    };
+    // (kts of this wave: wave, wave + WAVES, ...; loads past the last repeat it)
+    const int n = (kts - wave + WAVES - 1) / WAVES;
+    if (n > 0) {
+        const auto kt_of = [&](int i) { return wave + WAVES * min(i, n - 1); };
+#pragma unroll
+        for (int u = 0; u < U; ++u) load(ring[u], kt_of(u));
+        for (int i = 0; i < n; i += U) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (i + u < n) mul(ring[u]);
+                __builtin_amdgcn_sched_barrier(0);
+                load(ring[u], kt_of(i + u + U));
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    }
+    // the waves' sums, in order: wave w takes output units w, w + WAVES, ...
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+            *reinterpret_cast<f32x4_t*>(lds + ((wave * NT + j) * MT + i) * 4 * kWave + 4 * lane) = acc[j][i];
+    __syncthreads();
+    const auto total = [&](int j, int i) {
+        f32x4_t s = {};
+#pragma unroll
+        for (int v = 0; v < WAVES; ++v) s += *reinterpret_cast<const f32x4_t*>(lds + ((v * NT + j) * MT + i) * 4 * kWave + 4 * lane);
+        return s;
+    };
+    const int cols = SWIGLU ? g.w.part_rows() : g.w.N;
+    for (int unit = wave; unit < (SWIGLU ? 2 : NT) * MT; unit += WAVES) {
+        const int j = unit / MT, i = unit % MT;
+        const int b = t.b + j / 2, row = 16 * i + r16, in = 16 * (j & 1) + 4 * rho;
+        f32x4_t v = total(j, i);
+        if constexpr (SWIGLU) {
+            const f32x4_t up = total(j + 2, i);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = (v[k] * sigmoid(v[k])) * up[k];
+        }
+        if (b >= (SWIGLU ? twin : g.w.sbs()) || row >= t.rows || in >= g.w.rows(b)) continue;
+        if (g.row_scale) v *= g.row_scale[t.s0 + row];
+        *reinterpret_cast<u32x2_t*>(g.c + (t.s0 + row) * cols + g.w.row0(b) + in) =
+            u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    }
+    __syncthreads();
+}
+
+template <bool SWIGLU, int MT, int NSB, int GPT, bool HALF, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave, 2) void w4_gemm_kernel(W4Args g)
+{
+    __shared__ __attribute__((aligned(16))) float lds[WAVES * 2 * NSB * MT * 4 * kWave];
+    __shared__ int ptile[ET_MAX_EXPERTS + 1];     // prefix of the experts' slot tiles
+    __shared__ int32_t eoff[ET_MAX_EXPERTS + 1];  // expert_offsets below the capacity
+    constexpr int kRows = 16 * MT;
+    const int E = g.w.E, lane = lane_id();
+    if (threadIdx.x < kWave) {
+        int carry = 0;
+        for (int e0 = 0; e0 < E; e0 += kWave) {
+            const int e = e0 + lane;
+            int n = 0;
+            if (e < E) {
+                const int64_t lo = g.expert_offsets ? min<int64_t>(g.expert_offsets[e], g.cap) : 0;
+                const int64_t hi = g.expert_offsets ? min<int64_t>(g.expert_offsets[e + 1], g.cap) : g.cap;
+                eoff[e] = (int32_t)lo;
+                eoff[e + 1] = (int32_t)hi;   // (the next expert's lo)
+                n = (int)((max<int64_t>(0, hi - lo) + kRows - 1) / kRows);
+            }
+            const int inc = wave_incl_scan(n) + carry;
+            if (e < E) ptile[e + 1] = inc;
+            carry = __shfl(inc, kWave - 1, kWave);
+        }
+        if (lane == 0) ptile[0] = 0;
+    }
+    __syncthreads();
+    // units of superblocks: pairs of twins for SwiGLU, NSB side by side else
+    const int nb = SWIGLU ? g.w.part_sbs() : (g.w.sbs() + NSB - 1) / NSB;
+    const int64_t Q = (int64_t)__builtin_amdgcn_readfirstlane(ptile[E]) * nb;
+    const int64_t per = (Q + 7) / 8;
+    const int nloc = (int)(gridDim.x >> 3);
+    for (int64_t l = blockIdx.x >> 3; l < per; l += nloc) {
+        // XCD x (blocks b % 8 = x) takes a contiguous range; an expert's slot tiles are innermost
+        const int64_t q = (int64_t)(blockIdx.x & 7) * per + l;
+        if (q >= Q) break;
+        int lo = 0, hi = E;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (ptile[mid] <= q / nb) lo = mid;
+            else hi = mid;
+        }
+        W4Tile t;
+        t.e = __builtin_amdgcn_readfirstlane(lo);
+        const int p0 = __builtin_amdgcn_readfirstlane(ptile[t.e]);
+        const int mte = __builtin_amdgcn_readfirstlane(ptile[t.e + 1]) - p0;
+        const int qq = (int)(q - (int64_t)p0 * nb);
+        const int first = __builtin_amdgcn_readfirstlane(eoff[t.e]);
+        const int end = __builtin_amdgcn_readfirstlane(eoff[t.e + 1]);
+        t.s0 = first + (int64_t)(qq % mte) * kRows;
+        t.rows = min(kRows, end - (int)t.s0);
+        t.b = qq / mte * (SWIGLU ? 1 : NSB);
+        w4_tile<SWIGLU, MT, NSB, GPT, HALF, WAVES>(g, t, lds);
+    }
+}
+
+template <bool SWIGLU, int MT, bool HALF>
+int launch_w4(const W4Args& g, int cus, hipStream_t s)
+{
+    constexpr int WAVES = 4, NSB = 2;
+    const int64_t nb = SWIGLU ? g.w.part_sbs() : (g.w.sbs() + NSB - 1) / NSB;
+    const int64_t tiles = std::min<int64_t>(g.cap, g.cap / (16 * MT) + g.w.E);
+    const int64_t blocks = std::min<int64_t>(tiles * nb, (int64_t)cus * 4);
+    const dim3 grid((unsigned)(8 * ((blocks + 7) / 8))), block(WAVES * kWave);
+    switch (g.w.gpt()) {
+        case 1: w4_gemm_kernel<SWIGLU, MT, NSB, 1, HALF, WAVES><<<grid, block, 0, s>>>(g); break;
+        case 2: w4_gemm_kernel<SWIGLU, MT, NSB, 2, HALF, WAVES><<<grid, block, 0, s>>>(g); break;
+        default: w4_gemm_kernel<SWIGLU, MT, NSB, 4, HALF, WAVES><<<grid, block, 0, s>>>(g); break;
+    }
+    return check_launch("w4_gemm_kernel");
+}
+
+template <int MT>
+int launch_w4(bool swiglu, bool half, const W4Args& g, int cus, hipStream_t s)
+{
+    if (swiglu) return half ? launch_w4<true, MT, true>(g, cus, s) : launch_w4<true, MT, false>(g, cus, s);
+    return half ? launch_w4<false, MT, true>(g, cus, s) : launch_w4<false, MT, false>(g, cus, s);
+}
+
+int check_shape(const char* fn, int64_t E, int64_t N, int64_t K, int64_t group, int64_t parts)
+{
+    const std::string f(fn);
+    if (E < 1 || E > ET_MAX_EXPERTS) return fail(ET_ERR_INVALID_ARGUMENT, f + ": num_experts must be in [1, 1024]");
+    if (parts != 1 && parts != 2) return fail(ET_ERR_INVALID_ARGUMENT, f + ": parts must be 1 or 2");
+    if (N < 8 * parts || N % (8 * parts)) return fail(ET_ERR_INVALID_ARGUMENT, f + ": N must be a positive multiple of 8 for each part");
+    if (K < 8 || K % 8 || K >= (int64_t)1 << 22) return fail(ET_ERR_INVALID_ARGUMENT, f + ": K must be a positive multiple of 8 below 2^22");
+    if (group != 32 && group != 64 && group != 128) return fail(ET_ERR_INVALID_ARGUMENT, f + ": group must be 32, 64 or 128");
+    if (N >= (int64_t)1 << 24 || N * K >= (int64_t)1 << 31) return fail(ET_ERR_INVALID_ARGUMENT, f + ": N * K must be below 2^31, N below 2^24");
+    return ET_OK;
+}
+
+W4Shape shape_of(int64_t E, int64_t N, int64_t K, int64_t group, int64_t parts)
+{
+    return W4Shape{(int)E, (int)N, (int)K, (int)parts, (int)group};
+}
+
+int blocks_of(const char* fn, const W4Shape& w, unsigned& blocks)
+{
+    const int64_t n = (int64_t)w.E * w.sbs() * w.kts();
+    if (n >= (int64_t)1 << 31) return fail(ET_ERR_INVALID_ARGUMENT, std::string(fn) + ": the weight is too large");
+    blocks = (unsigned)n;
+    return ET_OK;
+}
+
+int check_ptr(const char* fn, const char* name, const void* p, uintptr_t align)
+{
+    if (!p) return fail(ET_ERR_INVALID_ARGUMENT, std::string(fn) + ": null " + name);
+    if ((uintptr_t)p % align) return fail(ET_ERR_INVALID_ARGUMENT, std::string(fn) + ": " + name + " is not aligned");
+    return ET_OK;
+}
+
+int check_scale_type(const char* fn, int t)
+{
+    if (t != ET_W4_SCALE_BF16 && t != ET_W4_SCALE_F16)
+        return fail(ET_ERR_INVALID_ARGUMENT, std::string(fn) + ": scale_type must be ET_W4_SCALE_BF16 or ET_W4_SCALE_F16");
+    return ET_OK;
+}
+
+}  // namespace
+}  // namespace et
+
+using namespace et;
+
+extern "C" size_t et_w4_packed_bytes(int64_t num_experts, int64_t N, int64_t K, int64_t parts)
+{
+    if (check_shape("et_w4_packed_bytes", num_experts, N, K, 128, parts)) return 0;
+    return (size_t)num_experts * shape_of(num_experts, N, K, 128, parts).expert_bytes();
+}
+
+extern "C" size_t et_w4_packed_scales(int64_t num_experts, int64_t N, int64_t K, int64_t group, int64_t parts)
+{
+    if (check_shape("et_w4_packed_scales", num_experts, N, K, group, parts)) return 0;
+    return (size_t)num_experts * shape_of(num_experts, N, K, group, parts).expert_scales();
+}
+
+extern "C" int et_w4_pack(const void* q, const void* scales, int64_t num_experts, int64_t N, int64_t K, int64_t group,
+                          int64_t parts, void* packed, void* packed_scales, void* stream)
+{
+    const char* fn = "et_w4_pack";
+    unsigned blocks = 0;
+    int rc = check_shape(fn, num_experts, N, K, group, parts);
+    if (rc) return rc;
+    const W4Shape w = shape_of(num_experts, N, K, group, parts);
+    rc = blocks_of(fn, w, blocks);
+    if (!rc) rc = check_ptr(fn, "q", q, 1);
+    if (!rc) rc = check_ptr(fn, "scales", scales, 2);
+    if (!rc) rc = check_ptr(fn, "packed", packed, 16);
+    if (!rc) rc = check_ptr(fn, "packed_scales", packed_scales, 16);
+    if (rc) return rc;
+    w4_pack_kernel<<<dim3(blocks), dim3(256), 0, (hipStream_t)stream>>>((const uint8_t*)q, (const uint16_t*)scales, w,
+                                                                       (uint32_t*)packed, (uint16_t*)packed_scales);
+    return check_launch("w4_pack_kernel");
+}
+
+extern "C" int et_w4_unpack(const void* packed, const void* packed_scales, int scale_type, const int32_t* expert_offsets,
+                            int64_t num_experts, int64_t N, int64_t K, int64_t group, int64_t parts,
+                            int64_t slot_capacity, void* w, void* stream)
+{
+    const char* fn = "et_w4_unpack";
+    unsigned blocks = 0;
+    int rc = check_shape(fn, num_experts, N, K, group, parts);
+    if (!rc) rc = check_scale_type(fn, scale_type);
+    if (rc) return rc;
+    const W4Shape sh = shape_of(num_experts, N, K, group, parts);
+    rc = blocks_of(fn, sh, blocks);
+    if (!rc) rc = check_ptr(fn, "packed", packed, 16);
+    if (!rc) rc = check_ptr(fn, "packed_scales", packed_scales, 16);
+    if (!rc) rc = check_ptr(fn, "w", w, 16);
+    if (rc) return rc;
+    if (slot_capacity < 0) return fail(ET_ERR_INVALID_ARGUMENT, "et_w4_unpack: slot_capacity must be >= 0");
+    w4_unpack_kernel<<<dim3(blocks), dim3(256), 0, (hipStream_t)stream>>>(
+        (const uint32_t*)packed, (const uint16_t*)packed_scales, scale_type == ET_W4_SCALE_F16, sh, expert_offsets,
+        slot_capacity, (uint16_t*)w);
+    return check_launch("w4_unpack_kernel");
+}
+
+namespace et {
+namespace {
+
+template <typename X>
+void launch_quantize(const void* w, int64_t rows, int64_t K, int64_t group, bool half, void* q, void* scales, hipStream_t s)
+{
+    const int64_t threads = rows * ((K + group - 1) / group * (group / 8));
+    const dim3 grid((unsigned)((threads + 255) / 256)), block(256);
+    switch (group) {
+        case 32: w4_quantize_kernel<X, 32><<<grid, block, 0, s>>>((const X*)w, rows, (int)K, half, (uint32_t*)q, (uint16_t*)scales); break;
+        case 64: w4_quantize_kernel<X, 64><<<grid, block, 0, s>>>((const X*)w, rows, (int)K, half, (uint32_t*)q, (uint16_t*)scales); break;
+        default: w4_quantize_kernel<X, 128><<<grid, block, 0, s>>>((const X*)w, rows, (int)K, half, (uint32_t*)q, (uint16_t*)scales); break;
+    }
+}
+
+int cus_of_device()
+{
+    static thread_local int cus[64] = {};
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+    if (!cus[dev] && (hipDeviceGetAttribute(&cus[dev], hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus[dev] < 1))
+        cus[dev] = 256;
+    return cus[dev];
+}
+
+}  // namespace
+}  // namespace et
+
+extern "C" int et_w4_quantize(const void* w, int dtype, int64_t num_experts, int64_t N, int64_t K, int64_t group,
+                              int scale_type, void* q, void* scales, void* stream)
+{
+    const char* fn = "et_w4_quantize";
+    int rc = check_shape(fn, num_experts, N, K, group, 1);
+    if (!rc) rc = check_scale_type(fn, scale_type);
+    if (rc) return rc;
+    if (dtype != ET_DTYPE_F32 && dtype != ET_DTYPE_BF16)
+        return fail(ET_ERR_INVALID_ARGUMENT, "et_w4_quantize: dtype must be ET_DTYPE_F32 or ET_DTYPE_BF16");
+    if (num_experts * N * (K / 8 + group) >= (int64_t)1 << 39)
+        return fail(ET_ERR_INVALID_ARGUMENT, "et_w4_quantize: the weight is too large");
+    rc = check_ptr(fn, "w", w, dtype == ET_DTYPE_F32 ? 4 : 2);
+    if (!rc) rc = check_ptr(fn, "q", q, 4);
+    if (!rc) rc = check_ptr(fn, "scales", scales, 2);
+    if (rc) return rc;
+    const bool half = scale_type == ET_W4_SCALE_F16;
+    if (dtype == ET_DTYPE_F32) launch_quantize<float>(w, num_experts * N, K, group, half, q, scales, (hipStream_t)stream);
+    else launch_quantize<uint16_t>(w, num_experts * N, K, group, half, q, scales, (hipStream_t)stream);
+    return check_launch("w4_quantize_kernel");
+}
+
+// max_slots: slots of one expert at most, as far as the host knows.
+extern "C" int et_expert_gemm_w4_impl(const void* a, int64_t a_rows, const int32_t* sorted_token, const void* packed,
+                                      const void* packed_scales, int scale_type, const int32_t* expert_offsets,
+                                      int64_t num_experts, int64_t K, int64_t N, int64_t group, int64_t parts,
+                                      int64_t slot_capacity, int epilogue, const float* row_scale, void* c,
+                                      int64_t max_slots, void* stream)
+{
+    const char* fn = "et_expert_gemm_w4";
+    int rc = check_shape(fn, num_experts, N, K, group, parts);
+    if (!rc) rc = check_scale_type(fn, scale_type);
+    if (rc) return rc;
+    if (epilogue != EPI_PLAIN && epilogue != EPI_ROW_SCALE && epilogue != EPI_SWIGLU)
+        return fail(ET_ERR_INVALID_ARGUMENT, "et_expert_gemm_w4: unknown epilogue");
+    if (epilogue == EPI_SWIGLU && parts != 2)
+        return fail(ET_ERR_INVALID_ARGUMENT, "et_expert_gemm_w4: SwiGLU needs a weight laid out in two parts");
+    if (slot_capacity < 0 || slot_capacity >= (int64_t)1 << 31 || a_rows < 0)
+        return fail(ET_ERR_INVALID_ARGUMENT, "et_expert_gemm_w4: slot_capacity must be in [0, 2^31), a_rows >= 0");
+    if (sorted_token && a_rows * K * 2 >= (int64_t)1 << 31)
+        return fail(ET_ERR_INVALID_ARGUMENT, "et_expert_gemm_w4: in gather mode the token matrix must be below 2 GiB");
+    if (!expert_offsets && num_experts != 1)
+        return fail(ET_ERR_INVALID_ARGUMENT, "et_expert_gemm_w4: more than one expert needs expert_offsets");
+    if (!expert_offsets && sorted_token)
+        return fail(ET_ERR_INVALID_ARGUMENT, "et_expert_gemm_w4: gather mode needs expert_offsets");
+    if (slot_capacity == 0) return ET_OK;
+    rc = check_ptr(fn, "a", a, 16);
+    if (!rc) rc = check_ptr(fn, "packed", packed, 16);
+    if (!rc) rc = check_ptr(fn, "packed_scales", packed_scales, 16);
+    if (!rc) rc = check_ptr(fn, "c", c, 16);
+    if (!rc && epilogue == EPI_ROW_SCALE) rc = check_ptr(fn, "row_scale", row_scale, 4);
+    if (rc) return rc;
+    W4Args g{(const uint16_t*)a, sorted_token, (const unsigned char*)packed, (const uint16_t*)packed_scales, expert_offsets,
+             (uint16_t*)c, epilogue == EPI_ROW_SCALE ? row_scale : nullptr, a_rows, slot_capacity,
+             shape_of(num_experts, N, K, group, parts)};
+    const bool swiglu = epilogue == EPI_SWIGLU, half = scale_type == ET_W4_SCALE_F16;
+    const int cus = cus_of_device();
+    const int64_t most = std::min(max_slots, slot_capacity);
+    if (most <= 16) return launch_w4<1>(swiglu, half, g, cus, (hipStream_t)stream);
+    return launch_w4<2>(swiglu, half, g, cus, (hipStream_t)stream);
+}
+
+extern "C" int et_expert_gemm_w4(const void* a, int64_t a_rows, const int32_t* sorted_token, const void* packed,
+                                 const void* packed_scales, int scale_type, const int32_t* expert_offsets,
+                                 int64_t num_experts, int64_t K, int64_t N, int64_t group, int64_t parts,
+                                 int64_t slot_capacity, int epilogue, const float* row_scale, void* c, void* stream)
+{
+    return et_expert_gemm_w4_impl(a, a_rows, sorted_token, packed, packed_scales, scale_type, expert_offsets, num_experts, K,
+                                  N, group, parts, slot_capacity, epilogue, row_scale, c, slot_capacity, stream);
+}

@@ -108,3 +108,35 @@ def test_layer_norm_rejects_bad_arguments(et):
     assert bwd(dw=None) == ET_ERR_INVALID_ARGUMENT and "dweight" in _err(et)
     assert bwd(wsb=4) == ET_ERR_WORKSPACE_TOO_SMALL and "workspace" in _err(et)
     assert bwd(ws=ctypes.c_void_p(0x1002)) == ET_ERR_INVALID_ARGUMENT
+
+
+def test_w4_rejects_bad_arguments(et):
+    lib = et.lib()
+    p = ctypes.c_void_p(0x1000)
+    assert lib.et_w4_packed_bytes(3, 40, 136, 1) == 3 * 2 * 2 * 2048
+    assert lib.et_w4_packed_bytes(1, 48, 128, 2) == 2 * 2048          # 24 rows of each part to 32
+    assert lib.et_w4_packed_scales(1, 32, 136, 64, 1) == 2 * 2 * 32
+    assert lib.et_w4_packed_bytes(0, 32, 128, 1) == 0 and lib.et_w4_packed_scales(1, 32, 128, 48, 1) == 0
+    assert lib.et_w4_pack(p, p, 1, 12, 128, 128, 1, p, p, None) == ET_ERR_INVALID_ARGUMENT and "N must" in _err(et)
+    assert lib.et_w4_pack(p, p, 1, 16, 12, 128, 1, p, p, None) == ET_ERR_INVALID_ARGUMENT and "K must" in _err(et)
+    assert lib.et_w4_pack(p, p, 1, 16, 128, 16, 1, p, p, None) == ET_ERR_INVALID_ARGUMENT and "group" in _err(et)
+    assert lib.et_w4_pack(p, p, 1, 16, 128, 128, 0, p, p, None) == ET_ERR_INVALID_ARGUMENT and "parts" in _err(et)
+    assert lib.et_w4_pack(p, p, 1, 16, 128, 128, 1, ctypes.c_void_p(0x1008), p, None) == ET_ERR_INVALID_ARGUMENT
+    assert lib.et_w4_quantize(p, 3, 1, 16, 128, 128, 0, p, p, None) == ET_ERR_INVALID_ARGUMENT and "dtype" in _err(et)
+    assert lib.et_w4_quantize(p, 0, 1, 16, 128, 128, 2, p, p, None) == ET_ERR_INVALID_ARGUMENT and "scale_type" in _err(et)
+    assert lib.et_w4_unpack(p, p, 0, None, 1, 16, 128, 128, 1, -1, p, None) == ET_ERR_INVALID_ARGUMENT
+
+    def gemm(a=p, rows=4, tok=None, st=0, eo=p, E=2, K=128, N=32, group=128, parts=1, cap=4, epi=0, rs=None, c=p):
+        return lib.et_expert_gemm_w4(a, rows, tok, p, p, st, eo, E, K, N, group, parts, cap, epi, rs, c, None)
+
+    assert gemm(E=0) == ET_ERR_INVALID_ARGUMENT and "num_experts" in _err(et)
+    assert gemm(st=5) == ET_ERR_INVALID_ARGUMENT
+    assert gemm(epi=3) == ET_ERR_INVALID_ARGUMENT and "epilogue" in _err(et)
+    assert gemm(epi=2) == ET_ERR_INVALID_ARGUMENT and "parts" in _err(et)
+    assert gemm(epi=1) == ET_ERR_INVALID_ARGUMENT and "row_scale" in _err(et)
+    assert gemm(eo=None) == ET_ERR_INVALID_ARGUMENT and "expert_offsets" in _err(et)
+    assert gemm(eo=None, E=1, tok=p) == ET_ERR_INVALID_ARGUMENT and "gather" in _err(et)
+    assert gemm(tok=p, rows=1 << 23) == ET_ERR_INVALID_ARGUMENT and "2 GiB" in _err(et)
+    assert gemm(cap=-1) == ET_ERR_INVALID_ARGUMENT
+    assert gemm(a=ctypes.c_void_p(0x1008)) == ET_ERR_INVALID_ARGUMENT and "aligned" in _err(et)
+    assert gemm(cap=0) == 0

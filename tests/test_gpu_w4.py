@@ -1,0 +1,316 @@
+"""Products with 4-bit weights against a plain implementation in 64 bits, with
+bounds derived from the formula's roundings; the layout and the quantiser
+against the written definition."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+BF = 2.0 ** -8
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+def _weight(g, E, N, K, group, sdt):
+    q = torch.randint(0, 256, (E, N, K // 2), generator=g, dtype=torch.uint8)
+    s = (torch.exp(torch.randn(E, N, -(-K // group), generator=g) * 0.5) * 0.02).to(sdt)
+    return q, s
+
+
+def _values(q, s, group, K):
+    """float64 (q - 8) * scale [E, N, K]."""
+    v = torch.stack([q & 15, q >> 4], -1).reshape(*q.shape[:-1], K).double() - 8
+    return v * s.double().repeat_interleave(group, -1)[..., :K]
+
+
+def _product64(a, w):
+    """(a @ w^T, bound of what 32-bit sums add).  A group's partial sums reach
+    (136 + 15 + 128) |a| at most: K additions in MFMAs (a few ULPs of the largest partial sum
+    each), one product and one addition for each of the groups."""
+    a, w = a.double(), w.double()
+    p = a @ w.t()
+    K = a.shape[1]
+    size = a.abs() @ torch.ones(K, 1, dtype=torch.float64) * 280 * w.abs().amax(1)
+    chain = 40 + K / 32
+    return p, size * U * chain / 8 + (a.abs() @ w.abs().t()) * U * chain
+
+
+def _swiglu(p, e):
+    F = p.shape[1] // 2
+    g, u = p[:, :F], p[:, F:]
+    eg, eu = e[:, :F], e[:, F:]
+    s = torch.sigmoid(g)
+    h = g * s * u
+    # |d silu| <= 1.1, 8 roundings
+    return h, 1.1 * eg * (u.abs() + eu) + (g * s).abs() * eu + 8 * U * h.abs()
+
+
+def _close(got, want, err):
+    got = got.cpu().double()
+    return torch.all((got - want).abs() <= err + BF * (want.abs() + err))
+
+
+# N and K of every kind: one vector, below a tile, odd tiles, whole ones, several chunks of a wave
+SHAPES = [(8, 8), (24, 40), (32, 128), (40, 136), (72, 512), (264, 520), (520, 1032), (96, 2104)]
+
+
+@pytest.mark.parametrize("N,K", SHAPES)
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("sdt", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("T", [1, 3, 16, 17, 50, 130])
+def test_linear_against_64_bits(et, dev, N, K, group, sdt, T):
+    g = torch.Generator().manual_seed(N * K + T)
+    q, s = _weight(g, 1, N, K, group, sdt)
+    x = torch.randn(T, K, generator=g).to(BF16)
+    w = et.pack_w4(q[0].to(dev), s[0].to(dev), group=group)
+    want, err = _product64(x, _values(q, s, group, K)[0])
+    got = et.linear_w4(x.to(dev), w)
+    assert _close(got, want, err)
+    assert torch.equal(got, et.linear_w4(x.to(dev), w))
+    scale = torch.randn(T, generator=g)
+    got = et.linear_w4(x.to(dev), w, epilogue="row_scale", row_scale=scale.to(dev))
+    assert _close(got, want * scale.double()[:, None], (err + U * want.abs()) * scale.double().abs()[:, None])
+    if N % 16 == 0:
+        w = et.pack_w4(q[0].to(dev), s[0].to(dev), group=group, parts=2)
+        assert _close(et.linear_w4(x.to(dev), w, epilogue="swiglu"), *_swiglu(want, err))
+        assert _close(et.linear_w4(x.to(dev), w), want, err)
+
+
+def _plan(et, dev, chosen, capacity=None, known=False):
+    """A plan of a [T, E] mask on the device, its arrays those of routing."""
+    T, E = chosen.shape
+    expert, token = chosen.t().nonzero(as_tuple=True)
+    counts = chosen.sum(0)
+    offsets = torch.cat([counts.new_zeros(1), counts.cumsum(0)])
+    S = len(token)
+    cap = S if capacity is None else capacity
+    by_token = torch.argsort(token * E + expert)
+    to = torch.searchsorted(token[by_token].contiguous(), torch.arange(T + 1))
+    pad = lambda t: torch.nn.functional.pad(t, (0, max(0, cap - S)), value=-7)[:cap].to(dev)  # noqa: E731
+    i32 = torch.int32
+    plan = et.RoutingPlan(counts.to(dev, i32), offsets.to(dev, i32), to.to(dev, i32), pad(token.to(i32)),
+                          pad(torch.rand(S)), pad(by_token.to(i32)), T, E, cap, S if known else None)
+    return plan, expert, token
+
+
+MASKS = {
+    "one_token": lambda g, T, E: torch.randperm(E, generator=g)[None].argsort(1) < 3,
+    "few": lambda g, T, E: torch.rand(T, E, generator=g) < 0.3,
+    "skewed": lambda g, T, E: torch.rand(T, E, generator=g) < torch.linspace(1, 0, E) ** 4,
+    "one_expert": lambda g, T, E: (torch.arange(E) == E // 2).expand(T, E),
+    "none": lambda g, T, E: torch.zeros(T, E, dtype=torch.bool),
+    "last_only": lambda g, T, E: (torch.arange(E) == E - 1).expand(T, E),
+}
+
+
+@pytest.mark.parametrize("mask", MASKS)
+@pytest.mark.parametrize("T,E", [(1, 7), (9, 70), (45, 5), (150, 3)])
+@pytest.mark.parametrize("N,K,group", [(48, 200, 64), (96, 264, 32), (160, 1032, 128)])
+def test_experts_against_64_bits(et, dev, mask, T, E, N, K, group):
+    g = torch.Generator().manual_seed(T * E + K)
+    q, s = _weight(g, E, N, K, group, BF16)
+    vals = _values(q, s, group, K)
+    chosen = MASKS[mask](g, T if mask != "one_token" else 1, E)
+    T = len(chosen)
+    plan, expert, token = _plan(et, dev, chosen)
+    x = torch.randn(T, K, generator=g).to(BF16)
+    rows = x[token]
+    want, err = torch.zeros(len(token), N, dtype=torch.float64), torch.zeros(len(token), N, dtype=torch.float64)
+    for e in range(E):
+        at = expert == e
+        want[at], err[at] = _product64(rows[at], vals[e])
+    w1, w2 = (et.pack_w4(q.to(dev), s.to(dev), group=group, parts=p) for p in (1, 2))
+    xd, rd = x.to(dev), rows.to(dev)
+    assert _close(et.expert_gemm_w4(xd, w1, plan), want, err)
+    gate = plan.slot_gate.cpu().double()[:, None]
+    assert _close(et.expert_gemm_w4(rd, w1, plan, gather=False, epilogue="row_scale", row_scale=plan.slot_gate),
+                  want * gate, (err + U * want.abs()) * gate)
+    a = et.expert_gemm_w4(xd, w2, plan, epilogue="swiglu")
+    assert _close(a, *_swiglu(want, err))
+    assert torch.equal(a, et.expert_gemm_w4(rd, w2, plan, gather=False, epilogue="swiglu"))
+
+
+@pytest.mark.parametrize("known", [False, True])
+def test_capacity_smaller_and_larger_than_the_slots(et, dev, known):
+    g = torch.Generator().manual_seed(4)
+    T, E, N, K = 30, 6, 64, 256
+    q, s = _weight(g, E, N, K, 128, BF16)
+    w = et.pack_w4(q.to(dev), s.to(dev))
+    chosen = torch.rand(T, E, generator=g) < 0.5
+    x = torch.randn(T, K, generator=g).to(BF16).to(dev)
+    plan, _, token = _plan(et, dev, chosen)
+    full = et.expert_gemm_w4(x, w, plan)
+    S = len(token)
+    for cap in (T * E, S + 1, S - 1, S - 40, 1):
+        small, _, _ = _plan(et, dev, chosen, capacity=cap)
+        out = torch.full((cap, N), 3.0, dtype=BF16, device=dev)
+        et.expert_gemm_w4(x, w, small, out=out)
+        n = min(cap, S)
+        assert torch.equal(out[:n], full[:n]) and torch.all(out[n:] == 3.0)
+
+
+def test_invalid_tokens_read_nothing(et, dev):
+    """Token ids out of range take part as rows of zeros."""
+    g = torch.Generator().manual_seed(8)
+    q, s = _weight(g, 2, 32, 128, 128, BF16)
+    w = et.pack_w4(q.to(dev), s.to(dev))
+    plan, _, token = _plan(et, dev, torch.ones(4, 2, dtype=torch.bool))
+    plan.sorted_token[1] = 1 << 20
+    plan.sorted_token[6] = -1
+    out = et.expert_gemm_w4(torch.randn(4, 128, generator=g).to(BF16).to(dev), w, plan)
+    assert torch.all(out[1] == 0) and torch.all(out[6] == 0) and torch.isfinite(out).all()
+
+
+def test_non_finite_rows_stay_alone(et, dev):
+    g = torch.Generator().manual_seed(9)
+    q, s = _weight(g, 1, 64, 512, 64, BF16)
+    w = et.pack_w4(q[0].to(dev), s[0].to(dev), group=64)
+    x = torch.randn(20, 512, generator=g).to(BF16).to(dev)
+    clean = et.linear_w4(x, w)
+    for bad in (float("nan"), float("inf")):
+        z = x.clone()
+        z[5, 100] = bad
+        out = et.linear_w4(z, w)
+        keep = torch.arange(20, device=dev) != 5
+        assert torch.equal(out[keep], clean[keep]) and torch.isnan(out[5]).all()
+    # a scale that is not a number spoils its row of the weight alone
+    s2 = s.clone()
+    s2[0, 7, 3] = float("nan")
+    out = et.linear_w4(x, et.pack_w4(q[0].to(dev), s2[0].to(dev), group=64))
+    cols = torch.arange(64, device=dev) != 7
+    assert torch.isnan(out[:, 7]).all() and torch.equal(out[:, cols], clean[:, cols])
+
+
+@pytest.mark.parametrize("parts", [1, 2])
+@pytest.mark.parametrize("N,K,group", [(16, 8, 32), (48, 264, 64), (208, 1032, 128), (32, 40, 32)])
+@pytest.mark.parametrize("sdt", [BF16, F16], ids=["bf16", "f16"])
+def test_unpack_gives_the_weight_back(et, dev, parts, N, K, group, sdt):
+    g = torch.Generator().manual_seed(N + K)
+    q, s = _weight(g, 3, N, K, group, sdt)
+    w = et.pack_w4(q.to(dev), s.to(dev), group=group, parts=parts)
+    # (the product of 4 and 11 bits is exact in binary32)
+    want = _values(q, s, group, K).float().to(BF16)
+    assert torch.equal(et.unpack_w4(w).cpu(), want)
+    chosen = torch.zeros(2, 3, dtype=torch.bool)
+    chosen[1, 1] = True
+    plan, _, _ = _plan(et, dev, chosen)
+    out = torch.full((3, N, K), 2.0, dtype=BF16, device=dev)
+    et.unpack_w4(w, plan, out=out)
+    assert torch.equal(out[1].cpu(), want[1]) and torch.all(out[0] == 2.0) and torch.all(out[2] == 2.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("sdt", [BF16, F16], ids=["sbf16", "sf16"])
+@pytest.mark.parametrize("E,N,K,group", [(1, 8, 8, 32), (2, 40, 264, 64), (3, 16, 1000, 128), (1, 24, 4096, 32)])
+def test_quantize_is_the_definition(et, dev, dtype, sdt, E, N, K, group):
+    g = torch.Generator().manual_seed(K)
+    w = (torch.randn(E, N, K, generator=g) * torch.exp(torch.randn(E, N, 1, generator=g))).to(dtype)
+    w[0, 0] = 0.0
+    w[0, 1, :] = -w[0, 1, :].abs()
+    q, s = et.quantize_w4(w.to(dev), group=group, scale_dtype=sdt)
+    pad = torch.nn.functional.pad(w.float(), (0, -K % group)).view(E, N, -1, group)
+    hi, lo = pad.amax(-1).clamp(min=0), pad.amin(-1).clamp(max=0)
+    scale = torch.maximum(hi / torch.tensor(7.0), lo / torch.tensor(-8.0)).to(sdt)
+    assert torch.equal(s.cpu(), scale)
+    sf = scale.float()[..., None]
+    n = torch.where(sf > 0, torch.round(pad / sf), 0.0).clamp(-8, 7) + 8
+    n = n.view(E, N, -1)[..., :K].to(torch.uint8)
+    assert torch.equal(q.cpu(), n[..., 0::2] | n[..., 1::2] << 4)
+    # every value within half a scale (and what rounding the scale to 16 bits holds back at the ends)
+    back = _values(q.cpu(), s.cpu(), group, K)
+    slack = 8 * (BF if sdt == BF16 else 2.0 ** -11)
+    each = scale.double().repeat_interleave(group, -1)[..., :K]
+    assert torch.all((back - w.double()).abs() <= (0.5 + slack) * each + 1e-7)
+
+
+def test_quantize_marks_groups_that_are_not_finite(et, dev):
+    w = torch.randn(8, 256, device=dev)
+    w[2, 200] = float("inf")
+    w[3, 10] = float("nan")
+    q, s = et.quantize_w4(w)
+    assert torch.isnan(s).tolist() == [[False, False]] * 2 + [[False, True], [True, False]] + [[False, False]] * 4
+    assert torch.all(q[2, 64:] == 0x88) and torch.all(q[3, :64] == 0x88)
+
+
+def test_dense_slices_and_strides_are_refused_or_right(et, dev):
+    g = torch.Generator().manual_seed(1)
+    q, s = _weight(g, 1, 32, 128, 128, BF16)
+    w = et.pack_w4(q[0].to(dev), s[0].to(dev))
+    x = torch.randn(8, 256, generator=g).to(BF16).to(dev)
+    with pytest.raises(ValueError, match="contiguous"):
+        et.linear_w4(x[:, :128], w)
+    y = x[:, :128].contiguous()
+    assert torch.equal(et.linear_w4(y[2:5], w), et.linear_w4(y, w)[2:5])
+    assert et.linear_w4(y[:0], w).shape == (0, 32)
+
+
+def test_side_stream_and_graph_replays(et, dev):
+    g = torch.Generator().manual_seed(2)
+    E, N, K = 8, 128, 512
+    q, s = _weight(g, E, N, K, 128, BF16)
+    w = et.pack_w4(q.to(dev), s.to(dev), parts=2)
+    chosen = torch.rand(12, E, generator=g) < 0.4
+    plan, _, _ = _plan(et, dev, chosen)
+    x = torch.randn(12, K, generator=g).to(BF16).to(dev)
+    want = et.expert_gemm_w4(x, w, plan, epilogue="swiglu")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = et.expert_gemm_w4(x, w, plan, epilogue="swiglu")
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = et.expert_gemm_w4(x, w, plan, epilogue="swiglu")
+    for _ in range(4):
+        x.mul_(0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, et.expert_gemm_w4(x, w, plan, epilogue="swiglu"))
+        torch.cuda.synchronize()
+
+
+def test_refusals(et, dev):
+    q = torch.zeros(2, 32, 64, dtype=torch.uint8, device=dev)
+    s = torch.ones(2, 32, 1, dtype=BF16, device=dev)
+    w = et.pack_w4(q, s)
+    x = torch.zeros(4, 128, dtype=BF16, device=dev)
+    plan, _, _ = _plan(et, dev, torch.ones(4, 2, dtype=torch.bool))
+    with pytest.raises(ValueError, match="HIP device"):
+        et.pack_w4(q.cpu(), s)
+    with pytest.raises(TypeError, match="uint8"):
+        et.pack_w4(q.to(torch.int8), s)
+    with pytest.raises(TypeError, match="scales"):
+        et.pack_w4(q, s.float())
+    with pytest.raises(ValueError, match="scales"):
+        et.pack_w4(q, s, group=64)
+    with pytest.raises(ValueError, match="group"):
+        et.pack_w4(q, s, group=100)
+    with pytest.raises(ValueError, match="parts"):
+        et.pack_w4(q, s, parts=3)
+    with pytest.raises(ValueError, match="multiple of 8"):
+        et.pack_w4(q[:, :20].contiguous(), s[:, :20].contiguous())
+    with pytest.raises(ValueError, match="multiple of 8"):
+        et.pack_w4(q[:, :24].contiguous(), s[:, :24].contiguous(), parts=2)
+    with pytest.raises(TypeError, match="W4Weight"):
+        et.linear_w4(x, q)
+    with pytest.raises(ValueError, match="experts"):
+        et.linear_w4(x, w)
+    with pytest.raises(TypeError, match="bfloat16"):
+        et.expert_gemm_w4(x.float(), w, plan)
+    with pytest.raises(ValueError, match="row length"):
+        et.expert_gemm_w4(x[:, :64].contiguous(), w, plan)
+    with pytest.raises(ValueError, match="tokens"):
+        et.expert_gemm_w4(x[:3], w, plan)
+    with pytest.raises(ValueError, match="slots"):
+        et.expert_gemm_w4(x, w, plan, gather=False)
+    with pytest.raises(ValueError, match="parts=2"):
+        et.expert_gemm_w4(x, w, plan, epilogue="swiglu")
+    with pytest.raises(ValueError, match="row_scale"):
+        et.expert_gemm_w4(x, w, plan, epilogue="row_scale")
+    with pytest.raises(ValueError, match="epilogue"):
+        et.expert_gemm_w4(x, w, plan, epilogue="gelu")
+    with pytest.raises(TypeError, match="scale_dtype"):
+        et.quantize_w4(torch.zeros(8, 128, device=dev), scale_dtype=torch.float32)
+    with pytest.raises(ValueError, match="contiguous"):
+        et.quantize_w4(torch.zeros(128, 8, device=dev).t())
