@@ -338,20 +338,31 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void layer_norm_bwd_kernel(
 }
 
 // Column sums of the blocks' partials, in a fixed order: 64 columns to a
-// block, wave w the partials w, w + 4, ...
-__global__ __launch_bounds__(256) void layer_norm_cols_kernel(const float* partial, int64_t blocks, int d, float* dweight,
-                                                              float* dbias)
+// block, wave w of 16 the partials w, w + 16, ..., eight loads at a time.
+constexpr int kColWaves = 16;
+
+__global__ __launch_bounds__(kColWaves * kWave) void layer_norm_cols_kernel(const float* partial, int blocks, int d,
+                                                                            float* dweight, float* dbias)
 {
-    __shared__ float part[4][kWave];
+    __shared__ float part[kColWaves][kWave];
     const int lane = lane_id(), wave = (int)threadIdx.x / kWave;
     const int col = (int)blockIdx.x * kWave + lane;
+    const int at = min(col, 2 * d - 1);
     float s = 0.0f;
-    if (col < 2 * d)
-        for (int64_t b = wave; b < blocks; b += 4) s += partial[b * 2 * d + col];
+    int b = wave;
+    for (; b + 7 * kColWaves < blocks; b += 8 * kColWaves) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = partial[(int64_t)(b + j * kColWaves) * 2 * d + at];
+        s += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+    }
+    for (; b < blocks; b += kColWaves) s += partial[(int64_t)b * 2 * d + at];
     part[wave][lane] = s;
     __syncthreads();
     if (wave == 0 && col < 2 * d) {
-        s = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+        s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kColWaves; ++w) s += part[w][lane];
         if (col < d) dweight[col] = s;
         else if (dbias) dbias[col - d] = s;
     }
@@ -498,8 +509,7 @@ extern "C" int et_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* 
     else rc = weight_dtype == ET_DTYPE_F32 ? launch_bwd<uint16_t, float>(a, blocks, s)
                                            : launch_bwd<uint16_t, uint16_t>(a, blocks, s);
     if (rc) return rc;
-    layer_norm_cols_kernel<<<dim3((unsigned)((2 * d + kWave - 1) / kWave)), dim3(256), 0, s>>>((const float*)workspace,
-                                                                                             blocks, (int)d, dweight,
-                                                                                             dbias);
+    layer_norm_cols_kernel<<<dim3((unsigned)((2 * d + kWave - 1) / kWave)), dim3(kColWaves * kWave), 0, s>>>(
+        (const float*)workspace, (int)blocks, (int)d, dweight, dbias);
     return check_launch("layer_norm_cols_kernel");
 }
