@@ -52,6 +52,7 @@ struct Row {
     static constexpr int V = Elem<X>::V;
     u32x4_t v[NV];
     float tail;
+    X raw;
 
     __device__ __forceinline__ void load(const X* row, int d, int t)
     {
@@ -64,6 +65,29 @@ struct Row {
         }
         tail = 0.0f;
         if (t < d % V) tail = Elem<X>::to_float(row[nvec * V + t]);
+    }
+    // The same without a branch, so that rows can be loaded ahead of the one
+    // that is worked on (behind branches every wait is for all loads): what a
+    // thread does not have is read from the row's last vector or element and
+    // replaced by 0.  d >= V; TAIL: d is no multiple of V.
+    template <bool TAIL>
+    __device__ __forceinline__ void load_ahead(const X* row, int d, int t)
+    {
+        const int nvec = d / V;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int k = t + TPR * i;
+            v[i] = *reinterpret_cast<const u32x4_any_t*>(row + (int64_t)min(k, nvec - 1) * V);
+        }
+        if constexpr (TAIL) raw = row[min(nvec * V + t, d - 1)];
+    }
+    template <bool TAIL>
+    __device__ __forceinline__ void settle(int d, int t)
+    {
+        const int nvec = d / V;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = t + TPR * i < nvec ? v[i] : u32x4_t{};
+        tail = TAIL && t < d % V ? Elem<X>::to_float(raw) : 0.0f;
     }
     // f(vector, its first column, whether the row holds it) and g(tail, its column), in a fixed order
     template <typename F, typename G>
@@ -133,12 +157,14 @@ struct FwdArgs {
     float eps;
 };
 
-// WPR waves per row; blocks of 256 threads (WPR = 16: 1024).
+// WPR waves per row; blocks of one row, or of four waves.
+constexpr int norm_threads(int wpr) { return wpr > 4 ? wpr * kWave : 256; }
+
 template <typename X, typename W, int WPR, int NV>
-__global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void layer_norm_fwd_kernel(FwdArgs a)
+__global__ __launch_bounds__(norm_threads(WPR)) void layer_norm_fwd_kernel(FwdArgs a)
 {
-    constexpr int TPR = WPR * kWave, V = Elem<X>::V, kRows = WPR == 16 ? 1 : 4 / WPR;
-    __shared__ float slots[2][WPR == 16 ? 16 : 4][1];
+    constexpr int TPR = WPR * kWave, V = Elem<X>::V, kRows = norm_threads(WPR) / TPR;
+    __shared__ float slots[2][WPR][1];
     const int t = (int)threadIdx.x % TPR, wave = t / kWave;
     const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
     if (row >= a.T) return;               // (whole waves; whole blocks where there are barriers)
@@ -224,13 +250,16 @@ struct BwdArgs {
 };
 
 // A block walks rows blockIdx, blockIdx + gridDim, ... (4 / WPR at a time), its
-// threads keeping their columns' sums for the weight and the bias.
-template <typename X, typename W, int WPR, int NV>
-__global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void layer_norm_bwd_kernel(BwdArgs a)
+// threads keeping their columns' sums for the weight and the bias.  DSUM: a
+// gradient past the norm is added.
+template <typename X, typename W, int WPR, int NV, int D, bool TAIL, bool DSUM>
+__global__ __launch_bounds__(norm_threads(WPR)) void layer_norm_bwd_kernel(BwdArgs a)
 {
-    constexpr int TPR = WPR * kWave, V = Elem<X>::V, kRows = WPR == 16 ? 1 : 4 / WPR;
-    __shared__ float slots[2][WPR == 16 ? 16 : 4][2];
-    const int t = (int)threadIdx.x % TPR, wave = t / kWave, sub = (int)threadIdx.x / TPR;
+    constexpr int TPR = WPR * kWave, V = Elem<X>::V, kRows = norm_threads(WPR) / TPR;
+    constexpr bool kLean = WPR == 16 || NV * V > 16;   // (registers are better spent on rows)
+    __shared__ float slots[2][WPR][2];
+    const int t = (int)threadIdx.x % TPR, wave = t / kWave;
+    const int sub = __builtin_amdgcn_readfirstlane((int)threadIdx.x / TPR);
     const int d = a.d;
     const W* const w = (const W*)a.weight;
     float dw[NV][V], db[NV][V], dwt = 0.0f, dbt = 0.0f;
@@ -238,61 +267,100 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void layer_norm_bwd_kernel(
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) dw[i][j] = db[i][j] = 0.0f;
-    int turn = 0;
-    for (int64_t row = (int64_t)blockIdx.x * kRows + sub; row < a.T; row += (int64_t)gridDim.x * kRows, turn ^= 1) {
-        Row<X, TPR, NV> x, dy, ds;
-        x.load((const X*)a.x + row * a.ldx, d, t);
-        dy.load((const X*)a.dy + row * a.lddy, d, t);
-        if (a.dsum) ds.load((const X*)a.dsum + row * a.ldds, d, t);
-        const float mean = a.mean[row], rstd = a.rstd[row];
-        float s[2] = {0.0f, 0.0f};
-        x.each(
-            d, t,
-            [&](u32x4_t& v, int col, int i) {
-                float wv[V];
-                load_weights(w, col, wv);
+    // the weight stays in registers: read twice a row it would be as much L1
+    // traffic as the rows are
+    float wr[NV][V], wt = 0.0f;
+    const int nvec = d / V;
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float xh = (Elem<X>::get(v, j) - mean) * rstd, dyv = Elem<X>::get(dy.v[i], j);
-                    const float g = dyv * wv[j];
-                    s[0] += g;
-                    s[1] = __builtin_fmaf(g, xh, s[1]);
-                    dw[i][j] = __builtin_fmaf(dyv, xh, dw[i][j]);
-                    db[i][j] += dyv;
-                }
-            },
-            [&](float v, int col) {
-                const float xh = (v - mean) * rstd, g = dy.tail * Elem<W>::to_float(w[col]);
+    for (int i = 0; i < NV; ++i) {
+        const bool in = t + TPR * i < nvec;
+        if (!kLean) load_weights(w, in ? (t + TPR * i) * V : 0, wr[i]);
+#pragma unroll
+        for (int j = 0; j < V; ++j) wr[i][j] = in ? wr[i][j] : 0.0f;
+    }
+    if (TAIL && t < d % V) wt = Elem<W>::to_float(w[nvec * V + t]);
+    struct Rows {
+        Row<X, TPR, NV> x, dy, ds;
+        float mean, rstd;
+    } ring[D];
+    const auto load = [&](Rows& r, int64_t row) {
+        row = min(row, a.T - 1);
+        r.x.template load_ahead<TAIL>((const X*)a.x + row * a.ldx, d, t);
+        r.dy.template load_ahead<TAIL>((const X*)a.dy + row * a.lddy, d, t);
+        if constexpr (DSUM) r.ds.template load_ahead<TAIL>((const X*)a.dsum + row * a.ldds, d, t);
+        r.mean = a.mean[row];
+        r.rstd = a.rstd[row];
+    };
+    const auto weights_of = [&](int i) {
+        if constexpr (kLean) load_weights(w, min(t + TPR * i, nvec - 1) * V, wr[i]);
+    };
+    const int64_t step = (int64_t)gridDim.x * kRows;
+    int64_t row = (int64_t)blockIdx.x * kRows + sub;
+    int turn = 0;
+    const auto process = [&](Rows& cur) {
+        cur.x.template settle<TAIL>(d, t);
+        cur.dy.template settle<TAIL>(d, t);
+        if constexpr (DSUM) cur.ds.template settle<TAIL>(d, t);
+        const float mean = cur.mean, rstd = cur.rstd;
+        float s[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            weights_of(i);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float xh = (Elem<X>::get(cur.x.v[i], j) - mean) * rstd, dyv = Elem<X>::get(cur.dy.v[i], j);
+                const float g = dyv * wr[i][j];
                 s[0] += g;
                 s[1] = __builtin_fmaf(g, xh, s[1]);
-                dwt = __builtin_fmaf(dy.tail, xh, dwt);
-                dbt += dy.tail;
-            });
+                dw[i][j] = __builtin_fmaf(dyv, xh, dw[i][j]);
+                db[i][j] += dyv;
+            }
+        }
+        if constexpr (TAIL) {
+            const float xh = (cur.x.tail - mean) * rstd, g = cur.dy.tail * wt;
+            s[0] += g;
+            s[1] = __builtin_fmaf(g, xh, s[1]);
+            dwt = __builtin_fmaf(cur.dy.tail, xh, dwt);
+            dbt += cur.dy.tail;
+        }
         row_sums<WPR, 2>(s, slots[turn], wave);
         const float c1 = s[0] / (float)d, c2 = s[1] / (float)d;
         X* const dx = (X*)a.dx + row * d;
-        x.each(
-            d, t,
-            [&](u32x4_t& v, int col, int i) {
-                float wv[V], out[V];
-                load_weights(w, col, wv);
+        const auto gradient = [&](float x, float dy, float wv, float ds) {
+            const float xh = (x - mean) * rstd;
+            const float g = rstd * __builtin_fmaf(-xh, c2, __builtin_fmaf(dy, wv, -c1));
+            return DSUM ? g + ds : g;
+        };
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float xh = (Elem<X>::get(v, j) - mean) * rstd;
-                    const float g = __builtin_fmaf(Elem<X>::get(dy.v[i], j), wv[j], -c1);
-                    out[j] = rstd * __builtin_fmaf(-xh, c2, g) + (a.dsum ? Elem<X>::get(ds.v[i], j) : 0.0f);
-                }
-                *reinterpret_cast<u32x4_any_t*>(dx + col) = Elem<X>::pack(out);
-            },
-            [&](float v, int col) {
-                const float xh = (v - mean) * rstd;
-                const float g = __builtin_fmaf(dy.tail, Elem<W>::to_float(w[col]), -c1);
-                dx[col] = Elem<X>::from_float(rstd * __builtin_fmaf(-xh, c2, g) + (a.dsum ? ds.tail : 0.0f));
-            });
+        for (int i = 0; i < NV; ++i) {
+            float out[V];
+            weights_of(i);
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                out[j] = gradient(Elem<X>::get(cur.x.v[i], j), Elem<X>::get(cur.dy.v[i], j), wr[i][j],
+                                  DSUM ? Elem<X>::get(cur.ds.v[i], j) : 0.0f);
+            if (t + TPR * i < nvec)
+                *reinterpret_cast<u32x4_any_t*>(dx + (t + TPR * i) * V) = Elem<X>::pack(out);
+        }
+        if (TAIL && t < d % V)
+            dx[nvec * V + t] = Elem<X>::from_float(gradient(cur.x.tail, cur.dy.tail, wt, DSUM ? cur.ds.tail : 0.0f));
+        turn ^= 1;
+    };
+    // rows in flight: the one that is worked on and D - 1 behind it
+#pragma unroll
+    for (int u = 0; u < D - 1; ++u) load(ring[u], row + u * step);
+    for (bool more = true; more;) {
+#pragma unroll
+        for (int u = 0; u < D; ++u) {
+            more = row < a.T;
+            if (!more) break;
+            load(ring[(u + D - 1) % D], row + (D - 1) * step);
+            process(ring[u]);
+            row += step;
+        }
     }
     // the block's sums; with several rows at a time their threads' are added first
     float* const out = a.partial + (int64_t)blockIdx.x * 2 * d;
-    const int nvec = d / V;
     if constexpr (kRows > 1) {
         constexpr int kCols = TPR * NV * V;
         __shared__ float cols[2][kCols + kWave];
@@ -369,9 +437,9 @@ __global__ __launch_bounds__(kColWaves * kWave) void layer_norm_cols_kernel(cons
 }
 
 constexpr int kMaxWidth = ET_MAX_NORM_WIDTH;
-constexpr int64_t kMaxBlocks = 1024;
+constexpr int64_t kMaxBlocks = 256;
 
-int64_t bwd_blocks(int64_t T) { return std::max<int64_t>(1, std::min<int64_t>((T + 3) / 4, kMaxBlocks)); }
+int64_t bwd_blocks(int64_t T) { return std::max<int64_t>(1, std::min(T, kMaxBlocks)); }
 
 // Vectors of a row of d elements for each of `threads`.
 int vectors(int64_t d, int V, int threads) { return (int)((d / V + threads - 1) / threads); }
@@ -380,35 +448,100 @@ template <typename X, typename W>
 int launch_fwd(const FwdArgs& a, hipStream_t s)
 {
     constexpr int V = Elem<X>::V;
-    const auto go = [&](auto kernel, int rows, int threads) {
-        kernel<<<dim3((unsigned)((a.T + rows - 1) / rows)), dim3(threads), 0, s>>>(a);
+    const auto go = [&](auto kernel, int wpr) {
+        const int64_t rows = norm_threads(wpr) / (wpr * kWave);
+        kernel<<<dim3((unsigned)((a.T + rows - 1) / rows)), dim3(norm_threads(wpr)), 0, s>>>(a);
         return check_launch("layer_norm_fwd_kernel");
     };
-    const int n1 = vectors(a.d, V, 64), n4 = vectors(a.d, V, 256);
-    if (n1 <= 1) return go(layer_norm_fwd_kernel<X, W, 1, 1>, 4, 256);
-    if (n1 <= 2) return go(layer_norm_fwd_kernel<X, W, 1, 2>, 4, 256);
-    if (n1 <= 4) return go(layer_norm_fwd_kernel<X, W, 1, 4>, 4, 256);
-    if (n4 <= 2) return go(layer_norm_fwd_kernel<X, W, 4, 2>, 1, 256);
-    if (n4 <= 4) return go(layer_norm_fwd_kernel<X, W, 4, 4>, 1, 256);
-    return go(layer_norm_fwd_kernel<X, W, 16, 16 / V>, 1, 1024);
+    const auto fits = [&](int wpr, int nv) { return vectors(a.d, V, wpr * kWave) <= nv; };
+    if (fits(1, 1)) return go(layer_norm_fwd_kernel<X, W, 1, 1>, 1);
+    if (fits(1, 2)) return go(layer_norm_fwd_kernel<X, W, 1, 2>, 1);
+    if (fits(1, 4)) return go(layer_norm_fwd_kernel<X, W, 1, 4>, 1);
+    if (fits(4, 2)) return go(layer_norm_fwd_kernel<X, W, 4, 2>, 4);
+    if (fits(4, 4)) return go(layer_norm_fwd_kernel<X, W, 4, 4>, 4);
+    return go(layer_norm_fwd_kernel<X, W, 16, 16 / V>, 16);
+}
+
+template <typename X, typename W, bool TAIL, bool DSUM>
+int launch_bwd(const BwdArgs& a, int64_t blocks, hipStream_t s)
+{
+    constexpr int V = Elem<X>::V;
+    const auto go = [&](auto kernel, int wpr) {
+        kernel<<<dim3((unsigned)blocks), dim3(norm_threads(wpr)), 0, s>>>(a);
+        return check_launch("layer_norm_bwd_kernel");
+    };
+    const auto fits = [&](int wpr, int nv) { return vectors(a.d, V, wpr * kWave) <= nv; };
+    if (fits(1, 1)) return go(layer_norm_bwd_kernel<X, W, 1, 1, 4, TAIL, DSUM>, 1);
+    if (fits(1, 2)) return go(layer_norm_bwd_kernel<X, W, 1, 2, 2, TAIL, DSUM>, 1);
+    if (fits(4, 1)) return go(layer_norm_bwd_kernel<X, W, 4, 1, 3, TAIL, DSUM>, 4);
+    if (fits(4, 2)) return go(layer_norm_bwd_kernel<X, W, 4, 2, 2, TAIL, DSUM>, 4);
+    if (fits(8, 2)) return go(layer_norm_bwd_kernel<X, W, 8, 2, 2, TAIL, DSUM>, 8);
+    if constexpr (sizeof(X) == 2) {
+        return go(layer_norm_bwd_kernel<X, W, 16, 2, 1, TAIL, DSUM>, 16);
+    } else {
+        if (fits(8, 4)) return go(layer_norm_bwd_kernel<X, W, 8, 4, 2, TAIL, DSUM>, 8);
+        return go(layer_norm_bwd_kernel<X, W, 16, 4, 1, TAIL, DSUM>, 16);
+    }
+}
+
+// Rows of fewer than V elements: nothing to do in vectors, and no more than 7
+// columns; a thread for each of them and 256 rows a block.
+template <typename X, typename W>
+__global__ __launch_bounds__(256) void layer_norm_bwd_narrow_kernel(BwdArgs a)
+{
+    __shared__ float part[4][2][8];
+    const int d = a.d;
+    float dw[8], db[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) dw[c] = db[c] = 0.0f;
+    for (int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x; row < a.T; row += (int64_t)gridDim.x * 256) {
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        float xh[8], dy[8], g[8], s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            if (c >= d) break;
+            xh[c] = (Elem<X>::to_float(((const X*)a.x)[row * a.ldx + c]) - mean) * rstd;
+            dy[c] = Elem<X>::to_float(((const X*)a.dy)[row * a.lddy + c]);
+            g[c] = dy[c] * Elem<W>::to_float(((const W*)a.weight)[c]);
+            s0 += g[c];
+            s1 = __builtin_fmaf(g[c], xh[c], s1);
+            dw[c] = __builtin_fmaf(dy[c], xh[c], dw[c]);
+            db[c] += dy[c];
+        }
+        const float c1 = s0 / (float)d, c2 = s1 / (float)d;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            if (c >= d) break;
+            const float v = rstd * __builtin_fmaf(-xh[c], c2, g[c] - c1);
+            ((X*)a.dx)[row * d + c] =
+                Elem<X>::from_float(a.dsum ? v + Elem<X>::to_float(((const X*)a.dsum)[row * a.ldds + c]) : v);
+        }
+    }
+    for (int c = 0; c < d; ++c) {
+        const float sw = wave_sum_dpp(dw[c]), sb = wave_sum_dpp(db[c]);
+        if (lane_id() == 0) {
+            part[threadIdx.x / kWave][0][c] = sw;
+            part[threadIdx.x / kWave][1][c] = sb;
+        }
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < 2 * d) {
+        const int k = (int)threadIdx.x / d, c = (int)threadIdx.x % d;
+        a.partial[(int64_t)blockIdx.x * 2 * d + threadIdx.x] =
+            (part[0][k][c] + part[1][k][c]) + (part[2][k][c] + part[3][k][c]);
+    }
 }
 
 template <typename X, typename W>
 int launch_bwd(const BwdArgs& a, int64_t blocks, hipStream_t s)
 {
-    constexpr int V = Elem<X>::V;
-    const auto go = [&](auto kernel, int threads) {
-        kernel<<<dim3((unsigned)blocks), dim3(threads), 0, s>>>(a);
-        return check_launch("layer_norm_bwd_kernel");
-    };
-    const int n1 = vectors(a.d, V, 64), n4 = vectors(a.d, V, 256), n16 = vectors(a.d, V, 1024);
-    if (n1 <= 1) return go(layer_norm_bwd_kernel<X, W, 1, 1>, 256);
-    if (n1 <= 2) return go(layer_norm_bwd_kernel<X, W, 1, 2>, 256);
-    if (n4 <= 1) return go(layer_norm_bwd_kernel<X, W, 4, 1>, 256);
-    if (n4 <= 2) return go(layer_norm_bwd_kernel<X, W, 4, 2>, 256);
-    if (n16 <= 1) return go(layer_norm_bwd_kernel<X, W, 16, 1>, 1024);
-    if (sizeof(X) == 2 || n16 <= 2) return go(layer_norm_bwd_kernel<X, W, 16, 2>, 1024);
-    if constexpr (sizeof(X) == 4) return go(layer_norm_bwd_kernel<X, W, 16, 4>, 1024);
+    if (a.d < Elem<X>::V) {
+        layer_norm_bwd_narrow_kernel<X, W><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(a);
+        return check_launch("layer_norm_bwd_narrow_kernel");
+    }
+    if (a.d % Elem<X>::V)
+        return a.dsum ? launch_bwd<X, W, true, true>(a, blocks, s) : launch_bwd<X, W, true, false>(a, blocks, s);
+    return a.dsum ? launch_bwd<X, W, false, true>(a, blocks, s) : launch_bwd<X, W, false, false>(a, blocks, s);
 }
 
 // Checks that both directions share.
@@ -505,11 +638,13 @@ extern "C" int et_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* 
     const int64_t blocks = bwd_blocks(rows);
     const BwdArgs a{dy, x, dsum, weight, mean, rstd, dx, (float*)workspace, dy_stride, x_stride, dsum_stride, rows, (int)d};
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == ET_DTYPE_F32) rc = launch_bwd<float, float>(a, blocks, s);
+    // (the kernels read rows ahead, the last one at least: they are for rows > 0)
+    if (rows == 0) rc = ET_OK;
+    else if (dtype == ET_DTYPE_F32) rc = launch_bwd<float, float>(a, blocks, s);
     else rc = weight_dtype == ET_DTYPE_F32 ? launch_bwd<uint16_t, float>(a, blocks, s)
                                            : launch_bwd<uint16_t, uint16_t>(a, blocks, s);
     if (rc) return rc;
     layer_norm_cols_kernel<<<dim3((unsigned)((2 * d + kWave - 1) / kWave)), dim3(kColWaves * kWave), 0, s>>>(
-        (const float*)workspace, (int)blocks, (int)d, dweight, dbias);
+        (const float*)workspace, rows ? (int)blocks : 0, (int)d, dweight, dbias);
     return check_launch("layer_norm_cols_kernel");
 }
