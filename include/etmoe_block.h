@@ -170,7 +170,7 @@ int et_adamw8(void* const* params, const void* const* grads, uint8_t* const* m8,
  * K columns each:
  *   w[e, n, k] = (q[e, n, k] - 8) * scale[e, n, k / group],  q in 0..15
  * group 32, 64 or 128; the last group of a row may be short.  K a multiple of 8 below
- * 2^22, N*K below 2^31.  q is given as bytes [E, N, K / 2], the even k in the
+ * 2^22, N below 2^22, N*K below 2^31.  q is given as bytes [E, N, K / 2], the even k in the
  * low half, scales as 16-bit numbers [E, N, ceil(K / group)].
  *
  * et_w4_pack lays both out once in the order in which the product reads them:

@@ -22,6 +22,7 @@
 // other, and their scales lie in the lanes' order: a wave's loads are whole
 // KiBs of consecutive addresses.
 #include <algorithm>
+#include <utility>
 
 #include "et_gemm_common.hpp"
 #include "etmoe_block.h"
@@ -35,20 +36,20 @@ constexpr int kTileBytes = 1024;
 constexpr uint32_t kMagic = 0x43004300u;    // bf16 128 | q
 constexpr uint32_t kOffset = 0xC308C308u;   // bf16 -136, twice
 
+// Sizes of a weight; the derived ones are the host's (a division takes a wave
+// some 40 instructions).
 struct W4Shape {
     int E, N, K, parts, group;
-    __host__ __device__ int part_rows() const { return N / parts; }
-    __host__ __device__ int part_sbs() const { return (N / parts + kSb - 1) / kSb; }
-    __host__ __device__ int sbs() const { return parts * part_sbs(); }
-    __host__ __device__ int kts() const { return (K + kKt - 1) / kKt; }
+    int part_rows, part_sbs;   // rows of a part, and its superblocks
+    int sbs, kts;              // superblocks of an expert, tiles along K
     __host__ __device__ int gpt() const { return kKt / group; }               // groups of a tile
-    __host__ __device__ int64_t expert_bytes() const { return (int64_t)sbs() * kts() * 2 * kTileBytes; }
-    __host__ __device__ int64_t expert_scales() const { return (int64_t)sbs() * kts() * gpt() * kSb; }
+    __host__ __device__ int64_t expert_bytes() const { return (int64_t)sbs * kts * 2 * kTileBytes; }
+    __host__ __device__ int64_t expert_scales() const { return (int64_t)sbs * kts * gpt() * kSb; }
     // the first weight row of superblock b, and how many of its rows there are
-    __host__ __device__ int row0(int b) const { return b / part_sbs() * part_rows() + b % part_sbs() * kSb; }
+    __host__ __device__ int row0(int b) const { return b < part_sbs ? b * kSb : part_rows + (b - part_sbs) * kSb; }
     __host__ __device__ int rows(int b) const
     {
-        const int left = part_rows() - b % part_sbs() * kSb;
+        const int left = part_rows - (b < part_sbs ? b : b - part_sbs) * kSb;
         return left < kSb ? left : kSb;
     }
 };
@@ -76,12 +77,12 @@ __device__ __forceinline__ int scale_row(int i) { return 16 * (i >> 2 & 1) + 4 *
 __global__ __launch_bounds__(256) void w4_pack_kernel(const uint8_t* q, const uint16_t* scales, W4Shape w, uint32_t* packed,
                                                       uint16_t* packed_scales)
 {
-    const int kts = w.kts(), gpt = w.gpt(), groups = (w.K + w.group - 1) / w.group;
+    const int kts = w.kts, gpt = w.gpt(), groups = (w.K + w.group - 1) / w.group;
     // one block: the tiles of one superblock at one k range
     const int64_t blk = blockIdx.x;
     const int kt = (int)(blk % kts);
-    const int b = (int)(blk / kts % w.sbs());
-    const int e = (int)(blk / kts / w.sbs());
+    const int b = (int)(blk / kts % w.sbs);
+    const int e = (int)(blk / kts / w.sbs);
     const int row0 = w.row0(b), rows = w.rows(b);
     for (int i = (int)threadIdx.x; i < 2 * kTileBytes / 4; i += 256) {
         const int tile = i >> 8, lane = i >> 2 & 63, s = i & 3;
@@ -110,11 +111,11 @@ __global__ __launch_bounds__(256) void w4_unpack_kernel(const uint32_t* packed, 
                                                         W4Shape w, const int32_t* expert_offsets, int64_t cap,
                                                         uint16_t* out)
 {
-    const int kts = w.kts(), gpt = w.gpt();
+    const int kts = w.kts, gpt = w.gpt();
     const int64_t blk = blockIdx.x;
     const int kt = (int)(blk % kts);
-    const int b = (int)(blk / kts % w.sbs());
-    const int e = (int)(blk / kts / w.sbs());
+    const int b = (int)(blk / kts % w.sbs);
+    const int e = (int)(blk / kts / w.sbs);
     if (expert_offsets && min<int64_t>(expert_offsets[e], cap) >= min<int64_t>(expert_offsets[e + 1], cap)) return;
     const int row0 = w.row0(b), rows = w.rows(b);
     for (int i = (int)threadIdx.x; i < 2 * kTileBytes / 4; i += 256) {
@@ -203,129 +204,201 @@ struct W4Tile {
     int b;          // first superblock (SwiGLU: of the gate part)
 };
 
+// Lane i of each row of 16 lanes, to the whole row.
+template <int I>
+__device__ __forceinline__ float row_bcast(float x)
+{
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x150 + I, 0xf, 0xf, true));
+}
+
+// f(0), f(1), ... with the numbers as constants.
+template <int... I, typename F>
+__device__ __forceinline__ void constants(std::integer_sequence<int, I...>, F f)
+{
+    (f(std::integral_constant<int, I>{}), ...);
+}
+
+// The two constants of unpacking, kept in registers.
+struct Unpack {
+    uint32_t mask = 0x000F000Fu, magic = kMagic;
+    __device__ __forceinline__ Unpack()
+    {
+        asm("" : "+s"(mask));
+        asm("" : "+v"(magic));
+    }
+};
+
+// Scales of R = 4 turns (4 GPT groups) of the superblocks of a wave: lane
+// (rho, i) loads those of group i for the rows that lanes (rho, *) add up, 16
+// bytes; a broadcast of lane i along its row hands them out.  (Loaded group by
+// group, the same 64 bytes in all of a row's lanes, they cost 8 to 13% of a
+// call of 4 to 16 tokens.)
+constexpr int kTurns = 4;
+template <int NSB, bool HALF>
+struct Scales {
+    u32x4_t raw[NSB];
+    float f[NSB][8];
+    __device__ __forceinline__ void convert()
+    {
+#pragma unroll
+        for (int j = 0; j < NSB; ++j)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[j][k] = scale16(k & 1 ? raw[j][k / 2] >> 16 : raw[j][k / 2] & 0xFFFFu, HALF);
+    }
+};
+
+// acc += one k range of 128 of NT tiles (two to a superblock) by MT tiles of 16
+// slots; a(i, s) is the fragment of slots 16 i.. at k-step s, TURN the place of
+// the range among those that the scales at hand are for.
+template <int MT, int NT, int GPT, int TURN, bool HALF, typename A>
+__device__ __forceinline__ void w4_mul(const u32x4_t (&w)[NT], const Scales<NT / 2, HALF>& scales, const Unpack& un, A a,
+                                       f32x4_t (&acc)[NT][MT])
+{
+    constexpr int SPG = 4 / GPT;
+    const bf16x8_t offset = __builtin_bit_cast(bf16x8_t, u32x4_t{kOffset, kOffset, kOffset, kOffset});
+    constants(std::make_integer_sequence<int, GPT>{}, [&](auto group) {
+        constexpr int q = decltype(group)::value;
+        bf16x8_t x[MT][SPG];
+        f32x4_t base[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            base[i] = f32x4_t{};
+#pragma unroll
+            for (int s = 0; s < SPG; ++s) {
+                x[i][s] = __builtin_bit_cast(bf16x8_t, a(i, q * SPG + s));
+                base[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(offset, x[i][s], base[i], 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            // (a tile at a time: the scheduler would else unpack them all first)
+            __builtin_amdgcn_sched_barrier(0);
+            f32x4_t p[MT];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) p[i] = base[i];
+#pragma unroll
+            for (int s = 0; s < SPG; ++s) {
+                u32x4_t f;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) f[k] = unpack2(w[j][q * SPG + s], 4 * k, un.mask, un.magic);
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+                    p[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, f), x[i][s], p[i], 0, 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float scale = row_bcast<TURN * GPT + q>(scales.f[j / 2][4 * (j & 1) + r]);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) acc[j][i][r] = __builtin_fmaf(scale, p[i][r], acc[j][i][r]);
+            }
+        }
+    });
+}
+
+// Where a wave reads the weights and scales of superblock b (clamped to the last).
+struct W4Rows {
+    const unsigned char* w;
+    const uint16_t* s;
+    __device__ __forceinline__ W4Rows() {}
+    __device__ __forceinline__ W4Rows(const W4Args& g, int e, int b, int gpt)
+    {
+        b = min(b, g.w.sbs - 1);
+        w = g.packed + e * g.w.expert_bytes() + (int64_t)b * g.w.kts * 2 * kTileBytes;
+        s = g.scales + e * g.w.expert_scales() + (int64_t)b * g.w.kts * gpt * kSb;
+    }
+};
+
+// Rows of A of a tile as a buffer, and the offset of row r in it (out of range
+// past the tile and for invalid tokens, which read 0).
+struct W4Acts {
+    __amdgpu_buffer_rsrc_t res;
+    __device__ __forceinline__ W4Acts(const W4Args& g, const W4Tile& t)
+    {
+        const int K = g.w.K;
+        res = g.sorted_token
+                  ? __builtin_amdgcn_make_buffer_rsrc((void*)g.a, (short)0, (int)(g.a_rows * K * 2), kBufDword3)
+                  : __builtin_amdgcn_make_buffer_rsrc((void*)(g.a + t.s0 * K), (short)0, t.rows * K * 2, kBufDword3);
+    }
+    __device__ __forceinline__ uint32_t row(const W4Args& g, const W4Tile& t, int r) const
+    {
+        if (r >= t.rows) return kOOR;
+        uint32_t at = (uint32_t)r;
+        if (g.sorted_token) {
+            at = (uint32_t)g.sorted_token[t.s0 + r];
+            if (at >= (uint32_t)g.a_rows) return kOOR;
+        }
+        return at * (uint32_t)g.w.K * 2u;
+    }
+    // 16 bytes from column k (uniform) + in of the row at byte offset `at`; 0 past K
+    __device__ __forceinline__ u32x4_t load(uint32_t at, int k, int in, int K) const
+    {
+        return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                                               res, (int)(k + in < K ? at + 2u * (uint32_t)in : kOOR), 2 * k, 0));
+    }
+};
+
 // One block's tile: 16 MT slots x NSB superblocks (SwiGLU: one of the gate
 // part, its twin of the up part), the k range dealt to the block's waves one
 // 128 at a time, their sums joined through LDS in the waves' order.
 template <bool SWIGLU, int MT, int NSB, int GPT, bool HALF, int WAVES>
 __device__ __forceinline__ void w4_tile(const W4Args& g, const W4Tile& t, float* lds)
 {
-    constexpr int NT = 2 * NSB, SPG = 4 / GPT, U = 2;
+    constexpr int NT = 2 * NSB, U = 2;
     const int lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
     const int r16 = lane & 15, rho = lane >> 4;
-    const int K = g.w.K, kts = g.w.kts(), twin = g.w.part_sbs();
-    const unsigned char* const wq = g.packed + t.e * g.w.expert_bytes();
-    const uint16_t* const ws = g.scales + t.e * g.w.expert_scales();
-    const unsigned char* wp[NSB];
-    const uint16_t* sp[NSB];
+    const int K = g.w.K, kts = g.w.kts, twin = g.w.part_sbs;
+    W4Rows rows[NSB];
 #pragma unroll
-    for (int j = 0; j < NSB; ++j) {
-        const int b = min(t.b + (SWIGLU ? j * twin : j), g.w.sbs() - 1);
-        wp[j] = wq + (int64_t)b * kts * 2 * kTileBytes;
-        sp[j] = ws + (int64_t)b * kts * GPT * kSb;
-    }
-    const bool gather = g.sorted_token != nullptr;
-    const __amdgpu_buffer_rsrc_t ares =
-        gather ? __builtin_amdgcn_make_buffer_rsrc((void*)g.a, (short)0, (int)(g.a_rows * K * 2), kBufDword3)
-               : __builtin_amdgcn_make_buffer_rsrc((void*)(g.a + t.s0 * K), (short)0, t.rows * K * 2, kBufDword3);
+    for (int j = 0; j < NSB; ++j) rows[j] = W4Rows(g, t.e, t.b + (SWIGLU ? j * twin : j), GPT);
+    const W4Acts acts(g, t);
     uint32_t ao[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const int r = 16 * i + r16;
-        ao[i] = kOOR;
-        if (r < t.rows) {
-            uint32_t at = (uint32_t)r;
-            if (gather) at = (uint32_t)g.sorted_token[t.s0 + r];
-            if (!gather || at < (uint32_t)g.a_rows) ao[i] = (at * (uint32_t)K + 8u * rho) * 2u;
-        }
-    }
+    for (int i = 0; i < MT; ++i) ao[i] = acts.row(g, t, 16 * i + r16);
+    // (kts of this wave: wave, wave + WAVES, ...; loads past the last repeat it)
+    const int n = (kts - wave + WAVES - 1) / WAVES;
+    const auto kt_of = [&](int i) { return wave + WAVES * min(i, n - 1); };
     struct Step {
-        u32x4_t w[NT], s[NSB][GPT], a[MT][4];
+        u32x4_t w[NT], a[MT][4];
     } ring[U];
-    const auto load = [&](Step& x, int kt) {
+    const auto load = [&](Step& x, int i) {
+        const int kt = kt_of(i);
+        const uint32_t at = (uint32_t)kt * (2 * kTileBytes);
 #pragma unroll
-        for (int j = 0; j < NSB; ++j) {
+        for (int j = 0; j < NT; ++j)
+            x.w[j] = *reinterpret_cast<const u32x4_t*>(rows[j / 2].w + at + (j & 1) * kTileBytes + 16 * lane);
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                x.w[2 * j + h] = *reinterpret_cast<const u32x4_t*>(wp[j] + (int64_t)kt * 2 * kTileBytes + h * kTileBytes +
-                                                                   16 * lane);
+        for (int s = 0; s < 4; ++s)
 #pragma unroll
-            for (int q = 0; q < GPT; ++q)
-                x.s[j][q] = *reinterpret_cast<const u32x4_t*>(sp[j] + (kt * GPT + q) * kSb + 8 * rho);
-        }
+            for (int m = 0; m < MT; ++m) x.a[m][s] = acts.load(ao[m], kt * kKt, 32 * s + 8 * rho, K);
+    };
+    Scales<NSB, HALF> scales;
+    const auto load_scales = [&](int i) {
+        const int at = (kt_of(i + min(r16 / GPT, kTurns - 1)) * GPT + r16 % GPT) * kSb + 8 * rho;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const bool in = kt * kKt + 32 * s + 8 * rho < K;
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-                x.a[i][s] = __builtin_bit_cast(
-                    u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(ares, (int)(in ? ao[i] : kOOR), kt * kKt * 2 + 64 * s, 0));
-        }
+        for (int j = 0; j < NSB; ++j) scales.raw[j] = *reinterpret_cast<const u32x4_t*>(rows[j].s + at);
     };
     f32x4_t acc[NT][MT];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[j][i] = f32x4_t{};
-    const bf16x8_t offset = __builtin_bit_cast(bf16x8_t, u32x4_t{kOffset, kOffset, kOffset, kOffset});
-    uint32_t mask = 0x000F000Fu, magic = kMagic;
-    asm("" : "+s"(mask));
-    asm("" : "+v"(magic));
-    const auto mul = [&](const Step& x) {
-#pragma unroll
-        for (int q = 0; q < GPT; ++q) {
-            f32x4_t base[MT];
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                base[i] = f32x4_t{};
-#pragma unroll
-                for (int s = 0; s < SPG; ++s)
-                    base[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                        offset, __builtin_bit_cast(bf16x8_t, x.a[i][q * SPG + s]), base[i], 0, 0, 0);
-            }
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                // (a tile at a time: the scheduler would else unpack them all first)
-                __builtin_amdgcn_sched_barrier(0);
-                f32x4_t p[MT];
-#pragma unroll
-                for (int i = 0; i < MT; ++i) p[i] = base[i];
-#pragma unroll
-                for (int s = 0; s < SPG; ++s) {
-                    const uint32_t v = x.w[j][q * SPG + s];
-                    u32x4_t f;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) f[k] = unpack2(v, 4 * k, mask, magic);
-#pragma unroll
-                    for (int i = 0; i < MT; ++i)
-                        p[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, f),
-                                                                       __builtin_bit_cast(bf16x8_t, x.a[i][q * SPG + s]),
-                                                                       p[i], 0, 0, 0);
-                }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const uint32_t pair = x.s[j / 2][q][2 * (j & 1) + r / 2];
-                    const float sc = scale16(r & 1 ? pair >> 16 : pair & 0xFFFFu, HALF);
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) acc[j][i][r] = __builtin_fmaf(sc, p[i][r], acc[j][i][r]);
-                }
-            }
-        }
-    };
-    // (kts of this wave: wave, wave + WAVES, ...; loads past the last repeat it)
-    const int n = (kts - wave + WAVES - 1) / WAVES;
+    const Unpack un;
     if (n > 0) {
-        const auto kt_of = [&](int i) { return wave + WAVES * min(i, n - 1); };
+        load_scales(0);
 #pragma unroll
-        for (int u = 0; u < U; ++u) load(ring[u], kt_of(u));
-        for (int i = 0; i < n; i += U) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (i + u < n) mul(ring[u]);
+        for (int u = 0; u < U; ++u) load(ring[u], u);
+        for (int i = 0; i < n; i += kTurns) {
+            scales.convert();
+            load_scales(i + kTurns);
+            constants(std::make_integer_sequence<int, kTurns>{}, [&](auto turn) {
+                constexpr int v = decltype(turn)::value;
+                const Step& x = ring[v % U];
+                if (i + v < n) w4_mul<MT, NT, GPT, v, HALF>(x.w, scales, un, [&](int m, int s) { return x.a[m][s]; }, acc);
                 __builtin_amdgcn_sched_barrier(0);
-                load(ring[u], kt_of(i + u + U));
+                load(ring[v % U], i + v + U);
                 __builtin_amdgcn_sched_barrier(0);
-            }
+            });
         }
     }
     // the waves' sums, in order: wave w takes output units w, w + WAVES, ...
@@ -341,7 +414,7 @@ __device__ __forceinline__ void w4_tile(const W4Args& g, const W4Tile& t, float*
         for (int v = 0; v < WAVES; ++v) s += *reinterpret_cast<const f32x4_t*>(lds + ((v * NT + j) * MT + i) * 4 * kWave + 4 * lane);
         return s;
     };
-    const int cols = SWIGLU ? g.w.part_rows() : g.w.N;
+    const int cols = SWIGLU ? g.w.part_rows : g.w.N;
     for (int unit = wave; unit < (SWIGLU ? 2 : NT) * MT; unit += WAVES) {
         const int j = unit / MT, i = unit % MT;
         const int b = t.b + j / 2, row = 16 * i + r16, in = 16 * (j & 1) + 4 * rho;
@@ -351,7 +424,7 @@ __device__ __forceinline__ void w4_tile(const W4Args& g, const W4Tile& t, float*
 #pragma unroll
             for (int k = 0; k < 4; ++k) v[k] = (v[k] * sigmoid(v[k])) * up[k];
         }
-        if (b >= (SWIGLU ? twin : g.w.sbs()) || row >= t.rows || in >= g.w.rows(b)) continue;
+        if (b >= (SWIGLU ? twin : g.w.sbs) || row >= t.rows || in >= g.w.rows(b)) continue;
         if (g.row_scale) v *= g.row_scale[t.s0 + row];
         *reinterpret_cast<u32x2_t*>(g.c + (t.s0 + row) * cols + g.w.row0(b) + in) =
             u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
@@ -359,70 +432,265 @@ __device__ __forceinline__ void w4_tile(const W4Args& g, const W4Tile& t, float*
     __syncthreads();
 }
 
-template <bool SWIGLU, int MT, int NSB, int GPT, bool HALF, int WAVES>
-__global__ __launch_bounds__(WAVES * kWave, 2) void w4_gemm_kernel(W4Args g)
+// Tiles of more slots: the waves lie side by side in the weight rows, 64 each
+// (SwiGLU: 32 gate rows and their 32 up rows), every one over the whole of K, and
+// share the rows of A, 128 k at a time, through two LDS buffers (one barrier
+// each): read from L2 by every wave, as above, they are 2 to 4 times the weight's
+// bytes at 32 and 64 slots.
+constexpr int kWideWaves = 4;
+constexpr int kWidePitch = 2 * kKt + 16;               // bytes of a row of A in LDS
+constexpr int kWideBuf = 64 * kWidePitch;
+
+template <bool SWIGLU, int MT, int GPT, bool HALF>
+__device__ __forceinline__ void w4_wide_tile(const W4Args& g, const W4Tile& t, unsigned char* lds)
 {
-    __shared__ __attribute__((aligned(16))) float lds[WAVES * 2 * NSB * MT * 4 * kWave];
-    __shared__ int ptile[ET_MAX_EXPERTS + 1];     // prefix of the experts' slot tiles
-    __shared__ int32_t eoff[ET_MAX_EXPERTS + 1];  // expert_offsets below the capacity
-    constexpr int kRows = 16 * MT;
-    const int E = g.w.E, lane = lane_id();
-    if (threadIdx.x < kWave) {
-        int carry = 0;
+    constexpr int NSB = 2, NT = 4, U = 2;
+    const int lane = lane_id();
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+    const int r16 = lane & 15, rho = lane >> 4;
+    const int K = g.w.K, kts = g.w.kts, twin = g.w.part_sbs;
+    const int b0 = t.b + wave * (SWIGLU ? 1 : NSB);      // the wave's first superblock
+    W4Rows rows[NSB];
+#pragma unroll
+    for (int j = 0; j < NSB; ++j) rows[j] = W4Rows(g, t.e, b0 + (SWIGLU ? j * twin : j), GPT);
+    u32x4_t ring[U][NT];
+    const auto load_w = [&](int kt, int u) {
+        const uint32_t at = (uint32_t)min(kt, kts - 1) * (2 * kTileBytes);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+            ring[u][j] = *reinterpret_cast<const u32x4_t*>(rows[j / 2].w + at + (j & 1) * kTileBytes + 16 * lane);
+    };
+    Scales<NSB, HALF> scales;
+    const auto load_scales = [&](int kt) {
+        const int at = (min(kt + min(r16 / GPT, kTurns - 1), kts - 1) * GPT + r16 % GPT) * kSb + 8 * rho;
+#pragma unroll
+        for (int j = 0; j < NSB; ++j) scales.raw[j] = *reinterpret_cast<const u32x4_t*>(rows[j].s + at);
+    };
+    load_scales(0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) load_w(u, u);
+    // thread i: 16 bytes from column 8 (i % 16) of rows i / 16 + 16 m
+    const W4Acts acts(g, t);
+    const int seg = (int)threadIdx.x & 15, sr = (int)threadIdx.x >> 4;
+    uint32_t ao[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) ao[m] = acts.row(g, t, 16 * m + sr);
+    u32x4_t stage[MT];
+    const auto load_a = [&](int kt) {
+        kt = min(kt, kts - 1);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) stage[m] = acts.load(ao[m], kt * kKt, 8 * seg, K);
+    };
+    const auto store_a = [&](int b) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+            *reinterpret_cast<u32x4_t*>(lds + b * kWideBuf + (16 * m + sr) * kWidePitch + 16 * seg) = stage[m];
+    };
+    f32x4_t acc[NT][MT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[j][i] = f32x4_t{};
+    const Unpack un;
+    load_a(0);
+    store_a(0);
+    load_a(1);
+    __syncthreads();
+    for (int kt = 0; kt < kts; kt += kTurns) {
+        scales.convert();
+        load_scales(kt + kTurns);
+        constants(std::make_integer_sequence<int, kTurns>{}, [&](auto turn) {
+            constexpr int v = decltype(turn)::value;
+            if (kt + v < kts) {      // (the same for the whole block)
+                // range kt + v is in buffer v % 2; the next one goes to the
+                // other, which every wave has read before the last barrier
+                store_a((v & 1) ^ 1);
+                load_a(kt + v + 2);
+                __builtin_amdgcn_sched_barrier(0);
+                const unsigned char* const x = lds + (v & 1) * kWideBuf + r16 * kWidePitch + 16 * rho;
+                w4_mul<MT, NT, GPT, v, HALF>(ring[v % U], scales, un, [&](int m, int s) {
+                    return *reinterpret_cast<const u32x4_t*>(x + 16 * m * kWidePitch + 64 * s);
+                }, acc);
+                __builtin_amdgcn_sched_barrier(0);
+                load_w(kt + v + U, v % U);
+                __builtin_amdgcn_sched_barrier(0);
+                __syncthreads();
+            }
+        });
+    }
+    const int cols = SWIGLU ? g.w.part_rows : g.w.N;
+    const __amdgpu_buffer_rsrc_t cres =
+        __builtin_amdgcn_make_buffer_rsrc((void*)(g.c + t.s0 * cols), (short)0, t.rows * cols * 2, kBufDword3);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int row = 16 * i + r16;
+        float scale = 1.0f;
+        if (g.row_scale) scale = g.row_scale[t.s0 + min(row, t.rows - 1)];
+#pragma unroll
+        for (int j = 0; j < (SWIGLU ? 1 : NSB); ++j) {
+            const int b = b0 + j;
+            if (b >= (SWIGLU ? twin : g.w.sbs)) break;
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                v[k] = acc[2 * j + k / 4][i][k % 4];
+                if constexpr (SWIGLU) v[k] = (v[k] * sigmoid(v[k])) * acc[2 + k / 4][i][k % 4];
+                else if (g.row_scale) v[k] *= scale;
+            }
+            store_pair16(v, cres, row < t.rows, (uint32_t)row * (uint32_t)cols, g.w.row0(b), g.w.row0(b) + g.w.rows(b), rho);
+        }
+    }
+}
+
+// Inclusive sums along the wave, with DPP moves only.
+__device__ __forceinline__ int wave_scan_dpp(int v)
+{
+    v += (int)dpp_mov_u32<0x111>((uint32_t)v);        // row_shr:1
+    v += (int)dpp_mov_u32<0x112>((uint32_t)v);
+    v += (int)dpp_mov_u32<0x114>((uint32_t)v);
+    v += (int)dpp_mov_u32<0x118>((uint32_t)v);
+    v += (int)dpp_mov_u32<0x142, 0xA>((uint32_t)v);   // row_bcast:15 into rows 1 and 3
+    v += (int)dpp_mov_u32<0x143, 0xC>((uint32_t)v);   // row_bcast:31 into rows 2 and 3
+    return v;
+}
+
+// Slot tile `at` of 1 << LOG slots, counted over the experts' slots: its
+// expert, first slot and slots.  False past the last.  Every wave for itself
+// (E loads, 64 at a time): no barrier before the first weight is asked for.
+template <int LOG>
+__device__ __forceinline__ bool find_slots(const W4Args& g, int at, W4Tile& t)
+{
+    if (!g.expert_offsets) {
+        t.e = 0;
+        t.s0 = (int64_t)at << LOG;
+        t.rows = (int)min<int64_t>(g.cap - t.s0, 1 << LOG);
+        return t.rows > 0;
+    }
+    const int lane = lane_id(), E = g.w.E, cap = (int)g.cap;
+    int before = 0;
+    for (int e0 = 0; e0 < E; e0 += kWave) {
+        const int e = e0 + lane;
+        const int lo = min(g.expert_offsets[min(e, E)], cap), hi = min(g.expert_offsets[min(e + 1, E)], cap);
+        const int n = max(hi - lo, 0);
+        const int tiles = (n + (1 << LOG) - 1) >> LOG;
+        const int upto = wave_scan_dpp(tiles) + before;
+        const uint64_t past = __ballot(upto > at);
+        if (past) {
+            const int who = __builtin_ctzll(past);
+            const int in = at - __builtin_amdgcn_readlane(upto - tiles, who);
+            t.e = e0 + who;
+            t.s0 = __builtin_amdgcn_readlane(lo, who) + (in << LOG);
+            t.rows = min(__builtin_amdgcn_readlane(n, who) - (in << LOG), 1 << LOG);
+            return true;
+        }
+        before = __builtin_amdgcn_readlane(upto, kWave - 1);
+    }
+    return false;
+}
+
+// Tile q of the wide kernel: an expert's slot tiles (64 slots) times nb blocks
+// of weight rows, the slot tile the faster.  q below the count.
+__device__ __forceinline__ void find_tile(const W4Args& g, uint32_t q, uint32_t nb, W4Tile& t)
+{
+    constexpr int LOG = 6;
+    const int lane = lane_id(), E = g.w.E, cap = (int)g.cap;
+    int first = 0, n = cap, before = 0;
+    t.e = 0;
+    if (g.expert_offsets) {
         for (int e0 = 0; e0 < E; e0 += kWave) {
             const int e = e0 + lane;
-            int n = 0;
-            if (e < E) {
-                const int64_t lo = g.expert_offsets ? min<int64_t>(g.expert_offsets[e], g.cap) : 0;
-                const int64_t hi = g.expert_offsets ? min<int64_t>(g.expert_offsets[e + 1], g.cap) : g.cap;
-                eoff[e] = (int32_t)lo;
-                eoff[e + 1] = (int32_t)hi;   // (the next expert's lo)
-                n = (int)((max<int64_t>(0, hi - lo) + kRows - 1) / kRows);
+            const int lo = min(g.expert_offsets[min(e, E)], cap), hi = min(g.expert_offsets[min(e + 1, E)], cap);
+            const int rows = max(hi - lo, 0), tiles = (rows + (1 << LOG) - 1) >> LOG;
+            const int upto = wave_scan_dpp(tiles) + before;
+            const uint64_t past = __ballot((uint32_t)upto * nb > q);
+            if (past) {
+                const int who = __builtin_ctzll(past);
+                t.e = e0 + who;
+                first = __builtin_amdgcn_readlane(lo, who);
+                n = __builtin_amdgcn_readlane(rows, who);
+                before = __builtin_amdgcn_readlane(upto - tiles, who);
+                break;
             }
-            const int inc = wave_incl_scan(n) + carry;
-            if (e < E) ptile[e + 1] = inc;
-            carry = __shfl(inc, kWave - 1, kWave);
+            before = __builtin_amdgcn_readlane(upto, kWave - 1);
         }
-        if (lane == 0) ptile[0] = 0;
     }
-    __syncthreads();
+    const uint32_t in = q - (uint32_t)before * nb, mine = (uint32_t)(n + (1 << LOG) - 1) >> LOG;
+    const int at = (int)(in % mine) << LOG;
+    t.b = (int)(in / mine);
+    t.s0 = first + at;
+    t.rows = min(n - at, 1 << LOG);
+}
+
+template <bool SWIGLU, int MT, int NSB, int GPT, bool HALF, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave, WAVES > 8 ? 4 : 2) void w4_gemm_kernel(W4Args g)
+{
+    constexpr int LOG = MT == 1 ? 4 : MT == 2 ? 5 : 6;
+    __shared__ __attribute__((aligned(16))) float lds[WAVES * 2 * NSB * MT * 4 * kWave];
     // units of superblocks: pairs of twins for SwiGLU, NSB side by side else
-    const int nb = SWIGLU ? g.w.part_sbs() : (g.w.sbs() + NSB - 1) / NSB;
-    const int64_t Q = (int64_t)__builtin_amdgcn_readfirstlane(ptile[E]) * nb;
-    const int64_t per = (Q + 7) / 8;
-    const int nloc = (int)(gridDim.x >> 3);
-    for (int64_t l = blockIdx.x >> 3; l < per; l += nloc) {
-        // XCD x (blocks b % 8 = x) takes a contiguous range; an expert's slot tiles are innermost
-        const int64_t q = (int64_t)(blockIdx.x & 7) * per + l;
-        if (q >= Q) break;
-        int lo = 0, hi = E;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (ptile[mid] <= q / nb) lo = mid;
-            else hi = mid;
-        }
+    const uint32_t nb = (uint32_t)(SWIGLU ? g.w.part_sbs : (g.w.sbs + NSB - 1) / NSB);
+    for (uint32_t q = blockIdx.x;; q += gridDim.x) {
         W4Tile t;
-        t.e = __builtin_amdgcn_readfirstlane(lo);
-        const int p0 = __builtin_amdgcn_readfirstlane(ptile[t.e]);
-        const int mte = __builtin_amdgcn_readfirstlane(ptile[t.e + 1]) - p0;
-        const int qq = (int)(q - (int64_t)p0 * nb);
-        const int first = __builtin_amdgcn_readfirstlane(eoff[t.e]);
-        const int end = __builtin_amdgcn_readfirstlane(eoff[t.e + 1]);
-        t.s0 = first + (int64_t)(qq % mte) * kRows;
-        t.rows = min(kRows, end - (int)t.s0);
-        t.b = qq / mte * (SWIGLU ? 1 : NSB);
+        if (!find_slots<LOG>(g, (int)(q / nb), t)) break;
+        // (uniform as they are, but the compiler has to know)
+        t.e = __builtin_amdgcn_readfirstlane(t.e);
+        t.s0 = __builtin_amdgcn_readfirstlane((int)t.s0);
+        t.rows = __builtin_amdgcn_readfirstlane(t.rows);
+        t.b = (int)(q % nb) * (SWIGLU ? 1 : NSB);
         w4_tile<SWIGLU, MT, NSB, GPT, HALF, WAVES>(g, t, lds);
     }
 }
 
+// Slot tiles of 1 << LOG slots of all experts.
+template <int LOG>
+__device__ __forceinline__ int count_slots(const W4Args& g)
+{
+    const int E = g.w.E, cap = (int)g.cap;
+    if (!g.expert_offsets) return (cap + (1 << LOG) - 1) >> LOG;
+    int tiles = 0;
+    for (int e = lane_id(); e < E; e += kWave)
+        tiles += (max(min(g.expert_offsets[e + 1], cap) - min(g.expert_offsets[e], cap), 0) + (1 << LOG) - 1) >> LOG;
+    return __builtin_amdgcn_readlane(wave_scan_dpp(tiles), kWave - 1);
+}
+
+template <bool SWIGLU, int GPT, bool HALF>
+__global__ __launch_bounds__(kWideWaves * kWave, 2) void w4_wide_kernel(W4Args g)
+{
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * kWideBuf];
+    constexpr int kSbs = kWideWaves * (SWIGLU ? 1 : 2);      // superblocks of a tile (SwiGLU: of the gate part)
+    const uint32_t nb = (uint32_t)(((SWIGLU ? g.w.part_sbs : g.w.sbs) + kSbs - 1) / kSbs);
+    // XCD x (blocks b % 8 = x) takes a contiguous range of tiles, an expert's
+    // slot tiles innermost, so that they read its weight through the same L2
+    const uint32_t Q = (uint32_t)__builtin_amdgcn_readfirstlane(count_slots<6>(g)) * nb;
+    const uint32_t per = (Q + 7) / 8;
+    for (uint32_t l = blockIdx.x >> 3; l < per; l += gridDim.x >> 3) {
+        const uint32_t q = (blockIdx.x & 7) * per + l;
+        if (q >= Q) break;
+        W4Tile t;
+        find_tile(g, q, nb, t);
+        t.e = __builtin_amdgcn_readfirstlane(t.e);
+        t.s0 = __builtin_amdgcn_readfirstlane((int)t.s0);
+        t.rows = __builtin_amdgcn_readfirstlane(t.rows);
+        t.b = __builtin_amdgcn_readfirstlane(t.b) * kSbs;
+        __syncthreads();        // (the last tile's reads of LDS)
+        if (t.rows <= 16) w4_wide_tile<SWIGLU, 1, GPT, HALF>(g, t, lds);
+        else if (t.rows <= 32) w4_wide_tile<SWIGLU, 2, GPT, HALF>(g, t, lds);
+        else w4_wide_tile<SWIGLU, 4, GPT, HALF>(g, t, lds);
+    }
+}
+
+#ifndef V_WAVES
+#define V_WAVES 4
+#define V_NSB 2
+#define V_BPC 4
+#endif
 template <bool SWIGLU, int MT, bool HALF>
 int launch_w4(const W4Args& g, int cus, hipStream_t s)
 {
-    constexpr int WAVES = 4, NSB = 2;
-    const int64_t nb = SWIGLU ? g.w.part_sbs() : (g.w.sbs() + NSB - 1) / NSB;
+    constexpr int WAVES = V_WAVES, NSB = SWIGLU ? 2 : V_NSB;
+    const int64_t nb = SWIGLU ? g.w.part_sbs : (g.w.sbs + NSB - 1) / NSB;
     const int64_t tiles = std::min<int64_t>(g.cap, g.cap / (16 * MT) + g.w.E);
-    const int64_t blocks = std::min<int64_t>(tiles * nb, (int64_t)cus * 4);
-    const dim3 grid((unsigned)(8 * ((blocks + 7) / 8))), block(WAVES * kWave);
+    const int64_t blocks = std::min<int64_t>(tiles * nb, (int64_t)cus * V_BPC);
+    const dim3 grid((unsigned)blocks), block(WAVES * kWave);
     switch (g.w.gpt()) {
         case 1: w4_gemm_kernel<SWIGLU, MT, NSB, 1, HALF, WAVES><<<grid, block, 0, s>>>(g); break;
         case 2: w4_gemm_kernel<SWIGLU, MT, NSB, 2, HALF, WAVES><<<grid, block, 0, s>>>(g); break;
@@ -431,11 +699,33 @@ int launch_w4(const W4Args& g, int cus, hipStream_t s)
     return check_launch("w4_gemm_kernel");
 }
 
+template <bool SWIGLU, bool HALF>
+int launch_wide(const W4Args& g, int cus, hipStream_t s)
+{
+    constexpr int kSbs = kWideWaves * (SWIGLU ? 1 : 2);
+    const int64_t nb = ((SWIGLU ? g.w.part_sbs : g.w.sbs) + kSbs - 1) / kSbs;
+    const int64_t tiles = std::min<int64_t>(g.cap, g.cap / 64 + g.w.E);
+    const int64_t blocks = std::min<int64_t>(tiles * nb, (int64_t)cus * 2);
+    const dim3 grid((unsigned)(8 * ((blocks + 7) / 8))), block(kWideWaves * kWave);
+    switch (g.w.gpt()) {
+        case 1: w4_wide_kernel<SWIGLU, 1, HALF><<<grid, block, 0, s>>>(g); break;
+        case 2: w4_wide_kernel<SWIGLU, 2, HALF><<<grid, block, 0, s>>>(g); break;
+        default: w4_wide_kernel<SWIGLU, 4, HALF><<<grid, block, 0, s>>>(g); break;
+    }
+    return check_launch("w4_wide_kernel");
+}
+
 template <int MT>
 int launch_w4(bool swiglu, bool half, const W4Args& g, int cus, hipStream_t s)
 {
     if (swiglu) return half ? launch_w4<true, MT, true>(g, cus, s) : launch_w4<true, MT, false>(g, cus, s);
     return half ? launch_w4<false, MT, true>(g, cus, s) : launch_w4<false, MT, false>(g, cus, s);
+}
+
+int launch_wide(bool swiglu, bool half, const W4Args& g, int cus, hipStream_t s)
+{
+    if (swiglu) return half ? launch_wide<true, true>(g, cus, s) : launch_wide<true, false>(g, cus, s);
+    return half ? launch_wide<false, true>(g, cus, s) : launch_wide<false, false>(g, cus, s);
 }
 
 int check_shape(const char* fn, int64_t E, int64_t N, int64_t K, int64_t group, int64_t parts)
@@ -446,18 +736,20 @@ int check_shape(const char* fn, int64_t E, int64_t N, int64_t K, int64_t group, 
     if (N < 8 * parts || N % (8 * parts)) return fail(ET_ERR_INVALID_ARGUMENT, f + ": N must be a positive multiple of 8 for each part");
     if (K < 8 || K % 8 || K >= (int64_t)1 << 22) return fail(ET_ERR_INVALID_ARGUMENT, f + ": K must be a positive multiple of 8 below 2^22");
     if (group != 32 && group != 64 && group != 128) return fail(ET_ERR_INVALID_ARGUMENT, f + ": group must be 32, 64 or 128");
-    if (N >= (int64_t)1 << 24 || N * K >= (int64_t)1 << 31) return fail(ET_ERR_INVALID_ARGUMENT, f + ": N * K must be below 2^31, N below 2^24");
+    if (N >= (int64_t)1 << 22 || N * K >= (int64_t)1 << 31) return fail(ET_ERR_INVALID_ARGUMENT, f + ": N * K must be below 2^31, N below 2^22");
     return ET_OK;
 }
 
 W4Shape shape_of(int64_t E, int64_t N, int64_t K, int64_t group, int64_t parts)
 {
-    return W4Shape{(int)E, (int)N, (int)K, (int)parts, (int)group};
+    const int rows = (int)(N / parts), part_sbs = (rows + kSb - 1) / kSb;
+    return W4Shape{(int)E, (int)N, (int)K, (int)parts, (int)group, rows, part_sbs, (int)parts * part_sbs,
+                   (int)((K + kKt - 1) / kKt)};
 }
 
 int blocks_of(const char* fn, const W4Shape& w, unsigned& blocks)
 {
-    const int64_t n = (int64_t)w.E * w.sbs() * w.kts();
+    const int64_t n = (int64_t)w.E * w.sbs * w.kts;
     if (n >= (int64_t)1 << 31) return fail(ET_ERR_INVALID_ARGUMENT, std::string(fn) + ": the weight is too large");
     blocks = (unsigned)n;
     return ET_OK;
@@ -618,10 +910,17 @@ extern "C" int et_expert_gemm_w4_impl(const void* a, int64_t a_rows, const int32
              (uint16_t*)c, epilogue == EPI_ROW_SCALE ? row_scale : nullptr, a_rows, slot_capacity,
              shape_of(num_experts, N, K, group, parts)};
     const bool swiglu = epilogue == EPI_SWIGLU, half = scale_type == ET_W4_SCALE_F16;
+    // (tiles are counted in 32 bits: 16 slots by 32 rows at the least)
+    if ((slot_capacity / 16 + num_experts + 1) * (int64_t)g.w.sbs >= (int64_t)1 << 31)
+        return fail(ET_ERR_INVALID_ARGUMENT, "et_expert_gemm_w4: slot_capacity times N is too large");
     const int cus = cus_of_device();
     const int64_t most = std::min(max_slots, slot_capacity);
     if (most <= 16) return launch_w4<1>(swiglu, half, g, cus, (hipStream_t)stream);
+#ifdef V_NOWIDE
     return launch_w4<2>(swiglu, half, g, cus, (hipStream_t)stream);
+#else
+    return launch_wide(swiglu, half, g, cus, (hipStream_t)stream);
+#endif
 }
 
 extern "C" int et_expert_gemm_w4(const void* a, int64_t a_rows, const int32_t* sorted_token, const void* packed,

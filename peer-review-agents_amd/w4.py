@@ -47,8 +47,8 @@ def _check_sizes(E: int, N: int, K: int, group: int, parts: int) -> None:
         raise ValueError(f"K must be a positive multiple of 8 below 2^22, got {K}")
     if group not in _GROUPS:
         raise ValueError(f"group must be one of {_GROUPS}, got {group}")
-    if N * K >= 1 << 31 or N >= 1 << 24:
-        raise ValueError("N * K must be below 2^31 and N below 2^24")
+    if N * K >= 1 << 31 or N >= 1 << 22:
+        raise ValueError("N * K must be below 2^31 and N below 2^22")
 
 
 def quantize_w4(w: torch.Tensor, *, group: int = 128,
