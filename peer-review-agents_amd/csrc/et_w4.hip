@@ -195,6 +195,7 @@ struct W4Args {
     const float* row_scale;
     int64_t a_rows, cap;
     W4Shape w;
+    bool half;                      // scales f16, else bf16
 };
 
 struct W4Tile {
@@ -234,24 +235,32 @@ struct Unpack {
 // group, the same 64 bytes in all of a row's lanes, they cost 8 to 13% of a
 // call of 4 to 16 tokens.)
 constexpr int kTurns = 4;
-template <int NSB, bool HALF>
+template <int NSB>
 struct Scales {
     u32x4_t raw[NSB];
     float f[NSB][8];
-    __device__ __forceinline__ void convert()
+    __device__ __forceinline__ void convert(bool half)
     {
+        // (a branch of the whole grid: each way 8 instructions for 4 turns)
+        if (half) {
 #pragma unroll
-        for (int j = 0; j < NSB; ++j)
+            for (int j = 0; j < NSB; ++j)
 #pragma unroll
-            for (int k = 0; k < 8; ++k) f[j][k] = scale16(k & 1 ? raw[j][k / 2] >> 16 : raw[j][k / 2] & 0xFFFFu, HALF);
+                for (int k = 0; k < 8; ++k) f[j][k] = scale16(raw[j][k / 2] >> (16 * (k & 1)) & 0xFFFFu, true);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NSB; ++j)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) f[j][k] = k & 1 ? bf16hi(raw[j][k / 2]) : bf16lo(raw[j][k / 2]);
+        }
     }
 };
 
 // acc += one k range of 128 of NT tiles (two to a superblock) by MT tiles of 16
 // slots; a(i, s) is the fragment of slots 16 i.. at k-step s, TURN the place of
 // the range among those that the scales at hand are for.
-template <int MT, int NT, int GPT, int TURN, bool HALF, typename A>
-__device__ __forceinline__ void w4_mul(const u32x4_t (&w)[NT], const Scales<NT / 2, HALF>& scales, const Unpack& un, A a,
+template <int MT, int NT, int GPT, int TURN, typename A>
+__device__ __forceinline__ void w4_mul(const u32x4_t (&w)[NT], const Scales<NT / 2>& scales, const Unpack& un, A a,
                                        f32x4_t (&acc)[NT][MT])
 {
     constexpr int SPG = 4 / GPT;
@@ -337,13 +346,14 @@ struct W4Acts {
     }
 };
 
-// One block's tile: 16 MT slots x NSB superblocks (SwiGLU: one of the gate
-// part, its twin of the up part), the k range dealt to the block's waves one
-// 128 at a time, their sums joined through LDS in the waves' order.
-template <bool SWIGLU, int MT, int NSB, int GPT, bool HALF, int WAVES>
-__device__ __forceinline__ void w4_tile(const W4Args& g, const W4Tile& t, float* lds)
+// Tiles of few slots: 16 slots x NSB superblocks (SwiGLU: one of the gate part,
+// its twin of the up part) to a block, the k range dealt to the block's waves
+// one 128 at a time, their sums joined through LDS in the waves' order.
+template <bool SWIGLU, int NSB, int GPT, int WAVES>
+__device__ __forceinline__ void w4_split_tile(const W4Args& g, const W4Tile& t, float* lds)
 {
-    constexpr int NT = 2 * NSB, U = 2;
+    constexpr int NT = 2 * NSB, U = 2, MT = 1;
+    const bool half = g.half;
     const int lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
     const int r16 = lane & 15, rho = lane >> 4;
@@ -352,14 +362,12 @@ __device__ __forceinline__ void w4_tile(const W4Args& g, const W4Tile& t, float*
 #pragma unroll
     for (int j = 0; j < NSB; ++j) rows[j] = W4Rows(g, t.e, t.b + (SWIGLU ? j * twin : j), GPT);
     const W4Acts acts(g, t);
-    uint32_t ao[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) ao[i] = acts.row(g, t, 16 * i + r16);
+    const uint32_t ao = acts.row(g, t, r16);
     // (kts of this wave: wave, wave + WAVES, ...; loads past the last repeat it)
     const int n = (kts - wave + WAVES - 1) / WAVES;
     const auto kt_of = [&](int i) { return wave + WAVES * min(i, n - 1); };
     struct Step {
-        u32x4_t w[NT], a[MT][4];
+        u32x4_t w[NT], a[4];
     } ring[U];
     const auto load = [&](Step& x, int i) {
         const int kt = kt_of(i);
@@ -368,11 +376,9 @@ __device__ __forceinline__ void w4_tile(const W4Args& g, const W4Tile& t, float*
         for (int j = 0; j < NT; ++j)
             x.w[j] = *reinterpret_cast<const u32x4_t*>(rows[j / 2].w + at + (j & 1) * kTileBytes + 16 * lane);
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
-#pragma unroll
-            for (int m = 0; m < MT; ++m) x.a[m][s] = acts.load(ao[m], kt * kKt, 32 * s + 8 * rho, K);
+        for (int s = 0; s < 4; ++s) x.a[s] = acts.load(ao, kt * kKt, 32 * s + 8 * rho, K);
     };
-    Scales<NSB, HALF> scales;
+    Scales<NSB> scales;
     const auto load_scales = [&](int i) {
         const int at = (kt_of(i + min(r16 / GPT, kTurns - 1)) * GPT + r16 % GPT) * kSb + 8 * rho;
 #pragma unroll
@@ -380,53 +386,48 @@ __device__ __forceinline__ void w4_tile(const W4Args& g, const W4Tile& t, float*
     };
     f32x4_t acc[NT][MT];
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) acc[j][i] = f32x4_t{};
+    for (int j = 0; j < NT; ++j) acc[j][0] = f32x4_t{};
     const Unpack un;
     if (n > 0) {
         load_scales(0);
 #pragma unroll
         for (int u = 0; u < U; ++u) load(ring[u], u);
         for (int i = 0; i < n; i += kTurns) {
-            scales.convert();
+            scales.convert(half);
             load_scales(i + kTurns);
             constants(std::make_integer_sequence<int, kTurns>{}, [&](auto turn) {
                 constexpr int v = decltype(turn)::value;
                 const Step& x = ring[v % U];
-                if (i + v < n) w4_mul<MT, NT, GPT, v, HALF>(x.w, scales, un, [&](int m, int s) { return x.a[m][s]; }, acc);
+                if (i + v < n) w4_mul<MT, NT, GPT, v>(x.w, scales, un, [&](int, int s) { return x.a[s]; }, acc);
                 __builtin_amdgcn_sched_barrier(0);
                 load(ring[v % U], i + v + U);
                 __builtin_amdgcn_sched_barrier(0);
             });
         }
     }
-    // the waves' sums, in order: wave w takes output units w, w + WAVES, ...
+    // the waves' sums, in order: wave w takes tiles w, w + WAVES, ...
 #pragma unroll
     for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-            *reinterpret_cast<f32x4_t*>(lds + ((wave * NT + j) * MT + i) * 4 * kWave + 4 * lane) = acc[j][i];
+        *reinterpret_cast<f32x4_t*>(lds + (wave * NT + j) * 4 * kWave + 4 * lane) = acc[j][0];
     __syncthreads();
-    const auto total = [&](int j, int i) {
+    const auto total = [&](int j) {
         f32x4_t s = {};
 #pragma unroll
-        for (int v = 0; v < WAVES; ++v) s += *reinterpret_cast<const f32x4_t*>(lds + ((v * NT + j) * MT + i) * 4 * kWave + 4 * lane);
+        for (int v = 0; v < WAVES; ++v) s += *reinterpret_cast<const f32x4_t*>(lds + (v * NT + j) * 4 * kWave + 4 * lane);
         return s;
     };
     const int cols = SWIGLU ? g.w.part_rows : g.w.N;
-    for (int unit = wave; unit < (SWIGLU ? 2 : NT) * MT; unit += WAVES) {
-        const int j = unit / MT, i = unit % MT;
-        const int b = t.b + j / 2, row = 16 * i + r16, in = 16 * (j & 1) + 4 * rho;
-        f32x4_t v = total(j, i);
+    for (int j = wave; j < (SWIGLU ? 2 : NT); j += WAVES) {
+        const int b = t.b + j / 2, in = 16 * (j & 1) + 4 * rho;
+        f32x4_t v = total(j);
         if constexpr (SWIGLU) {
-            const f32x4_t up = total(j + 2, i);
+            const f32x4_t up = total(j + 2);
 #pragma unroll
             for (int k = 0; k < 4; ++k) v[k] = (v[k] * sigmoid(v[k])) * up[k];
         }
-        if (b >= (SWIGLU ? twin : g.w.sbs) || row >= t.rows || in >= g.w.rows(b)) continue;
-        if (g.row_scale) v *= g.row_scale[t.s0 + row];
-        *reinterpret_cast<u32x2_t*>(g.c + (t.s0 + row) * cols + g.w.row0(b) + in) =
+        if (b >= (SWIGLU ? twin : g.w.sbs) || r16 >= t.rows || in >= g.w.rows(b)) continue;
+        if (g.row_scale) v *= g.row_scale[t.s0 + r16];
+        *reinterpret_cast<u32x2_t*>(g.c + (t.s0 + r16) * cols + g.w.row0(b) + in) =
             u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
     }
     __syncthreads();
@@ -439,12 +440,14 @@ __device__ __forceinline__ void w4_tile(const W4Args& g, const W4Tile& t, float*
 // bytes at 32 and 64 slots.
 constexpr int kWideWaves = 4;
 constexpr int kWidePitch = 2 * kKt + 16;               // bytes of a row of A in LDS
-constexpr int kWideBuf = 64 * kWidePitch;
+// MAXMT tiles of 16 slots at most: 32 or 64 slots
+constexpr int wide_buf(int maxmt) { return 16 * maxmt * kWidePitch; }
 
-template <bool SWIGLU, int MT, int GPT, bool HALF>
+template <bool SWIGLU, int MT, int MAXMT, int GPT>
 __device__ __forceinline__ void w4_wide_tile(const W4Args& g, const W4Tile& t, unsigned char* lds)
 {
-    constexpr int NSB = 2, NT = 4, U = 2;
+    constexpr int NSB = 2, NT = 4, U = 2, kBuf = wide_buf(MAXMT);
+    const bool half = g.half;
     const int lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
     const int r16 = lane & 15, rho = lane >> 4;
@@ -460,7 +463,7 @@ __device__ __forceinline__ void w4_wide_tile(const W4Args& g, const W4Tile& t, u
         for (int j = 0; j < NT; ++j)
             ring[u][j] = *reinterpret_cast<const u32x4_t*>(rows[j / 2].w + at + (j & 1) * kTileBytes + 16 * lane);
     };
-    Scales<NSB, HALF> scales;
+    Scales<NSB> scales;
     const auto load_scales = [&](int kt) {
         const int at = (min(kt + min(r16 / GPT, kTurns - 1), kts - 1) * GPT + r16 % GPT) * kSb + 8 * rho;
 #pragma unroll
@@ -484,7 +487,7 @@ __device__ __forceinline__ void w4_wide_tile(const W4Args& g, const W4Tile& t, u
     const auto store_a = [&](int b) {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
-            *reinterpret_cast<u32x4_t*>(lds + b * kWideBuf + (16 * m + sr) * kWidePitch + 16 * seg) = stage[m];
+            *reinterpret_cast<u32x4_t*>(lds + b * kBuf + (16 * m + sr) * kWidePitch + 16 * seg) = stage[m];
     };
     f32x4_t acc[NT][MT];
 #pragma unroll
@@ -497,7 +500,7 @@ __device__ __forceinline__ void w4_wide_tile(const W4Args& g, const W4Tile& t, u
     load_a(1);
     __syncthreads();
     for (int kt = 0; kt < kts; kt += kTurns) {
-        scales.convert();
+        scales.convert(half);
         load_scales(kt + kTurns);
         constants(std::make_integer_sequence<int, kTurns>{}, [&](auto turn) {
             constexpr int v = decltype(turn)::value;
@@ -507,8 +510,8 @@ __device__ __forceinline__ void w4_wide_tile(const W4Args& g, const W4Tile& t, u
                 store_a((v & 1) ^ 1);
                 load_a(kt + v + 2);
                 __builtin_amdgcn_sched_barrier(0);
-                const unsigned char* const x = lds + (v & 1) * kWideBuf + r16 * kWidePitch + 16 * rho;
-                w4_mul<MT, NT, GPT, v, HALF>(ring[v % U], scales, un, [&](int m, int s) {
+                const unsigned char* const x = lds + (v & 1) * kBuf + r16 * kWidePitch + 16 * rho;
+                w4_mul<MT, NT, GPT, v>(ring[v % U], scales, un, [&](int m, int s) {
                     return *reinterpret_cast<const u32x4_t*>(x + 16 * m * kWidePitch + 64 * s);
                 }, acc);
                 __builtin_amdgcn_sched_barrier(0);
@@ -588,11 +591,12 @@ __device__ __forceinline__ bool find_slots(const W4Args& g, int at, W4Tile& t)
     return false;
 }
 
-// Tile q of the wide kernel: an expert's slot tiles (64 slots) times nb blocks
-// of weight rows, the slot tile the faster.  q below the count.
+// Tile q of the wide kernel: an expert's slot tiles (1 << LOG slots at most, the
+// expert's slots dealt evenly in sixteens) times nb blocks of weight rows, the
+// slot tile the faster.  q below the count.
+template <int LOG>
 __device__ __forceinline__ void find_tile(const W4Args& g, uint32_t q, uint32_t nb, W4Tile& t)
 {
-    constexpr int LOG = 6;
     const int lane = lane_id(), E = g.w.E, cap = (int)g.cap;
     int first = 0, n = cap, before = 0;
     t.e = 0;
@@ -615,17 +619,18 @@ __device__ __forceinline__ void find_tile(const W4Args& g, uint32_t q, uint32_t 
         }
     }
     const uint32_t in = q - (uint32_t)before * nb, mine = (uint32_t)(n + (1 << LOG) - 1) >> LOG;
-    const int at = (int)(in % mine) << LOG;
+    const int share = (int)(((uint32_t)(n + 15) / 16 + mine - 1) / mine) * 16;
+    const int at = (int)(in % mine) * share;
     t.b = (int)(in / mine);
     t.s0 = first + at;
-    t.rows = min(n - at, 1 << LOG);
+    t.rows = min(n - at, share);
 }
 
-template <bool SWIGLU, int MT, int NSB, int GPT, bool HALF, int WAVES>
-__global__ __launch_bounds__(WAVES * kWave, WAVES > 8 ? 4 : 2) void w4_gemm_kernel(W4Args g)
+template <bool SWIGLU, int NSB, int GPT, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave, 2) void w4_split_kernel(W4Args g)
 {
-    constexpr int LOG = MT == 1 ? 4 : MT == 2 ? 5 : 6;
-    __shared__ __attribute__((aligned(16))) float lds[WAVES * 2 * NSB * MT * 4 * kWave];
+    constexpr int LOG = 4;
+    __shared__ __attribute__((aligned(16))) float lds[WAVES * 2 * NSB * 4 * kWave];
     // units of superblocks: pairs of twins for SwiGLU, NSB side by side else
     const uint32_t nb = (uint32_t)(SWIGLU ? g.w.part_sbs : (g.w.sbs + NSB - 1) / NSB);
     for (uint32_t q = blockIdx.x;; q += gridDim.x) {
@@ -636,7 +641,7 @@ __global__ __launch_bounds__(WAVES * kWave, WAVES > 8 ? 4 : 2) void w4_gemm_kern
         t.s0 = __builtin_amdgcn_readfirstlane((int)t.s0);
         t.rows = __builtin_amdgcn_readfirstlane(t.rows);
         t.b = (int)(q % nb) * (SWIGLU ? 1 : NSB);
-        w4_tile<SWIGLU, MT, NSB, GPT, HALF, WAVES>(g, t, lds);
+        w4_split_tile<SWIGLU, NSB, GPT, WAVES>(g, t, lds);
     }
 }
 
@@ -652,80 +657,137 @@ __device__ __forceinline__ int count_slots(const W4Args& g)
     return __builtin_amdgcn_readlane(wave_scan_dpp(tiles), kWave - 1);
 }
 
-template <bool SWIGLU, int GPT, bool HALF>
-__global__ __launch_bounds__(kWideWaves * kWave, 2) void w4_wide_kernel(W4Args g)
+// Blocks of the wide kernel to a CU: 168 registers allow three of those with
+// 32 slots, whose time is the weight's stream (61 tokens, 32 experts, K = 2048,
+// N = 7168, groups of 32: 60.5 us against 65.6 with two).
+constexpr int wide_blocks(int maxmt) { return maxmt == 2 ? 3 : 2; }
+
+template <bool SWIGLU, int MAXMT, int GPT>
+__global__ __launch_bounds__(kWideWaves * kWave, wide_blocks(MAXMT)) void w4_wide_kernel(W4Args g)
 {
-    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * kWideBuf];
+    constexpr int LOG = MAXMT == 2 ? 5 : 6;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * wide_buf(MAXMT)];
     constexpr int kSbs = kWideWaves * (SWIGLU ? 1 : 2);      // superblocks of a tile (SwiGLU: of the gate part)
     const uint32_t nb = (uint32_t)(((SWIGLU ? g.w.part_sbs : g.w.sbs) + kSbs - 1) / kSbs);
     // XCD x (blocks b % 8 = x) takes a contiguous range of tiles, an expert's
     // slot tiles innermost, so that they read its weight through the same L2
-    const uint32_t Q = (uint32_t)__builtin_amdgcn_readfirstlane(count_slots<6>(g)) * nb;
+    const uint32_t Q = (uint32_t)__builtin_amdgcn_readfirstlane(count_slots<LOG>(g)) * nb;
     const uint32_t per = (Q + 7) / 8;
     for (uint32_t l = blockIdx.x >> 3; l < per; l += gridDim.x >> 3) {
         const uint32_t q = (blockIdx.x & 7) * per + l;
         if (q >= Q) break;
         W4Tile t;
-        find_tile(g, q, nb, t);
+        find_tile<LOG>(g, q, nb, t);
         t.e = __builtin_amdgcn_readfirstlane(t.e);
         t.s0 = __builtin_amdgcn_readfirstlane((int)t.s0);
         t.rows = __builtin_amdgcn_readfirstlane(t.rows);
         t.b = __builtin_amdgcn_readfirstlane(t.b) * kSbs;
         __syncthreads();        // (the last tile's reads of LDS)
-        if (t.rows <= 16) w4_wide_tile<SWIGLU, 1, GPT, HALF>(g, t, lds);
-        else if (t.rows <= 32) w4_wide_tile<SWIGLU, 2, GPT, HALF>(g, t, lds);
-        else w4_wide_tile<SWIGLU, 4, GPT, HALF>(g, t, lds);
+        if (t.rows <= 16) {
+            w4_wide_tile<SWIGLU, 1, MAXMT, GPT>(g, t, lds);
+        } else if (MAXMT == 2 || t.rows <= 32) {
+            w4_wide_tile<SWIGLU, 2, MAXMT, GPT>(g, t, lds);
+        } else if constexpr (MAXMT == 4) {
+            if (t.rows <= 48) w4_wide_tile<SWIGLU, 3, MAXMT, GPT>(g, t, lds);
+            else w4_wide_tile<SWIGLU, 4, MAXMT, GPT>(g, t, lds);
+        }
     }
 }
 
-#ifndef V_WAVES
-#define V_WAVES 4
-#define V_NSB 2
-#define V_BPC 4
-#endif
-template <bool SWIGLU, int MT, bool HALF>
-int launch_w4(const W4Args& g, int cus, hipStream_t s)
+// What the host knows of a call, and what follows from it.
+struct W4Load {
+    int64_t busy, mean;    // experts with slots, and slots of one, as far as the capacity tells
+    int64_t cus;
+};
+
+// Units of the split kernel: 64 weight rows (SwiGLU: 32 hidden units) by 16
+// slots; tiles of the wide one: 256 weight rows by 32 slots.  A mean of n slots
+// makes about n / 16 + 1/2 slot tiles of 16.
+int64_t split_units(const W4Args& g, bool swiglu, const W4Load& l)
 {
-    constexpr int WAVES = V_WAVES, NSB = SWIGLU ? 2 : V_NSB;
-    const int64_t nb = SWIGLU ? g.w.part_sbs : (g.w.sbs + NSB - 1) / NSB;
-    const int64_t tiles = std::min<int64_t>(g.cap, g.cap / (16 * MT) + g.w.E);
-    const int64_t blocks = std::min<int64_t>(tiles * nb, (int64_t)cus * V_BPC);
-    const dim3 grid((unsigned)blocks), block(WAVES * kWave);
-    switch (g.w.gpt()) {
-        case 1: w4_gemm_kernel<SWIGLU, MT, NSB, 1, HALF, WAVES><<<grid, block, 0, s>>>(g); break;
-        case 2: w4_gemm_kernel<SWIGLU, MT, NSB, 2, HALF, WAVES><<<grid, block, 0, s>>>(g); break;
-        default: w4_gemm_kernel<SWIGLU, MT, NSB, 4, HALF, WAVES><<<grid, block, 0, s>>>(g); break;
-    }
-    return check_launch("w4_gemm_kernel");
+    return l.busy * std::max<int64_t>(16, l.mean + 8) * (swiglu ? g.w.part_sbs : (g.w.sbs + 1) / 2) / 16;
 }
 
-template <bool SWIGLU, bool HALF>
+int64_t wide_tiles(const W4Args& g, bool swiglu, const W4Load& l)
+{
+    const int sbs = kWideWaves * (swiglu ? 1 : 2);
+    return l.busy * std::max<int64_t>(32, l.mean + 16) * (((swiglu ? g.w.part_sbs : g.w.sbs) + sbs - 1) / sbs) / 32;
+}
+
+enum W4Route { kSplit4 = 0, kSplit8 = 1, kWide32 = 2, kWide64 = 3 };
+
+// Which kernel a call takes.
+//
+// Split K or lay the waves side by side.  Where the weights' stream is what
+// counts the split kernel is 9% faster up to a mean of 2 slots, they are equal at 4
+// and the wide one is 2 to 27% faster from 6 on (us, split / wide; K = 4096,
+// N = 4096, 128 experts, 17 to 128 tokens: 141 / 155, 177 / 194, 201 / 204, 226 / 208;
+// 32 experts, K = 2048, N = 7168, 24 and 61 tokens: 54 / 53, 79 / 58).  In calls of few
+// tiles a wide one takes 33 us at K = 4096 however few they are, and 768 of them
+// (three to a CU) little more, while 45 units of the split kernel pass in a us:
+// 8 experts, 40 tokens 20 / 34, dense, 48 and 200 tokens: 8.6 / 32, 42 / 33.
+//
+// Eight waves on one superblock where there are then no more blocks than CUs
+// (dense, one token, K = N = 4096: 5.4 us against 7.7 with four waves on two; 48
+// tokens, 384 blocks: 14.4 against 8.6).
+//
+// Slot tiles of 64 where there are many slots and tiles (32 experts of 75 slots,
+// K = 2048, N = 7168: 111 us against 123; up to a mean of 64 equal, in calls of few
+// tiles 35% slower: dense, 64 tokens, K = N = 4096 45 against 33).
+int w4_route(const W4Args& g, bool swiglu, const W4Load& l, int64_t most)
+{
+    const int64_t units = split_units(g, swiglu, l), tiles = wide_tiles(g, swiglu, l);
+    if (most > 16 && l.mean > 4 && units * 3 * l.cus > 1500 * std::max<int64_t>(3 * l.cus, tiles))
+        return l.mean > 64 && tiles >= 4 * l.cus ? kWide64 : kWide32;
+    return 2 * units <= l.cus ? kSplit8 : kSplit4;
+}
+
+template <bool SWIGLU, int NSB, int WAVES>
+int launch_split(const W4Args& g, int cus, hipStream_t s)
+{
+    const int64_t nb = SWIGLU ? g.w.part_sbs : (g.w.sbs + NSB - 1) / NSB;
+    const int64_t tiles = std::min<int64_t>(g.cap, g.cap / 16 + g.w.E);
+    // (12 waves to a CU are what the registers allow)
+    const dim3 grid((unsigned)std::min<int64_t>(tiles * nb, (int64_t)cus * (12 / WAVES))), block(WAVES * kWave);
+    switch (g.w.gpt()) {
+        case 1: w4_split_kernel<SWIGLU, NSB, 1, WAVES><<<grid, block, 0, s>>>(g); break;
+        case 2: w4_split_kernel<SWIGLU, NSB, 2, WAVES><<<grid, block, 0, s>>>(g); break;
+        default: w4_split_kernel<SWIGLU, NSB, 4, WAVES><<<grid, block, 0, s>>>(g); break;
+    }
+    return check_launch("w4_split_kernel");
+}
+
+template <bool SWIGLU, int MAXMT>
 int launch_wide(const W4Args& g, int cus, hipStream_t s)
 {
     constexpr int kSbs = kWideWaves * (SWIGLU ? 1 : 2);
     const int64_t nb = ((SWIGLU ? g.w.part_sbs : g.w.sbs) + kSbs - 1) / kSbs;
-    const int64_t tiles = std::min<int64_t>(g.cap, g.cap / 64 + g.w.E);
-    const int64_t blocks = std::min<int64_t>(tiles * nb, (int64_t)cus * 2);
+    const int64_t tiles = std::min<int64_t>(g.cap, g.cap / (16 * MAXMT) + g.w.E);
+    const int64_t blocks = std::min<int64_t>(tiles * nb, (int64_t)cus * wide_blocks(MAXMT));
     const dim3 grid((unsigned)(8 * ((blocks + 7) / 8))), block(kWideWaves * kWave);
     switch (g.w.gpt()) {
-        case 1: w4_wide_kernel<SWIGLU, 1, HALF><<<grid, block, 0, s>>>(g); break;
-        case 2: w4_wide_kernel<SWIGLU, 2, HALF><<<grid, block, 0, s>>>(g); break;
-        default: w4_wide_kernel<SWIGLU, 4, HALF><<<grid, block, 0, s>>>(g); break;
+        case 1: w4_wide_kernel<SWIGLU, MAXMT, 1><<<grid, block, 0, s>>>(g); break;
+        case 2: w4_wide_kernel<SWIGLU, MAXMT, 2><<<grid, block, 0, s>>>(g); break;
+        default: w4_wide_kernel<SWIGLU, MAXMT, 4><<<grid, block, 0, s>>>(g); break;
     }
     return check_launch("w4_wide_kernel");
 }
 
-template <int MT>
-int launch_w4(bool swiglu, bool half, const W4Args& g, int cus, hipStream_t s)
+template <bool SWIGLU>
+int launch_w4(const W4Args& g, int route, int cus, hipStream_t s)
 {
-    if (swiglu) return half ? launch_w4<true, MT, true>(g, cus, s) : launch_w4<true, MT, false>(g, cus, s);
-    return half ? launch_w4<false, MT, true>(g, cus, s) : launch_w4<false, MT, false>(g, cus, s);
+    switch (route) {
+        case kSplit4: return launch_split<SWIGLU, 2, 4>(g, cus, s);
+        case kSplit8: return launch_split<SWIGLU, SWIGLU ? 2 : 1, 8>(g, cus, s);
+        case kWide32: return launch_wide<SWIGLU, 2>(g, cus, s);
+        default: return launch_wide<SWIGLU, 4>(g, cus, s);
+    }
 }
 
-int launch_wide(bool swiglu, bool half, const W4Args& g, int cus, hipStream_t s)
+W4Load load_of(int64_t num_experts, int64_t slot_capacity, int64_t most, int64_t cus)
 {
-    if (swiglu) return half ? launch_wide<true, true>(g, cus, s) : launch_wide<true, false>(g, cus, s);
-    return half ? launch_wide<false, true>(g, cus, s) : launch_wide<false, false>(g, cus, s);
+    const int64_t busy = std::max<int64_t>(1, std::min(num_experts, slot_capacity));
+    return W4Load{busy, std::min(most, (slot_capacity + busy - 1) / busy), cus};
 }
 
 int check_shape(const char* fn, int64_t E, int64_t N, int64_t K, int64_t group, int64_t parts)
@@ -876,12 +938,23 @@ extern "C" int et_w4_quantize(const void* w, int dtype, int64_t num_experts, int
     return check_launch("w4_quantize_kernel");
 }
 
-// max_slots: slots of one expert at most, as far as the host knows.
+// The kernel that et_expert_gemm_w4_impl takes of itself (W4Route).
+extern "C" int et_w4_route_impl(int64_t num_experts, int64_t K, int64_t N, int64_t group, int64_t parts,
+                                int64_t slot_capacity, int epilogue, int64_t max_slots, int64_t cus)
+{
+    W4Args g = {};
+    g.w = shape_of(num_experts, N, K, group, parts);
+    const int64_t most = std::min(max_slots, slot_capacity);
+    return w4_route(g, epilogue == EPI_SWIGLU, load_of(num_experts, slot_capacity, most, cus), most);
+}
+
+// max_slots: slots of one expert at most, as far as the host knows.  route: a
+// W4Route, or -1 for the one that w4_route says.
 extern "C" int et_expert_gemm_w4_impl(const void* a, int64_t a_rows, const int32_t* sorted_token, const void* packed,
                                       const void* packed_scales, int scale_type, const int32_t* expert_offsets,
                                       int64_t num_experts, int64_t K, int64_t N, int64_t group, int64_t parts,
                                       int64_t slot_capacity, int epilogue, const float* row_scale, void* c,
-                                      int64_t max_slots, void* stream)
+                                      int64_t max_slots, int route, void* stream)
 {
     const char* fn = "et_expert_gemm_w4";
     int rc = check_shape(fn, num_experts, N, K, group, parts);
@@ -908,19 +981,15 @@ extern "C" int et_expert_gemm_w4_impl(const void* a, int64_t a_rows, const int32
     if (rc) return rc;
     W4Args g{(const uint16_t*)a, sorted_token, (const unsigned char*)packed, (const uint16_t*)packed_scales, expert_offsets,
              (uint16_t*)c, epilogue == EPI_ROW_SCALE ? row_scale : nullptr, a_rows, slot_capacity,
-             shape_of(num_experts, N, K, group, parts)};
-    const bool swiglu = epilogue == EPI_SWIGLU, half = scale_type == ET_W4_SCALE_F16;
+             shape_of(num_experts, N, K, group, parts), scale_type == ET_W4_SCALE_F16};
     // (tiles are counted in 32 bits: 16 slots by 32 rows at the least)
     if ((slot_capacity / 16 + num_experts + 1) * (int64_t)g.w.sbs >= (int64_t)1 << 31)
         return fail(ET_ERR_INVALID_ARGUMENT, "et_expert_gemm_w4: slot_capacity times N is too large");
-    const int cus = cus_of_device();
     const int64_t most = std::min(max_slots, slot_capacity);
-    if (most <= 16) return launch_w4<1>(swiglu, half, g, cus, (hipStream_t)stream);
-#ifdef V_NOWIDE
-    return launch_w4<2>(swiglu, half, g, cus, (hipStream_t)stream);
-#else
-    return launch_wide(swiglu, half, g, cus, (hipStream_t)stream);
-#endif
+    const bool swiglu = epilogue == EPI_SWIGLU;
+    const int cus = cus_of_device();
+    if (route < kSplit4 || route > kWide64) route = w4_route(g, swiglu, load_of(num_experts, slot_capacity, most, cus), most);
+    return swiglu ? launch_w4<true>(g, route, cus, (hipStream_t)stream) : launch_w4<false>(g, route, cus, (hipStream_t)stream);
 }
 
 extern "C" int et_expert_gemm_w4(const void* a, int64_t a_rows, const int32_t* sorted_token, const void* packed,
@@ -929,5 +998,5 @@ extern "C" int et_expert_gemm_w4(const void* a, int64_t a_rows, const int32_t* s
                                  int64_t slot_capacity, int epilogue, const float* row_scale, void* c, void* stream)
 {
     return et_expert_gemm_w4_impl(a, a_rows, sorted_token, packed, packed_scales, scale_type, expert_offsets, num_experts, K,
-                                  N, group, parts, slot_capacity, epilogue, row_scale, c, slot_capacity, stream);
+                                  N, group, parts, slot_capacity, epilogue, row_scale, c, slot_capacity, -1, stream);
 }

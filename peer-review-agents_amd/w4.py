@@ -122,7 +122,8 @@ def unpack_w4(w: W4Weight, plan: Optional[RoutingPlan] = None, out: Optional[tor
     return out
 
 
-def _gemm(a, w: W4Weight, rows: int, sorted_token, offsets, epilogue: str, row_scale, out, max_slots: int):
+def _gemm(a, w: W4Weight, rows: int, sorted_token, offsets, epilogue: str, row_scale, out, max_slots: int,
+          route: int = -1):
     dev = a.device
     if epilogue not in _EPILOGUES:
         raise ValueError(f"epilogue must be one of {sorted(_EPILOGUES)}, got {epilogue!r}")
@@ -142,7 +143,7 @@ def _gemm(a, w: W4Weight, rows: int, sorted_token, offsets, epilogue: str, row_s
         raise ValueError("a and out must be 16-byte aligned")
     _call("et_expert_gemm_w4_impl", dev, _vp(a), a.shape[0], sorted_token, _vp(w.packed), _vp(w.scales),
           _SCALE_TYPES[w.scales.dtype], offsets, w.num_experts, w.K, w.N, w.group, w.parts, rows, _EPILOGUES[epilogue],
-          _vp(row_scale) if epilogue == "row_scale" else None, _vp(c), max_slots)
+          _vp(row_scale) if epilogue == "row_scale" else None, _vp(c), max_slots, route)
     return c
 
 

@@ -3,6 +3,8 @@ before any device work."""
 import ctypes
 import importlib
 
+import pytest
+
 ET_ERR_INVALID_ARGUMENT = -1
 ET_ERR_WORKSPACE_TOO_SMALL = -2
 
@@ -140,3 +142,14 @@ def test_w4_rejects_bad_arguments(et):
     assert gemm(cap=-1) == ET_ERR_INVALID_ARGUMENT
     assert gemm(a=ctypes.c_void_p(0x1008)) == ET_ERR_INVALID_ARGUMENT and "aligned" in _err(et)
     assert gemm(cap=0) == 0
+
+
+@pytest.mark.parametrize("E,K,N,swiglu,capacity,most,route", [
+    # (us of the kernels beside each other: see w4_route)
+    (1, 4096, 4096, 0, 1, 1, 1), (1, 7168, 8192, 0, 1, 1, 1), (1, 4096, 4096, 0, 48, 48, 0), (1, 4096, 8192, 0, 200, 200, 2),
+    (128, 4096, 4096, 1, 8, 1, 0), (128, 4096, 4096, 1, 128, 16, 0), (128, 4096, 4096, 1, 256, 32, 0),
+    (128, 4096, 4096, 1, 1024, 128, 2), (32, 2048, 7168, 0, 488, 61, 2), (8, 4096, 4096, 1, 80, 40, 0),
+    (64, 2048, 2816, 1, 4072, 509, 2), (32, 2048, 7168, 0, 2400, 300, 3)])
+def test_w4_kernel_choice(et, E, K, N, swiglu, capacity, most, route):
+    got = et.lib().et_w4_route_impl(E, K, N, 128, 1 + swiglu, capacity, 2 * swiglu, most, 256)
+    assert got == route
