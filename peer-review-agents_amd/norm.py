@@ -8,8 +8,8 @@ from typing import Optional
 
 import torch
 
-from ._lib import ET_DTYPE_F32, ET_MAX_NORM_WIDTH, lib
-from .expert_threshold import _act_dtype, _call, _out_or_new, _require, _require_device, _vp
+from ._lib import ET_MAX_NORM_WIDTH, lib
+from .expert_threshold import _ACT_DTYPES, _act_dtype, _call, _out_or_new, _require, _require_device, _vp
 
 
 def _require_rows(t, name: str, dtype=None, shape=None, device=None) -> int:
@@ -28,6 +28,13 @@ def _require_rows(t, name: str, dtype=None, shape=None, device=None) -> int:
     if (inner != 1 and d > 1) or (along < d and rows > 1):
         raise ValueError(f"the rows of {name} must be contiguous and must not overlap, got strides {t.stride()}")
     return max(along, d)
+
+
+def _new_rows(out, x, name: str):
+    """`out` checked, or new dense rows like x."""
+    if out is None:
+        return torch.empty_like(x, memory_format=torch.contiguous_format)
+    return _out_or_new(out, tuple(x.shape), x.dtype, x.device, name)
 
 
 def _check_width(d: int) -> None:
@@ -57,23 +64,37 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
         y | (y, sum) | (y, mean, rstd) | (y, sum, mean, rstd)
     Binary32 arithmetic, one rounding of y, identical bits on repeated calls.
     """
-    ldx = _require_rows(x, "x")
-    dt = _act_dtype(x, "x")
-    rows, d = x.shape
+    if not isinstance(x, torch.Tensor) or not isinstance(weight, torch.Tensor):
+        raise TypeError("x and weight must be torch.Tensors")
     dev, dtype = x.device, x.dtype
-    _check_width(d)
-    wdt = _require_weight(weight, "weight", d, dtype, dev)
-    if bias is not None and _require_weight(bias, "bias", d, dtype, dev) != wdt:
-        raise TypeError("weight and bias must have the same dtype")
+    # (a call on a few rows takes 4 us on the device: dense tensors pass one test)
+    if (x.is_cuda and x.dim() == 2 and x.is_contiguous() and dtype in _ACT_DTYPES and weight.dim() == 1
+            and weight.is_contiguous() and weight.device == dev and weight.shape[0] == x.shape[1] <= ET_MAX_NORM_WIDTH
+            and (weight.dtype == dtype or weight.dtype == torch.float32)
+            and (bias is None or (bias.dtype == weight.dtype and bias.device == dev and bias.is_contiguous()
+                                  and bias.shape == weight.shape)) and x.shape[1]):
+        rows, d = x.shape
+        ldx, dt, wdt = d, _ACT_DTYPES[dtype], _ACT_DTYPES[weight.dtype]
+    else:
+        ldx = _require_rows(x, "x")
+        dt = _act_dtype(x, "x")
+        rows, d = x.shape
+        _check_width(d)
+        wdt = _require_weight(weight, "weight", d, dtype, dev)
+        if bias is not None and _require_weight(bias, "bias", d, dtype, dev) != wdt:
+            raise TypeError("weight and bias must have the same dtype")
     if not 0.0 <= eps < float("inf"):
         raise ValueError(f"eps must be finite and >= 0, got {eps}")
     ldr = 0
     if residual is not None:
-        ldr = _require_rows(residual, "residual", dtype, x.shape, dev)
-        out_sum = _out_or_new(out_sum, (rows, d), dtype, dev, "out_sum")
+        if residual.dtype == dtype and residual.shape == x.shape and residual.device == dev and residual.is_contiguous():
+            ldr = d
+        else:
+            ldr = _require_rows(residual, "residual", dtype, x.shape, dev)
+        out_sum = _new_rows(out_sum, x, "out_sum")
     elif out_sum is not None:
         raise ValueError("out_sum needs a residual")
-    y = _out_or_new(out, (rows, d), dtype, dev, "out")
+    y = _new_rows(out, x, "out")
     if stats:
         mean, rstd = (torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(2))
     else:

@@ -31,11 +31,15 @@ _data_ptr = torch.Tensor.data_ptr
 _numel = torch.Tensor.numel
 _get_device = torch.Tensor.get_device
 _is_contiguous = torch.Tensor.is_contiguous
-_is_tensor = torch.is_tensor
 
 
 def _array(ptrs):
+    """A host array of pointers, as ctypes passes it."""
     return (ctypes.c_void_p * len(ptrs))(*ptrs)
+
+
+def _pointers(ts):
+    return _array(list(map(_data_ptr, ts)))
 
 
 def _numel_array(sizes):
@@ -49,11 +53,12 @@ def _check_list(ts, name: str, dtypes, device: int, sizes) -> None:
         raise TypeError(f"{name} must be a list or a tuple of tensors")
     if len(ts) != len(sizes):
         raise ValueError(f"{name} has {len(ts)} tensors, params has {len(sizes)}")
-    if not all(map(_is_tensor, ts)):
-        raise TypeError(f"{name} must hold torch.Tensors")
-    if (list(map(_numel, ts)) == sizes and all(map(_is_contiguous, ts)) and set(map(_get_device, ts)) <= {device}
-            and {t.dtype for t in ts} <= dtypes):
-        return
+    try:        # (the unbound methods refuse what is no tensor)
+        if (list(map(_numel, ts)) == sizes and all(map(_is_contiguous, ts)) and set(map(_get_device, ts)) <= {device}
+                and {t.dtype for t in ts} <= dtypes):
+            return
+    except TypeError:
+        raise TypeError(f"{name} must hold torch.Tensors") from None
     for i, t in enumerate(ts):
         _require_device(t, f"{name}[{i}]")
         if t.dtype not in dtypes:
@@ -144,7 +149,7 @@ def grad_norm(grads: Sequence[torch.Tensor], max_norm: Optional[float] = None, *
     out = torch.empty(2, dtype=torch.float32, device=dev)
     norm = out.data_ptr()
     dtypes = (ctypes.c_int32 * len(sizes))(*[_DTYPES[t.dtype] for t in grads])
-    _call("et_grad_norm", dev, _array(list(map(_data_ptr, grads))), numel, dtypes, len(sizes),
+    _call("et_grad_norm", dev, _pointers(grads), numel, dtypes, len(sizes),
           0.0 if max_norm is None else float(max_norm), norm, None if max_norm is None else norm + 4, _vp(workspace),
           workspace.numel() * workspace.element_size())
     return out[0], None if max_norm is None else out[1]
@@ -170,9 +175,9 @@ def _step(fn: str, dev, params, grads, states, masters, sizes, scalars, grad_sca
             return ts if at is None else [ts[i] for i in at]
         p, g = take(params), take(grads)
         low = p[0].dtype == torch.bfloat16
-        _call(fn, dev, _array(list(map(_data_ptr, p))), _array(list(map(_data_ptr, g))),
-              *(_array(list(map(_data_ptr, take(s)))) for s in states),
-              _array(list(map(_data_ptr, take(masters)))) if low else None, _numel_array(take(sizes)), len(p),
+        _call(fn, dev, _pointers(p), _pointers(g),
+              *(_pointers(take(s)) for s in states),
+              _pointers(take(masters)) if low else None, _numel_array(take(sizes)), len(p),
               _DTYPES[p[0].dtype], _DTYPES[g[0].dtype], scalars, _vp(grad_scale), *more)
 
 
@@ -290,7 +295,8 @@ class AdamW:
         _check_masters(self.params, masters, self._index, self._sizes)
         self.masters = None if masters is None else list(masters)
         # (the states' own buffers never move)
-        self._tables = [_array(list(map(_data_ptr, s))) for s in self._states]
+        self._one_type = len(set(self._dtypes)) == 1
+        self._tables = [_pointers(s) for s in self._states]
         self._numel = _numel_array(self._sizes)
 
     def step(self, grads: Sequence[Optional[torch.Tensor]], *, grad_scale: Optional[torch.Tensor] = None,
@@ -306,7 +312,11 @@ class AdamW:
         if [p.dtype for p in params] != self._dtypes:
             raise TypeError("a parameter changed its type")
         _check_list(params, "params", _DTYPES.keys(), self._index, sizes)
-        whole = all(g is not None for g in grads)
+        whole = True
+        for g in grads:
+            if g is None:
+                whole = False
+                break
         if not whole:
             at = [i for i, g in enumerate(grads) if g is not None]
             params, grads, sizes = ([ts[i] for i in at] for ts in (params, grads, sizes))
@@ -318,9 +328,9 @@ class AdamW:
         fn, more = "et_adamw", ()
         if self.state == "e4m3":
             fn, more = "et_adamw8", (int(self.stochastic), (self.seed + self.steps + 1) & 0xFFFFFFFF)
-        if whole and len(set(self._dtypes)) == 1 and len({g.dtype for g in grads}) == 1:
-            _call(fn, dev, _array(list(map(_data_ptr, params))), _array(list(map(_data_ptr, grads))), *self._tables,
-                  None if masters is None else _array(list(map(_data_ptr, masters))), self._numel, len(params),
+        if whole and self._one_type and len({g.dtype for g in grads}) == 1:
+            _call(fn, dev, _pointers(params), _pointers(grads), *self._tables,
+                  None if masters is None else _pointers(masters), self._numel, len(params),
                   _DTYPES[self._dtypes[0]], _DTYPES[grads[0].dtype], scalars, _vp(grad_scale), *more)
         elif params:
             _step(fn, dev, params, grads, states, masters, sizes, scalars, grad_scale, *more)
