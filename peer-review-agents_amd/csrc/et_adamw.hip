@@ -458,11 +458,13 @@ int check_step(const char* fn, int param_dtype, int grad_dtype, const void* mast
 }
 
 // Walks the tensors with elements in launches of up to N of them: put(slot, i,
-// index of its first element) fills a slot, go(blocks) enqueues.
+// element of tensor i that the slot begins at, that element's index in the
+// call) fills a slot, go(blocks) enqueues.  A launch has less than 2^32 threads: a
+// tensor of more is dealt to several slots.
 template <int N, typename Put, typename Go>
 int each_launch(const int64_t* numel, int64_t count, int chunk, Spans<N>& spans, Put put, Go go)
 {
-    constexpr int64_t kMostBlocks = (int64_t)1 << 30;
+    constexpr int64_t kMostBlocks = ((int64_t)1 << 32) / kThreads - 1;
     uint64_t element = 0;
     int slot = 0;
     int64_t blocks = 0;
@@ -477,20 +479,30 @@ int each_launch(const int64_t* numel, int64_t count, int chunk, Spans<N>& spans,
         return rc;
     };
     for (int64_t i = 0; i < count; ++i) {
-        const int64_t n = chunks(numel[i], chunk);
-        if (n > 0) {
-            if (slot == N || blocks + n > kMostBlocks) {
+        int64_t from = 0;
+        while (from < numel[i]) {
+            if (slot == N || blocks == kMostBlocks) {
                 const int rc = flush();
                 if (rc) return rc;
             }
+            const int64_t n = std::min(chunks(numel[i] - from, chunk), kMostBlocks - blocks);
+            const int64_t size = std::min(numel[i] - from, n * chunk);
             spans.first[slot] = (uint32_t)blocks;
-            spans.numel[slot] = numel[i];
-            put(slot++, i, (uint32_t)element);
+            spans.numel[slot] = size;
+            put(slot++, i, from, (uint32_t)(element + (uint64_t)from));
             blocks += n;
+            from += size;
         }
         element += (uint64_t)chunks(numel[i], ET_ADAMW8_BLOCK) * ET_ADAMW8_BLOCK;
     }
     return flush();
+}
+
+// Entry i of a list, `from` elements of `size` bytes on.
+template <typename T>
+T* at(T* p, int64_t from, int64_t size)
+{
+    return p ? (T*)((uintptr_t)p + (uintptr_t)(from * size)) : p;
 }
 
 }  // namespace
@@ -537,8 +549,8 @@ extern "C" int et_grad_norm(const void* const* grads, const int64_t* numel, cons
     args.partial = partial;
     rc = each_launch<kNormTensors>(
         numel, count, kNormChunk, args.spans,
-        [&](int slot, int64_t i, uint32_t) {
-            args.grad[slot] = grads[i];
+        [&](int slot, int64_t i, int64_t from, uint32_t) {
+            args.grad[slot] = at(grads[i], from, dtypes[i] == ET_DTYPE_BF16 ? 2 : 4);
             args.bf16[slot] = dtypes[i] == ET_DTYPE_BF16;
         },
         [&](unsigned blocks) {
@@ -558,7 +570,7 @@ extern "C" int et_adamw(void* const* params, const void* const* grads, float* co
 {
     const char* fn = "et_adamw";
     const auto list = [](auto* p) { return (const void* const*)p; };
-    const uintptr_t pa = param_dtype == ET_DTYPE_BF16 ? 2 : 4, ga = grad_dtype == ET_DTYPE_BF16 ? 2 : 4;
+    const int pa = param_dtype == ET_DTYPE_BF16 ? 2 : 4, ga = grad_dtype == ET_DTYPE_BF16 ? 2 : 4;   // bytes
     int rc = check_list(fn, numel, count);
     if (!rc) rc = check_step(fn, param_dtype, grad_dtype, masters);
     if (!rc) rc = check_pointers(fn, "params", list(params), numel, count, pa);
@@ -574,12 +586,12 @@ extern "C" int et_adamw(void* const* params, const void* const* grads, float* co
     args.grad_scale = grad_scale;
     return each_launch<kTensors>(
         numel, count, kChunk, args.spans,
-        [&](int slot, int64_t i, uint32_t) {
-            args.param[slot] = params[i];
-            args.grad[slot] = grads[i];
-            args.m[slot] = m[i];
-            args.v[slot] = v[i];
-            args.master[slot] = masters ? masters[i] : nullptr;
+        [&](int slot, int64_t i, int64_t from, uint32_t) {
+            args.param[slot] = at(params[i], from, pa);
+            args.grad[slot] = at(grads[i], from, ga);
+            args.m[slot] = m[i] + from;
+            args.v[slot] = v[i] + from;
+            args.master[slot] = masters ? masters[i] + from : nullptr;
         },
         [&](unsigned blocks) {
             const dim3 grid(blocks), block(kThreads);
@@ -620,7 +632,7 @@ extern "C" int et_adamw8(void* const* params, const void* const* grads, uint8_t*
 {
     const char* fn = "et_adamw8";
     const auto list = [](auto* p) { return (const void* const*)p; };
-    const uintptr_t pa = param_dtype == ET_DTYPE_BF16 ? 2 : 4, ga = grad_dtype == ET_DTYPE_BF16 ? 2 : 4;
+    const int pa = param_dtype == ET_DTYPE_BF16 ? 2 : 4, ga = grad_dtype == ET_DTYPE_BF16 ? 2 : 4;   // bytes
     int rc = check_list(fn, numel, count);
     if (!rc) rc = check_step(fn, param_dtype, grad_dtype, masters);
     if (!rc) rc = check_pointers(fn, "params", list(params), numel, count, pa);
@@ -642,14 +654,14 @@ extern "C" int et_adamw8(void* const* params, const void* const* grads, uint8_t*
     args.seed = seed;
     return each_launch<kTensors8>(
         numel, count, kChunk, args.spans,
-        [&](int slot, int64_t i, uint32_t element) {
-            args.param[slot] = params[i];
-            args.grad[slot] = grads[i];
-            args.m8[slot] = m8[i];
-            args.m_scale[slot] = m_scale[i];
-            args.u8[slot] = u8[i];
-            args.u_scale[slot] = u_scale[i];
-            args.master[slot] = masters ? masters[i] : nullptr;
+        [&](int slot, int64_t i, int64_t from, uint32_t element) {
+            args.param[slot] = at(params[i], from, pa);
+            args.grad[slot] = at(grads[i], from, ga);
+            args.m8[slot] = m8[i] + from;
+            args.m_scale[slot] = m_scale[i] + from / ET_ADAMW8_BLOCK;
+            args.u8[slot] = u8[i] + from;
+            args.u_scale[slot] = u_scale[i] + from / ET_ADAMW8_BLOCK;
+            args.master[slot] = masters ? masters[i] + from : nullptr;
             args.origin[slot] = element;
         },
         [&](unsigned blocks) {

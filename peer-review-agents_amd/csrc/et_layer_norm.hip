@@ -448,10 +448,25 @@ template <typename X, typename W>
 int launch_fwd(const FwdArgs& a, hipStream_t s)
 {
     constexpr int V = Elem<X>::V;
-    const auto go = [&](auto kernel, int wpr) {
-        const int64_t rows = norm_threads(wpr) / (wpr * kWave);
-        kernel<<<dim3((unsigned)((a.T + rows - 1) / rows)), dim3(norm_threads(wpr)), 0, s>>>(a);
-        return check_launch("layer_norm_fwd_kernel");
+    const auto go = [&](auto kernel, int wpr) -> int {
+        // (a launch has less than 2^32 threads)
+        const int64_t rows = norm_threads(wpr) / (wpr * kWave), most = (((int64_t)1 << 32) / norm_threads(wpr) - 1) * rows;
+        for (int64_t from = 0; from < a.T; from += most) {
+            FwdArgs part = a;
+            const int64_t es = sizeof(X);
+            const auto skip = [&](const void* p, int64_t bytes) { return p ? (const char*)p + from * bytes : nullptr; };
+            part.T = std::min(most, a.T - from);
+            part.x = skip(a.x, a.ldx * es);
+            part.residual = skip(a.residual, a.ldr * es);
+            part.y = (void*)skip(a.y, a.d * es);
+            part.sum = (void*)skip(a.sum, a.d * es);
+            part.mean = (float*)skip(a.mean, 4);
+            part.rstd = (float*)skip(a.rstd, 4);
+            kernel<<<dim3((unsigned)((part.T + rows - 1) / rows)), dim3(norm_threads(wpr)), 0, s>>>(part);
+            const int rc = check_launch("layer_norm_fwd_kernel");
+            if (rc) return rc;
+        }
+        return ET_OK;
     };
     const auto fits = [&](int wpr, int nv) { return vectors(a.d, V, wpr * kWave) <= nv; };
     if (fits(1, 1)) return go(layer_norm_fwd_kernel<X, W, 1, 1>, 1);

@@ -74,62 +74,64 @@ __device__ __forceinline__ float scale16(uint32_t bits16, bool half)
 // first tile, then its 4 rows of the second.
 __device__ __forceinline__ int scale_row(int i) { return 16 * (i >> 2 & 1) + 4 * (i >> 3) + (i & 3); }
 
-__global__ __launch_bounds__(256) void w4_pack_kernel(const uint8_t* q, const uint16_t* scales, W4Shape w, uint32_t* packed,
-                                                      uint16_t* packed_scales)
+__global__ __launch_bounds__(256) void w4_pack_kernel(const uint8_t* q, const uint16_t* scales, W4Shape w, int64_t blocks,
+                                                      uint32_t* packed, uint16_t* packed_scales)
 {
     const int kts = w.kts, gpt = w.gpt(), groups = (w.K + w.group - 1) / w.group;
-    // one block: the tiles of one superblock at one k range
-    const int64_t blk = blockIdx.x;
-    const int kt = (int)(blk % kts);
-    const int b = (int)(blk / kts % w.sbs);
-    const int e = (int)(blk / kts / w.sbs);
-    const int row0 = w.row0(b), rows = w.rows(b);
-    for (int i = (int)threadIdx.x; i < 2 * kTileBytes / 4; i += 256) {
-        const int tile = i >> 8, lane = i >> 2 & 63, s = i & 3;
-        const int r = 16 * tile + (lane & 15), k = kt * kKt + 32 * s + 8 * (lane >> 4);
-        uint32_t out = 0x88888888u;
-        if (r < rows && k < w.K) {     // (K a multiple of 8: all of the 8 or none)
-            const uint8_t* src = q + (((int64_t)e * w.N + row0 + r) * w.K + k) / 2;
-            out = 0;
+    // a block at a time: the tiles of one superblock at one k range
+    for (int64_t blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
+        const int kt = (int)(blk % kts);
+        const int b = (int)(blk / kts % w.sbs);
+        const int e = (int)(blk / kts / w.sbs);
+        const int row0 = w.row0(b), rows = w.rows(b);
+        for (int i = (int)threadIdx.x; i < 2 * kTileBytes / 4; i += 256) {
+            const int tile = i >> 8, lane = i >> 2 & 63, s = i & 3;
+            const int r = 16 * tile + (lane & 15), k = kt * kKt + 32 * s + 8 * (lane >> 4);
+            uint32_t out = 0x88888888u;
+            if (r < rows && k < w.K) {     // (K a multiple of 8: all of the 8 or none)
+                const uint8_t* src = q + (((int64_t)e * w.N + row0 + r) * w.K + k) / 2;
+                out = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                out |= (uint32_t)(src[j] & 15) << (4 * j);
-                out |= (uint32_t)(src[j] >> 4) << (16 + 4 * j);
+                for (int j = 0; j < 4; ++j) {
+                    out |= (uint32_t)(src[j] & 15) << (4 * j);
+                    out |= (uint32_t)(src[j] >> 4) << (16 + 4 * j);
+                }
             }
+            packed[blk * (2 * kTileBytes / 4) + i] = out;
         }
-        packed[blk * (2 * kTileBytes / 4) + i] = out;
-    }
-    for (int i = (int)threadIdx.x; i < gpt * kSb; i += 256) {
-        const int r = scale_row(i % kSb), g = kt * gpt + i / kSb;
-        packed_scales[blk * gpt * kSb + i] =
-            r < rows && g < groups ? scales[((int64_t)e * w.N + row0 + r) * groups + g] : (uint16_t)0;
+        for (int i = (int)threadIdx.x; i < gpt * kSb; i += 256) {
+            const int r = scale_row(i % kSb), g = kt * gpt + i / kSb;
+            packed_scales[blk * gpt * kSb + i] =
+                r < rows && g < groups ? scales[((int64_t)e * w.N + row0 + r) * groups + g] : (uint16_t)0;
+        }
     }
 }
 
 // bf16 [E, N, K] of the experts with slots (all without offsets).
 __global__ __launch_bounds__(256) void w4_unpack_kernel(const uint32_t* packed, const uint16_t* packed_scales, bool half,
-                                                        W4Shape w, const int32_t* expert_offsets, int64_t cap,
-                                                        uint16_t* out)
+                                                        W4Shape w, int64_t blocks, const int32_t* expert_offsets,
+                                                        int64_t cap, uint16_t* out)
 {
     const int kts = w.kts, gpt = w.gpt();
-    const int64_t blk = blockIdx.x;
-    const int kt = (int)(blk % kts);
-    const int b = (int)(blk / kts % w.sbs);
-    const int e = (int)(blk / kts / w.sbs);
-    if (expert_offsets && min<int64_t>(expert_offsets[e], cap) >= min<int64_t>(expert_offsets[e + 1], cap)) return;
-    const int row0 = w.row0(b), rows = w.rows(b);
-    for (int i = (int)threadIdx.x; i < 2 * kTileBytes / 4; i += 256) {
-        const int tile = i >> 8, lane = i >> 2 & 63, s = i & 3;
-        const int r = 16 * tile + (lane & 15), in = 32 * s + 8 * (lane >> 4), k = kt * kKt + in;
-        if (r >= rows || k >= w.K) continue;
-        const uint32_t v = packed[blk * (2 * kTileBytes / 4) + i];
-        const int at = 8 * ((r & 15) >> 2) + 4 * (r >> 4) + (r & 3);
-        const float sc = scale16(packed_scales[(blk * gpt + in / w.group) * kSb + at], half);
-        u32x4_t o;
+    for (int64_t blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
+        const int kt = (int)(blk % kts);
+        const int b = (int)(blk / kts % w.sbs);
+        const int e = (int)(blk / kts / w.sbs);
+        if (expert_offsets && min<int64_t>(expert_offsets[e], cap) >= min<int64_t>(expert_offsets[e + 1], cap)) continue;
+        const int row0 = w.row0(b), rows = w.rows(b);
+        for (int i = (int)threadIdx.x; i < 2 * kTileBytes / 4; i += 256) {
+            const int tile = i >> 8, lane = i >> 2 & 63, s = i & 3;
+            const int r = 16 * tile + (lane & 15), in = 32 * s + 8 * (lane >> 4), k = kt * kKt + in;
+            if (r >= rows || k >= w.K) continue;
+            const uint32_t v = packed[blk * (2 * kTileBytes / 4) + i];
+            const int at = 8 * ((r & 15) >> 2) + 4 * (r >> 4) + (r & 3);
+            const float sc = scale16(packed_scales[(blk * gpt + in / w.group) * kSb + at], half);
+            u32x4_t o;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            o[j] = pack_bf16x2((float)((int)(v >> (4 * j) & 15) - 8) * sc, (float)((int)(v >> (16 + 4 * j) & 15) - 8) * sc);
-        *reinterpret_cast<u32x4_t*>(out + ((int64_t)e * w.N + row0 + r) * w.K + k) = o;
+            for (int j = 0; j < 4; ++j)
+                o[j] = pack_bf16x2((float)((int)(v >> (4 * j) & 15) - 8) * sc, (float)((int)(v >> (16 + 4 * j) & 15) - 8) * sc);
+            *reinterpret_cast<u32x4_t*>(out + ((int64_t)e * w.N + row0 + r) * w.K + k) = o;
+        }
     }
 }
 
@@ -141,43 +143,45 @@ __global__ __launch_bounds__(256) void w4_quantize_kernel(const X* w, int64_t ro
                                                           uint16_t* scales)
 {
     const int cols = (K + G - 1) / G * (G / 8);     // threads of a row, whole groups
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t row = i / cols;
-    const int k = (int)(i % cols) * 8;
-    const bool in = row < rows && k < K;
-    float v[8];
+    // (whole waves take part in every turn)
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i - lane_id() < rows * cols; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / cols;
+        const int k = (int)(i % cols) * 8;
+        const bool in = row < rows && k < K;
+        float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        v[j] = 0.0f;
-        if (in) {
-            if constexpr (sizeof(X) == 2) v[j] = u2f((uint32_t)w[row * K + k + j] << 16);
-            else v[j] = w[row * K + k + j];
+        for (int j = 0; j < 8; ++j) {
+            v[j] = 0.0f;
+            if (in) {
+                if constexpr (sizeof(X) == 2) v[j] = u2f((uint32_t)w[row * K + k + j] << 16);
+                else v[j] = w[row * K + k + j];
+            }
         }
-    }
-    float hi = 0.0f, lo = 0.0f;
-    bool nan = false;
+        float hi = 0.0f, lo = 0.0f;
+        bool nan = false;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        hi = __builtin_fmaxf(hi, v[j]);
-        lo = __builtin_fminf(lo, v[j]);
-        nan |= !(__builtin_fabsf(v[j]) < __builtin_inff());
-    }
-    float s = nan ? __builtin_inff() : __builtin_fmaxf(hi / 7.0f, lo / -8.0f);
+        for (int j = 0; j < 8; ++j) {
+            hi = __builtin_fmaxf(hi, v[j]);
+            lo = __builtin_fminf(lo, v[j]);
+            nan |= !(__builtin_fabsf(v[j]) < __builtin_inff());
+        }
+        float s = nan ? __builtin_inff() : __builtin_fmaxf(hi / 7.0f, lo / -8.0f);
 #pragma unroll
-    for (int off = G / 16; off >= 1; off >>= 1) s = __builtin_fmaxf(s, __shfl_xor(s, off, kWave));
-    const uint16_t bits = half ? __builtin_bit_cast(uint16_t, (_Float16)s) : (uint16_t)f32_to_bf16_bits(s);
-    const float sc = scale16(bits, half);
-    uint32_t out = 0;
+        for (int off = G / 16; off >= 1; off >>= 1) s = __builtin_fmaxf(s, __shfl_xor(s, off, kWave));
+        const uint16_t bits = half ? __builtin_bit_cast(uint16_t, (_Float16)s) : (uint16_t)f32_to_bf16_bits(s);
+        const float sc = scale16(bits, half);
+        uint32_t out = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        // (a group whose scale is not finite, or 0, is all 8: its products are NaN, or 0)
-        const float t = sc > 0.0f && sc < __builtin_inff() ? __builtin_rintf(v[j] / sc) : 0.0f;
-        const int n = (int)__builtin_fminf(__builtin_fmaxf(t, -8.0f), 7.0f) + 8;
-        out |= (uint32_t)n << (4 * j);
-    }
-    if (in) {
-        q[(row * K + k) / 8] = out;
-        if (k % G == 0) scales[row * ((K + G - 1) / G) + k / G] = sc < __builtin_inff() ? bits : (uint16_t)(half ? 0x7E00 : 0x7FC0);
+        for (int j = 0; j < 8; ++j) {
+            // (a group whose scale is not finite, or 0, is all 8: its products are NaN, or 0)
+            const float t = sc > 0.0f && sc < __builtin_inff() ? __builtin_rintf(v[j] / sc) : 0.0f;
+            const int n = (int)__builtin_fminf(__builtin_fmaxf(t, -8.0f), 7.0f) + 8;
+            out |= (uint32_t)n << (4 * j);
+        }
+        if (in) {
+            q[(row * K + k) / 8] = out;
+            if (k % G == 0) scales[row * ((K + G - 1) / G) + k / G] = sc < __builtin_inff() ? bits : (uint16_t)(half ? 0x7E00 : 0x7FC0);
+        }
     }
 }
 
@@ -809,13 +813,9 @@ W4Shape shape_of(int64_t E, int64_t N, int64_t K, int64_t group, int64_t parts)
                    (int)((K + kKt - 1) / kKt)};
 }
 
-int blocks_of(const char* fn, const W4Shape& w, unsigned& blocks)
-{
-    const int64_t n = (int64_t)w.E * w.sbs * w.kts;
-    if (n >= (int64_t)1 << 31) return fail(ET_ERR_INVALID_ARGUMENT, std::string(fn) + ": the weight is too large");
-    blocks = (unsigned)n;
-    return ET_OK;
-}
+// Blocks of the layout kernels, and of a launch of them (less than 2^32 threads).
+int64_t blocks_of(const W4Shape& w) { return (int64_t)w.E * w.sbs * w.kts; }
+dim3 layout_grid(int64_t blocks) { return dim3((unsigned)std::min<int64_t>(blocks, (int64_t)1 << 22)); }
 
 int check_ptr(const char* fn, const char* name, const void* p, uintptr_t align)
 {
@@ -852,18 +852,17 @@ extern "C" int et_w4_pack(const void* q, const void* scales, int64_t num_experts
                           int64_t parts, void* packed, void* packed_scales, void* stream)
 {
     const char* fn = "et_w4_pack";
-    unsigned blocks = 0;
     int rc = check_shape(fn, num_experts, N, K, group, parts);
     if (rc) return rc;
     const W4Shape w = shape_of(num_experts, N, K, group, parts);
-    rc = blocks_of(fn, w, blocks);
-    if (!rc) rc = check_ptr(fn, "q", q, 1);
+    rc = check_ptr(fn, "q", q, 1);
     if (!rc) rc = check_ptr(fn, "scales", scales, 2);
     if (!rc) rc = check_ptr(fn, "packed", packed, 16);
     if (!rc) rc = check_ptr(fn, "packed_scales", packed_scales, 16);
     if (rc) return rc;
-    w4_pack_kernel<<<dim3(blocks), dim3(256), 0, (hipStream_t)stream>>>((const uint8_t*)q, (const uint16_t*)scales, w,
-                                                                       (uint32_t*)packed, (uint16_t*)packed_scales);
+    const int64_t blocks = blocks_of(w);
+    w4_pack_kernel<<<layout_grid(blocks), dim3(256), 0, (hipStream_t)stream>>>(
+        (const uint8_t*)q, (const uint16_t*)scales, w, blocks, (uint32_t*)packed, (uint16_t*)packed_scales);
     return check_launch("w4_pack_kernel");
 }
 
@@ -872,19 +871,18 @@ extern "C" int et_w4_unpack(const void* packed, const void* packed_scales, int s
                             int64_t slot_capacity, void* w, void* stream)
 {
     const char* fn = "et_w4_unpack";
-    unsigned blocks = 0;
     int rc = check_shape(fn, num_experts, N, K, group, parts);
     if (!rc) rc = check_scale_type(fn, scale_type);
     if (rc) return rc;
     const W4Shape sh = shape_of(num_experts, N, K, group, parts);
-    rc = blocks_of(fn, sh, blocks);
-    if (!rc) rc = check_ptr(fn, "packed", packed, 16);
+    rc = check_ptr(fn, "packed", packed, 16);
     if (!rc) rc = check_ptr(fn, "packed_scales", packed_scales, 16);
     if (!rc) rc = check_ptr(fn, "w", w, 16);
     if (rc) return rc;
     if (slot_capacity < 0) return fail(ET_ERR_INVALID_ARGUMENT, "et_w4_unpack: slot_capacity must be >= 0");
-    w4_unpack_kernel<<<dim3(blocks), dim3(256), 0, (hipStream_t)stream>>>(
-        (const uint32_t*)packed, (const uint16_t*)packed_scales, scale_type == ET_W4_SCALE_F16, sh, expert_offsets,
+    const int64_t blocks = blocks_of(sh);
+    w4_unpack_kernel<<<layout_grid(blocks), dim3(256), 0, (hipStream_t)stream>>>(
+        (const uint32_t*)packed, (const uint16_t*)packed_scales, scale_type == ET_W4_SCALE_F16, sh, blocks, expert_offsets,
         slot_capacity, (uint16_t*)w);
     return check_launch("w4_unpack_kernel");
 }
@@ -896,7 +894,7 @@ template <typename X>
 void launch_quantize(const void* w, int64_t rows, int64_t K, int64_t group, bool half, void* q, void* scales, hipStream_t s)
 {
     const int64_t threads = rows * ((K + group - 1) / group * (group / 8));
-    const dim3 grid((unsigned)((threads + 255) / 256)), block(256);
+    const dim3 grid = layout_grid((threads + 255) / 256), block(256);
     switch (group) {
         case 32: w4_quantize_kernel<X, 32><<<grid, block, 0, s>>>((const X*)w, rows, (int)K, half, (uint32_t*)q, (uint16_t*)scales); break;
         case 64: w4_quantize_kernel<X, 64><<<grid, block, 0, s>>>((const X*)w, rows, (int)K, half, (uint32_t*)q, (uint16_t*)scales); break;
@@ -926,8 +924,6 @@ extern "C" int et_w4_quantize(const void* w, int dtype, int64_t num_experts, int
     if (rc) return rc;
     if (dtype != ET_DTYPE_F32 && dtype != ET_DTYPE_BF16)
         return fail(ET_ERR_INVALID_ARGUMENT, "et_w4_quantize: dtype must be ET_DTYPE_F32 or ET_DTYPE_BF16");
-    if (num_experts * N * (K / 8 + group) >= (int64_t)1 << 39)
-        return fail(ET_ERR_INVALID_ARGUMENT, "et_w4_quantize: the weight is too large");
     rc = check_ptr(fn, "w", w, dtype == ET_DTYPE_F32 ? 4 : 2);
     if (!rc) rc = check_ptr(fn, "q", q, 4);
     if (!rc) rc = check_ptr(fn, "scales", scales, 2);

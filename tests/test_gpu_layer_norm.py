@@ -135,6 +135,19 @@ def test_many_rows(et, dev):
         assert torch.all((dw.double() - rw).abs() <= 2 * ew) and torch.all((db.double() - rb).abs() <= 2 * eb)
 
 
+def test_more_rows_than_one_launch_takes(et, dev):
+    """67108865 rows of 8: the forward's launches hold 2^24 - 1 blocks of 4 rows."""
+    T = 4 * (2 ** 24 - 1) + 5
+    x = torch.empty(T, 8, dtype=BF16, device=dev)
+    for i in range(0, T, 1 << 24):
+        x[i:i + (1 << 24)].normal_()
+    w = torch.arange(1.0, 9.0, device=dev)
+    y, s, mean, rstd = et.layer_norm(x, w, residual=x, stats=True)
+    for a, b in ((0, 1000), (T - 1000, T), (4 * (2 ** 24 - 1) - 500, 4 * (2 ** 24 - 1) + 3)):
+        part = et.layer_norm(x[a:b].clone(), w, residual=x[a:b].clone(), stats=True)
+        assert all(torch.equal(p, q[a:b]) for p, q in zip(part, (y, s, mean, rstd)))
+
+
 def test_gradients_against_differences(et, dev):
     """<dL, v> against central differences of L = sum(c1 y) + sum(c2 sum) in f32
     rows of 33: a step of 2^-7 leaves a truncation of about step^2 and U * |L| /
