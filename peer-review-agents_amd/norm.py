@@ -99,8 +99,9 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
         mean, rstd = (torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(2))
     else:
         mean = rstd = None
-    _call("et_layer_norm_fwd", dev, _vp(x), ldx, _vp(residual), ldr, _vp(weight), _vp(bias), rows, d, dt, wdt, eps,
-          _vp(y), _vp(out_sum), _vp(mean), _vp(rstd))
+    _call("et_layer_norm_fwd", dev, x.data_ptr(), ldx, None if residual is None else residual.data_ptr(), ldr,
+          weight.data_ptr(), None if bias is None else bias.data_ptr(), rows, d, dt, wdt, eps, y.data_ptr(),
+          None if residual is None else out_sum.data_ptr(), _vp(mean), _vp(rstd))
     if residual is None:
         return (y, mean, rstd) if stats else y
     return (y, out_sum, mean, rstd) if stats else (y, out_sum)

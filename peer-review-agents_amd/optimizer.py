@@ -251,7 +251,7 @@ class AdamW:
     for each kind, ``flat[name]``, each tensor from a multiple of 256 elements
     on.  ``step(grads)`` takes one gradient for each parameter, or None for one
     that has none this time.  The parameters' own storage may move between
-    steps (``p.data = ...``) as long as type, shape and device stay.
+    steps (``p.data = ...``) as long as type, shape, layout and device stay.
     """
 
     def __init__(self, params: Sequence[torch.Tensor], *, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
@@ -296,6 +296,8 @@ class AdamW:
         self.masters = None if masters is None else list(masters)
         # (the states' own buffers never move)
         self._one_type = len(set(self._dtypes)) == 1
+        self._at = list(map(_data_ptr, self.params))
+        self._param_table = _array(self._at)
         self._tables = [_pointers(s) for s in self._states]
         self._numel = _numel_array(self._sizes)
 
@@ -309,19 +311,22 @@ class AdamW:
             raise TypeError("grads must be a list or a tuple of tensors")
         if len(grads) != len(params):
             raise ValueError(f"grads has {len(grads)} tensors, params has {len(params)}")
-        if [p.dtype for p in params] != self._dtypes:
-            raise TypeError("a parameter changed its type")
-        _check_list(params, "params", _DTYPES.keys(), self._index, sizes)
+        at = list(map(_data_ptr, params))
+        if at != self._at or list(map(_numel, params)) != sizes:      # storage that has moved is looked over again
+            _check_list(params, "params", _DTYPES.keys(), self._index, sizes)
+            if [p.dtype for p in params] != self._dtypes:
+                raise TypeError("a parameter changed its type")
+            self._at, self._param_table = at, _array(at)
         whole = True
         for g in grads:
             if g is None:
                 whole = False
                 break
         if not whole:
-            at = [i for i, g in enumerate(grads) if g is not None]
-            params, grads, sizes = ([ts[i] for i in at] for ts in (params, grads, sizes))
-            states = [[s[i] for i in at] for s in states]
-            masters = None if masters is None else [masters[i] for i in at]
+            some = [i for i, g in enumerate(grads) if g is not None]
+            params, grads, sizes = ([ts[i] for i in some] for ts in (params, grads, sizes))
+            states = [[s[i] for i in some] for s in states]
+            masters = None if masters is None else [masters[i] for i in some]
         _check_list(grads, "grads", _DTYPES.keys(), self._index, sizes)
         _check_scale(grad_scale, dev)
         scalars = _scalars(self.steps + 1, self.lr if lr is None else lr, self.betas, self.eps, self.weight_decay)
@@ -329,7 +334,7 @@ class AdamW:
         if self.state == "e4m3":
             fn, more = "et_adamw8", (int(self.stochastic), (self.seed + self.steps + 1) & 0xFFFFFFFF)
         if whole and self._one_type and len({g.dtype for g in grads}) == 1:
-            _call(fn, dev, _pointers(params), _pointers(grads), *self._tables,
+            _call(fn, dev, self._param_table, _pointers(grads), *self._tables,
                   None if masters is None else _pointers(masters), self._numel, len(params),
                   _DTYPES[self._dtypes[0]], _DTYPES[grads[0].dtype], scalars, _vp(grad_scale), *more)
         elif params:

@@ -138,12 +138,14 @@ def _gemm(a, w: W4Weight, rows: int, sorted_token, offsets, epilogue: str, row_s
         _require(row_scale, "row_scale", torch.float32, 1, dev)
         if row_scale.shape[0] < rows:
             raise ValueError(f"row_scale has {row_scale.shape[0]} entries, out has {rows} rows")
-    c = _out_or_new(out, (rows, w.N // 2 if swiglu else w.N), torch.bfloat16, dev, "out")
-    if a.data_ptr() % 16 or c.data_ptr() % 16:
+    shape = (rows, w.N // 2 if swiglu else w.N)
+    c = a.new_empty(shape) if out is None else _out_or_new(out, shape, torch.bfloat16, dev, "out")
+    at, to = a.data_ptr(), c.data_ptr()
+    if at % 16 or to % 16:
         raise ValueError("a and out must be 16-byte aligned")
-    _call("et_expert_gemm_w4_impl", dev, _vp(a), a.shape[0], sorted_token, _vp(w.packed), _vp(w.scales),
+    _call("et_expert_gemm_w4_impl", dev, at, a.shape[0], sorted_token, w.packed.data_ptr(), w.scales.data_ptr(),
           _SCALE_TYPES[w.scales.dtype], offsets, w.num_experts, w.K, w.N, w.group, w.parts, rows, _EPILOGUES[epilogue],
-          _vp(row_scale) if epilogue == "row_scale" else None, _vp(c), max_slots, route)
+          row_scale.data_ptr() if epilogue == "row_scale" else None, to, max_slots, route)
     return c
 
 
