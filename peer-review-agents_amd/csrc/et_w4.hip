@@ -120,10 +120,11 @@ __global__ __launch_bounds__(256) void w4_unpack_kernel(const uint32_t* packed, 
         if (expert_offsets && min<int64_t>(expert_offsets[e], cap) >= min<int64_t>(expert_offsets[e + 1], cap)) continue;
         const int row0 = w.row0(b), rows = w.rows(b);
         for (int i = (int)threadIdx.x; i < 2 * kTileBytes / 4; i += 256) {
-            const int tile = i >> 8, lane = i >> 2 & 63, s = i & 3;
-            const int r = 16 * tile + (lane & 15), in = 32 * s + 8 * (lane >> 4), k = kt * kKt + in;
+            // (16 threads write 256 bytes of one row)
+            const int tile = i >> 8, r16 = i >> 4 & 15, s = i >> 2 & 3, rho = i & 3;
+            const int r = 16 * tile + r16, in = 32 * s + 8 * rho, k = kt * kKt + in;
             if (r >= rows || k >= w.K) continue;
-            const uint32_t v = packed[blk * (2 * kTileBytes / 4) + i];
+            const uint32_t v = packed[blk * (2 * kTileBytes / 4) + 256 * tile + 4 * (16 * rho + r16) + s];
             const int at = 8 * ((r & 15) >> 2) + 4 * (r >> 4) + (r & 3);
             const float sc = scale16(packed_scales[(blk * gpt + in / w.group) * kSb + at], half);
             u32x4_t o;
@@ -442,6 +443,16 @@ __device__ __forceinline__ void w4_split_tile(const W4Args& g, const W4Tile& t, 
 // share the rows of A, 128 k at a time, through two LDS buffers (one barrier
 // each): read from L2 by every wave, as above, they are 2 to 4 times the weight's
 // bytes at 32 and 64 slots.
+//
+// What bounds them at 64 slots is the issue of instructions: 80 MFMAs and 204
+// others for a wave's 4 KiB of weights.  (On one SIMD 32 MFMAs of one wave take
+// 584 cycles, 256 v_and_or and shifts of another 1218, both at once 1471: an MFMA costs the
+// other wave 8 cycles.)  64 experts of 64 slots, K = 2048, N = 2816: matrix pipe busy
+// 42% of the CUs' time, the others issued in 42% of it; a quarter of the time is the
+// last, partly filled round of tiles.  The order in which a wave issues them, its
+// priority, a ring of four k ranges and a third block to a CU change nothing.
+// Against the bf16 GEMM on unpacked weights (us): mean of 62 slots 110 / 216, 256
+// 318 / 353, 1026 1098 / 987, 2061 2250 / 1872 (32 experts, K = 2048, N = 7168).
 constexpr int kWideWaves = 4;
 constexpr int kWidePitch = 2 * kKt + 16;               // bytes of a row of A in LDS
 // MAXMT tiles of 16 slots at most: 32 or 64 slots
