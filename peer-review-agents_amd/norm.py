@@ -30,6 +30,16 @@ def _require_rows(t, name: str, dtype=None, shape=None, device=None) -> int:
     return max(along, d)
 
 
+def _dense_rows(t, dtype, shape, device) -> bool:
+    return (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2 and t.dtype == dtype and t.shape == shape
+            and t.device == device and t.is_contiguous())
+
+
+def _stat(t, h) -> bool:
+    return (isinstance(t, torch.Tensor) and t.dtype == torch.float32 and t.device == h.device and t.is_contiguous()
+            and t.shape == h.shape[:1])
+
+
 def _new_rows(out, x, name: str):
     """`out` checked, or new dense rows like x."""
     if out is None:
@@ -122,30 +132,40 @@ def layer_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor,
     the norm.  dx has h's type, dweight and dbias are f32 [d] (dbias None
     without ``need_dbias``).
     """
-    ldh = _require_rows(h, "h")
-    dt = _act_dtype(h, "h")
-    rows, d = h.shape
     dev, dtype = h.device, h.dtype
-    _check_width(d)
-    lddy = _require_rows(dy, "dy", dtype, h.shape, dev)
-    ldds = 0 if dsum is None else _require_rows(dsum, "dsum", dtype, h.shape, dev)
-    wdt = _require_weight(weight, "weight", d, dtype, dev)
-    for t, name in ((mean, "mean"), (rstd, "rstd")):
-        _require(t, name, torch.float32, 1, dev)
-        if t.shape[0] != rows:
-            raise ValueError(f"{name} has {t.shape[0]} entries, h has {rows} rows")
-    dx = _out_or_new(out_dx, (rows, d), dtype, dev, "out_dx")
-    dweight = _out_or_new(out_dweight, (d,), torch.float32, dev, "out_dweight")
+    if not (_dense_rows(h, dtype, h.shape, dev) and dtype in _ACT_DTYPES and weight.is_contiguous()
+            and weight.device == dev and weight.shape == h.shape[1:] and 0 < h.shape[1] <= ET_MAX_NORM_WIDTH
+            and (weight.dtype == dtype or weight.dtype == torch.float32) and _stat(mean, h) and _stat(rstd, h)):
+        _require_rows(h, "h")
+        _act_dtype(h, "h")
+        _check_width(h.shape[1])
+        _require_weight(weight, "weight", h.shape[1], dtype, dev)
+        for t, name in ((mean, "mean"), (rstd, "rstd")):
+            _require(t, name, torch.float32, 1, dev)
+            if t.shape[0] != h.shape[0]:
+                raise ValueError(f"{name} has {t.shape[0]} entries, h has {h.shape[0]} rows")
+    rows, d = h.shape
+    ldh = d if h.is_contiguous() else _require_rows(h, "h")
+    lddy = d if _dense_rows(dy, dtype, h.shape, dev) else _require_rows(dy, "dy", dtype, h.shape, dev)
+    ldds = 0
+    if dsum is not None:
+        ldds = d if _dense_rows(dsum, dtype, h.shape, dev) else _require_rows(dsum, "dsum", dtype, h.shape, dev)
+    dx = _new_rows(out_dx, h, "out_dx")
+    dweight = mean.new_empty(d) if out_dweight is None else _out_or_new(out_dweight, (d,), torch.float32, dev,
+                                                                        "out_dweight")
     dbias = None
-    if need_dbias or out_dbias is not None:
+    if out_dbias is not None:
         dbias = _out_or_new(out_dbias, (d,), torch.float32, dev, "out_dbias")
+    elif need_dbias:
+        dbias = mean.new_empty(d)
     wsb = layer_norm_backward_workspace_bytes(rows, d)
     if workspace is None:
-        workspace = torch.empty(wsb, dtype=torch.uint8, device=dev)
+        workspace = mean.new_empty(wsb // 4)
     elif workspace.device != dev or workspace.numel() * workspace.element_size() < wsb:
         raise ValueError(f"workspace must hold {wsb} bytes on {dev}")
-    _call("et_layer_norm_bwd", dev, _vp(dy), lddy, _vp(h), ldh, _vp(dsum), ldds, _vp(weight), _vp(mean), _vp(rstd),
-          rows, d, dt, wdt, _vp(dx), _vp(dweight), _vp(dbias), _vp(workspace), wsb)
+    _call("et_layer_norm_bwd", dev, dy.data_ptr(), lddy, h.data_ptr(), ldh, _vp(dsum), ldds, weight.data_ptr(),
+          mean.data_ptr(), rstd.data_ptr(), rows, d, _ACT_DTYPES[dtype], _ACT_DTYPES[weight.dtype], dx.data_ptr(),
+          dweight.data_ptr(), _vp(dbias), workspace.data_ptr(), wsb)
     return dx, dweight, dbias
 
 
