@@ -214,9 +214,9 @@ int et_w4_unpack(const void* packed, const void* packed_scales, int scale_type, 
  * those of et_expert_gemm; ET_GEMM_SWIGLU needs parts 2.  expert_offsets NULL
  * (with one expert and sorted_token NULL) is the dense layer: every slot below
  * slot_capacity.  Binary32 sums in a fixed order: repeated calls give
- * identical bits.  The inner sum is taken as sum a * (128 + q) from
- * -136 * sum a on, so a row of a that holds an infinity (or values above
- * 2^120) gives NaN.  a and c 16-byte aligned.
+ * identical bits.  The inner sum is taken as sum a * (16 + q) from
+ * -24 * sum a on, so a row of a that holds an infinity (or values whose
+ * 24 |a| add up to 2^128 within a group) gives NaN.  a and c 16-byte aligned.
  * Implements a 4-bit form of the expert GEMM (no reference counterpart).
  */
 int et_expert_gemm_w4(const void* a, int64_t a_rows, const int32_t* sorted_token, const void* packed,

@@ -8,14 +8,18 @@
 // 16 weight rows x 128 k, 1 KiB: lane l of the wave that reads it takes 16
 // bytes, its dword s the 8 values of row l % 16 at k = 32 s + 8 (l / 16) + 0..7,
 // the operand fragment of v_mfma_f32_16x16x32_bf16 as it is.  Value 2 i of a
-// dword is at bit 4 i, value 2 i + 1 at bit 16 + 4 i, so shifting by 4 i and
-// masking gives two of them, and the bits 0x4300 above each make the bf16
-// number 128 + q: 7 instructions for 8 weights, where a conversion through f32
-// takes 12.  The 128 too much (and the 8) go out again through the
-// accumulator: a group's MFMAs begin at -136 * sum(a), which is an MFMA chain
-// of the same activations with a constant operand, shared by the tiles of a
-// wave.  (q - 8) * a is summed exactly as it would be in binary32 but for
-// the size of the partial sums, up to 17 times larger: 4 bits of 24.
+// dword is at bit 4 i + 3, value 2 i + 1 at bit 16 + 4 i + 3 (modulo 32), so turning
+// it by 4 i and masking gives two of them, each on the upper four fraction bits
+// of a bf16 number, and the bits 0x4180 around them make that 16 + q: 7
+// instructions for 8 weights, where a conversion through f32 takes 12.  The 16
+// too much (and the 8) go out again through the accumulator: a group's MFMAs
+// begin at -24 * sum(a), which is an MFMA chain of the same activations with a
+// constant operand, shared by the tiles of a wave.  (q - 8) * a is summed as it
+// would be in binary32 but for the size of the partial sums, up to 4 times
+// larger: 2 bits of 24.  (16 is the least power of two that all of 0..15 lie
+// behind without a step of the exponent.  128 + q, whose bits need no turning, makes them up
+// to 17 times larger: where sums of 512 products cancel, 2.2e-5 to 1.1e-4 was
+// left of them, and 1.5e-6 to 6.9e-6 is now, at the same speed.)
 // A group's sum is then scaled and added in binary32.
 //
 // Two tiles (32 rows) of one k range are neighbours, their k ranges follow each
@@ -33,8 +37,9 @@ namespace {
 constexpr int kSb = 32;                 // weight rows of a superblock: two tiles
 constexpr int kKt = 128;                // k of a tile
 constexpr int kTileBytes = 1024;
-constexpr uint32_t kMagic = 0x43004300u;    // bf16 128 | q
-constexpr uint32_t kOffset = 0xC308C308u;   // bf16 -136, twice
+constexpr uint32_t kMask = 0x00780078u;     // the bits of two values
+constexpr uint32_t kMagic = 0x41804180u;    // bf16 16, twice
+constexpr uint32_t kOffset = 0xC1C0C1C0u;   // bf16 -24, twice
 
 // Sizes of a weight; the derived ones are the host's (a division takes a wave
 // some 40 instructions).
@@ -54,11 +59,14 @@ struct W4Shape {
     }
 };
 
-// (v >> shift & 0x000F000F) | 0x43004300 in one instruction behind the shift:
-// v_and_or_b32 takes one scalar register and no two literals.
-__device__ __forceinline__ uint32_t unpack2(uint32_t v, int shift, uint32_t mask_s, uint32_t magic_v)
+// Values 2 i and 2 i + 1 of a dword as bf16 16 + q, `turn` = 4 i: one instruction
+// behind the turning (v_and_or_b32 takes one scalar register and no two literals).
+__device__ __forceinline__ uint32_t turned(uint32_t v, int turn) { return v >> turn | v << (-turn & 31); }
+
+__device__ __forceinline__ uint32_t unpack2(uint32_t v, int turn, uint32_t mask_s, uint32_t magic_v)
 {
-    return ((v >> shift) & mask_s) | magic_v;
+    // (only the last two wrap; a shift's encoding is half as long)
+    return ((turn < 12 ? v >> turn : turned(v, turn)) & mask_s) | magic_v;
 }
 
 __device__ __forceinline__ float scale16(uint32_t bits16, bool half)
@@ -87,7 +95,7 @@ __global__ __launch_bounds__(256) void w4_pack_kernel(const uint8_t* q, const ui
         for (int i = (int)threadIdx.x; i < 2 * kTileBytes / 4; i += 256) {
             const int tile = i >> 8, lane = i >> 2 & 63, s = i & 3;
             const int r = 16 * tile + (lane & 15), k = kt * kKt + 32 * s + 8 * (lane >> 4);
-            uint32_t out = 0x88888888u;
+            uint32_t out = 0x88888888u;    // value 2 j at bit 4 j, value 2 j + 1 at bit 16 + 4 j
             if (r < rows && k < w.K) {     // (K a multiple of 8: all of the 8 or none)
                 const uint8_t* src = q + (((int64_t)e * w.N + row0 + r) * w.K + k) / 2;
                 out = 0;
@@ -97,7 +105,7 @@ __global__ __launch_bounds__(256) void w4_pack_kernel(const uint8_t* q, const ui
                     out |= (uint32_t)(src[j] >> 4) << (16 + 4 * j);
                 }
             }
-            packed[blk * (2 * kTileBytes / 4) + i] = out;
+            packed[blk * (2 * kTileBytes / 4) + i] = turned(out, 29);
         }
         for (int i = (int)threadIdx.x; i < gpt * kSb; i += 256) {
             const int r = scale_row(i % kSb), g = kt * gpt + i / kSb;
@@ -124,7 +132,7 @@ __global__ __launch_bounds__(256) void w4_unpack_kernel(const uint32_t* packed, 
             const int tile = i >> 8, r16 = i >> 4 & 15, s = i >> 2 & 3, rho = i & 3;
             const int r = 16 * tile + r16, in = 32 * s + 8 * rho, k = kt * kKt + in;
             if (r >= rows || k >= w.K) continue;
-            const uint32_t v = packed[blk * (2 * kTileBytes / 4) + 256 * tile + 4 * (16 * rho + r16) + s];
+            const uint32_t v = turned(packed[blk * (2 * kTileBytes / 4) + 256 * tile + 4 * (16 * rho + r16) + s], 3);
             const int at = 8 * ((r & 15) >> 2) + 4 * (r >> 4) + (r & 3);
             const float sc = scale16(packed_scales[(blk * gpt + in / w.group) * kSb + at], half);
             u32x4_t o;
@@ -226,7 +234,7 @@ __device__ __forceinline__ void constants(std::integer_sequence<int, I...>, F f)
 
 // The two constants of unpacking, kept in registers.
 struct Unpack {
-    uint32_t mask = 0x000F000Fu, magic = kMagic;
+    uint32_t mask = kMask, magic = kMagic;
     __device__ __forceinline__ Unpack()
     {
         asm("" : "+s"(mask));
