@@ -293,7 +293,8 @@ class AdamW:
                 if v is not None:
                     v.copy_(p.detach())
         _check_masters(self.params, masters, self._index, self._sizes)
-        self.masters = None if masters is None else list(masters)
+        # (a list of None alone, for float32 parameters only, is no masters)
+        self.masters = list(masters) if torch.bfloat16 in self._dtypes else None
         # (the states' own buffers never move)
         self._one_type = len(set(self._dtypes)) == 1
         self._at = list(map(_data_ptr, self.params))

@@ -499,3 +499,15 @@ def test_refusals(et, dev):
     with pytest.raises(ValueError, match="expected"):
         opt.load_state_dict({"steps": 3})
     assert ctypes.sizeof(ctypes.c_void_p) == 8
+
+
+def test_masters_that_are_all_none(et, dev):
+    g = [torch.randn(33, device=dev), torch.randn(5, device=dev)]
+    p, q = ([torch.ones(33, device=dev), torch.ones(5, device=dev)] for _ in range(2))
+    a, b = et.AdamW(p, masters=[None, None]), et.AdamW(q)
+    for _ in range(2):
+        a.step(g), b.step(g)
+        a.step([g[0], None]), b.step([g[0], None])
+    assert all(torch.equal(x, y) for x, y in zip(p, q))
+    b.load_state_dict(a.state_dict())
+    a.load_state_dict(b.state_dict())
