@@ -250,7 +250,9 @@ class AdamW:
     masters of bfloat16 parameters, unless given) are views of one allocation
     for each kind, ``flat[name]``, each tensor from a multiple of 256 elements
     on.  ``step(grads)`` takes one gradient for each parameter, or None for one
-    that has none this time.  The parameters' own storage may move between
+    that has none this time: it stays as it is, and the step number in its bias
+    corrections counts its own steps.  ``steps`` counts the calls; setting it sets
+    every parameter's number.  The parameters' own storage may move between
     steps (``p.data = ...``) as long as type, shape, layout and device stay.
     """
 
@@ -265,7 +267,7 @@ class AdamW:
         if state not in ("f32", "e4m3"):
             raise ValueError(f"state must be 'f32' or 'e4m3', got {state!r}")
         self.lr, self.betas, self.eps, self.weight_decay = lr, betas, eps, weight_decay
-        self.state, self.stochastic, self.seed, self.steps = state, bool(stochastic), int(seed), 0
+        self.state, self.stochastic, self.seed, self.steps = state, bool(stochastic), int(seed), 0     # (and _counts)
         self._starts, n = [], 0
         for size in self._sizes:
             self._starts.append(n)
@@ -302,9 +304,18 @@ class AdamW:
         self._tables = [_pointers(s) for s in self._states]
         self._numel = _numel_array(self._sizes)
 
+    @property
+    def steps(self) -> int:
+        return self._steps
+
+    @steps.setter
+    def steps(self, number: int) -> None:
+        self._steps = number
+        self._counts = None         # each parameter's steps, where they are not all this number
+
     def step(self, grads: Sequence[Optional[torch.Tensor]], *, grad_scale: Optional[torch.Tensor] = None,
              lr: Optional[float] = None) -> None:
-        """One step; ``lr`` for this step only.  The step number counts the steps
+        """One step; ``lr`` for this step only.  The step numbers count the steps
         that a grad_scale that is not finite made the device skip, too."""
         params, sizes, states, masters = self.params, self._sizes, self._states, self.masters
         dev = params[0].device
@@ -323,6 +334,8 @@ class AdamW:
             if g is None:
                 whole = False
                 break
+        number, counts = self._steps, self._counts
+        some = range(len(params))
         if not whole:
             some = [i for i, g in enumerate(grads) if g is not None]
             params, grads, sizes = ([ts[i] for i in some] for ts in (params, grads, sizes))
@@ -330,29 +343,43 @@ class AdamW:
             masters = None if masters is None else [masters[i] for i in some]
         _check_list(grads, "grads", _DTYPES.keys(), self._index, sizes)
         _check_scale(grad_scale, dev)
-        scalars = _scalars(self.steps + 1, self.lr if lr is None else lr, self.betas, self.eps, self.weight_decay)
+        hyper = self.lr if lr is None else lr, self.betas, self.eps, self.weight_decay
+        scalars = _scalars(number + 1, *hyper)
         fn, more = "et_adamw", ()
         if self.state == "e4m3":
-            fn, more = "et_adamw8", (int(self.stochastic), (self.seed + self.steps + 1) & 0xFFFFFFFF)
-        if whole and self._one_type and len({g.dtype for g in grads}) == 1:
+            fn, more = "et_adamw8", (int(self.stochastic), (self.seed + number + 1) & 0xFFFFFFFF)
+        if counts is not None:          # one step number to a call
+            ages = [counts[i] for i in some]
+            for age in dict.fromkeys(ages):
+                at = [j for j, n in enumerate(ages) if n == age]
+                of = lambda ts: [ts[j] for j in at]  # noqa: E731
+                _step(fn, dev, of(params), of(grads), [of(s) for s in states], None if masters is None else of(masters),
+                      of(sizes), _scalars(age + 1, *hyper), grad_scale, *more)
+        elif whole and self._one_type and len({g.dtype for g in grads}) == 1:
             _call(fn, dev, self._param_table, _pointers(grads), *self._tables,
                   None if masters is None else _pointers(masters), self._numel, len(params),
                   _DTYPES[self._dtypes[0]], _DTYPES[grads[0].dtype], scalars, _vp(grad_scale), *more)
         elif params:
             _step(fn, dev, params, grads, states, masters, sizes, scalars, grad_scale, *more)
-        self.steps += 1
+        if counts is None and not whole:
+            counts = self._counts = [number] * len(self.params)
+        if counts is not None:
+            for i in some:
+                counts[i] += 1
+        self._steps = number + 1
 
     def state_dict(self) -> dict:
-        """Copies of the states and masters (flat), and the step number."""
+        """Copies of the states and masters (flat), the step number and each parameter's."""
         held = {k: v.clone() for k, v in self.flat.items()}
         if self.masters is not None and "masters" not in held:
             held["masters"] = [None if m is None else m.clone() for m in self.masters]
-        return dict(held, steps=self.steps)
+        return dict(held, steps=self.steps, counts=[self.steps] * len(self.params) if self._counts is None else list(self._counts))
 
     def load_state_dict(self, held: dict) -> None:
-        """Takes over :meth:`state_dict`'s values; the parameters are the caller's."""
+        """Takes over :meth:`state_dict`'s values; the parameters are the caller's.
+        Without ``counts`` every parameter has had ``steps`` steps."""
         names = set(self.flat) | ({"masters"} if self.masters is not None else set()) | {"steps"}
-        if set(held) != names:
+        if set(held) - {"counts"} != names:
             raise ValueError(f"state has {sorted(held)}, expected {sorted(names)}")
         for k, v in self.flat.items():
             if held[k].shape != v.shape or held[k].dtype != v.dtype:
@@ -366,3 +393,5 @@ class AdamW:
         for k, v in self.flat.items():
             v.copy_(held[k])
         self.steps = int(held["steps"])
+        if any(n != self.steps for n in held.get("counts", ())):
+            self._counts = list(held["counts"])

@@ -511,3 +511,65 @@ def test_masters_that_are_all_none(et, dev):
     assert all(torch.equal(x, y) for x, y in zip(p, q))
     b.load_state_dict(a.state_dict())
     a.load_state_dict(b.state_dict())
+
+
+# --------------------------------------------------------------------------- #
+# parameters of different ages, copies, what a state may hold
+# --------------------------------------------------------------------------- #
+
+@pytest.mark.parametrize("state", ["f32", "e4m3"])
+@pytest.mark.parametrize("dtypes", [(torch.float32,) * 3, (torch.bfloat16, torch.float32, torch.bfloat16)], ids=["one", "two"])
+def test_a_parameter_without_gradients_keeps_its_step_number(et, dev, state, dtypes):
+    """A parameter whose first gradient arrives late takes its first step: the
+    bits of an optimizer of its own that began then."""
+    late = 1000
+    shapes = [(700,), (3, 5), (300,)]
+    g = torch.Generator().manual_seed(2)
+    p = [torch.randn(s, generator=g).to(dev).to(t) for s, t in zip(shapes, dtypes)]
+    q = [t.clone() for t in p]
+    kw = dict(state=state, stochastic=False, **HYPER)
+    opt, alone = et.AdamW(p, **kw), [et.AdamW([t], **kw) for t in q]
+    opt.steps = late                # (as after so many steps with every gradient)
+    alone[0].steps = alone[2].steps = late
+    opt._counts = [late, 0, late]   # but for the second parameter, which had none
+    for turn in range(4):
+        grads = [torch.randn(s, generator=g).to(dev) for s in shapes]
+        if turn == 2:
+            grads[2] = None
+        opt.step(grads)
+        for a, t in zip(alone, grads):
+            if t is not None:
+                a.step([t])
+        assert opt.steps == late + turn + 1
+        assert all(torch.equal(x, y) for x, y in zip(p, q)), turn
+        if turn == 2:               # a state that is loaded goes on the same way
+            held = opt.state_dict()
+            opt = et.AdamW(p, **kw)
+            opt.load_state_dict(held)
+
+
+def test_step_numbers_against_64_bits(et, dev):
+    """Four parameters, gradients in some of twelve steps: every weight is that
+    of the formula with its own number of steps."""
+    g = torch.Generator().manual_seed(7)
+    w = [torch.randn(50, generator=g) for _ in range(4)]
+    p = [t.to(dev) for t in w]
+    opt = et.AdamW(p, **HYPER)
+    (b1, b2), lr, eps, wd = HYPER["betas"], HYPER["lr"], HYPER["eps"], HYPER["weight_decay"]
+    w, m, v, n = [t.double() for t in w], [0.0] * 4, [0.0] * 4, [0] * 4
+    for turn in range(12):
+        # gradients of one sign: the denominator stays away from 0
+        grads = [torch.rand(50, generator=g) + 0.5 for _ in range(4)]
+        has = [True, turn >= 9, turn % 3 == 1, turn < 2]
+        opt.step([t.to(dev) if h else None for t, h in zip(grads, has)])
+        for i in range(4):
+            if has[i]:
+                x = grads[i].double()
+                n[i] += 1
+                m[i], v[i] = b1 * m[i] + (1 - b1) * x, b2 * v[i] + (1 - b2) * x * x
+                w[i] = w[i] * (1 - lr * wd) - lr / (1 - b1 ** n[i]) * m[i] / ((v[i] / (1 - b2 ** n[i])).sqrt() + eps)
+    for i in range(4):
+        # a step moves a weight by 1.3 lr at most (m and sqrt(v) are averages of [0.5, 1.5]) with some 40
+        # roundings (of the constants and of both averages' histories), and rounds it three times
+        bound = n[i] * (1.3 * lr * 40 * U + 3 * U * (w[i].abs() + 1.3 * lr * n[i]))
+        assert torch.all((p[i].cpu().double() - w[i]).abs() <= bound), i
