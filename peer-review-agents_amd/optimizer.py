@@ -272,37 +272,64 @@ class AdamW:
         for size in self._sizes:
             self._starts.append(n)
             n += adamw8_scales(size) * ADAMW8_BLOCK
-        self.flat = {}
-
-        def views(name, dtype, per=1):
-            flat = self.flat[name] = torch.zeros(n // per, dtype=dtype, device=dev)
-            if per > 1:
-                return [flat[a // per:a // per + adamw8_scales(s)] for a, s in zip(self._starts, self._sizes)]
-            return [flat[a:a + s].view(p.shape) for a, s, p in zip(self._starts, self._sizes, self.params)]
-
+        if masters is not None:
+            _check_masters(self.params, masters, self._index, self._sizes)
+        # (a list of None alone, for float32 parameters only, is no masters)
+        self.masters = list(masters) if masters is not None and torch.bfloat16 in self._dtypes else None
         if state == "f32":
-            self.exp_avg, self.exp_avg_sq = (views(k, torch.float32) for k in ("exp_avg", "exp_avg_sq"))
-            self._states = self.exp_avg, self.exp_avg_sq
+            kinds = dict(exp_avg=torch.float32, exp_avg_sq=torch.float32)
         else:
-            self.exp_avg, self.exp_avg_root = (views(k, torch.float8_e4m3fn) for k in ("exp_avg", "exp_avg_root"))
-            self.exp_avg_scale, self.exp_avg_root_scale = (
-                views(k, torch.float32, ADAMW8_BLOCK) for k in ("exp_avg_scale", "exp_avg_root_scale"))
-            self._states = self.exp_avg, self.exp_avg_scale, self.exp_avg_root, self.exp_avg_root_scale
-        if masters is None and torch.bfloat16 in self._dtypes:
-            masters = [v if p.dtype == torch.bfloat16 else None
-                       for v, p in zip(views("masters", torch.float32), self.params)]
-            for v, p in zip(masters, self.params):
+            e4m3 = torch.float8_e4m3fn
+            kinds = dict(exp_avg=e4m3, exp_avg_scale=torch.float32, exp_avg_root=e4m3, exp_avg_root_scale=torch.float32)
+        self._names = tuple(kinds)
+        own = masters is None and torch.bfloat16 in self._dtypes
+        if own:
+            kinds["masters"] = torch.float32
+        self.flat = {k: torch.zeros(n // self._per(k), dtype=t, device=dev) for k, t in kinds.items()}
+        self._lay_out()
+        if own:
+            for v, p in zip(self.masters, self.params):
                 if v is not None:
                     v.copy_(p.detach())
-        _check_masters(self.params, masters, self._index, self._sizes)
-        # (a list of None alone, for float32 parameters only, is no masters)
-        self.masters = list(masters) if torch.bfloat16 in self._dtypes else None
-        # (the states' own buffers never move)
+
+    @staticmethod
+    def _per(name: str) -> int:
+        """Elements of a parameter for each of a state's."""
+        return ADAMW8_BLOCK if name.endswith("_scale") else 1
+
+    def _views(self, name: str) -> list:
+        flat, per = self.flat[name], self._per(name)
+        if per > 1:
+            return [flat[a // per:a // per + adamw8_scales(s)] for a, s in zip(self._starts, self._sizes)]
+        return [flat[a:a + s].view(p.shape) for a, s, p in zip(self._starts, self._sizes, self.params)]
+
+    def _lay_out(self) -> None:
+        """The states as views of `flat`, and the tables of pointers that a step of
+        all tensors hands over (the states' own buffers never move)."""
+        self._states = tuple(map(self._views, self._names))
+        for name, views in zip(self._names, self._states):
+            setattr(self, name, views)
+        if "masters" in self.flat:
+            self.masters = [v if t == torch.bfloat16 else None for v, t in zip(self._views("masters"), self._dtypes)]
         self._one_type = len(set(self._dtypes)) == 1
         self._at = list(map(_data_ptr, self.params))
         self._param_table = _array(self._at)
         self._tables = [_pointers(s) for s in self._states]
         self._numel = _numel_array(self._sizes)
+
+    def __getstate__(self) -> dict:
+        """What a copy or a pickle holds: all but the views and the pointers."""
+        state = dict(self.__dict__)
+        for name in self._names + ("_states", "_at", "_param_table", "_tables", "_numel"):
+            del state[name]
+        if "masters" in self.flat:
+            del state["masters"]
+        return state
+
+    def __setstate__(self, state: dict) -> None:
+        self.__dict__.update(state)
+        self._index, _ = _check_params(self.params)     # (on another device, perhaps; never on the host)
+        self._lay_out()
 
     @property
     def steps(self) -> int:

@@ -573,3 +573,34 @@ def test_step_numbers_against_64_bits(et, dev):
         # roundings (of the constants and of both averages' histories), and rounds it three times
         bound = n[i] * (1.3 * lr * 40 * U + 3 * U * (w[i].abs() + 1.3 * lr * n[i]))
         assert torch.all((p[i].cpu().double() - w[i]).abs() <= bound), i
+
+
+@pytest.mark.parametrize("state", ["f32", "e4m3"])
+@pytest.mark.parametrize("given", [False, True])
+def test_copies_and_pickles_go_on_alike(et, dev, state, given):
+    import copy
+    import io
+    p = _random_params(dev, torch.bfloat16)
+    opt = et.AdamW(p, state=state, masters=[t.float() for t in p] if given else None, **HYPER)
+    g = [[torch.randn(t.shape, device=dev) for t in p] for _ in range(3)]
+    opt.step(g[0])
+    opt.step([None] + g[0][1:])
+    buf = io.BytesIO()
+    torch.save(opt, buf)
+    buf.seek(0)
+    others = [copy.deepcopy(opt), torch.load(buf, weights_only=False)]
+    buf.seek(0)
+    with pytest.raises(ValueError, match="HIP device"):
+        torch.load(buf, weights_only=False, map_location="cpu")
+    for other in others:
+        assert all(a.data_ptr() != b.data_ptr() for a, b in zip(opt.params, other.params))
+        assert all(v.untyped_storage().data_ptr() == other.flat["exp_avg"].untyped_storage().data_ptr()
+                   for v in other.exp_avg)
+        other.step(g[1]), other.step(g[2])
+    mid = [t.clone() for t in p]
+    opt.step(g[1]), opt.step(g[2])
+    assert not all(torch.equal(a, b) for a, b in zip(mid, p))
+    for other in others:
+        assert all(torch.equal(a, b) for a, b in zip(p, other.params))
+        assert all(torch.equal(a, b) for a, b in zip(opt.masters, other.masters))
+        assert other.steps == 4
