@@ -408,17 +408,30 @@ class AdamW:
         names = set(self.flat) | ({"masters"} if self.masters is not None else set()) | {"steps"}
         if set(held) - {"counts"} != names:
             raise ValueError(f"state has {sorted(held)}, expected {sorted(names)}")
+        # (everything is looked over before anything changes: copy_ would broadcast)
+        def check(t, like, name):
+            if not isinstance(t, torch.Tensor) or t.dtype != like.dtype or t.shape != like.shape:
+                got = f"{t.dtype} of shape {tuple(t.shape)}" if isinstance(t, torch.Tensor) else type(t).__name__
+                raise ValueError(f"{name} must be {like.dtype} of shape {tuple(like.shape)}, got {got}")
+
         for k, v in self.flat.items():
-            if held[k].shape != v.shape or held[k].dtype != v.dtype:
-                raise ValueError(f"{k} must be {v.dtype} of shape {tuple(v.shape)}")
+            check(held[k], v, k)
+        pairs = [(v, held[k]) for k, v in self.flat.items()]
         if "masters" in held and "masters" not in self.flat:
-            if len(held["masters"]) != len(self.masters):
-                raise ValueError("masters must have one entry for each parameter")
-            for mine, other in zip(self.masters, held["masters"]):
+            if not isinstance(held["masters"], (list, tuple)) or len(held["masters"]) != len(self.masters):
+                raise ValueError("masters must be a list of one entry for each parameter")
+            for i, (mine, other) in enumerate(zip(self.masters, held["masters"])):
                 if mine is not None:
-                    mine.copy_(other)
-        for k, v in self.flat.items():
-            v.copy_(held[k])
-        self.steps = int(held["steps"])
-        if any(n != self.steps for n in held.get("counts", ())):
-            self._counts = list(held["counts"])
+                    check(other, mine, f"masters[{i}]")
+                    pairs.append((mine, other))
+        steps = int(held["steps"])
+        counts = list(map(int, held.get("counts", [steps] * len(self.params))))
+        if steps < 0:
+            raise ValueError(f"steps must be >= 0, got {steps}")
+        if len(counts) != len(self.params) or not all(0 <= n <= steps for n in counts):
+            raise ValueError("counts must hold a number of steps for each parameter, none above steps")
+        for mine, other in pairs:
+            mine.copy_(other)
+        self.steps = steps
+        if any(n != steps for n in counts):
+            self._counts = counts

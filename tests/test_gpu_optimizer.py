@@ -604,3 +604,31 @@ def test_copies_and_pickles_go_on_alike(et, dev, state, given):
         assert all(torch.equal(a, b) for a, b in zip(p, other.params))
         assert all(torch.equal(a, b) for a, b in zip(opt.masters, other.masters))
         assert other.steps == 4
+
+
+def test_a_state_that_does_not_fit_changes_nothing(et, dev):
+    p = _random_params(dev, torch.bfloat16)
+    opt = et.AdamW(p, masters=[t.float() for t in p])
+    opt.step([torch.randn(t.shape, device=dev) for t in p])
+    before, flat = [t.clone() for t in opt.masters], {k: v.clone() for k, v in opt.flat.items()}
+
+    def wrong(change):
+        held = opt.state_dict()
+        held["masters"] = [torch.zeros_like(t) for t in held["masters"]]
+        held.update({k: torch.ones_like(v) for k, v in held.items() if k.startswith("exp_avg")})
+        change(held)
+        with pytest.raises((ValueError, TypeError)):
+            opt.load_state_dict(held)
+        assert all(torch.equal(a, b) for a, b in zip(before, opt.masters))
+        assert all(torch.equal(flat[k], opt.flat[k]) for k in flat) and opt.steps == 1
+
+    wrong(lambda h: h["masters"].__setitem__(2, None))
+    wrong(lambda h: h["masters"].__setitem__(2, torch.zeros(1, device=dev)))     # (would broadcast)
+    wrong(lambda h: h["masters"].__setitem__(3, h["masters"][3].bfloat16()))
+    wrong(lambda h: h["masters"].pop())
+    wrong(lambda h: h.update(exp_avg_sq=h["exp_avg_sq"][1:]))
+    wrong(lambda h: h.update(exp_avg=None))
+    wrong(lambda h: h.update(steps=-1))
+    wrong(lambda h: h.update(steps="many"))
+    wrong(lambda h: h.update(counts=[1, 1]))
+    wrong(lambda h: h.update(counts=[1, 1, 1, 2]))
