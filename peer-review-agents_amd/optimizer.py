@@ -97,6 +97,14 @@ def _check_masters(params, masters, device, sizes) -> None:
                 [n for n, b in zip(sizes, low) if b])
 
 
+def _check_apart(ts, name: str) -> None:
+    """No two of the tensors share memory: a step reads and writes each at once."""
+    spans = sorted((t.data_ptr(), t.numel() * t.element_size()) for t in ts if t is not None and t.numel())
+    for (at, size), (next_at, _) in zip(spans, spans[1:]):
+        if at + size > next_at:
+            raise ValueError(f"{name} overlap in memory (or hold a tensor more than once)")
+
+
 def _scalars(step: int, lr: float, betas, eps: float, weight_decay: float) -> AdamWScalars:
     step = int(step)
     b1, b2 = (float(b) for b in betas)
@@ -195,7 +203,8 @@ def adamw_step_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], e
     w being its float32 master (``masters[i]``, None for float32 parameters).
     exp_avg (m) and exp_avg_sq (v) are float32; grads float32 or bfloat16.
     ``grad_scale`` is one float32 value on the device (:func:`grad_norm`'s); the
-    step is skipped, every bit kept, where it is not finite.
+    step is skipped, every bit kept, where it is not finite.  No two tensors may
+    share memory.
     """
     index, sizes = _check_params(params)
     dev = params[0].device
@@ -274,6 +283,7 @@ class AdamW:
             n += adamw8_scales(size) * ADAMW8_BLOCK
         if masters is not None:
             _check_masters(self.params, masters, self._index, self._sizes)
+        _check_apart(self.params + list(masters or ()), "parameters and masters")
         # (a list of None alone, for float32 parameters only, is no masters)
         self.masters = list(masters) if masters is not None and torch.bfloat16 in self._dtypes else None
         if state == "f32":

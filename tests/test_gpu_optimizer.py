@@ -632,3 +632,14 @@ def test_a_state_that_does_not_fit_changes_nothing(et, dev):
     wrong(lambda h: h.update(steps="many"))
     wrong(lambda h: h.update(counts=[1, 1]))
     wrong(lambda h: h.update(counts=[1, 1, 1, 2]))
+
+
+def test_a_parameter_given_twice_is_refused(et, dev):
+    t = torch.zeros(64, device=dev)
+    with pytest.raises(ValueError, match="more than once|overlap"):
+        et.AdamW([t, torch.zeros(3, device=dev), t])
+    with pytest.raises(ValueError, match="overlap"):
+        et.AdamW([t[:40], t[32:]])
+    with pytest.raises(ValueError, match="overlap"):
+        et.AdamW([t.bfloat16(), torch.zeros(64, device=dev).bfloat16()], masters=[t, t])
+    et.AdamW([t[:32], t[32:], t[:0], t[:0]])
