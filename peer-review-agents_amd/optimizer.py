@@ -46,17 +46,18 @@ def _numel_array(sizes):
     return (ctypes.c_int64 * len(sizes))(*sizes)
 
 
-def _check_list(ts, name: str, dtypes, device: int, sizes) -> None:
+def _check_list(ts, name: str, dtypes, device: int, sizes) -> set:
     """Every tensor of `ts` contiguous, on HIP device `device`, of one of
-    `dtypes` and of as many elements as `sizes` says."""
+    `dtypes` and of as many elements as `sizes` says.  Returns their dtypes."""
     if not isinstance(ts, (list, tuple)):
         raise TypeError(f"{name} must be a list or a tuple of tensors")
     if len(ts) != len(sizes):
         raise ValueError(f"{name} has {len(ts)} tensors, params has {len(sizes)}")
     try:        # (the unbound methods refuse what is no tensor)
-        if (list(map(_numel, ts)) == sizes and all(map(_is_contiguous, ts)) and set(map(_get_device, ts)) <= {device}
-                and {t.dtype for t in ts} <= dtypes):
-            return
+        if list(map(_numel, ts)) == sizes and all(map(_is_contiguous, ts)) and set(map(_get_device, ts)) <= {device}:
+            found = {t.dtype for t in ts}
+            if found <= dtypes:
+                return found
     except TypeError:
         raise TypeError(f"{name} must hold torch.Tensors") from None
     for i, t in enumerate(ts):
@@ -69,6 +70,7 @@ def _check_list(ts, name: str, dtypes, device: int, sizes) -> None:
             raise ValueError(f"{name}[{i}] has {t.numel()} elements, expected {sizes[i]}")
         if t.get_device() != device:
             raise ValueError(f"{name}[{i}] is on {t.device}, expected cuda:{device}")
+    return {t.dtype for t in ts}
 
 
 def _check_params(params) -> tuple:
@@ -176,6 +178,11 @@ def _kinds(params, grads):
     return [[i for i, q in enumerate(pairs) if q == pair] for pair in dict.fromkeys(pairs)]
 
 
+# The parameters have changed: a backward that kept one of them as it was before
+# raises, as behind any in-place operation of torch (55 ns a tensor).
+_changed = torch.autograd.graph.increment_version
+
+
 def _step(fn: str, dev, params, grads, states, masters, sizes, scalars, grad_scale, *more) -> None:
     """The library calls of one step, its lists checked."""
     for at in _kinds(params, grads):
@@ -215,6 +222,7 @@ def adamw_step_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], e
     _check_scale(grad_scale, dev)
     _step("et_adamw", dev, params, grads, (exp_avg, exp_avg_sq), masters, sizes,
           _scalars(step, lr, betas, eps, weight_decay), grad_scale)
+    _changed(params)
 
 
 def adamw8_scales(numel: int) -> int:
@@ -249,6 +257,7 @@ def adamw8_step_(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], 
     _check_scale(grad_scale, dev)
     _step("et_adamw8", dev, params, grads, (exp_avg, exp_avg_scale, exp_avg_root, exp_avg_root_scale), masters, sizes,
           _scalars(step, lr, betas, eps, weight_decay), grad_scale, int(seed is not None), (seed or 0) & 0xFFFFFFFF)
+    _changed(params)
 
 
 class AdamW:
@@ -378,7 +387,7 @@ class AdamW:
             params, grads, sizes = ([ts[i] for i in some] for ts in (params, grads, sizes))
             states = [[s[i] for i in some] for s in states]
             masters = None if masters is None else [masters[i] for i in some]
-        _check_list(grads, "grads", _DTYPES.keys(), self._index, sizes)
+        grad_types = _check_list(grads, "grads", _DTYPES.keys(), self._index, sizes)
         _check_scale(grad_scale, dev)
         hyper = self.lr if lr is None else lr, self.betas, self.eps, self.weight_decay
         scalars = _scalars(number + 1, *hyper)
@@ -392,12 +401,13 @@ class AdamW:
                 of = lambda ts: [ts[j] for j in at]  # noqa: E731
                 _step(fn, dev, of(params), of(grads), [of(s) for s in states], None if masters is None else of(masters),
                       of(sizes), _scalars(age + 1, *hyper), grad_scale, *more)
-        elif whole and self._one_type and len({g.dtype for g in grads}) == 1:
+        elif whole and self._one_type and len(grad_types) == 1:
             _call(fn, dev, self._param_table, _pointers(grads), *self._tables,
                   None if masters is None else _pointers(masters), self._numel, len(params),
                   _DTYPES[self._dtypes[0]], _DTYPES[grads[0].dtype], scalars, _vp(grad_scale), *more)
         elif params:
             _step(fn, dev, params, grads, states, masters, sizes, scalars, grad_scale, *more)
+        _changed(params)
         if counts is None and not whole:
             counts = self._counts = [number] * len(self.params)
         if counts is not None:

@@ -643,3 +643,29 @@ def test_a_parameter_given_twice_is_refused(et, dev):
     with pytest.raises(ValueError, match="overlap"):
         et.AdamW([t.bfloat16(), torch.zeros(64, device=dev).bfloat16()], masters=[t, t])
     et.AdamW([t[:32], t[32:], t[:0], t[:0]])
+
+
+def test_steps_count_as_changes_of_the_parameters(et, dev):
+    """A weight that the forward kept and a step has changed since is an error in
+    the backward, not a gradient of another weight."""
+    for state, dtype in (("f32", torch.float32), ("e4m3", torch.bfloat16)):
+        x = torch.randn(4, 8, device=dev, dtype=dtype, requires_grad=True)
+        w = torch.randn(8, 8, device=dev, dtype=dtype, requires_grad=True)
+        opt = et.AdamW([w], state=state)
+        y = (x.float() @ w.float().mul(w.float())).sum() + (x * w[0]).sum()
+        opt.step([torch.randn(8, 8, device=dev)])
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+        z = lambda dt=torch.float32, n=64: [torch.zeros(n, dtype=dt, device=dev)]  # noqa: E731
+        e4 = torch.float8_e4m3fn
+        p, s = z(), w._version
+        et.adamw_step_(p, z(), z(), z(), step=1, lr=0.1)
+        assert p[0]._version == 1
+        et.adamw8_step_(p, z(), z(e4), z(n=1), z(e4), z(n=1), step=1, lr=0.1)
+        assert p[0]._version == 2
+        opt.step([None])
+        assert w._version == s
+    with torch.inference_mode():
+        w = torch.ones(8, device=dev)
+        et.AdamW([w]).step([torch.ones(8, device=dev)])
+        assert torch.all(w < 1)
