@@ -26,6 +26,7 @@ from dataclasses import dataclass, replace
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._lib import (ET_DTYPE_BF16, ET_DTYPE_F32, ET_GEMM_PLAIN, ET_GEMM_ROW_SCALE, ET_GEMM_SWIGLU,
                    ET_MAX_EXPERTS, ET_MAX_ROUTER_EXPERTS, check, lib)
@@ -832,6 +833,7 @@ class _DispatchFn(torch.autograd.Function):
         return dispatch(x, plan)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dxp):
         return dispatch_backward(dxp.contiguous(), ctx.plan), None
 
@@ -844,6 +846,7 @@ class _CombineFn(torch.autograd.Function):
         return combine(yp, plan)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         (yp,) = ctx.saved_tensors
         dyp, _dgate, dl = combine_backward(dy.contiguous(), yp, ctx.plan,
@@ -852,14 +855,16 @@ class _CombineFn(torch.autograd.Function):
 
 
 def dispatch_autograd(x: torch.Tensor, plan: RoutingPlan) -> torch.Tensor:
-    """dispatch() with a backward that runs dispatch_backward()."""
+    """dispatch() with a backward that runs dispatch_backward().  A second
+    derivative raises."""
     return _DispatchFn.apply(x, plan)
 
 
 def combine_autograd(yp: torch.Tensor, logits: torch.Tensor, plan: RoutingPlan) -> torch.Tensor:
     """combine() differentiable in yp and in the router logits (through the
     gates, which are sigmoid(logits) at the routed pairs; the routing mask
-    itself is piecewise constant and has no gradient)."""
+    itself is piecewise constant and has no gradient).  A second derivative
+    raises."""
     return _CombineFn.apply(yp, logits, plan)
 
 

@@ -7,6 +7,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._lib import ET_MAX_NORM_WIDTH, lib
 from .expert_threshold import _ACT_DTYPES, _act_dtype, _call, _out_or_new, _require, _require_device, _vp
@@ -181,6 +182,7 @@ class _LayerNormFn(torch.autograd.Function):
         return y if residual is None else (y, h)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy, dsum=None):
         h, weight, mean, rstd = ctx.saved_tensors
         has_bias, has_residual = ctx.has
@@ -195,5 +197,5 @@ class _LayerNormFn(torch.autograd.Function):
 def layer_norm_autograd(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
                         eps: float = 1e-5, residual: Optional[torch.Tensor] = None):
     """:func:`layer_norm` (y, or (y, sum) with a residual) with a backward that
-    runs :func:`layer_norm_backward`."""
+    runs :func:`layer_norm_backward`.  A second derivative raises."""
     return _LayerNormFn.apply(x, weight, bias, eps, residual)

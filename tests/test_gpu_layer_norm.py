@@ -323,3 +323,23 @@ def test_refusals(et, dev):
         et.layer_norm_backward(x[:, :8], x, w, m, m)
     with pytest.raises(ValueError, match="workspace"):
         et.layer_norm_backward(x, x, w, m, m, workspace=torch.zeros(8, dtype=torch.uint8, device=dev))
+
+
+def test_a_second_derivative_is_an_error(et, dev):
+    """Not a gradient that lacks the terms through this one."""
+    def refuses(f, x):
+        grad, = torch.autograd.grad(f(x).float().square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            (grad.square().sum() + x.float().square().sum()).backward()
+
+    w = torch.ones(40, device=dev, requires_grad=True)
+    rows = lambda: torch.randn(5, 40, device=dev, requires_grad=True)  # noqa: E731
+    r = rows()
+    refuses(lambda x: et.layer_norm_autograd(x, w), rows())
+    refuses(lambda x: et.layer_norm_autograd(x, w, residual=r)[0], rows())
+    refuses(lambda x: torch.ops.etmoe.layer_norm(x, w, None, 1e-5)[0], rows())
+    refuses(lambda x: torch.ops.etmoe.add_layer_norm(x, r, w, None, 1e-5)[0], rows())
+    plan = et.route(torch.randn(5, 4, device=dev), torch.full((4,), 0.5, device=dev))
+    refuses(lambda x: et.dispatch_autograd(x, plan), rows())
+    yp = torch.randn(plan.rows, 40, device=dev, requires_grad=True)
+    refuses(lambda x: et.combine_autograd(x, torch.zeros(5, 4, device=dev), plan), yp)
