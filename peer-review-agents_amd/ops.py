@@ -35,7 +35,7 @@ Gradients: dispatch -> dispatch_backward; combine -> combine_backward, with
 respect to yp, to the router logits (through the gates, which are the
 sigmoid scores at the routed pairs: dlogits) and to slot_gate (dgate);
 layer_norm and add_layer_norm -> layer_norm_backward, with respect to the rows,
-the weight and the bias (mean and rstd are not differentiable).  The routing
+the weight and the bias (mean and rstd are marked as not differentiable).  The routing
 itself is piecewise constant and has no gradient.
 """
 from typing import Optional, Tuple
@@ -262,6 +262,7 @@ def _norm_grads(ctx, dy, h, dsum):
 def _layer_norm_setup(ctx, inputs, output):
     x, weight, bias, _eps = inputs
     ctx.has_bias = bias is not None
+    ctx.mark_non_differentiable(output[1], output[2])
     ctx.save_for_backward(weight, output[1], output[2], x)
 
 
@@ -275,6 +276,7 @@ torch.library.register_autograd("etmoe::layer_norm", _layer_norm_grad, setup_con
 def _add_layer_norm_setup(ctx, inputs, output):
     _x, _residual, weight, bias, _eps = inputs
     ctx.has_bias = bias is not None
+    ctx.mark_non_differentiable(output[2], output[3])
     ctx.save_for_backward(weight, output[2], output[3], output[1])
 
 

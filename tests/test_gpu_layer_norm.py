@@ -343,3 +343,12 @@ def test_a_second_derivative_is_an_error(et, dev):
     refuses(lambda x: et.dispatch_autograd(x, plan), rows())
     yp = torch.randn(plan.rows, 40, device=dev, requires_grad=True)
     refuses(lambda x: et.combine_autograd(x, torch.zeros(5, 4, device=dev), plan), yp)
+
+
+def test_statistics_carry_no_gradient(et, dev):
+    x, r = (torch.randn(5, 40, device=dev, requires_grad=True) for _ in range(2))
+    w = torch.ones(40, device=dev, requires_grad=True)
+    y, mean, rstd = torch.ops.etmoe.layer_norm(x, w, None, 1e-5)
+    assert y.requires_grad and not mean.requires_grad and not rstd.requires_grad
+    y, s, mean, rstd = torch.ops.etmoe.add_layer_norm(x, r, w, None, 1e-5)
+    assert y.requires_grad and s.requires_grad and not mean.requires_grad and not rstd.requires_grad
