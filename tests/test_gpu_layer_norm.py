@@ -352,3 +352,41 @@ def test_statistics_carry_no_gradient(et, dev):
     assert y.requires_grad and not mean.requires_grad and not rstd.requires_grad
     y, s, mean, rstd = torch.ops.etmoe.add_layer_norm(x, r, w, None, 1e-5)
     assert y.requires_grad and s.requires_grad and not mean.requires_grad and not rstd.requires_grad
+
+
+def test_add_layer_norm_operator(et, dev):
+    """torch.ops.etmoe.add_layer_norm under torch.compile, both outputs used."""
+    x, r = (torch.randn(33, 96, device=dev, requires_grad=True) for _ in range(2))
+    w, b = (torch.randn(96, device=dev, requires_grad=True) for _ in range(2))
+
+    def f(x, r, w, b):
+        y, s, _, _ = torch.ops.etmoe.add_layer_norm(x, r, w, b, 1e-5)
+        return (y ** 2).sum() + (s ** 3).sum()
+
+    torch.compile(f, fullgraph=True, backend="aot_eager")(x, r, w, b).backward()
+    got = x.grad, r.grad, w.grad, b.grad
+    leaves = [t.detach().clone().requires_grad_(True) for t in (x, r, w, b)]
+    y, s = et.layer_norm_autograd(leaves[0], leaves[2], leaves[3], residual=leaves[1])
+    ((y ** 2).sum() + (s ** 3).sum()).backward()
+    assert all(torch.equal(p, q.grad) for p, q in zip(got, leaves))
+    # one output alone
+    for pick in (0, 1):
+        for t in (x, r):
+            t.grad = None
+        torch.ops.etmoe.add_layer_norm(x, r, w, None, 1e-5)[pick].sum().backward()
+        assert torch.equal(x.grad, r.grad) and (pick == 0 or torch.all(x.grad == 1))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_opcheck(et, dev, dtype):
+    x, r = (torch.randn(9, 40, device=dev).to(dtype).requires_grad_(True) for _ in range(2))
+    w, b = (torch.randn(40, device=dev, requires_grad=True) for _ in range(2))
+    tests = ("test_schema", "test_faketensor", "test_autograd_registration")
+    ops = torch.ops.etmoe
+    for bias in (b, None):
+        torch.library.opcheck(ops.layer_norm.default, (x, w, bias, 1e-5), test_utils=tests)
+        torch.library.opcheck(ops.add_layer_norm.default, (x, r, w, bias, 1e-5), test_utils=tests)
+    _, mean, rstd = ops.layer_norm(x.detach(), w.detach(), None, 1e-5)
+    for ds in (None, r.detach()):
+        torch.library.opcheck(ops.layer_norm_backward.default, (r.detach(), x.detach(), w.detach(), mean, rstd, ds),
+                              test_utils=("test_schema", "test_faketensor"))
