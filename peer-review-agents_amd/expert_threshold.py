@@ -85,6 +85,13 @@ def _require(t: torch.Tensor, name: str, dtype, ndim: int, device=None) -> None:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
 
 
+def _require_workspace(t: torch.Tensor, nbytes: int, dev: torch.device, name: str) -> None:
+    """`t` has so many bytes of its own: elements that lie apart, or on one
+    another (an expanded tensor), do not make memory that a kernel can fill."""
+    if t.device != dev or not t.is_contiguous() or t.numel() * t.element_size() < nbytes:
+        raise ValueError(f"{name} must hold {nbytes} bytes on {dev}, contiguous")
+
+
 def _act_dtype(t: torch.Tensor, name: str) -> int:
     if t.dtype not in _ACT_DTYPES:
         raise TypeError(f"{name} must be float32 or bfloat16, got {t.dtype}")
@@ -193,8 +200,8 @@ def route(logits: torch.Tensor, thr: torch.Tensor, *, slot_capacity: Optional[in
     wsb = route_workspace_bytes(T, E)
     if workspace is None:
         workspace = torch.empty(wsb, dtype=torch.uint8, device=dev)
-    elif workspace.device != dev or workspace.numel() * workspace.element_size() < wsb:
-        raise ValueError(f"workspace must hold {wsb} bytes on {dev}")
+    else:
+        _require_workspace(workspace, wsb, dev, "workspace")
     _call("et_route", dev, _vp(logits), _vp(thr), T, E, _vp(counts), _vp(eo), _vp(to), _vp(st), _vp(sg), _vp(ts), cap,
           _vp(workspace), wsb)
     plan = RoutingPlan(counts, eo, to, st, sg, ts, T, E, cap)
@@ -308,8 +315,8 @@ def combine_backward(dy: torch.Tensor, yp: torch.Tensor, plan: RoutingPlan, *,
     wsb = combine_backward_workspace_bytes(T, plan.rows, d, dy.dtype)
     if workspace is None:
         workspace = torch.empty(max(wsb, 1), dtype=torch.uint8, device=dev)
-    elif workspace.device != dev or workspace.numel() * workspace.element_size() < wsb:
-        raise ValueError(f"workspace must hold {wsb} bytes on {dev}")
+    else:
+        _require_workspace(workspace, wsb, dev, "workspace")
     _call("et_combine_bwd", dev, _vp(dy), _vp(yp), _vp(plan.slot_gate), _vp(plan.sorted_token),
           _vp(plan.token_offsets), _vp(plan.token_slot), _vp(plan.expert_offsets), T, E, d, dt, plan.rows, _vp(dyp),
           _vp(dgate), _vp(dl), _vp(workspace), workspace.numel() * workspace.element_size())
@@ -350,8 +357,8 @@ def dispatch_backward(dxp: torch.Tensor, plan: RoutingPlan, out: Optional[torch.
     wsb = int(lib().et_dispatch_bwd_router_workspace_bytes(plan.rows))
     if workspace is None:
         workspace = torch.empty(max(wsb, 1), dtype=torch.uint8, device=dev)
-    elif workspace.device != dev or workspace.numel() * workspace.element_size() < wsb:
-        raise ValueError(f"workspace must hold {wsb} bytes on {dev}")
+    else:
+        _require_workspace(workspace, wsb, dev, "workspace")
     _call("et_dispatch_bwd_router", dev, _vp(dxp), _vp(plan.token_offsets), _vp(plan.token_slot), T, d, dt, plan.rows,
           _vp(plan.slot_gate), _vp(dgate), _vp(plan.expert_offsets), E, _vp(router_weight), _vp(dx), _vp(workspace),
           wsb)
@@ -381,8 +388,8 @@ def router_weight_grad(dlogits: torch.Tensor, x: torch.Tensor, out: Optional[tor
     wsb = int(lib().et_router_wgrad_workspace_bytes(T, d, E))
     if workspace is None:
         workspace = torch.empty(max(wsb, 16), dtype=torch.uint8, device=dev)
-    elif workspace.device != dev or workspace.numel() * workspace.element_size() < wsb:
-        raise ValueError(f"workspace must hold {wsb} bytes on {dev}")
+    else:
+        _require_workspace(workspace, wsb, dev, "workspace")
     _call("et_router_wgrad", dev, _vp(dlogits), _vp(x), T, d, E, _vp(dw), _vp(workspace), wsb)
     return dw
 
@@ -671,8 +678,8 @@ def threshold_update_(thr: torch.Tensor, logits: torch.Tensor, k_target: int,
     wsb = threshold_workspace_bytes(T, E)
     if workspace is None:
         workspace = torch.empty(wsb, dtype=torch.uint8, device=dev)
-    elif workspace.device != dev or workspace.numel() * workspace.element_size() < wsb:
-        raise ValueError(f"workspace must hold {wsb} bytes on {dev}")
+    else:
+        _require_workspace(workspace, wsb, dev, "workspace")
     _call("et_threshold_update", dev, _vp(logits), _vp(thr), T, E, int(k_target), float(momentum), _vp(stat),
           _vp(workspace), wsb)
     return stat
@@ -716,12 +723,12 @@ def route_update(logits: torch.Tensor, thr: torch.Tensor, k_target: int, momentu
     rwsb, twsb = route_workspace_bytes(T, E), threshold_workspace_bytes(T, E)
     if workspace is None:
         workspace = torch.empty(rwsb, dtype=torch.uint8, device=dev)
-    elif workspace.device != dev or workspace.numel() * workspace.element_size() < rwsb:
-        raise ValueError(f"workspace must hold {rwsb} bytes on {dev}")
+    else:
+        _require_workspace(workspace, rwsb, dev, "workspace")
     if thr_workspace is None:
         thr_workspace = torch.empty(twsb, dtype=torch.uint8, device=dev)
-    elif thr_workspace.device != dev or thr_workspace.numel() * thr_workspace.element_size() < twsb:
-        raise ValueError(f"thr_workspace must hold {twsb} bytes on {dev}")
+    else:
+        _require_workspace(thr_workspace, twsb, dev, "thr_workspace")
     a, b = workspace.data_ptr(), thr_workspace.data_ptr()
     if a < b + twsb and b < a + rwsb:
         raise ValueError("workspace and thr_workspace must not overlap")
@@ -812,8 +819,8 @@ def router_route(x: torch.Tensor, w: torch.Tensor, thr: torch.Tensor, *, slot_ca
     wsb = router_route_workspace_bytes(T, E)
     if workspace is None:
         workspace = torch.empty(wsb, dtype=torch.uint8, device=dev)
-    elif workspace.device != dev or workspace.numel() * workspace.element_size() < wsb:
-        raise ValueError(f"workspace must hold {wsb} bytes on {dev}")
+    else:
+        _require_workspace(workspace, wsb, dev, "workspace")
     _call("et_router_route", dev, _vp(x), _vp(w), _vp(thr), T, d, E, _vp(counts), _vp(eo), _vp(to), _vp(st), _vp(sg),
           _vp(ts), cap, _vp(L), _vp(workspace), wsb)
     plan = RoutingPlan(counts, eo, to, st, sg, ts, T, E, cap)

@@ -10,7 +10,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from ._lib import ET_MAX_NORM_WIDTH, lib
-from .expert_threshold import _ACT_DTYPES, _act_dtype, _call, _out_or_new, _require, _require_device, _vp
+from .expert_threshold import (_ACT_DTYPES, _act_dtype, _call, _out_or_new, _require, _require_device,
+                               _require_workspace, _vp)
 
 
 def _require_rows(t, name: str, dtype=None, shape=None, device=None) -> int:
@@ -162,8 +163,8 @@ def layer_norm_backward(dy: torch.Tensor, h: torch.Tensor, weight: torch.Tensor,
     wsb = layer_norm_backward_workspace_bytes(rows, d)
     if workspace is None:
         workspace = mean.new_empty(wsb // 4)
-    elif workspace.device != dev or workspace.numel() * workspace.element_size() < wsb:
-        raise ValueError(f"workspace must hold {wsb} bytes on {dev}")
+    else:
+        _require_workspace(workspace, wsb, dev, "workspace")
     _call("et_layer_norm_bwd", dev, dy.data_ptr(), lddy, h.data_ptr(), ldh, _vp(dsum), ldds, weight.data_ptr(),
           mean.data_ptr(), rstd.data_ptr(), rows, d, _ACT_DTYPES[dtype], _ACT_DTYPES[weight.dtype], dx.data_ptr(),
           dweight.data_ptr(), _vp(dbias), workspace.data_ptr(), wsb)

@@ -18,7 +18,7 @@ from typing import Optional, Sequence
 import torch
 
 from ._lib import ET_DTYPE_BF16, ET_DTYPE_F32, AdamWScalars, lib
-from .expert_threshold import _call, _require, _require_device, _vp
+from .expert_threshold import _call, _require, _require_device, _require_workspace, _vp
 
 # Elements that share one scale of the 8-bit states.
 ADAMW8_BLOCK = 256
@@ -154,8 +154,8 @@ def grad_norm(grads: Sequence[torch.Tensor], max_norm: Optional[float] = None, *
     wsb = int(lib().et_grad_norm_workspace_bytes(numel, len(sizes)))
     if workspace is None:
         workspace = torch.empty(max(wsb, 8), dtype=torch.uint8, device=dev)
-    elif workspace.device != dev or workspace.numel() * workspace.element_size() < wsb:
-        raise ValueError(f"workspace must hold {wsb} bytes on {dev}")
+    else:
+        _require_workspace(workspace, wsb, dev, "workspace")
     out = torch.empty(2, dtype=torch.float32, device=dev)
     norm = out.data_ptr()
     dtypes = (ctypes.c_int32 * len(sizes))(*[_DTYPES[t.dtype] for t in grads])

@@ -390,3 +390,12 @@ def test_opcheck(et, dev, dtype):
     for ds in (None, r.detach()):
         torch.library.opcheck(ops.layer_norm_backward.default, (r.detach(), x.detach(), w.detach(), mean, rstd, ds),
                               test_utils=("test_schema", "test_faketensor"))
+
+
+def test_workspaces_that_only_look_large_are_refused(et, dev):
+    """A workspace of enough elements on one element of memory."""
+    x, w, m = torch.ones(400, 64, device=dev), torch.ones(64, device=dev), torch.ones(400, device=dev)
+    small = torch.zeros(4, device=dev)
+    for bad in (small[:1].expand(1 << 20), small[:1].expand(1 << 10, 1 << 10), torch.zeros(1 << 17, device=dev)[::2]):
+        with pytest.raises(ValueError, match="workspace"):
+            et.layer_norm_backward(x, x, w, m, m, workspace=bad)

@@ -120,3 +120,24 @@ def test_compiled_layer_is_bit_identical_to_eager(dev, dtype):
         comp.scale.grad = None
     # the EMA moved the thresholds, and the logits received gradient only at routed pairs
     assert not torch.equal(eager.thr, torch.full_like(eager.thr, 0.7))
+
+
+def test_workspaces_that_only_look_large_are_refused(et, dev):
+    """A workspace of enough elements on one element of memory."""
+    T, E, d = 300, 8, 64
+    logits, thr = torch.randn(T, E, device=dev), torch.zeros(E, device=dev)
+    x, w = (torch.randn(n, d, device=dev).bfloat16() for n in (T, E))
+    plan = et.route(logits, thr)
+    yp = torch.randn(plan.rows, d, device=dev).bfloat16()
+    dgate = torch.zeros(plan.rows, device=dev)
+    bad = torch.zeros(4, device=dev)[:1].expand(1 << 24)
+    for call in (lambda ws: et.route(logits, thr, workspace=ws),
+                 lambda ws: et.route_update(logits, thr, 2, workspace=ws),
+                 lambda ws: et.route_update(logits, thr, 2, thr_workspace=ws),
+                 lambda ws: et.threshold_update_(thr, logits, 2, workspace=ws),
+                 lambda ws: et.router_route(x, w, thr, workspace=ws),
+                 lambda ws: et.router_weight_grad(logits, x, workspace=ws),
+                 lambda ws: et.combine_backward(x, yp, plan, workspace=ws),
+                 lambda ws: et.dispatch_backward(yp, plan, router_weight=w, dgate=dgate, workspace=ws)):
+        with pytest.raises(ValueError, match="workspace"):
+            call(bad)

@@ -669,3 +669,11 @@ def test_steps_count_as_changes_of_the_parameters(et, dev):
         w = torch.ones(8, device=dev)
         et.AdamW([w]).step([torch.ones(8, device=dev)])
         assert torch.all(w < 1)
+
+
+def test_workspaces_that_only_look_large_are_refused(et, dev):
+    """A workspace of enough elements on one element of memory."""
+    small = torch.zeros(2, dtype=torch.float64, device=dev)
+    for bad in (small[:1].expand(4096), small[:1].expand(64, 64), torch.zeros(9000, device=dev)[::2]):
+        with pytest.raises(ValueError, match="workspace"):
+            et.grad_norm([torch.ones(1 << 20, device=dev)], workspace=bad)
