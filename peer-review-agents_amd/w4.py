@@ -31,6 +31,23 @@ class W4Weight:
     group: int
     parts: int
 
+    def __post_init__(self) -> None:
+        # (the products read as much as these sizes say)
+        _check_sizes(self.num_experts, self.N, self.K, self.group, self.parts)
+        L = lib()
+        for t, name, dtypes, n in (
+                (self.packed, "packed", (torch.uint8,), L.et_w4_packed_bytes(self.num_experts, self.N, self.K, self.parts)),
+                (self.scales, "scales", tuple(_SCALE_TYPES),
+                 L.et_w4_packed_scales(self.num_experts, self.N, self.K, self.group, self.parts))):
+            if not isinstance(t, torch.Tensor) or t.dtype not in dtypes:
+                raise TypeError(f"{name} must be a tensor of {' or '.join(map(str, dtypes))}")
+            if not t.is_contiguous() or t.numel() != n:
+                raise ValueError(f"{name} must be contiguous with {n} elements, got shape {tuple(t.shape)}")
+            if t.data_ptr() % 16:
+                raise ValueError(f"{name} must be 16-byte aligned")
+        if self.scales.device != self.packed.device:
+            raise ValueError(f"scales are on {self.scales.device}, packed is on {self.packed.device}")
+
     @property
     def device(self) -> torch.device:
         return self.packed.device

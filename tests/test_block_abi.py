@@ -153,3 +153,30 @@ def test_w4_rejects_bad_arguments(et):
 def test_w4_kernel_choice(et, E, K, N, swiglu, capacity, most, route):
     got = et.lib().et_w4_route_impl(E, K, N, 128, 1 + swiglu, capacity, 2 * swiglu, most, 256)
     assert got == route
+
+
+def test_a_4_bit_weight_holds_what_its_sizes_say(et):
+    """The products read by num_experts, N, K, group and parts; a weight whose tensors are
+    smaller is refused where it is made."""
+    import copy
+    import dataclasses
+
+    import torch
+
+    def weight(packed=2 * 2 * 2048, scales=2 * 2 * 32, E=1, N=40, K=136, group=128, parts=1, pt=torch.uint8,
+               st=torch.bfloat16, at=0):
+        p = torch.zeros(packed + at, dtype=pt)[at:]
+        return et.W4Weight(p, torch.zeros(scales, dtype=st), E, N, K, group, parts)
+
+    w = weight()
+    assert copy.deepcopy(w).packed.numel() == w.packed.numel()
+    assert dataclasses.replace(w, scales=w.scales.half()).scales.dtype == torch.float16
+    for bad in (dict(packed=2 * 2048), dict(scales=32), dict(E=2), dict(K=264), dict(N=72), dict(group=64), dict(parts=3),
+                dict(at=1), dict(E=0), dict(group=48), dict(N=44)):
+        with pytest.raises(ValueError):
+            weight(**bad)
+    for bad in (dict(pt=torch.int8), dict(st=torch.float32)):
+        with pytest.raises(TypeError):
+            weight(**bad)
+    with pytest.raises(ValueError):
+        et.W4Weight(torch.zeros(1, dtype=torch.uint8).expand(8192), torch.zeros(128).bfloat16(), 1, 40, 136, 128, 1)
