@@ -319,9 +319,11 @@ __global__ __launch_bounds__(norm_threads(WPR)) void layer_norm_bwd_kernel(BwdAr
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             weights_of(i);
+            // (columns past the row have to add 0: 0 - mean, times a large rstd, may be an infinity)
+            const float mu = t + TPR * i < nvec ? mean : 0.0f;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float xh = (Elem<X>::get(cur.x.v[i], j) - mean) * rstd, dyv = Elem<X>::get(cur.dy.v[i], j);
+                const float xh = (Elem<X>::get(cur.x.v[i], j) - mu) * rstd, dyv = Elem<X>::get(cur.dy.v[i], j);
                 const float g = dyv * wr[i][j];
                 s[0] += g;
                 s[1] = __builtin_fmaf(g, xh, s[1]);
@@ -330,7 +332,7 @@ __global__ __launch_bounds__(norm_threads(WPR)) void layer_norm_bwd_kernel(BwdAr
             }
         }
         if constexpr (TAIL) {
-            const float xh = (cur.x.tail - mean) * rstd, g = cur.dy.tail * wt;
+            const float xh = (cur.x.tail - (t < d % V ? mean : 0.0f)) * rstd, g = cur.dy.tail * wt;
             s[0] += g;
             s[1] = __builtin_fmaf(g, xh, s[1]);
             dwt = __builtin_fmaf(cur.dy.tail, xh, dwt);

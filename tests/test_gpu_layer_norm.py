@@ -399,3 +399,19 @@ def test_workspaces_that_only_look_large_are_refused(et, dev):
     for bad in (small[:1].expand(1 << 20), small[:1].expand(1 << 10, 1 << 10), torch.zeros(1 << 17, device=dev)[::2]):
         with pytest.raises(ValueError, match="workspace"):
             et.layer_norm_backward(x, x, w, m, m, workspace=bad)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("d", [3, 9, 100, 1000, 1500, 2889, 6000, 9000])
+def test_backward_of_rows_far_from_zero(et, dev, dtype, d):
+    """Constant rows of 2^112: mean * rstd passes binary32's range, but x - mean is
+    0 in every column, so dx = rstd (g - mean(g)) + dsum is not large."""
+    g = torch.Generator().manual_seed(d)
+    x = torch.full((6, d), 2.0 ** 112, device=dev, dtype=dtype)
+    w = (1 + torch.randn(d, generator=g) * 0.3).to(dev)
+    mean, rstd = torch.full((6,), 2.0 ** 112, device=dev), torch.full((6,), 2.0 ** 20, device=dev)
+    dy, ds = (torch.randn(6, d, generator=g).to(dev).to(dtype) for _ in range(2))
+    got = et.layer_norm_backward(dy, x, w, mean, rstd, dsum=ds)
+    dx, dw, db, ex, ew, eb = _backward64(dy, x, w, mean, rstd, ds)
+    assert torch.all((got[0].double() - dx).abs() <= ex + HALF[dtype] * (dx.abs() + ex))
+    assert torch.all(got[1] == 0) and torch.all((got[2].double() - db).abs() <= eb)
