@@ -2,6 +2,7 @@
 // and its backward with the reductions of the weight's and bias's gradients
 // (gfx950).
 #include <algorithm>
+#include <cmath>
 
 #include "et_common.hpp"
 #include "etmoe_block.h"
@@ -9,6 +10,7 @@
 namespace et {
 namespace {
 
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 // 16 bytes at an address aligned to the element only: rows may start anywhere
 // (one global_load_dwordx4 all the same; a row that starts at a 16-byte
@@ -251,6 +253,7 @@ struct BwdArgs {
     float* partial;           // [blocks][2][d]: the blocks' sums of dy * xhat and of dy
     int64_t lddy, ldx, ldds, T;
     int d;
+    int fold;                 // turns (of D rows of a thread) between two foldings of its columns' sums
 };
 
 // With g = dy w and xhat = (x - mean) rstd: dx = rstd (g - mean(g) - xhat mean(g xhat)),
@@ -263,8 +266,14 @@ struct BwdArgs {
 // 3001 x 2889 f32 40.6 against 25.7).
 //
 // A block walks rows blockIdx, blockIdx + gridDim, ... (4 / WPR at a time), its
-// threads keeping their columns' sums for the weight and the bias.  DSUM: a
-// gradient past the norm is added.
+// threads keeping their columns' sums for the weight and the bias.  After as many rows as
+// the root of their number (32 at least) the sums are added to second ones and begin
+// anew, so that none is a chain of more (262144 rows of 520 in f32: 1.8e-7 of the sum's size
+// off, 6.0e-7 in one chain of 1024).  The second ones are in LDS, the thread's own places (a
+// wave a row: in registers they cost as much).  With 16 waves a row (rows of more than 8192)
+// the first are in LDS, which spares registers that would spill, and the second in memory,
+// every 64 rows (4096 x 16384 bf16 with DSUM 162 to 124 us, 2048 x 9000 f32 126 to 72; 32768 x
+// 16384, where memory's part counts, 702 to 734).  DSUM: a gradient past the norm is added.
 template <typename X, typename W, int WPR, int NV, int D, bool TAIL, bool DSUM>
 __global__ __launch_bounds__(norm_threads(WPR)) void layer_norm_bwd_kernel(BwdArgs a)
 {
@@ -280,10 +289,54 @@ __global__ __launch_bounds__(norm_threads(WPR)) void layer_norm_bwd_kernel(BwdAr
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) dw[i][j] = db[i][j] = 0.0f;
+    // the sums' second place; with 16 waves a row their first, the second being in memory
+    constexpr bool kInLds = WPR == 16;
+    float* const out = a.partial + (int64_t)blockIdx.x * 2 * d;
+    const int nvec = d / V;
+    __shared__ f32x4_t kept[NV][V / 4][2][norm_threads(WPR)];
+    const auto place = [&](int i, int q, int of) -> f32x4_t& { return kept[i][q][of][threadIdx.x]; };
+    float dwt_kept = 0.0f, dbt_kept = 0.0f;
+    bool folded = false;
+    // f(number, the place of four of the thread's sums, the sums, their address in the
+    // block's, whether the row has them)
+    const auto each_sum = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int q = 0; q < V / 4; ++q) {
+                const int n = 2 * (i * (V / 4) + q), k = t + TPR * i;
+                float* const at = out + k * V + 4 * q;
+                f(n, place(i, q, 0), &dw[i][4 * q], at, k < nvec);
+                f(n + 1, place(i, q, 1), &db[i][4 * q], at + d, k < nvec);
+            }
+    };
+    const auto add_to_memory = [&]() {
+        // (all loads before the first store: the compiler keeps their order)
+        f32x4_t there[2 * NV * V / 4];
+        each_sum([&](int n, f32x4_t&, float*, float* at, bool in) {
+            there[n] = f32x4_t{};
+            if (in && folded) there[n] = *reinterpret_cast<f32x4_any_t*>(at);
+        });
+        each_sum([&](int n, f32x4_t& sums, float*, float* at, bool in) {
+            if (in) *reinterpret_cast<f32x4_any_t*>(at) = there[n] + sums;
+        });
+    };
+    const auto fold = [&]() {
+        if constexpr (kInLds) add_to_memory();
+        each_sum([](int, f32x4_t& there, float* sum, float*, bool) {
+            if constexpr (kInLds) there = f32x4_t{};
+            else there += f32x4_t{sum[0], sum[1], sum[2], sum[3]};
+            sum[0] = sum[1] = sum[2] = sum[3] = 0.0f;
+        });
+        dwt_kept += dwt;
+        dbt_kept += dbt;
+        dwt = dbt = 0.0f;
+        folded = true;
+    };
+    each_sum([](int, f32x4_t& there, float*, float*, bool) { there = f32x4_t{}; });
     // the weight stays in registers: read twice a row it would be as much L1
     // traffic as the rows are
     float wr[NV][V], wt = 0.0f;
-    const int nvec = d / V;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const bool in = t + TPR * i < nvec;
@@ -321,14 +374,34 @@ __global__ __launch_bounds__(norm_threads(WPR)) void layer_norm_bwd_kernel(BwdAr
             weights_of(i);
             // (columns past the row have to add 0: 0 - mean, times a large rstd, may be an infinity)
             const float mu = t + TPR * i < nvec ? mean : 0.0f;
+            f32x4_t sw[V / 4], sb[V / 4];
+            if constexpr (kInLds) {
+#pragma unroll
+                for (int q = 0; q < V / 4; ++q) {
+                    sw[q] = place(i, q, 0);
+                    sb[q] = place(i, q, 1);
+                }
+            }
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const float xh = (Elem<X>::get(cur.x.v[i], j) - mu) * rstd, dyv = Elem<X>::get(cur.dy.v[i], j);
                 const float g = dyv * wr[i][j];
                 s[0] += g;
                 s[1] = __builtin_fmaf(g, xh, s[1]);
-                dw[i][j] = __builtin_fmaf(dyv, xh, dw[i][j]);
-                db[i][j] += dyv;
+                if constexpr (kInLds) {
+                    sw[j / 4][j % 4] = __builtin_fmaf(dyv, xh, sw[j / 4][j % 4]);
+                    sb[j / 4][j % 4] += dyv;
+                } else {
+                    dw[i][j] = __builtin_fmaf(dyv, xh, dw[i][j]);
+                    db[i][j] += dyv;
+                }
+            }
+            if constexpr (kInLds) {
+#pragma unroll
+                for (int q = 0; q < V / 4; ++q) {
+                    place(i, q, 0) = sw[q];
+                    place(i, q, 1) = sb[q];
+                }
             }
         }
         if constexpr (TAIL) {
@@ -364,6 +437,7 @@ __global__ __launch_bounds__(norm_threads(WPR)) void layer_norm_bwd_kernel(BwdAr
     // rows in flight: the one that is worked on and D - 1 behind it
 #pragma unroll
     for (int u = 0; u < D - 1; ++u) load(ring[u], row + u * step);
+    int turns = a.fold;
     for (bool more = true; more;) {
 #pragma unroll
         for (int u = 0; u < D; ++u) {
@@ -373,9 +447,20 @@ __global__ __launch_bounds__(norm_threads(WPR)) void layer_norm_bwd_kernel(BwdAr
             process(ring[u]);
             row += step;
         }
+        if (--turns == 0 && more) {
+            fold();
+            turns = a.fold;
+        }
     }
+    dwt += dwt_kept;
+    dbt += dbt_kept;
     // the block's sums; with several rows at a time their threads' are added first
-    float* const out = a.partial + (int64_t)blockIdx.x * 2 * d;
+    if constexpr (!kInLds) {
+        each_sum([](int, f32x4_t& there, float* sum, float*, bool) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum[k] += there[k];
+        });
+    }
     if constexpr (kRows > 1) {
         constexpr int kCols = TPR * NV * V;
         __shared__ float cols[2][kCols + kWave];
@@ -402,17 +487,10 @@ __global__ __launch_bounds__(norm_threads(WPR)) void layer_norm_bwd_kernel(BwdAr
             out[d + c] = cols[1][at];
         }
     } else {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int k = t + TPR * i;
-            if (k < nvec) {
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    out[k * V + j] = dw[i][j];
-                    out[d + k * V + j] = db[i][j];
-                }
-            }
-        }
+        if constexpr (kInLds) add_to_memory();
+        else each_sum([](int, f32x4_t&, float* sum, float* at, bool in) {
+            if (in) *reinterpret_cast<f32x4_any_t*>(at) = f32x4_t{sum[0], sum[1], sum[2], sum[3]};
+        });
         if (t < d % V) {
             out[nvec * V + t] = dwt;
             out[d + nvec * V + t] = dbt;
@@ -457,6 +535,14 @@ constexpr int64_t kMaxBlocks = 256;
 
 int64_t bwd_blocks(int64_t T) { return std::max<int64_t>(1, std::min(T, kMaxBlocks)); }
 
+// Rows whose sums a thread adds up before it folds them, of those that it has of T: as
+// many as it then has results, `least` at least.
+int rows_between_folds(int64_t T, int64_t walkers, int least)
+{
+    const int64_t rows = (T + walkers - 1) / walkers;
+    return std::max(least, (int)std::ceil(std::sqrt((double)rows)));
+}
+
 // Vectors of a row of d elements for each of `threads`.
 int vectors(int64_t d, int V, int threads) { return (int)((d / V + threads - 1) / threads); }
 
@@ -497,21 +583,24 @@ template <typename X, typename W, bool TAIL, bool DSUM>
 int launch_bwd(const BwdArgs& a, int64_t blocks, hipStream_t s)
 {
     constexpr int V = Elem<X>::V;
-    const auto go = [&](auto kernel, int wpr) {
-        kernel<<<dim3((unsigned)blocks), dim3(norm_threads(wpr)), 0, s>>>(a);
+    const auto go = [&](auto kernel, int wpr, int depth) {
+        BwdArgs b = a;
+        const int64_t walkers = blocks * (norm_threads(wpr) / (wpr * kWave));
+        b.fold = (rows_between_folds(a.T, walkers, wpr == 16 ? 64 : 32) + depth - 1) / depth;
+        kernel<<<dim3((unsigned)blocks), dim3(norm_threads(wpr)), 0, s>>>(b);
         return check_launch("layer_norm_bwd_kernel");
     };
     const auto fits = [&](int wpr, int nv) { return vectors(a.d, V, wpr * kWave) <= nv; };
-    if (fits(1, 1)) return go(layer_norm_bwd_kernel<X, W, 1, 1, 4, TAIL, DSUM>, 1);
-    if (fits(1, 2)) return go(layer_norm_bwd_kernel<X, W, 1, 2, 2, TAIL, DSUM>, 1);
-    if (fits(4, 1)) return go(layer_norm_bwd_kernel<X, W, 4, 1, 3, TAIL, DSUM>, 4);
-    if (fits(4, 2)) return go(layer_norm_bwd_kernel<X, W, 4, 2, 2, TAIL, DSUM>, 4);
-    if (fits(8, 2)) return go(layer_norm_bwd_kernel<X, W, 8, 2, 2, TAIL, DSUM>, 8);
+    if (fits(1, 1)) return go(layer_norm_bwd_kernel<X, W, 1, 1, 4, TAIL, DSUM>, 1, 4);
+    if (fits(1, 2)) return go(layer_norm_bwd_kernel<X, W, 1, 2, 2, TAIL, DSUM>, 1, 2);
+    if (fits(4, 1)) return go(layer_norm_bwd_kernel<X, W, 4, 1, 3, TAIL, DSUM>, 4, 3);
+    if (fits(4, 2)) return go(layer_norm_bwd_kernel<X, W, 4, 2, 2, TAIL, DSUM>, 4, 2);
+    if (fits(8, 2)) return go(layer_norm_bwd_kernel<X, W, 8, 2, 2, TAIL, DSUM>, 8, 2);
     if constexpr (sizeof(X) == 2) {
-        return go(layer_norm_bwd_kernel<X, W, 16, 2, 1, TAIL, DSUM>, 16);
+        return go(layer_norm_bwd_kernel<X, W, 16, 2, 1, TAIL, DSUM>, 16, 1);
     } else {
-        if (fits(8, 4)) return go(layer_norm_bwd_kernel<X, W, 8, 4, 2, TAIL, DSUM>, 8);
-        return go(layer_norm_bwd_kernel<X, W, 16, 4, 1, TAIL, DSUM>, 16);
+        if (fits(8, 4)) return go(layer_norm_bwd_kernel<X, W, 8, 4, 2, TAIL, DSUM>, 8, 2);
+        return go(layer_norm_bwd_kernel<X, W, 16, 4, 1, TAIL, DSUM>, 16, 1);
     }
 }
 
@@ -522,9 +611,10 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_narrow_kernel(BwdArgs a)
 {
     __shared__ float part[4][2][8];
     const int d = a.d;
-    float dw[8], db[8];
+    float dw[8], db[8], dw_kept[8], db_kept[8];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) dw[c] = db[c] = 0.0f;
+    for (int c = 0; c < 8; ++c) dw[c] = db[c] = dw_kept[c] = db_kept[c] = 0.0f;
+    int turns = a.fold;
     for (int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x; row < a.T; row += (int64_t)gridDim.x * 256) {
         const float mean = a.mean[row], rstd = a.rstd[row];
         float xh[8], dy[8], g[8], s0 = 0.0f, s1 = 0.0f;
@@ -547,9 +637,18 @@ __global__ __launch_bounds__(256) void layer_norm_bwd_narrow_kernel(BwdArgs a)
             ((X*)a.dx)[row * d + c] =
                 Elem<X>::from_float(a.dsum ? v + Elem<X>::to_float(((const X*)a.dsum)[row * a.ldds + c]) : v);
         }
+        if (--turns == 0) {
+            turns = a.fold;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                dw_kept[c] += dw[c];
+                db_kept[c] += db[c];
+                dw[c] = db[c] = 0.0f;
+            }
+        }
     }
     for (int c = 0; c < d; ++c) {
-        const float sw = wave_sum_dpp(dw[c]), sb = wave_sum_dpp(db[c]);
+        const float sw = wave_sum_dpp(dw[c] + dw_kept[c]), sb = wave_sum_dpp(db[c] + db_kept[c]);
         if (lane_id() == 0) {
             part[threadIdx.x / kWave][0][c] = sw;
             part[threadIdx.x / kWave][1][c] = sb;
@@ -567,7 +666,9 @@ template <typename X, typename W>
 int launch_bwd(const BwdArgs& a, int64_t blocks, hipStream_t s)
 {
     if (a.d < Elem<X>::V) {
-        layer_norm_bwd_narrow_kernel<X, W><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(a);
+        BwdArgs b = a;
+        b.fold = rows_between_folds(a.T, blocks * 256, 32);
+        layer_norm_bwd_narrow_kernel<X, W><<<dim3((unsigned)blocks), dim3(256), 0, s>>>(b);
         return check_launch("layer_norm_bwd_narrow_kernel");
     }
     if (a.d % Elem<X>::V)
@@ -667,7 +768,7 @@ extern "C" int et_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* 
         return fail(ET_ERR_WORKSPACE_TOO_SMALL, "et_layer_norm_bwd: workspace needs " + std::to_string(need) + " bytes");
     if ((uintptr_t)workspace % 4) return fail(ET_ERR_INVALID_ARGUMENT, "et_layer_norm_bwd: workspace is not aligned");
     const int64_t blocks = bwd_blocks(rows);
-    const BwdArgs a{dy, x, dsum, weight, mean, rstd, dx, (float*)workspace, dy_stride, x_stride, dsum_stride, rows, (int)d};
+    const BwdArgs a{dy, x, dsum, weight, mean, rstd, dx, (float*)workspace, dy_stride, x_stride, dsum_stride, rows, (int)d, 0};
     hipStream_t s = (hipStream_t)stream;
     // (the kernels read rows ahead, the last one at least: they are for rows > 0)
     if (rows == 0) rc = ET_OK;

@@ -415,3 +415,31 @@ def test_backward_of_rows_far_from_zero(et, dev, dtype, d):
     dx, dw, db, ex, ew, eb = _backward64(dy, x, w, mean, rstd, ds)
     assert torch.all((got[0].double() - dx).abs() <= ex + HALF[dtype] * (dx.abs() + ex))
     assert torch.all(got[1] == 0) and torch.all((got[2].double() - db).abs() <= eb)
+
+
+@pytest.mark.parametrize("dtype,d", [(F32, 3), (BF16, 64), (F32, 520), (BF16, 520), (F32, 8200), (BF16, 8200)])
+def test_column_sums_over_many_rows(et, dev, dtype, d):
+    """The error of dweight and dbias does not grow with the rows.  A sum of n
+    terms of deviation 1 and random signs in chains of lengths l_1, l_2, ... (a chain's
+    results are the next one's terms) is off by about 0.3 U sqrt(l_1 + l_2 + ...) times
+    its size, sqrt(n): an addition errs by 0.4 U (deviation) of a partial sum that
+    grows as the root.  Chains of 32 and T / 256 / 32 rows, 20 for the blocks, and one U of the
+    terms' own roundings: below 4 U up to 2^18 rows, where a single
+    chain of T / 256 gives 9 U."""
+    T = (1 << 18) if d < 4096 else (1 << 16)
+    g = torch.Generator(device=dev).manual_seed(d)
+    x, dy = torch.empty(T, d, dtype=dtype, device=dev), torch.empty(T, d, dtype=dtype, device=dev)
+    step = 1 << 13
+    for i in range(0, T, step):
+        x[i:i + step] = torch.randn(step, d, generator=g, device=dev)
+        dy[i:i + step] = torch.randn(step, d, generator=g, device=dev)
+    w = torch.ones(d, device=dev)
+    mean, rstd = torch.zeros(T, device=dev), torch.ones(T, device=dev)     # (xhat = x, exactly)
+    _, dw, db = et.layer_norm_backward(dy, x, w, mean, rstd)
+    rw, rb = (torch.zeros(d, dtype=torch.float64, device=dev) for _ in range(2))
+    for i in range(0, T, step):
+        a = dy[i:i + step].double()
+        rw += (a * x[i:i + step].double()).sum(0)
+        rb += a.sum(0)
+    for got, want in ((dw, rw), (db, rb)):
+        assert (got.double() - want).norm() <= 4 * U * (T * d) ** 0.5
