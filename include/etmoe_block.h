@@ -217,6 +217,8 @@ int et_w4_unpack(const void* packed, const void* packed_scales, int scale_type, 
  * identical bits.  The inner sum is taken as sum a * (16 + q) from
  * -24 * sum a on, so a row of a that holds an infinity (or values whose
  * 24 |a| add up to 2^128 within a group) gives NaN.  a and c 16-byte aligned.
+ * slot_capacity may be larger than the slots (T * E where no count is read back): which kernel
+ * runs is then decided on the device, by expert_offsets[num_experts].
  * Implements a 4-bit form of the expert GEMM (no reference counterpart).
  */
 int et_expert_gemm_w4(const void* a, int64_t a_rows, const int32_t* sorted_token, const void* packed,

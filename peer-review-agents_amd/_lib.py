@@ -69,7 +69,8 @@ _BLOCK_SIGNATURES = {
     "et_w4_unpack": (_int, [_p, _p, _int, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p]),
     "et_expert_gemm_w4": (_int, [_p, _i64, _p, _p, _p, _int, _p, _i64, _i64, _i64, _i64, _i64, _i64, _int, _p, _p, _p]),
     "et_expert_gemm_w4_impl": (_int, [_p, _i64, _p, _p, _p, _int, _p, _i64, _i64, _i64, _i64, _i64, _i64, _int, _p, _p,
-                                      _i64, _int, _p]),
+                                      _i64, _int, _int, _p]),
+    "et_w4_from_impl": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _int, _i64, _i64, _int]),
     "et_w4_route_impl": (_int, [_i64, _i64, _i64, _i64, _i64, _i64, _int, _i64, _i64]),
     "et_adamw8": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _int, _int, AdamWScalars, _p, _int, _u32, _p]),
 }

@@ -650,11 +650,12 @@ __device__ __forceinline__ void find_tile(const W4Args& g, uint32_t q, uint32_t 
     t.rows = min(n - at, share);
 }
 
+constexpr int split_lds(int nsb, int waves) { return waves * 2 * nsb * 4 * kWave; }    // floats
+
 template <bool SWIGLU, int NSB, int GPT, int WAVES>
-__global__ __launch_bounds__(WAVES * kWave, 2) void w4_split_kernel(W4Args g)
+__device__ __forceinline__ void w4_split(const W4Args& g, float* lds)
 {
     constexpr int LOG = 4;
-    __shared__ __attribute__((aligned(16))) float lds[WAVES * 2 * NSB * 4 * kWave];
     // units of superblocks: pairs of twins for SwiGLU, NSB side by side else
     const uint32_t nb = (uint32_t)(SWIGLU ? g.w.part_sbs : (g.w.sbs + NSB - 1) / NSB);
     for (uint32_t q = blockIdx.x;; q += gridDim.x) {
@@ -667,6 +668,13 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void w4_split_kernel(W4Args g)
         t.b = (int)(q % nb) * (SWIGLU ? 1 : NSB);
         w4_split_tile<SWIGLU, NSB, GPT, WAVES>(g, t, lds);
     }
+}
+
+template <bool SWIGLU, int NSB, int GPT, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave, 2) void w4_split_kernel(W4Args g)
+{
+    __shared__ __attribute__((aligned(16))) float lds[split_lds(NSB, WAVES)];
+    w4_split<SWIGLU, NSB, GPT, WAVES>(g, lds);
 }
 
 // Slot tiles of 1 << LOG slots of all experts.
@@ -686,16 +694,16 @@ __device__ __forceinline__ int count_slots(const W4Args& g)
 // N = 7168, groups of 32: 60.5 us against 65.6 with two).
 constexpr int wide_blocks(int maxmt) { return maxmt == 2 ? 3 : 2; }
 
+// `tiles`: the experts' slot tiles.
 template <bool SWIGLU, int MAXMT, int GPT>
-__global__ __launch_bounds__(kWideWaves * kWave, wide_blocks(MAXMT)) void w4_wide_kernel(W4Args g)
+__device__ __forceinline__ void w4_wide(const W4Args& g, unsigned char* lds, int tiles)
 {
     constexpr int LOG = MAXMT == 2 ? 5 : 6;
-    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * wide_buf(MAXMT)];
     constexpr int kSbs = kWideWaves * (SWIGLU ? 1 : 2);      // superblocks of a tile (SwiGLU: of the gate part)
     const uint32_t nb = (uint32_t)(((SWIGLU ? g.w.part_sbs : g.w.sbs) + kSbs - 1) / kSbs);
     // XCD x (blocks b % 8 = x) takes a contiguous range of tiles, an expert's
     // slot tiles innermost, so that they read its weight through the same L2
-    const uint32_t Q = (uint32_t)__builtin_amdgcn_readfirstlane(count_slots<LOG>(g)) * nb;
+    const uint32_t Q = (uint32_t)__builtin_amdgcn_readfirstlane(tiles) * nb;
     const uint32_t per = (Q + 7) / 8;
     for (uint32_t l = blockIdx.x >> 3; l < per; l += gridDim.x >> 3) {
         const uint32_t q = (blockIdx.x & 7) * per + l;
@@ -718,6 +726,36 @@ __global__ __launch_bounds__(kWideWaves * kWave, wide_blocks(MAXMT)) void w4_wid
     }
 }
 
+// All slots, where the host doesn't know them.
+__device__ __forceinline__ int slots_of(const W4Args& g) { return min(g.expert_offsets[g.w.E], (int)g.cap); }
+
+// from: the slots below which another kernel does the work (0: none does).
+template <bool SWIGLU, int MAXMT, int GPT>
+__global__ __launch_bounds__(kWideWaves * kWave, wide_blocks(MAXMT)) void w4_wide_kernel(W4Args g, int from)
+{
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * wide_buf(MAXMT)];
+    if (from && slots_of(g) < from) return;
+    w4_wide<SWIGLU, MAXMT, GPT>(g, lds, count_slots<MAXMT == 2 ? 5 : 6>(g));
+}
+
+// The same choice as the host's (w4_route) with the slots that there are: split
+// below `wide` of them, wide below `wide64`, where w4_wide_kernel's 64-slot tiles take over.
+// A program that doesn't read the count back gives a capacity with room to spare, T * E for certain;
+// chosen by that, 100 tokens of two experts of 8 (K = 4096, N = 2048) took 39.2 us, and
+// 18.2 so (18.1 with the count known), 70 of two of 64 (2048, 2816) 43.6 and 40.1 (38.5: the launch
+// that finds no work takes the rest).  At an exact capacity that the host doesn't know to be exact
+// it costs nothing measurable.
+template <bool SWIGLU, int GPT>
+__global__ __launch_bounds__(kWideWaves * kWave, wide_blocks(2)) void w4_choose_kernel(W4Args g, int wide, int wide64)
+{
+    __shared__ __attribute__((aligned(16))) unsigned char lds[std::max<int>(2 * wide_buf(2), 4 * split_lds(2, 4))];
+    // (both loads at once: one wait in front of the work)
+    const int tiles = count_slots<5>(g), slots = slots_of(g);
+    if (slots >= wide64) return;
+    if (slots >= wide) w4_wide<SWIGLU, 2, GPT>(g, lds, tiles);
+    else w4_split<SWIGLU, 2, GPT, 4>(g, (float*)lds);
+}
+
 // What the host knows of a call, and what follows from it.
 struct W4Load {
     int64_t busy, mean;    // experts with slots, and slots of one, as far as the capacity tells
@@ -737,6 +775,11 @@ int64_t wide_tiles(const W4Args& g, bool swiglu, const W4Load& l)
     const int sbs = kWideWaves * (swiglu ? 1 : 2);
     return l.busy * std::max<int64_t>(32, l.mean + 16) * (((swiglu ? g.w.part_sbs : g.w.sbs) + sbs - 1) / sbs) / 32;
 }
+
+// Slots from which the wide kernels are taken.
+struct W4From {
+    int64_t wide, wide64;
+};
 
 enum W4Route { kSplit4 = 0, kSplit8 = 1, kWide32 = 2, kWide64 = 3 };
 
@@ -782,7 +825,7 @@ int launch_split(const W4Args& g, int cus, hipStream_t s)
 }
 
 template <bool SWIGLU, int MAXMT>
-int launch_wide(const W4Args& g, int cus, hipStream_t s)
+int launch_wide(const W4Args& g, int cus, hipStream_t s, int from = 0)
 {
     constexpr int kSbs = kWideWaves * (SWIGLU ? 1 : 2);
     const int64_t nb = ((SWIGLU ? g.w.part_sbs : g.w.sbs) + kSbs - 1) / kSbs;
@@ -790,11 +833,28 @@ int launch_wide(const W4Args& g, int cus, hipStream_t s)
     const int64_t blocks = std::min<int64_t>(tiles * nb, (int64_t)cus * wide_blocks(MAXMT));
     const dim3 grid((unsigned)(8 * ((blocks + 7) / 8))), block(kWideWaves * kWave);
     switch (g.w.gpt()) {
-        case 1: w4_wide_kernel<SWIGLU, MAXMT, 1><<<grid, block, 0, s>>>(g); break;
-        case 2: w4_wide_kernel<SWIGLU, MAXMT, 2><<<grid, block, 0, s>>>(g); break;
-        default: w4_wide_kernel<SWIGLU, MAXMT, 4><<<grid, block, 0, s>>>(g); break;
+        case 1: w4_wide_kernel<SWIGLU, MAXMT, 1><<<grid, block, 0, s>>>(g, from); break;
+        case 2: w4_wide_kernel<SWIGLU, MAXMT, 2><<<grid, block, 0, s>>>(g, from); break;
+        default: w4_wide_kernel<SWIGLU, MAXMT, 4><<<grid, block, 0, s>>>(g, from); break;
     }
     return check_launch("w4_wide_kernel");
+}
+
+template <bool SWIGLU>
+int launch_choose(const W4Args& g, const W4From& from, int cus, hipStream_t s)
+{
+    const int64_t nb = SWIGLU ? g.w.part_sbs : (g.w.sbs + 1) / 2;
+    const int64_t tiles = std::min<int64_t>(g.cap, g.cap / 16 + g.w.E);
+    const int64_t blocks = std::min<int64_t>(tiles * nb, (int64_t)cus * wide_blocks(2));
+    const dim3 grid((unsigned)(8 * ((blocks + 7) / 8))), block(kWideWaves * kWave);
+    const int wide = (int)from.wide, wide64 = (int)from.wide64;
+    switch (g.w.gpt()) {
+        case 1: w4_choose_kernel<SWIGLU, 1><<<grid, block, 0, s>>>(g, wide, wide64); break;
+        case 2: w4_choose_kernel<SWIGLU, 2><<<grid, block, 0, s>>>(g, wide, wide64); break;
+        default: w4_choose_kernel<SWIGLU, 4><<<grid, block, 0, s>>>(g, wide, wide64); break;
+    }
+    const int rc = check_launch("w4_choose_kernel");
+    return rc || from.wide64 > g.cap ? rc : launch_wide<SWIGLU, 4>(g, cus, s, wide64);
 }
 
 template <bool SWIGLU>
@@ -808,10 +868,33 @@ int launch_w4(const W4Args& g, int route, int cus, hipStream_t s)
     }
 }
 
-W4Load load_of(int64_t num_experts, int64_t slot_capacity, int64_t most, int64_t cus)
+W4Load load_of(int64_t num_experts, int64_t slots, int64_t most, int64_t cus)
 {
-    const int64_t busy = std::max<int64_t>(1, std::min(num_experts, slot_capacity));
-    return W4Load{busy, std::min(most, (slot_capacity + busy - 1) / busy), cus};
+    const int64_t busy = std::max<int64_t>(1, std::min(num_experts, slots));
+    return W4Load{busy, std::min(most, (slots + busy - 1) / busy), cus};
+}
+
+// The kernel for a number of slots.
+int route_of(const W4Args& g, bool swiglu, int64_t slots, int64_t max_slots, int64_t cus)
+{
+    const int64_t most = std::min(max_slots, slots);
+    return w4_route(g, swiglu, load_of(g.w.E, slots, most, cus), most);
+}
+
+// The fewest slots, of 1 to the capacity, that take a wide kernel, and the one of 64-slot tiles: more than the
+// capacity where none do.  (A route never comes before another's with more slots.)
+W4From from_of(const W4Args& g, bool swiglu, int64_t max_slots, int64_t cus)
+{
+    const auto first = [&](int route) {
+        int64_t lo = 1, hi = g.cap + 1;
+        while (lo < hi) {
+            const int64_t mid = (lo + hi) / 2;
+            if (route_of(g, swiglu, mid, max_slots, cus) >= route) hi = mid;
+            else lo = mid + 1;
+        }
+        return lo;
+    };
+    return W4From{first(kWide32), first(kWide64)};
 }
 
 int check_shape(const char* fn, int64_t E, int64_t N, int64_t K, int64_t group, int64_t parts)
@@ -960,17 +1043,29 @@ extern "C" int et_w4_route_impl(int64_t num_experts, int64_t K, int64_t N, int64
 {
     W4Args g = {};
     g.w = shape_of(num_experts, N, K, group, parts);
-    const int64_t most = std::min(max_slots, slot_capacity);
-    return w4_route(g, epilogue == EPI_SWIGLU, load_of(num_experts, slot_capacity, most, cus), most);
+    return route_of(g, epilogue == EPI_SWIGLU, slot_capacity, max_slots, cus);
+}
+
+// The slots from which it takes a wide one (which 0) or that of 64-slot tiles (1), where
+// the slots are known on the device alone.
+extern "C" int64_t et_w4_from_impl(int64_t num_experts, int64_t K, int64_t N, int64_t group, int64_t parts,
+                                   int64_t slot_capacity, int epilogue, int64_t max_slots, int64_t cus, int which)
+{
+    W4Args g = {};
+    g.w = shape_of(num_experts, N, K, group, parts);
+    g.cap = slot_capacity;
+    const W4From from = from_of(g, epilogue == EPI_SWIGLU, max_slots, cus);
+    return which ? from.wide64 : from.wide;
 }
 
 // max_slots: slots of one expert at most, as far as the host knows.  route: a
-// W4Route, or -1 for the one that w4_route says.
+// W4Route, or -1 for the one that w4_route says.  known: the slots are as many as the
+// capacity; else they may be fewer, and where that decides, the device chooses.
 extern "C" int et_expert_gemm_w4_impl(const void* a, int64_t a_rows, const int32_t* sorted_token, const void* packed,
                                       const void* packed_scales, int scale_type, const int32_t* expert_offsets,
                                       int64_t num_experts, int64_t K, int64_t N, int64_t group, int64_t parts,
                                       int64_t slot_capacity, int epilogue, const float* row_scale, void* c,
-                                      int64_t max_slots, int route, void* stream)
+                                      int64_t max_slots, int route, int known, void* stream)
 {
     const char* fn = "et_expert_gemm_w4";
     int rc = check_shape(fn, num_experts, N, K, group, parts);
@@ -1001,10 +1096,16 @@ extern "C" int et_expert_gemm_w4_impl(const void* a, int64_t a_rows, const int32
     // (tiles are counted in 32 bits: 16 slots by 32 rows at the least)
     if ((slot_capacity / 16 + num_experts + 1) * (int64_t)g.w.sbs >= (int64_t)1 << 31)
         return fail(ET_ERR_INVALID_ARGUMENT, "et_expert_gemm_w4: slot_capacity times N is too large");
-    const int64_t most = std::min(max_slots, slot_capacity);
     const bool swiglu = epilogue == EPI_SWIGLU;
     const int cus = cus_of_device();
-    if (route < kSplit4 || route > kWide64) route = w4_route(g, swiglu, load_of(num_experts, slot_capacity, most, cus), most);
+    if (route < kSplit4 || route > kWide64) {
+        route = route_of(g, swiglu, slot_capacity, max_slots, cus);
+        if (!known && expert_offsets && route >= kWide32) {
+            const W4From from = from_of(g, swiglu, max_slots, cus);
+            return swiglu ? launch_choose<true>(g, from, cus, (hipStream_t)stream)
+                          : launch_choose<false>(g, from, cus, (hipStream_t)stream);
+        }
+    }
     return swiglu ? launch_w4<true>(g, route, cus, (hipStream_t)stream) : launch_w4<false>(g, route, cus, (hipStream_t)stream);
 }
 
@@ -1014,5 +1115,5 @@ extern "C" int et_expert_gemm_w4(const void* a, int64_t a_rows, const int32_t* s
                                  int64_t slot_capacity, int epilogue, const float* row_scale, void* c, void* stream)
 {
     return et_expert_gemm_w4_impl(a, a_rows, sorted_token, packed, packed_scales, scale_type, expert_offsets, num_experts, K,
-                                  N, group, parts, slot_capacity, epilogue, row_scale, c, slot_capacity, -1, stream);
+                                  N, group, parts, slot_capacity, epilogue, row_scale, c, slot_capacity, -1, 0, stream);
 }

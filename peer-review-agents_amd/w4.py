@@ -140,7 +140,7 @@ def unpack_w4(w: W4Weight, plan: Optional[RoutingPlan] = None, out: Optional[tor
 
 
 def _gemm(a, w: W4Weight, rows: int, sorted_token, offsets, epilogue: str, row_scale, out, max_slots: int,
-          route: int = -1):
+          route: int = -1, known: int = 1):
     dev = a.device
     if epilogue not in _EPILOGUES:
         raise ValueError(f"epilogue must be one of {sorted(_EPILOGUES)}, got {epilogue!r}")
@@ -162,7 +162,7 @@ def _gemm(a, w: W4Weight, rows: int, sorted_token, offsets, epilogue: str, row_s
         raise ValueError("a and out must be 16-byte aligned")
     _call("et_expert_gemm_w4_impl", dev, at, a.shape[0], sorted_token, w.packed.data_ptr(), w.scales.data_ptr(),
           _SCALE_TYPES[w.scales.dtype], offsets, w.num_experts, w.K, w.N, w.group, w.parts, rows, _EPILOGUES[epilogue],
-          row_scale.data_ptr() if epilogue == "row_scale" else None, to, max_slots, route)
+          row_scale.data_ptr() if epilogue == "row_scale" else None, to, max_slots, route, known)
     return c
 
 
@@ -195,5 +195,6 @@ def expert_gemm_w4(a: torch.Tensor, w: W4Weight, plan: RoutingPlan, *, gather: b
             raise ValueError("in gather mode the token matrix must be below 2 GiB")
     elif a.shape[0] != plan.rows:
         raise ValueError(f"a has {a.shape[0]} rows, plan has {plan.rows} slots")
+    most, known = _known_counts(plan)
     return _gemm(a, w, plan.rows, _vp(plan.sorted_token) if gather else None, _vp(plan.expert_offsets), epilogue,
-                 row_scale, out, _known_counts(plan)[0])
+                 row_scale, out, most, known=known)

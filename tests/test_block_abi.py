@@ -180,3 +180,22 @@ def test_a_4_bit_weight_holds_what_its_sizes_say(et):
             weight(**bad)
     with pytest.raises(ValueError):
         et.W4Weight(torch.zeros(1, dtype=torch.uint8).expand(8192), torch.zeros(128).bfloat16(), 1, 40, 136, 128, 1)
+
+
+@pytest.mark.parametrize("E,K,N,swiglu,T", [(128, 4096, 4096, 1, 17), (128, 4096, 4096, 1, 32), (128, 4096, 4096, 1, 65),
+                                            (128, 4096, 4096, 1, 128), (64, 2048, 2816, 1, 70), (8, 4096, 2048, 0, 100),
+                                            (32, 2048, 7168, 0, 300), (8, 4096, 4096, 0, 1), (1, 512, 4096, 0, 40)])
+def test_w4_choice_with_room_for_every_expert(et, E, K, N, swiglu, T):
+    """A call whose capacity is T * E takes the kernel of the slots that there are: the
+    device compares them with thresholds, which have to say what the choice at
+    an exact capacity says."""
+    lib, args = et.lib(), (E, K, N, 128, 1 + swiglu)
+    wide, wide64 = (lib.et_w4_from_impl(*args, T * E, 2 * swiglu, T, 256, which) for which in (0, 1))
+    assert 1 <= wide <= wide64 <= T * E + 1
+    for slots in {*range(1, min(T * E, 300)), *(T * k for k in range(1, E + 1)), T * E}:
+        route = lib.et_w4_route_impl(*args, slots, 2 * swiglu, T, 256)
+        # (the rule's whole-number divisions may turn back for a step or two of the slots at a threshold)
+        if all(abs(slots - at) > 2 * E for at in (wide, wide64)):
+            assert (slots >= wide, slots >= wide64) == (route >= 2, route == 3), slots
+    if (E, T) in ((128, 17), (128, 32), (64, 70), (8, 100)):        # two experts a token, or eight of 128
+        assert T * (8 if E == 128 else 2) < wide < T * E

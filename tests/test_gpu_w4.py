@@ -400,3 +400,50 @@ def test_sums_that_cancel(et, dev, route, group):
             p = _toward_zero(p + y @ v.t())
         model = (model + p).float().double()
     assert got.square().mean().sqrt() <= 2 * model.square().mean().sqrt()
+
+
+@pytest.mark.parametrize("E,T,chance,N,parts,kernel", [(8, 100, 0.25, 2048, 1, "split"), (64, 70, 0.04, 2816, 2, "split"),
+                                                       (8, 100, 0.9, 2048, 1, "wide"), (64, 70, 0.4, 2816, 2, "wide"),
+                                                       (32, 200, 0.5, 7168, 1, "wide64"), (16, 140, 0.0, 4096, 1, "split")])
+def test_room_for_every_expert(et, dev, E, T, chance, N, parts, kernel):
+    """A capacity of T * E, which alone would say wide tiles of 64 slots: the device
+    takes the kernel of the slots that there are, the same as with the count known, so the
+    same bits; rows past the slots are left as they were."""
+    g = torch.Generator().manual_seed(E + T)
+    K, group = 264, 64
+    q, s = _weight(g, E, N, K, group, BF16)
+    vals = _values(q, s, group, K)
+    chosen = torch.rand(T, E, generator=g) < chance
+    chosen[torch.arange(T) % 3 > 0, 0] = True
+    plan, expert, token = _plan(et, dev, chosen, known=True)
+    loose, _, _ = _plan(et, dev, chosen, capacity=T * E)
+    S, epi = len(token), 2 if parts == 2 else 0
+    cus = torch.cuda.get_device_properties(dev).multi_processor_count
+    froms = [et.lib().et_w4_from_impl(E, K, N, group, parts, T * E, epi, T, cus, which) for which in (0, 1)]
+    assert kernel == ("split" if S < froms[0] else "wide" if S < froms[1] else "wide64") and froms[0] < T * E
+    x = torch.randn(T, K, generator=g).to(BF16)
+    want, err = torch.zeros(S, N, dtype=torch.float64), torch.zeros(S, N, dtype=torch.float64)
+    for e in range(E):
+        at = expert == e
+        want[at], err[at] = _product64(x[token[at]], vals[e])
+    w = et.pack_w4(q.to(dev), s.to(dev), group=group, parts=parts)
+    epilogue = "swiglu" if parts == 2 else "none"
+    out = torch.full((T * E, N // parts), 3.0, dtype=BF16, device=dev)
+    et.expert_gemm_w4(x.to(dev), w, loose, epilogue=epilogue, out=out)
+    assert _close(out[:S], *(_swiglu(want, err) if parts == 2 else (want, err))) and torch.all(out[S:] == 3.0)
+    assert torch.equal(out[:S], et.expert_gemm_w4(x.to(dev), w, plan, epilogue=epilogue))
+    # captured, with other routings in the same buffers
+    graph = torch.cuda.CUDAGraph()
+    xd = x.to(dev)
+    with torch.cuda.graph(graph):
+        got = et.expert_gemm_w4(xd, w, loose, epilogue=epilogue)
+    for tokens in (T, 1, T // 2, 0, T):
+        part = chosen.clone()
+        part[tokens:] = False
+        small, _, tok = _plan(et, dev, part, capacity=T * E)
+        loose.expert_offsets.copy_(small.expert_offsets)
+        loose.sorted_token.copy_(small.sorted_token)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[:len(tok)], et.expert_gemm_w4(xd, w, small, epilogue=epilogue)[:len(tok)])
+        torch.cuda.synchronize()
