@@ -447,3 +447,22 @@ def test_room_for_every_expert(et, dev, E, T, chance, N, parts, kernel):
         torch.cuda.synchronize()
         assert torch.equal(got[:len(tok)], et.expert_gemm_w4(xd, w, small, epilogue=epilogue)[:len(tok)])
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("T,group", [(130, 128), (97, 32)])
+@pytest.mark.parametrize("route", [2, 3], ids=["wide32", "wide64"])
+def test_blocks_that_take_several_wide_tiles(et, dev, route, T, group):
+    """More tiles than blocks that a GPU holds (three to each of 256 CUs): the next tile's
+    activations go to the LDS of the last one's."""
+    g = torch.Generator().manual_seed(T)
+    N, K = 256 * 520 + 24, 264
+    q, s = _weight(g, 1, N, K, group, BF16)
+    x = torch.randn(T, K, generator=g).to(BF16)
+    assert -(-T // (32 if route == 2 else 64)) * 521 > 2 * 512
+    want, err = _product64(x, _values(q, s, group, K)[0])
+    gemm = importlib.import_module("peer-review-agents_amd.w4")._gemm
+    for parts, epilogue in ((1, "none"), (2, "swiglu")):
+        n = N if parts == 1 else 2 * 128 * 520
+        w = et.pack_w4(q[0, :n].to(dev), s[0, :n].to(dev), group=group, parts=parts)
+        got = gemm(x.to(dev), w, T, None, None, epilogue, None, None, T, route)
+        assert _close(got, *(_swiglu(want[:, :n], err[:, :n]) if parts == 2 else (want, err))), epilogue
