@@ -57,3 +57,58 @@ def test_block_gradients_against_differences(et, dev, example):
     exact = (dx.double() * v.double()).sum().item()
     diff = (c.double() * (up - down)).sum().item() / (2 * step)
     assert abs(exact - diff) <= 0.1 * abs(diff)
+
+
+def _float64_block(block, x, mask):
+    """The block in float64 by torch's autograd, the routing that of `mask`."""
+    gain, bias, w_router, w_gu, w_down = (p.detach().double().requires_grad_(True) for p in block.params)
+    x = x.double().requires_grad_(True)
+    c = x - x.mean(1, keepdim=True)
+    h = c / (c.square().mean(1, keepdim=True) + 1e-5).sqrt() * gain + bias
+    gate = torch.sigmoid(h @ w_router.t()) * mask
+    y = x
+    for e in range(len(w_gu)):
+        gate_up = h @ w_gu[e].t()
+        f = gate_up.shape[1] // 2
+        g = gate_up[:, :f]
+        y = y + gate[:, e:e + 1] * ((g * torch.sigmoid(g) * gate_up[:, f:]) @ w_down[e].t())
+    return y, x, [gain, bias, w_router, w_gu, w_down]
+
+
+@pytest.mark.parametrize("everyone", [True, False])
+def test_every_gradient_against_64_bits(et, dev, example, everyone):
+    """dx past the identity and the five parameters' gradients.  Ten roundings to
+    bf16 on the way (h, gu, a, yp, dyp, da, dgu, dxp, dh, dx), each of
+    2^-9 / sqrt(3) of a value at random, leave 0.4% of a gradient's size; dx, rounded
+    with the identity's part in it, 2^-9 |dy| / sqrt(3) more.  Three times that is
+    allowed.  The norm's own terms (the means over a row that it takes out of dh),
+    which are 6% of it, are also looked at alone."""
+    block = example.Block(256, 8, 128, 2, "cuda", 3)
+    block.router.eval()
+    g = torch.Generator(device=dev).manual_seed(5)
+    block.gain.add_(torch.randn(256, generator=g, device=dev) * 0.2)
+    block.bias.add_(torch.randn(256, generator=g, device=dev) * 0.2)
+    block.router.thr.fill_(0.0 if everyone else 0.6)
+    x = torch.randn(512, 256, generator=g, device=dev).bfloat16()
+    dy = torch.randn(512, 256, generator=g, device=dev).bfloat16()
+    y, kept = block.forward(x)
+    dx, grads = block.backward(dy, kept)
+    plan = kept[4]
+    mask = torch.zeros(512, 8, dtype=torch.float64, device=dev)
+    mask[plan.sorted_token.long(), torch.repeat_interleave(torch.arange(8, device=dev), plan.counts.long())] = 1.0
+    want_y, x64, params = _float64_block(block, x, mask)
+    want = torch.autograd.grad(want_y, [x64] + params, dy.double())
+    allowed = 3 * 0.004
+    assert (y.double() - want_y).norm() <= allowed * (want_y - x64).norm() + 2.0 ** -9 * want_y.norm()
+    past, want_past = dx.double() - dy.double(), want[0] - dy.double()
+    slack = 3 * 2.0 ** -9 / 3 ** 0.5 * dx.double().norm()
+    assert (past - want_past).norm() <= allowed * want_past.norm() + slack
+    for name, a, b in zip(("gain", "bias", "router", "gate_up", "down"), grads, want[1:]):
+        assert (a.double() - b).norm() <= allowed * b.norm(), name
+    # what the norm takes out of a row's gradient: its mean, and its share along xhat (both 0 of past)
+    c = x.double() - x.double().mean(1, keepdim=True)
+    xhat = c / c.square().mean(1, keepdim=True).sqrt()
+    for along in (torch.ones_like(xhat), xhat):
+        share = (past * along).sum(1) / 16.0        # (a row of 256: |along| = 16)
+        # the roundings' part along one direction of 256
+        assert share.norm() <= (allowed * want_past.norm() + slack) / 16.0
