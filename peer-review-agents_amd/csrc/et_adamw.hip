@@ -11,9 +11,12 @@ namespace {
 constexpr int kThreads = 256;
 // Elements of one block of the AdamW kernels: one vector of four for a thread,
 // one block of the 8-bit states for a wave.  HBM bounds the kernels, and blocks
-// that come and go keep the range in flight narrow: 201M elements, f32 states and
-// masters 1165 us (5.43 TB/s; 1184 with 4096 elements to a block, 1213 with 8192),
-// 8-bit states 584 (5.79 TB/s; 660 with 4096).
+// that come and go keep the range in flight narrow.  One tensor of 201.5M elements, f32
+// gradients, back to back on one card (us; 1024, 4096 and 8192 elements to a block):
+//   f32 parameters, f32 states, 28 bytes an element, 5.64 GB      919   923   938   6.14 TB/s
+//   bf16 parameters and masters, f32 states, 30 bytes, 6.04 GB    980   987   996   6.16
+//   f32 parameters, 8-bit states, 16.06 bytes, 3.24 GB            537   579   573   6.03
+//   bf16 and masters, 8-bit states, stochastic, 18.06, 3.64 GB    611   620   617   5.95
 constexpr int kChunk = 1024;
 constexpr int kNormChunk = 16384;     // elements of one block of the norm
 // Tensors of one launch: their table is a kernel argument of 4 KiB at most.
@@ -31,8 +34,8 @@ struct Spans {
 };
 
 // Chunk of a block: the last first.  Behind a gradient norm the gradients that
-// are still in the last-level cache are those at the end (201M elements with the
-// norm 1346 to 1335 us, 50M 324 to 317).
+// are still in the last-level cache are those at the end (201.5M elements with
+// masters and the norm 1133 to 1122 us).
 __device__ __forceinline__ uint32_t chunk_of_block() { return gridDim.x - 1 - blockIdx.x; }
 
 // The tensor of a chunk, found by the wave at once: lane i looks at entry i.
@@ -114,7 +117,8 @@ struct AdamWArgs {
 };
 
 // 28 bytes an element, 30 with a bf16 parameter and its f32 master, for some 20
-// operations: HBM bounds it (201M elements of 30 bytes, 6.04 GB, 996 to 1077 us).
+// operations: HBM bounds it (times at kChunk, from the second call on the same tensors;
+// 201.5M elements with masters, other ones every call: 996 and 1078 us on two cards).
 template <typename P, typename G>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(AdamWArgs t)
 {
@@ -241,7 +245,8 @@ __device__ __forceinline__ void from_e4m3x4(uint32_t w, float scale, float (&x)[
 
 // A block of 256 elements is a wave's, four to a lane, so its largest |m| and sqrt(v)
 // are found within the wave and nothing is read twice.  16 to 18 bytes an element: HBM
-// bounds it (201M elements of 18 bytes, 3.64 GB, 584 to 664 us).
+// bounds it (times at kChunk; 201.5M elements with masters, other ones every call: 652 and
+// 664 us on two cards).
 template <typename P, typename G, bool STOCHASTIC>
 __global__ __launch_bounds__(kThreads) void adamw8_kernel(AdamW8Args t)
 {
@@ -387,7 +392,7 @@ __device__ __forceinline__ double block_sum(double s)
 }
 
 // Each block's sum of squares in binary64, of squares in binary64.  Reading bounds it:
-// 842 MB 142 us, 5.95 TB/s (180 us with one load at a time instead of four).
+// 806 MB 136 us, 5.94 TB/s (140 with one load at a time instead of four).
 __global__ __launch_bounds__(kThreads) void grad_norm_kernel(NormArgs t)
 {
     const int i = find_tensor(t.spans, blockIdx.x);
@@ -399,8 +404,8 @@ __global__ __launch_bounds__(kThreads) void grad_norm_kernel(NormArgs t)
     if (threadIdx.x == 0) t.partial[blockIdx.x] = all;
 }
 
-// One block, eight loads of a thread at a time (12300 partials, of 200M elements:
-// 15 us one by one in 256 threads).
+// One block, eight loads of a thread at a time (12297 partials, of 201.5M elements: 5 us;
+// 15 one by one in 256 threads).
 constexpr int kFinishThreads = 1024;
 
 __global__ __launch_bounds__(kFinishThreads) void grad_norm_finish_kernel(const double* partial, int64_t n, float max_norm,
