@@ -456,7 +456,7 @@ __device__ __forceinline__ void w4_split_tile(const W4Args& g, const W4Tile& t, 
 // others for a wave's 4 KiB of weights.  (On one SIMD 32 MFMAs of one wave take
 // 584 cycles, 256 v_and_or and shifts of another 1218, both at once 1471: an MFMA costs the
 // other wave 8 cycles.)  With 32 slots a weight is unpacked twice as often.  64 experts of
-// a mean of 64 slots, K = 2048, N = 2816, 32 slots to a tile, 91 us: CUs busy 81% of the
+// a mean of 64 slots, K = 2048, N = 2816, 32 slots to a tile, 90 us: CUs busy 82% of the
 // time; of that the matrix pipes 39%, while 27 M vector instructions are issued (66% at 4
 // cycles each).  The order in which a wave issues them, its priority, a ring of four k
 // ranges and (at 64 slots) a third block to a CU change nothing.
