@@ -408,9 +408,8 @@ class AdamW:
         elif params:
             _step(fn, dev, params, grads, states, masters, sizes, scalars, grad_scale, *more)
         _changed(params)
-        if counts is None and not whole:
-            counts = self._counts = [number] * len(self.params)
-        if counts is not None:
+        if counts is not None or not whole:
+            counts = self._counts = [number] * len(self.params) if counts is None else list(counts)
             for i in some:
                 counts[i] += 1
         self._steps = number + 1

@@ -677,3 +677,14 @@ def test_workspaces_that_only_look_large_are_refused(et, dev):
     for bad in (small[:1].expand(4096), small[:1].expand(64, 64), torch.zeros(9000, device=dev)[::2]):
         with pytest.raises(ValueError, match="workspace"):
             et.grad_norm([torch.ones(1 << 20, device=dev)], workspace=bad)
+
+
+def test_a_shallow_copy_counts_for_itself(et, dev):
+    import copy
+    p = [torch.zeros(8, device=dev), torch.zeros(8, device=dev)]
+    g = torch.ones(8, device=dev)
+    opt = et.AdamW(p)
+    opt.step([g, None])
+    other = copy.copy(opt)
+    other.step([g, g])
+    assert opt.state_dict()["counts"] == [1, 0] and other.state_dict()["counts"] == [2, 1]
