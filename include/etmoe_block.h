@@ -23,7 +23,7 @@
 extern "C" {
 #endif
 
-#define ET_BLOCK_ABI_VERSION 1
+#define ET_BLOCK_ABI_VERSION 2      /* 2: the values of a packed 4-bit weight lie three bits further */
 
 int et_block_abi_version(void);
 
@@ -177,8 +177,8 @@ int et_adamw8(void* const* params, const void* const* grads, uint8_t* const* m8,
  * `packed` of et_w4_packed_bytes bytes and `packed_scales` of
  * et_w4_packed_scales 16-bit numbers, 16-byte aligned.  parts 2 lays the first and the
  * second half of the rows out each for itself, as SwiGLU's gate and up rows
- * need it (N a multiple of 8 for each part); 1 else.  Sizes are 0 for invalid
- * arguments.
+ * need it (N a multiple of 8 for each part); 1 else.  The layout is that of
+ * one ET_BLOCK_ABI_VERSION.  Sizes are 0 for invalid arguments.
  */
 size_t et_w4_packed_bytes(int64_t num_experts, int64_t N, int64_t K, int64_t parts);
 size_t et_w4_packed_scales(int64_t num_experts, int64_t N, int64_t K, int64_t group, int64_t parts);

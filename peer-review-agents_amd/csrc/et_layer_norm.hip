@@ -271,9 +271,10 @@ struct BwdArgs {
 // anew, so that none is a chain of more (262144 rows of 520 in f32: 1.8e-7 of the sum's size
 // off, 6.0e-7 in one chain of 1024).  The second ones are in LDS, the thread's own places (a
 // wave a row: in registers they cost as much).  With 16 waves a row (rows of more than 8192)
-// the first are in LDS, which spares registers that would spill, and the second in memory,
-// every 64 rows (4096 x 16384 bf16 with DSUM 162 to 124 us, 2048 x 9000 f32 126 to 72; 32768 x
-// 16384, where memory's part counts, 702 to 734).  DSUM: a gradient past the norm is added.
+// the first are in LDS, which spares registers that would spill (6 to 20 still do in f32 with
+// DSUM), and the second in memory, every 64 rows (4096 x 16384 bf16 with DSUM 162 to 124 us,
+// 2048 x 9000 f32 126 to 72; 32768 x 16384, where memory's part counts, 702 to 734).  DSUM: a
+// gradient past the norm is added.
 template <typename X, typename W, int WPR, int NV, int D, bool TAIL, bool DSUM>
 __global__ __launch_bounds__(norm_threads(WPR)) void layer_norm_bwd_kernel(BwdArgs a)
 {

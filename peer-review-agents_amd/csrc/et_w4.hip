@@ -691,7 +691,8 @@ __device__ __forceinline__ int count_slots(const W4Args& g)
 
 // Blocks of the wide kernel to a CU: 168 registers allow three of those with
 // 32 slots, whose time is the weight's stream (61 tokens, 32 experts, K = 2048,
-// N = 7168, groups of 32: 60.5 us against 65.6 with two).
+// N = 7168, groups of 32: 60.5 us against 65.6 with two).  With groups of 128 the
+// bounds make them spill 13 to 19 registers, of 64 2 or 3, outside the loop over k.
 constexpr int wide_blocks(int maxmt) { return maxmt == 2 ? 3 : 2; }
 
 // `tiles`: the experts' slot tiles.
@@ -894,7 +895,7 @@ W4From from_of(const W4Args& g, bool swiglu, int64_t max_slots, int64_t cus)
         }
         return lo;
     };
-    return W4From{first(kWide32), first(kWide64)};
+    return W4From{first(kWide32), route_of(g, swiglu, g.cap, max_slots, cus) < kWide64 ? g.cap + 1 : first(kWide64)};
 }
 
 int check_shape(const char* fn, int64_t E, int64_t N, int64_t K, int64_t group, int64_t parts)

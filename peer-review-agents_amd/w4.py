@@ -21,7 +21,8 @@ _GROUPS = (32, 64, 128)
 class W4Weight:
     """A 4-bit weight as the products read it: w = (q - 8) * scale of E experts
     (1: a dense layer), N rows, K columns, ``group`` columns to a scale.  Made by
-    :func:`pack_w4`; ``packed`` and ``scales`` are its layout, not for indexing."""
+    :func:`pack_w4`; ``packed`` and ``scales`` are its layout, not for indexing, and
+    that of one version of the library (a pickle of another version's raises)."""
 
     packed: torch.Tensor
     scales: torch.Tensor
@@ -30,6 +31,15 @@ class W4Weight:
     K: int
     group: int
     parts: int
+
+    def __getstate__(self) -> dict:
+        return {**self.__dict__, "layout": lib().et_block_abi_version()}
+
+    def __setstate__(self, state: dict) -> None:
+        state = dict(state)
+        if state.pop("layout", None) != lib().et_block_abi_version():
+            raise ValueError("the weight was packed by another version of the library: pack its values and scales again")
+        self.__dict__.update(state)
 
     def __post_init__(self) -> None:
         # (the products read as much as these sizes say)

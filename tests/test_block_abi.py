@@ -170,6 +170,11 @@ def test_a_4_bit_weight_holds_what_its_sizes_say(et):
 
     w = weight()
     assert copy.deepcopy(w).packed.numel() == w.packed.numel()
+    # a pickle of another version's layout, or of one without a version
+    state = w.__getstate__()
+    for layout in (et.lib().et_block_abi_version() - 1, None):
+        with pytest.raises(ValueError, match="pack"):
+            et.W4Weight.__new__(et.W4Weight).__setstate__({**state, "layout": layout})
     assert dataclasses.replace(w, scales=w.scales.half()).scales.dtype == torch.float16
     for bad in (dict(packed=2 * 2048), dict(scales=32), dict(E=2), dict(K=264), dict(N=72), dict(group=64), dict(parts=3),
                 dict(at=1), dict(E=0), dict(group=48), dict(N=44)):
