@@ -7,7 +7,7 @@ dispatch path), norm.py (layer norm), optimizer.py (AdamW, the gradient norm)
 and w4.py (products with 4-bit weights), and ops.py registers
 the path as PyTorch operators (torch.ops.etmoe.*).
 """
-from ._lib import BLOCK_HEADER_PATH, ETMoEError, LIB_PATH, header_symbols, lib  # noqa: F401
+from ._lib import BLOCK_HEADER_PATH, DENSE_HEADER_PATH, ETMoEError, LIB_PATH, header_symbols, lib  # noqa: F401
 from . import ops  # noqa: F401  (registers torch.ops.etmoe.*)
 from .expert_threshold import (  # noqa: F401
     ExpertThresholdRouter,
@@ -35,6 +35,12 @@ from .expert_threshold import (  # noqa: F401
     swiglu_backward,
     threshold_update_,
     threshold_workspace_bytes,
+)
+from .gated import (  # noqa: F401
+    gated_linear,
+    gated_linear_autograd,
+    gated_linear_backward,
+    gated_linear_backward_workspace_bytes,
 )
 from .norm import (  # noqa: F401
     layer_norm,

@@ -18,6 +18,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libetmoe.so")
 HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "etmoe.h")
 BLOCK_HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "etmoe_block.h")
+DENSE_HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "etmoe_dense.h")
 
 ET_DTYPE_F32 = 0
 ET_DTYPE_BF16 = 1
@@ -25,6 +26,7 @@ ET_MAX_EXPERTS = 1024
 ET_MAX_ROUTER_EXPERTS = 256
 ET_MAX_NORM_WIDTH = 16384
 ET_GEMM_PLAIN, ET_GEMM_ROW_SCALE, ET_GEMM_SWIGLU = 0, 1, 2
+ET_GATED_SILU, ET_GATED_GELU = 0, 1
 
 
 class ETMoEError(RuntimeError):
@@ -73,6 +75,15 @@ _BLOCK_SIGNATURES = {
     "et_w4_from_impl": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _int, _i64, _i64, _int]),
     "et_w4_route_impl": (_int, [_i64, _i64, _i64, _i64, _i64, _i64, _int, _i64, _i64]),
     "et_adamw8": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _int, _int, AdamWScalars, _p, _int, _u32, _p]),
+}
+
+# Names of include/etmoe_dense.h.
+_DENSE_SIGNATURES = {
+    "et_dense_abi_version": (_int, []),
+    "et_gated_linear": (_int, [_p, _i64, _p, _i64, _i64, _i64, _int, _p, _p]),
+    "et_gated_linear_impl": (_int, [_p, _i64, _p, _i64, _i64, _i64, _int, _p, _int, _p]),
+    "et_gated_linear_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "et_gated_linear_bwd": (_int, [_p, _p, _i64, _p, _i64, _i64, _i64, _int, _p, _p, _int, _p, _sz, _p]),
 }
 
 _SIGNATURES = {
@@ -136,7 +147,7 @@ def lib() -> ctypes.CDLL:
                 f"{LIB_PATH} is not built; run __graft_entry__.build() "
                 "(there is no CPU fallback for this path)")
         L = ctypes.CDLL(LIB_PATH)
-        for name, (res, args) in {**_SIGNATURES, **_BLOCK_SIGNATURES}.items():
+        for name, (res, args) in {**_SIGNATURES, **_BLOCK_SIGNATURES, **_DENSE_SIGNATURES}.items():
             fn = getattr(L, name)
             fn.restype = res
             fn.argtypes = args

@@ -1,6 +1,7 @@
 // et_abi.hip -- status plumbing of the C ABI (et_last_error, et_abi_version).
 #include "et_common.hpp"
 #include "etmoe_block.h"
+#include "etmoe_dense.h"
 
 namespace et {
 
@@ -27,5 +28,7 @@ int check_launch(const char* what)
 extern "C" int et_abi_version(void) { return ET_ABI_VERSION; }
 
 extern "C" int et_block_abi_version(void) { return ET_BLOCK_ABI_VERSION; }
+
+extern "C" int et_dense_abi_version(void) { return ET_DENSE_ABI_VERSION; }
 
 extern "C" const char* et_last_error(void) { return et::g_last_error.c_str(); }

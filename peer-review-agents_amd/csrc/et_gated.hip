@@ -1,0 +1,471 @@
+// et_gated.hip -- the gated projection of a dense (shared) expert, forward and
+// backward (gfx950):
+//
+//   g = x Wg^T,  u = x Wu^T       W [2F, K]: the F gate rows, then the F up rows
+//   h = act(g) * u                act: SiLU g sigmoid(g), or GELU g Phi(g)
+//
+//   dp = [dh u act'(g) | dh act(g)],  dx = dp W,  dW = dp^T x
+//
+// Forward: one kernel; a tile's weight rows are gate rows and the up rows of the
+// same hidden units, so a lane holds both of a unit in its accumulators and writes
+// h alone.  Backward: nothing but x and W is kept from the forward.  The same
+// product runs again with dh in its epilogue, which writes dp (bf16, the one
+// rounding between the two products: dp is an operand of the matrix units), and
+// two products follow, dx with W read down its columns and dW with dp and x both
+// read down their columns, its sum over the tokens split where there are too few
+// tiles to fill the GPU.
+#include "et_dense_gemm.hpp"
+#include "etmoe_dense.h"
+
+namespace et {
+namespace {
+
+constexpr float kRootHalf = 0.70710678118654752f, kInvRoot2Pi = 0.39894228040143268f;
+
+// act(g) and, for the backward, act'(g).
+// SiLU: s = sigmoid(g), g s, s (1 + g (1 - s)).  GELU: Phi(g) = erfc(-g / sqrt 2) / 2
+// (not 1 + erf, which cancels below 0), g Phi, Phi + g phi.
+template <int ACT>
+__device__ __forceinline__ float gate_value(float g)
+{
+    if constexpr (ACT == ET_GATED_SILU) return g * sigmoid(g);
+    else return g * (0.5f * erfcf(-g * kRootHalf));
+}
+
+template <int ACT>
+__device__ __forceinline__ void gate_slope(float g, float& value, float& slope)
+{
+    if constexpr (ACT == ET_GATED_SILU) {
+        const float s = sigmoid(g);
+        value = g * s;
+        slope = s * (1.0f + g * (1.0f - s));
+    } else {
+        const float p = 0.5f * erfcf(-g * kRootHalf);
+        value = g * p;
+        slope = p + g * (kInvRoot2Pi * expf(-0.5f * g * g));
+    }
+}
+
+struct GatedArgs {
+    const unsigned char* x;    // [T, K], row stride ldx
+    const unsigned char* w;    // [2F, K]
+    uint16_t* out;             // h [T, F], or dp [T, 2F]
+    const uint16_t* dh;        // [T, F]
+    int64_t T;
+    int ldx, K, F;
+    int nm, nn;
+};
+
+// x (rows) times gate and up rows: a wave's first NJ / 2 tiles are gate rows, the
+// others the up rows of the same hidden units.
+template <int SIDE, int ACT, bool BACKWARD>
+struct GatedPolicy {
+    static constexpr int MI = SIDE, NJ = SIDE;
+    static constexpr bool kACol = false, kBCol = false, kF16 = false;
+    static constexpr int kBlocks = SIDE == 8 ? 1 : 2;
+    static constexpr int BM = 32 * MI, BH = 16 * NJ;      // rows and hidden units of a tile
+    using Args = GatedArgs;
+    struct Tile : GemmTile {
+        int64_t m0;
+        int n0;
+    };
+    __device__ static int tiles(const Args& g) { return g.nm * g.nn; }
+    __device__ static void tile(const Args& g, int q, Tile& t)
+    {
+        const TileAt at = tile_at(q, g.nm, g.nn, 8);
+        t.m0 = (int64_t)at.m * BM;
+        t.n0 = at.n * BH;
+        t.a = g.x + t.m0 * g.ldx * 2;
+        t.b = g.w;
+        t.a_rows = (int)min<int64_t>(BM, g.T - t.m0);
+        t.b_rows = 2 * g.F;
+        t.lda = g.ldx;
+        t.ldb = g.K;
+        t.k = g.K;
+    }
+    // the weight row of the tile's rows R ..  R + 7 (F is a multiple of 8)
+    __device__ static int b_row(const Args& g, const Tile& t, int R)
+    {
+        const int tt = (R % (16 * NJ)) / 16;
+        const int hid = t.n0 + R / (16 * NJ) * (8 * NJ) + tt % (NJ / 2) * 16 + (R & 15);
+        return hid < g.F ? (tt >= NJ / 2 ? g.F + hid : hid) : -1;
+    }
+    __device__ static void epilogue(const Args& g, const Tile& t, f32x4_t (&acc)[MI][NJ], int wm, int wn, int r16, int rho)
+    {
+        const int F = g.F;
+        const int width = BACKWARD ? 2 * F : F;
+        const __amdgpu_buffer_rsrc_t res = dense_rsrc(g.out + t.m0 * width, t.a_rows * width * 2);
+        const __amdgpu_buffer_rsrc_t dres = dense_rsrc(BACKWARD ? g.dh + t.m0 * F : nullptr, t.a_rows * F * 2);
+        const int c0 = t.n0 + wn * (8 * NJ);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            __builtin_amdgcn_sched_barrier(0);       // one row tile at a time: few temporaries
+            const int row = (wm * MI + i) * 16 + r16;
+            const bool ok = row < t.a_rows;
+            u32x2_t d[NJ / 2];
+            if constexpr (BACKWARD) {
+#pragma unroll
+                for (int j = 0; j < NJ / 2; ++j) {
+                    const int col = c0 + j * 16 + 4 * rho;
+                    d[j] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(
+                        dres, ok && col < F ? (uint32_t)(row * F + col) * 2u : kOOR, 0, 0));
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < NJ / 2; j += 2) {
+                float v[8], w[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int jj = j + (e >> 2);
+                    const float gate = acc[i][jj][e & 3], up = acc[i][jj + NJ / 2][e & 3];
+                    if constexpr (BACKWARD) {
+                        const uint32_t word = d[jj][(e & 3) >> 1];
+                        const float dh = (e & 1) ? bf16hi(word) : bf16lo(word);
+                        float value, slope;
+                        gate_slope<ACT>(gate, value, slope);
+                        v[e] = dh * up * slope;
+                        w[e] = dh * value;
+                    } else {
+                        v[e] = gate_value<ACT>(gate) * up;
+                    }
+                }
+                store_pair<false>(v, res, ok, (uint32_t)(row * width), c0 + j * 16, F, rho);
+                if constexpr (BACKWARD)
+                    store_pair<false>(w, res, ok, (uint32_t)(row * width + F), c0 + j * 16, F, rho);
+            }
+        }
+    }
+};
+
+// dx [T, K] = dp [T, 2F] W, W read down its columns.
+struct InputGradArgs {
+    const unsigned char* dp;
+    const unsigned char* w;
+    uint16_t* dx;
+    int64_t T;
+    int K, F;
+    int nm, nn;
+};
+
+template <int SIDE>
+struct InputGradPolicy {
+    static constexpr int MI = SIDE, NJ = SIDE;
+    static constexpr bool kACol = false, kBCol = true, kF16 = false;
+    static constexpr int kBlocks = SIDE == 8 ? 1 : 2;
+    static constexpr int BM = 32 * MI, BN = 32 * NJ;
+    using Args = InputGradArgs;
+    struct Tile : GemmTile {
+        int64_t m0;
+        int n0;
+    };
+    __device__ static int tiles(const Args& g) { return g.nm * g.nn; }
+    __device__ static void tile(const Args& g, int q, Tile& t)
+    {
+        const TileAt at = tile_at(q, g.nm, g.nn, 8);
+        t.m0 = (int64_t)at.m * BM;
+        t.n0 = at.n * BN;
+        t.a = g.dp + t.m0 * (2 * g.F) * 2;
+        t.b = g.w + (int64_t)t.n0 * 2;
+        t.a_rows = (int)min<int64_t>(BM, g.T - t.m0);
+        t.b_rows = min(BN, g.K - t.n0);
+        t.lda = 2 * g.F;
+        t.ldb = g.K;
+        t.k = 2 * g.F;
+    }
+    __device__ static int b_row(const Args&, const Tile&, int) { return -1; }
+    __device__ static void epilogue(const Args& g, const Tile& t, f32x4_t (&acc)[MI][NJ], int wm, int wn, int r16, int rho)
+    {
+        const __amdgpu_buffer_rsrc_t res = dense_rsrc(g.dx + t.m0 * g.K, t.a_rows * g.K * 2);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            const int row = (wm * MI + i) * 16 + r16;
+#pragma unroll
+            for (int j = 0; j < NJ; j += 2) {
+                __builtin_amdgcn_sched_barrier(0);
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = acc[i][j + (e >> 2)][e & 3];
+                store_pair<false>(v, res, row < t.a_rows, (uint32_t)(row * g.K), t.n0 + (wn * NJ + j) * 16, g.K, rho);
+            }
+        }
+    }
+};
+
+// dW [2F, K] = dp^T x over tokens [split * step, + step): bf16, or f32 (dW itself,
+// or a split's partial sums).
+struct WeightGradArgs {
+    const unsigned char* dp;   // [T, 2F]
+    const unsigned char* x;    // [T, K], row stride ldx
+    void* dw;                  // [splits, 2F, K]
+    int64_t T, step;
+    int ldx, K, F;
+    int nm, nn, splits;
+    bool f32;
+};
+
+template <int SIDE>
+struct WeightGradPolicy {
+    static constexpr int MI = SIDE, NJ = SIDE;
+    static constexpr bool kACol = true, kBCol = true, kF16 = false;
+    static constexpr int kBlocks = SIDE == 8 ? 1 : 2;
+    static constexpr int BM = 32 * MI, BN = 32 * NJ;
+    using Args = WeightGradArgs;
+    struct Tile : GemmTile {
+        int split, m0, n0;
+    };
+    __device__ static int tiles(const Args& g) { return g.nm * g.nn * g.splits; }
+    __device__ static void tile(const Args& g, int q, Tile& t)
+    {
+        t.split = q / (g.nm * g.nn);
+        const TileAt at = tile_at(q - t.split * (g.nm * g.nn), g.nm, g.nn, 8);
+        t.m0 = at.m * BM;
+        t.n0 = at.n * BN;
+        const int64_t k0 = t.split * g.step;
+        t.a = g.dp + (k0 * (2 * g.F) + t.m0) * 2;
+        t.b = g.x + (k0 * g.ldx + t.n0) * 2;
+        t.a_rows = min(BM, 2 * g.F - t.m0);
+        t.b_rows = min(BN, g.K - t.n0);
+        t.lda = 2 * g.F;
+        t.ldb = g.ldx;
+        t.k = (int)min<int64_t>(g.step, g.T - k0);
+    }
+    __device__ static int b_row(const Args&, const Tile&, int) { return -1; }
+    __device__ static void epilogue(const Args& g, const Tile& t, f32x4_t (&acc)[MI][NJ], int wm, int wn, int r16, int rho)
+    {
+        const int es = g.f32 ? 4 : 2;
+        const int64_t first = ((int64_t)t.split * 2 * g.F + t.m0) * g.K;
+        const __amdgpu_buffer_rsrc_t res = dense_rsrc((unsigned char*)g.dw + first * es, t.a_rows * g.K * es);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            const int row = (wm * MI + i) * 16 + r16;
+            if (g.f32) {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    const int col = t.n0 + (wn * NJ + j) * 16 + 4 * rho;
+                    const uint32_t off = row < t.a_rows && col < g.K ? (uint32_t)(row * g.K + col) * 4u : kOOR;
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, acc[i][j]), res, off, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < NJ; j += 2) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = acc[i][j + (e >> 2)][e & 3];
+                    store_pair<false>(v, res, row < t.a_rows, (uint32_t)(row * g.K), t.n0 + (wn * NJ + j) * 16, g.K, rho);
+                }
+            }
+        }
+    }
+};
+
+// The splits' partial sums added in order (n a multiple of 8).
+__global__ __launch_bounds__(kDenseThreads) void gated_fold_kernel(const float* partial, int64_t n, int splits, void* dw, bool f32)
+{
+    for (int64_t at = ((int64_t)blockIdx.x * kDenseThreads + threadIdx.x) * 4; at < n;
+         at += (int64_t)gridDim.x * kDenseThreads * 4) {
+        f32x4_t v = *reinterpret_cast<const f32x4_t*>(partial + at);
+        for (int s = 1; s < splits; ++s) v += *reinterpret_cast<const f32x4_t*>(partial + s * n + at);
+        if (f32) *reinterpret_cast<f32x4_t*>((float*)dw + at) = v;
+        else *reinterpret_cast<u32x2_t*>((uint16_t*)dw + at) = u32x2_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    }
+}
+
+__global__ __launch_bounds__(kDenseThreads) void gated_zero_kernel(uint32_t* p, int64_t words)
+{
+    for (int64_t at = (int64_t)blockIdx.x * kDenseThreads + threadIdx.x; at < words; at += (int64_t)gridDim.x * kDenseThreads)
+        p[at] = 0u;
+}
+
+int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+template <template <int> class POLICY, class ARGS>
+int launch_sided(ARGS g, int side, int64_t tiles, hipStream_t s, const char* what)
+{
+    const int cus = dense_cus();
+    if (side == 8) dense_gemm_kernel<POLICY<8>><<<dim3(dense_grid(tiles, 1, cus)), dim3(kDenseThreads), 0, s>>>(g);
+    else dense_gemm_kernel<POLICY<4>><<<dim3(dense_grid(tiles, 2, cus)), dim3(kDenseThreads), 0, s>>>(g);
+    return check_launch(what);
+}
+
+template <int SIDE> using SiluFwd = GatedPolicy<SIDE, ET_GATED_SILU, false>;
+template <int SIDE> using GeluFwd = GatedPolicy<SIDE, ET_GATED_GELU, false>;
+template <int SIDE> using SiluBwd = GatedPolicy<SIDE, ET_GATED_SILU, true>;
+template <int SIDE> using GeluBwd = GatedPolicy<SIDE, ET_GATED_GELU, true>;
+
+// Tile side of a product of m x n outputs (8: 256 x 256 tiles, 4: 128 x 128).
+int dense_side(int64_t m, int64_t n, int64_t splits = 1)
+{
+    const int cus = dense_cus();
+    const int64_t big = up(m, 256) * up(n, 256) * splits, small = up(m, 128) * up(n, 128) * splits;
+    return 4 * up(big, cus) <= 3 * up(small, 2 * cus) ? 8 : 4;
+}
+
+int check_sizes(const char* fn, int64_t T, int64_t K, int64_t F, int64_t ldx, int act)
+{
+    const std::string at = fn;
+    if (T < 0 || T >= (int64_t)1 << 31) return fail(ET_ERR_INVALID_ARGUMENT, at + ": rows must be in [0, 2^31)");
+    if (K < 8 || K % 8 || K >= 1 << 21) return fail(ET_ERR_INVALID_ARGUMENT, at + ": K must be a positive multiple of 8 below 2^21");
+    if (F < 8 || F % 8 || F >= 1 << 20) return fail(ET_ERR_INVALID_ARGUMENT, at + ": F must be a positive multiple of 8 below 2^20");
+    if (2 * F * K * 2 >= (int64_t)1 << 31) return fail(ET_ERR_INVALID_ARGUMENT, at + ": the weight must be below 2 GiB");
+    if (ldx < K || ldx % 8 || ldx >= 1 << 22)
+        return fail(ET_ERR_INVALID_ARGUMENT, at + ": the row stride of x must be a multiple of 8, at least K and below 2^22");
+    if (act != ET_GATED_SILU && act != ET_GATED_GELU) return fail(ET_ERR_INVALID_ARGUMENT, at + ": unknown activation");
+    return ET_OK;
+}
+
+int check_pointer(const char* fn, const char* name, const void* p)
+{
+    if (!p) return fail(ET_ERR_INVALID_ARGUMENT, std::string(fn) + ": null " + name);
+    if ((uintptr_t)p % 16) return fail(ET_ERR_INVALID_ARGUMENT, std::string(fn) + ": " + name + " must be 16-byte aligned");
+    return ET_OK;
+}
+
+int launch_gated(GatedArgs g, int act, bool backward, int side, hipStream_t s)
+{
+    if (side == 0) side = dense_side(g.T, 2 * g.F);
+    g.nm = (int)up(g.T, 32 * side);
+    g.nn = (int)up(g.F, 16 * side);
+    const int64_t tiles = (int64_t)g.nm * g.nn;
+    if (act == ET_GATED_SILU)
+        return backward ? launch_sided<SiluBwd>(g, side, tiles, s, "gated_backward") : launch_sided<SiluFwd>(g, side, tiles, s, "gated_linear");
+    return backward ? launch_sided<GeluBwd>(g, side, tiles, s, "gated_backward") : launch_sided<GeluFwd>(g, side, tiles, s, "gated_linear");
+}
+
+// Splits of dW's sum over the tokens: as many blocks as the GPU holds, a split
+// of 512 tokens at least.
+struct Split {
+    int side, splits;
+    int64_t step;
+};
+Split split_tokens(int64_t T, int64_t K, int64_t F)
+{
+    const int cus = dense_cus();
+    if (up(2 * F, 256) * up(K, 256) * 4 >= 3 * cus) return {8, 1, T};
+    const int64_t tiles = up(2 * F, 128) * up(K, 128);
+    const int64_t most = std::max<int64_t>(1, 2 * cus / tiles);
+    const int64_t step = std::max<int64_t>(512, up(up(T, most), 64) * 64);
+    return {4, (int)std::max<int64_t>(1, up(T, step)), step};
+}
+
+}  // namespace
+}  // namespace et
+
+using namespace et;
+
+extern "C" int et_gated_linear_impl(const void* x, int64_t x_stride, const void* w, int64_t rows, int64_t K, int64_t F,
+                                    int activation, void* h, int side, void* stream)
+{
+    const char* fn = "et_gated_linear";
+    int rc = check_sizes(fn, rows, K, F, x_stride, activation);
+    if (rc || rows == 0) return rc;
+    for (const auto& [p, name] : {std::pair<const void*, const char*>{x, "x"}, {w, "w"}, {h, "h"}}) {
+        rc = check_pointer(fn, name, p);
+        if (rc) return rc;
+    }
+    GatedArgs g = {};
+    g.x = (const unsigned char*)x;
+    g.w = (const unsigned char*)w;
+    g.out = (uint16_t*)h;
+    g.T = rows;
+    g.ldx = (int)x_stride;
+    g.K = (int)K;
+    g.F = (int)F;
+    return launch_gated(g, activation, false, side, (hipStream_t)stream);
+}
+
+extern "C" int et_gated_linear(const void* x, int64_t x_stride, const void* w, int64_t rows, int64_t K, int64_t F,
+                               int activation, void* h, void* stream)
+{
+    return et_gated_linear_impl(x, x_stride, w, rows, K, F, activation, h, 0, stream);
+}
+
+extern "C" size_t et_gated_linear_bwd_workspace_bytes(int64_t rows, int64_t K, int64_t F)
+{
+    if (rows < 0 || K < 8 || F < 8) return 0;
+    const Split sp = split_tokens(rows, K, F);
+    const size_t dp = (size_t)up(rows * 2 * F * 2, 256) * 256;
+    return dp + (sp.splits > 1 ? (size_t)sp.splits * 2 * F * K * 4 : 0);
+}
+
+extern "C" int et_gated_linear_bwd(const void* dh, const void* x, int64_t x_stride, const void* w, int64_t rows, int64_t K,
+                                   int64_t F, int activation, void* dx, void* dw, int dw_dtype, void* workspace,
+                                   size_t workspace_bytes, void* stream)
+{
+    const char* fn = "et_gated_linear_bwd";
+    int rc = check_sizes(fn, rows, K, F, x_stride, activation);
+    if (rc) return rc;
+    if (dw_dtype != ET_DTYPE_F32 && dw_dtype != ET_DTYPE_BF16)
+        return fail(ET_ERR_INVALID_ARGUMENT, "et_gated_linear_bwd: dw_dtype must be ET_DTYPE_F32 or ET_DTYPE_BF16");
+    hipStream_t s = (hipStream_t)stream;
+    const bool f32 = dw_dtype == ET_DTYPE_F32;
+    if (dw && (rc = check_pointer(fn, "dw", dw))) return rc;
+    if (rows == 0) {
+        if (!dw) return ET_OK;
+        const int64_t words = 2 * F * K * (f32 ? 4 : 2) / 4;
+        gated_zero_kernel<<<dim3((unsigned)std::min<int64_t>(1024, up(words, kDenseThreads))), dim3(kDenseThreads), 0, s>>>(
+            (uint32_t*)dw, words);
+        return check_launch("gated_zero_kernel");
+    }
+    for (const auto& [p, name] : {std::pair<const void*, const char*>{dh, "dh"}, {x, "x"}, {w, "w"}}) {
+        rc = check_pointer(fn, name, p);
+        if (rc) return rc;
+    }
+    if (dx && (rc = check_pointer(fn, "dx", dx))) return rc;
+    const size_t need = et_gated_linear_bwd_workspace_bytes(rows, K, F);
+    if (workspace_bytes < need) return fail(ET_ERR_WORKSPACE_TOO_SMALL, "et_gated_linear_bwd: workspace needs " + std::to_string(need) + " bytes");
+    if ((rc = check_pointer(fn, "workspace", workspace))) return rc;
+    unsigned char* const dp = (unsigned char*)workspace;
+    GatedArgs g = {};
+    g.x = (const unsigned char*)x;
+    g.w = (const unsigned char*)w;
+    g.out = (uint16_t*)dp;
+    g.dh = (const uint16_t*)dh;
+    g.T = rows;
+    g.ldx = (int)x_stride;
+    g.K = (int)K;
+    g.F = (int)F;
+    rc = launch_gated(g, activation, true, 0, s);
+    if (rc) return rc;
+    if (dx) {
+        InputGradArgs a = {};
+        a.dp = dp;
+        a.w = (const unsigned char*)w;
+        a.dx = (uint16_t*)dx;
+        a.T = rows;
+        a.K = (int)K;
+        a.F = (int)F;
+        const int side = dense_side(rows, K);
+        a.nm = (int)up(rows, 32 * side);
+        a.nn = (int)up(K, 32 * side);
+        rc = launch_sided<InputGradPolicy>(a, side, (int64_t)a.nm * a.nn, s, "gated_input_grad");
+        if (rc) return rc;
+    }
+    if (dw) {
+        const Split sp = split_tokens(rows, K, F);
+        WeightGradArgs a = {};
+        a.dp = dp;
+        a.x = (const unsigned char*)x;
+        float* const partial = (float*)(dp + up(rows * 2 * F * 2, 256) * 256);
+        a.dw = sp.splits > 1 ? (void*)partial : dw;
+        a.f32 = f32 || sp.splits > 1;
+        a.T = rows;
+        a.step = sp.step;
+        a.splits = sp.splits;
+        a.ldx = (int)x_stride;
+        a.K = (int)K;
+        a.F = (int)F;
+        a.nm = (int)up(2 * F, 32 * sp.side);
+        a.nn = (int)up(K, 32 * sp.side);
+        rc = launch_sided<WeightGradPolicy>(a, sp.side, (int64_t)a.nm * a.nn * sp.splits, s, "gated_weight_grad");
+        if (rc) return rc;
+        if (sp.splits > 1) {
+            const int64_t n = 2 * F * K;
+            gated_fold_kernel<<<dim3((unsigned)std::min<int64_t>(4096, up(n, 4 * kDenseThreads))), dim3(kDenseThreads), 0, s>>>(
+                partial, n, sp.splits, dw, f32);
+            rc = check_launch("gated_fold_kernel");
+        }
+    }
+    return rc;
+}
