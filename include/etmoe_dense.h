@@ -60,6 +60,58 @@ int et_gated_linear_bwd(const void* dh, const void* x, int64_t x_stride, const v
                         int activation, void* dx, void* dw, int dw_dtype, void* workspace, size_t workspace_bytes,
                         void* stream);
 
+/* ------------------------------------------------------------------------ *
+ * Orthogonalised updates of matrices
+ * ------------------------------------------------------------------------ */
+
+/* Bytes of device workspace et_orthogonalize and et_muon need for `count` tensors
+ * of shapes[3 i] matrices of shapes[3 i + 1] rows and shapes[3 i + 2] columns (HOST
+ * array).  0 for invalid shapes. */
+size_t et_orthogonalize_workspace_bytes(const int64_t* shapes, int64_t count);
+
+/*
+ * Newton-Schulz steps on every matrix U [m, n] of every tensor:
+ *   X = U / (|U| + eps)                              (|U| the Frobenius norm)
+ *   `iterations` times:  A = X X^T,  X = (a + b A + c A A) X
+ * (with m > n: A = X^T X, X = X (a + b A + c A A), the same), X rounded to bf16.
+ * g, out and shapes are HOST arrays: device pointers (element-aligned) to
+ * [E, m, n] of `dtype` and bf16.  coefficients (HOST) a, b, c: a > 0, and the
+ * polynomial keeps singular values from [0, 1] below 1.9.  The sums are binary32,
+ * X, A and the polynomial are held in f16 with 11 bits: the result is 0.1 to 0.2%
+ * off in norm.  Fixed order: repeated calls give identical bits.  A matrix
+ * that is all zero gives zero; one with a value that is not finite gives NaN,
+ * and no other matrix does.  Sides below 65536.  workspace 256-byte aligned.
+ */
+int et_orthogonalize(const void* const* g, void* const* out, const int64_t* shapes, int64_t count, int dtype,
+                     int iterations, const float* coefficients, float eps, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
+/* The scalars of one step (passed by value from the host). */
+typedef struct {
+    float beta, one_minus_beta;
+    float decay;                /* 1 - lr * weight_decay */
+    float eps;
+    float a, b, c;
+    int32_t iterations;
+    int32_t nesterov;           /* 0 or 1 */
+} et_muon_scalars;
+
+/*
+ * One optimizer step, in place, on `count` tensors of matrices:
+ *   g = grad * grad_scale
+ *   m = beta * m + one_minus_beta * g
+ *   U = one_minus_beta * g + beta * m  (nesterov), or m
+ *   w = decay * w - step_sizes[i] * X   X as above, of U, not rounded to bf16
+ * params, grads, momentum (f32), masters and step_sizes are HOST arrays.
+ * param_dtype F32: w is the parameter and masters is NULL.  BF16: w is the f32
+ * master, and the parameter is w rounded.  grad_scale (f32 [1] on the device) may
+ * be NULL (1); where it is not finite every buffer keeps its bits.  Tensors must
+ * not overlap.
+ */
+int et_muon(void* const* params, const void* const* grads, float* const* momentum, float* const* masters,
+            const float* step_sizes, const int64_t* shapes, int64_t count, int param_dtype, int grad_dtype,
+            et_muon_scalars scalars, const float* grad_scale, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

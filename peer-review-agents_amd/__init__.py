@@ -42,6 +42,13 @@ from .gated import (  # noqa: F401
     gated_linear_backward,
     gated_linear_backward_workspace_bytes,
 )
+from .muon import (  # noqa: F401
+    MUON_COEFFICIENTS,
+    Muon,
+    muon_step_,
+    orthogonalize,
+    orthogonalize_workspace_bytes,
+)
 from .norm import (  # noqa: F401
     layer_norm,
     layer_norm_autograd,

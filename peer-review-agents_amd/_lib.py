@@ -77,13 +77,23 @@ _BLOCK_SIGNATURES = {
     "et_adamw8": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _i64, _int, _int, AdamWScalars, _p, _int, _u32, _p]),
 }
 
-# Names of include/etmoe_dense.h.
+class MuonScalars(ctypes.Structure):
+    """et_muon_scalars of include/etmoe_dense.h."""
+
+    _fields_ = [(name, _f) for name in ("beta", "one_minus_beta", "decay", "eps", "a", "b", "c")] + [
+        (name, ctypes.c_int32) for name in ("iterations", "nesterov")]
+
+
+# Names of include/etmoe_dense.h (lists of tensors are host arrays: _p too).
 _DENSE_SIGNATURES = {
     "et_dense_abi_version": (_int, []),
     "et_gated_linear": (_int, [_p, _i64, _p, _i64, _i64, _i64, _int, _p, _p]),
     "et_gated_linear_impl": (_int, [_p, _i64, _p, _i64, _i64, _i64, _int, _p, _int, _p]),
     "et_gated_linear_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "et_gated_linear_bwd": (_int, [_p, _p, _i64, _p, _i64, _i64, _i64, _int, _p, _p, _int, _p, _sz, _p]),
+    "et_orthogonalize_workspace_bytes": (_sz, [_p, _i64]),
+    "et_orthogonalize": (_int, [_p, _p, _p, _i64, _int, _int, _p, _f, _p, _sz, _p]),
+    "et_muon": (_int, [_p, _p, _p, _p, _p, _p, _i64, _int, _int, MuonScalars, _p, _p, _sz, _p]),
 }
 
 _SIGNATURES = {

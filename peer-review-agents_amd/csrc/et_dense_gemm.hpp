@@ -169,7 +169,7 @@ __global__ __launch_bounds__(kDenseThreads, P::kBlocks) void dense_gemm_kernel(t
     };
     const auto row_chunk = [&](const unsigned char* p, int rows, int ld, int k, int c) -> RowChunk {
         RowChunk r;
-        r.res = dense_rsrc(p, (rows - 1) * ld * 2 + k * 2);
+        r.res = dense_rsrc(p, (rows - 1) * ld * 2 + ((k + 7) & ~7) * 2);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
             r.at[i] = c * 64 + (seg0 ^ i) * 8 < k ? (uint32_t)((lane >> 3) * 2 * ld + (seg0 ^ i) * 16) : kOOR;
