@@ -112,6 +112,46 @@ int et_muon(void* const* params, const void* const* grads, float* const* momentu
             const float* step_sizes, const int64_t* shapes, int64_t count, int param_dtype, int grad_dtype,
             et_muon_scalars scalars, const float* grad_scale, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------ *
+ * Low-rank adapters of many requests
+ * ------------------------------------------------------------------------ */
+
+#define ET_MAX_ADAPTERS 4096
+#define ET_MAX_ADAPTER_RANK 128
+
+/* Entries of et_adapter_plan's items (-1 for invalid sizes). */
+int64_t et_adapter_plan_items(int64_t num_tokens, int64_t num_adapters);
+
+/*
+ * The tokens sorted by adapter, once for all projections of a step.  index
+ * [num_tokens]: each token's adapter; a value outside [0, num_adapters) is none.
+ * order [num_tokens]; items [et_adapter_plan_items()][4] (16-byte aligned): an
+ * adapter (-1: none) and a range of the order; num_items [1].  The order of the
+ * tokens of one adapter may change from call to call; it changes no result.
+ */
+int et_adapter_plan(const int32_t* index, int64_t num_tokens, int64_t num_adapters, int32_t* order, int32_t* items,
+                    int32_t* num_items, void* stream);
+
+/* Bytes of device workspace et_adapter_add needs (0 for invalid sizes). */
+size_t et_adapter_add_workspace_bytes(int64_t num_tokens, int64_t num_adapters, int64_t K, int64_t rank);
+
+/*
+ *   out[t, n] = y[t, n] + sum_r b[i, n, r] * (scale[i] * sum_k a[i, r, k] * x[t, k])
+ * with i token t's adapter in the plan (none: out[t] = y[t]).  bf16 x [num_tokens, K],
+ * y and out [num_tokens, N] with row strides in elements (multiples of 8), out may
+ * be y; bf16 a [num_adapters, rank, K] and b [num_adapters, N, rank], f32 scale
+ * [num_adapters].  K, N and rank multiples of 8, rank at most
+ * ET_MAX_ADAPTER_RANK.  order, items and num_items are those of et_adapter_plan for the
+ * same num_tokens and num_adapters.  Binary32 sums in a fixed order, the inner one
+ * kept to 16 bits, one rounding of out: repeated calls give identical bits.  An
+ * inner sum that is not finite gives NaN in its token's row.
+ * Pointers 16-byte aligned (scale, order and num_items 4).
+ */
+int et_adapter_add(const void* y, int64_t y_stride, const void* x, int64_t x_stride, const void* a, const void* b,
+                   const float* scale, const int32_t* order, const int32_t* items, const int32_t* num_items,
+                   int64_t num_tokens, int64_t num_adapters, int64_t K, int64_t N, int64_t rank, void* out,
+                   int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -36,6 +36,13 @@ from .expert_threshold import (  # noqa: F401
     threshold_update_,
     threshold_workspace_bytes,
 )
+from .adapters import (  # noqa: F401
+    AdapterBank,
+    AdapterPlan,
+    adapter_add,
+    adapter_add_workspace_bytes,
+    adapter_plan,
+)
 from .gated import (  # noqa: F401
     gated_linear,
     gated_linear_autograd,

@@ -27,6 +27,7 @@ ET_MAX_ROUTER_EXPERTS = 256
 ET_MAX_NORM_WIDTH = 16384
 ET_GEMM_PLAIN, ET_GEMM_ROW_SCALE, ET_GEMM_SWIGLU = 0, 1, 2
 ET_GATED_SILU, ET_GATED_GELU = 0, 1
+ET_MAX_ADAPTERS, ET_MAX_ADAPTER_RANK = 4096, 128
 
 
 class ETMoEError(RuntimeError):
@@ -94,6 +95,11 @@ _DENSE_SIGNATURES = {
     "et_orthogonalize_workspace_bytes": (_sz, [_p, _i64]),
     "et_orthogonalize": (_int, [_p, _p, _p, _i64, _int, _int, _p, _f, _p, _sz, _p]),
     "et_muon": (_int, [_p, _p, _p, _p, _p, _p, _i64, _int, _int, MuonScalars, _p, _p, _sz, _p]),
+    "et_adapter_plan_items": (_i64, [_i64, _i64]),
+    "et_adapter_plan": (_int, [_p, _i64, _i64, _p, _p, _p, _p]),
+    "et_adapter_add_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
+    "et_adapter_add": (_int, [_p, _i64, _p, _i64, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _i64, _p, _sz,
+                              _p]),
 }
 
 _SIGNATURES = {
