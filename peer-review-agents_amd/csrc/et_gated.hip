@@ -137,6 +137,75 @@ struct GatedPolicy {
     }
 };
 
+// The forward of up to 64 tokens, where reading the weight is the work: no LDS
+// stages, a wave's loads go straight into the operands.  A block owns 8 hidden
+// units, whose gate and up rows fill one MFMA tile of 16 rows, and TT tiles of 16
+// tokens; its 8 waves take K's chunks of 64 in turn (128 contiguous bytes of each
+// row), U at a time, and their sums meet in LDS.  F = 2048 then makes a block for
+// each CU, with the whole of a block's weights (128 KB at K = 4096) in flight at
+// once.  Chunks past K read 0 through the descriptors' range check.
+constexpr int kSkinnyWaves = 8;
+constexpr int kSkinnyTokens = 64;
+
+template <int TT, int U, int ACT>
+__global__ __launch_bounds__(kSkinnyWaves * kWave) void gated_skinny_kernel(GatedArgs g)
+{
+    __shared__ f32x4_t part[kSkinnyWaves][TT][kWave];
+    const int lane = lane_id(), wave = (int)threadIdx.x >> 6;
+    const int r16 = lane & 15, rho = lane >> 4;
+    const int hid0 = (int)blockIdx.x * 8;
+    const int T = (int)g.T, K = g.K, F = g.F;
+    const __amdgpu_buffer_rsrc_t wres = dense_rsrc(g.w, 2 * F * K * 2);
+    const __amdgpu_buffer_rsrc_t xres = dense_rsrc(g.x, ((T - 1) * g.ldx + K) * 2);
+    const uint32_t wrow = (uint32_t)(r16 < 8 ? hid0 + r16 : F + hid0 + r16 - 8) * (uint32_t)K * 2u;
+    uint32_t xrow[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) xrow[t] = (uint32_t)min(16 * t + r16, T - 1) * (uint32_t)g.ldx * 2u;
+    f32x4_t acc[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t) acc[t] = f32x4_t{};
+    for (int c = wave * 64 + 8 * rho; c - 8 * rho < K; c += kSkinnyWaves * 64 * U) {
+        u32x4_t fw[2 * U], fx[2 * U][TT];
+#pragma unroll
+        for (int u = 0; u < 2 * U; ++u) {
+            const int k = c + (u >> 1) * (kSkinnyWaves * 64) + (u & 1) * 32;
+            fw[u] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(wres, k < K ? wrow + 2 * k : kOOR, 0, 0));
+#pragma unroll
+            for (int t = 0; t < TT; ++t)
+                fx[u][t] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(xres, k < K ? xrow[t] + 2 * k : kOOR, 0, 0));
+        }
+#pragma unroll
+        for (int u = 0; u < 2 * U; ++u)
+#pragma unroll
+            for (int t = 0; t < TT; ++t)
+                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, fw[u]),
+                                                                 __builtin_bit_cast(bf16x8_t, fx[u][t]), acc[t], 0, 0, 0);
+    }
+#pragma unroll
+    for (int t = 0; t < TT; ++t) part[wave][t][lane] = acc[t];
+    __syncthreads();
+    // (row r of the tile, token c: lane 16 (r / 4) + c, element r % 4)
+    for (int q = (int)threadIdx.x; q < TT * 128; q += kSkinnyWaves * kWave) {
+        const int token = q >> 3, h = q & 7;
+        float gate = 0.0f, up = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kSkinnyWaves; ++w) {
+            gate += part[w][token >> 4][16 * (h >> 2) + (token & 15)][h & 3];
+            up += part[w][token >> 4][16 * (2 + (h >> 2)) + (token & 15)][h & 3];
+        }
+        if (token < T) g.out[(int64_t)token * F + hid0 + h] = (uint16_t)f32_to_bf16_bits(gate_value<ACT>(gate) * up);
+    }
+}
+
+template <int ACT>
+void launch_skinny(const GatedArgs& g, hipStream_t s)
+{
+    const dim3 grid((unsigned)(g.F / 8)), block(kSkinnyWaves * kWave);
+    if (g.T <= 16) gated_skinny_kernel<1, 4, ACT><<<grid, block, 0, s>>>(g);
+    else if (g.T <= 32) gated_skinny_kernel<2, 2, ACT><<<grid, block, 0, s>>>(g);
+    else gated_skinny_kernel<4, 2, ACT><<<grid, block, 0, s>>>(g);
+}
+
 // dx [T, K] = dp [T, 2F] W, W read down its columns.
 struct InputGradArgs {
     const unsigned char* dp;
@@ -324,6 +393,11 @@ int check_pointer(const char* fn, const char* name, const void* p)
 
 int launch_gated(GatedArgs g, int act, bool backward, int side, hipStream_t s)
 {
+    if (side == 0 && !backward && g.T <= kSkinnyTokens) {
+        if (act == ET_GATED_SILU) launch_skinny<ET_GATED_SILU>(g, s);
+        else launch_skinny<ET_GATED_GELU>(g, s);
+        return check_launch("gated_skinny_kernel");
+    }
     if (side == 0) side = dense_side(g.T, 2 * g.F);
     g.nm = (int)up(g.T, 32 * side);
     g.nn = (int)up(g.F, 16 * side);
