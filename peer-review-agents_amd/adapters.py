@@ -96,7 +96,7 @@ def adapter_add_workspace_bytes(num_tokens: int, bank: AdapterBank) -> int:
 
 
 def _rows(t: torch.Tensor, name: str, shape, dev) -> int:
-    if (isinstance(t, torch.Tensor) and t.dtype == torch.bfloat16 and t.is_cuda and t.shape == shape and t.device == dev
+    if (isinstance(t, torch.Tensor) and t.dtype == torch.bfloat16 and t.shape == shape and t.device == dev
             and t.is_contiguous()):
         stride = shape[1]
     else:
@@ -118,23 +118,24 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, bank: AdapterBank, plan: Adapt
     """
     if not isinstance(bank, AdapterBank) or not isinstance(plan, AdapterPlan):
         raise TypeError("bank must be an AdapterBank and plan an AdapterPlan")
-    n, rank, K = bank.a.shape
-    N, T, dev = bank.b.shape[1], plan.num_tokens, bank.a.device
+    a, b, order = bank.a, bank.b, plan.order
+    n, rank, K = a.shape
+    N, T, dev = b.shape[1], plan.num_tokens, a.device
     if plan.num_adapters != n:
         raise ValueError(f"the plan is of {plan.num_adapters} adapters, the bank has {n}")
-    if plan.order.device != dev:
-        raise ValueError(f"the plan is on {plan.order.device}, the bank on {dev}")
+    if order.device != dev:
+        raise ValueError(f"the plan is on {order.device}, the bank on {dev}")
     ldy, ldx = _rows(y, "y", (T, N), dev), _rows(x, "x", (T, K), dev)
     if out is None:
         out, ldo = y.new_empty((T, N)), N
     else:
         ldo = _rows(out, "out", (T, N), dev)
-    wsb = int(lib().et_adapter_add_workspace_bytes(T, n, K, rank))
+    wsb = lib().et_adapter_add_workspace_bytes(T, n, K, rank)
     if workspace is None:
-        workspace = torch.empty(wsb, dtype=torch.uint8, device=dev)
+        workspace = y.new_empty(wsb >> 1)       # (bf16 elements)
     else:
         _require_workspace(workspace, wsb, dev, "workspace")
-    _call("et_adapter_add", dev, y.data_ptr(), ldy, x.data_ptr(), ldx, bank.a.data_ptr(), bank.b.data_ptr(),
-          bank.scale.data_ptr(), plan.order.data_ptr(), plan.items.data_ptr(), plan.num_items.data_ptr(), T, n, K, N, rank,
-          out.data_ptr(), ldo, workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    _call("et_adapter_add", dev, y.data_ptr(), ldy, x.data_ptr(), ldx, a.data_ptr(), b.data_ptr(), bank.scale.data_ptr(),
+          order.data_ptr(), plan.items.data_ptr(), plan.num_items.data_ptr(), T, n, K, N, rank, out.data_ptr(), ldo,
+          workspace.data_ptr(), wsb)
     return out

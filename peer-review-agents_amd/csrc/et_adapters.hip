@@ -26,6 +26,7 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
+constexpr int kShrinkWaves = 8;
 
 struct Item {
     int adapter, first, rows, unused;
@@ -36,7 +37,8 @@ struct Item {
 // --------------------------------------------------------------------------
 
 // One block.  order: the tokens by adapter (those without one last); items and
-// their number.  Within an adapter the order is that in which the waves come.
+// their number.  Within an adapter the order is that in which the lanes' atomics
+// come.
 __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(const int32_t* index, int64_t T, int n, int tile,
                                                                     int32_t* order, Item* items, int32_t* num_items)
 {
@@ -51,21 +53,15 @@ __global__ __launch_bounds__(kPlanThreads) void adapter_plan_kernel(const int32_
         return (uint32_t)i < (uint32_t)n ? i : n;
     };
     for (int pass = 0; pass < 2; ++pass) {
-        for (int64_t t0 = 0; t0 < T; t0 += kPlanThreads) {
-            const int64_t t = t0 + tid;
-            const int a = t < T ? adapter_of(t) : -1;
-            uint64_t left = __ballot(a >= 0);
-            while (left) {
-                // the lanes with the first one's adapter
-                const int leader = (int)__builtin_ctzll(left);
-                const int which = __shfl(a, leader, kWave);
-                const uint64_t same = __ballot(a == which);
-                int base = 0;
-                if (lane == leader) base = atomicAdd(&at[which], (int)__popcll(same));
-                base = __shfl(base, leader, kWave);
-                if (pass == 1 && a == which) order[base + rank_below(same)] = (int32_t)t;
-                left &= ~same;
-            }
+        for (int64_t t = tid; t < T; t += kPlanThreads) {
+            // (tokens of one request follow each other: the lanes with the first one's
+            // adapter take their places at once)
+            const int a = adapter_of(t), first = __builtin_amdgcn_readfirstlane(a);
+            const uint64_t same = __ballot(a == first);
+            int place = 0;
+            if (a != first || rank_below(same) == 0) place = atomicAdd(&at[a], a == first ? (int)__popcll(same) : 1);
+            if (a == first) place = __builtin_amdgcn_readfirstlane(place) + rank_below(same);
+            if (pass == 1) order[place] = (int32_t)t;
         }
         __syncthreads();
         if (pass == 1) break;
@@ -119,20 +115,24 @@ struct AdapterArgs {
     unsigned char* out;
     int64_t ldx, ldy, ldo, T;
     int K, N, r, splits, step;   // step: the k of a split
+    int col_blocks, chunks;      // of an item, and of a wave, in the expand kernel
 };
 
-// RT: tiles of 16 rows of A; TT: tiles of 16 tokens.
-template <int RT, int TT>
-__global__ __launch_bounds__(kThreads) void adapter_shrink_kernel(AdapterArgs g)
+// RT: tiles of 16 rows of A; TT: tiles of 16 tokens; U: chunks of a wave in flight; 64
+// tokens of rank 128 leave room in LDS for the sums of 4 WAVES.
+// (items has room for every block: it is read beside their number)
+template <int RT, int TT, int U, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave) void adapter_shrink_kernel(AdapterArgs g)
 {
-    __shared__ f32x4_t part[kWaves][TT * RT][kWave];
-    if ((int)blockIdx.x >= *g.num_items) return;
+    __shared__ f32x4_t part[WAVES][TT * RT][kWave];
     const Item it = g.items[blockIdx.x];
-    if (it.adapter < 0) return;
+    if ((int)blockIdx.x >= *g.num_items || it.adapter < 0) return;
     const int lane = lane_id(), wave = (int)threadIdx.x >> 6;
     const int r16 = lane & 15, rho = lane >> 4;
     const int split = (int)blockIdx.y;
     const int k0 = split * g.step, k1 = min(g.K, k0 + g.step);
+    const __amdgpu_buffer_rsrc_t ares = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<unsigned char*>(g.a + (int64_t)it.adapter * g.r * g.K * 2), (short)0, g.r * g.K * 2, kBufDword3);
     const unsigned char* xr[TT];
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
@@ -140,49 +140,47 @@ __global__ __launch_bounds__(kThreads) void adapter_shrink_kernel(AdapterArgs g)
         const int64_t token = g.order[it.first + min(16 * t + r16, it.rows - 1)];
         xr[t] = g.x + token * g.ldx * 2;
     }
-    const unsigned char* ar[RT];
-#pragma unroll
-    for (int i = 0; i < RT; ++i) ar[i] = g.a + ((int64_t)it.adapter * g.r + min(16 * i + r16, g.r - 1)) * g.K * 2;
     f32x4_t acc[RT][TT];
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int t = 0; t < TT; ++t) acc[i][t] = f32x4_t{};
-    // chunks of 64 k, dealt to the waves in turn: a row's 128 bytes in two loads of
-    // one wave
-    const auto one = [&](int c) {
-        u32x4_t fa[2][RT], fx[2][TT];
+    // Chunks of 64 k, dealt to the waves in turn: a row's 128 bytes in two loads of
+    // one wave.  Past the end A is 0 (and x any of the row's own values: one that is
+    // not finite makes the token's sum so anyway).
+    const int chunks = (k1 - k0 + 63) / 64;
+    for (int c = wave; c < chunks; c += WAVES * U) {
+        u32x4_t fa[2 * U][RT], fx[2 * U][TT];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int k = k0 + 64 * c + 32 * h + 8 * rho;
-            const bool in = k < k1;
+        for (int u = 0; u < 2 * U; ++u) {
+            const int k = k0 + 64 * (c + (u >> 1) * WAVES) + 32 * (u & 1) + 8 * rho;
 #pragma unroll
-            for (int i = 0; i < RT; ++i) fa[h][i] = in ? *reinterpret_cast<const u32x4_t*>(ar[i] + 2 * (int64_t)k) : u32x4_t{};
+            for (int i = 0; i < RT; ++i)
+                fa[u][i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                    ares, k < k1 ? (uint32_t)(min(16 * i + r16, g.r - 1) * g.K + k) * 2u : kOOR, 0, 0));
 #pragma unroll
-            for (int t = 0; t < TT; ++t) fx[h][t] = in ? *reinterpret_cast<const u32x4_t*>(xr[t] + 2 * (int64_t)k) : u32x4_t{};
+            for (int t = 0; t < TT; ++t) fx[u][t] = *reinterpret_cast<const u32x4_t*>(xr[t] + 2 * (int64_t)min(k, g.K - 8));
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int u = 0; u < 2 * U; ++u)
 #pragma unroll
             for (int i = 0; i < RT; ++i)
 #pragma unroll
                 for (int t = 0; t < TT; ++t)
-                    acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, fa[h][i]),
-                                                                        __builtin_bit_cast(bf16x8_t, fx[h][t]), acc[i][t], 0, 0, 0);
-    };
-    const int chunks = (k1 - k0 + 63) / 64;
-    for (int c = wave; c < chunks; c += kWaves) one(c);
+                    acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, fa[u][i]),
+                                                                        __builtin_bit_cast(bf16x8_t, fx[u][t]), acc[i][t], 0, 0, 0);
+    }
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int t = 0; t < TT; ++t) part[wave][i * TT + t][lane] = acc[i][t];
     __syncthreads();
     const float scale = g.scale[it.adapter];
-    for (int q = (int)threadIdx.x; q < RT * TT * kWave; q += kThreads) {
+    for (int q = (int)threadIdx.x; q < RT * TT * kWave; q += WAVES * kWave) {
         const int tile = q >> 6, l = q & 63;
         f32x4_t sum = part[0][tile][l];
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) sum += part[w][tile][l];
+        for (int w = 1; w < WAVES; ++w) sum += part[w][tile][l];
         const int row = 16 * (tile / TT) + 4 * (l >> 4), token = 16 * (tile % TT) + (l & 15);
         if (row < g.r && token < it.rows)
             *reinterpret_cast<f32x4_t*>(g.v + ((int64_t)split * g.T + it.first + token) * g.r + row) = sum * scale;
@@ -194,97 +192,122 @@ __global__ __launch_bounds__(kThreads) void adapter_shrink_kernel(AdapterArgs g)
 // --------------------------------------------------------------------------
 
 // KS: k-steps of 32 over v's two parts (2 r / 32, rounded up).  A wave's 64 columns
-// are dealt to four MFMA tiles so that a lane holds 16 consecutive ones of a token:
-// row i of tile j is column 16 (i / 4) + 4 j + i % 4.
-template <int KS, int TT>
+// are dealt to four MFMA tiles so that a lane holds 8 consecutive ones of a token
+// twice and four lanes 64 contiguous bytes: row i of tile j is column
+// 32 (j / 2) + 8 (i / 4) + 4 (j % 2) + i % 4.
+// A wave goes through g.chunks chunks of columns with its tokens' v in registers (v
+// is as many bytes as a chunk of y at rank 32), the next chunk's y on its way.
+// Blocks take an item's columns in turn, so that those that run together cover
+// whole rows of y.
+template <int KS, int TT, bool EVEN>
 __global__ __launch_bounds__(kThreads) void adapter_expand_kernel(AdapterArgs g)
 {
-    if ((int)blockIdx.x >= *g.num_items) return;
-    const Item it = g.items[blockIdx.x];
+    const int item = (int)(blockIdx.x / (uint32_t)g.col_blocks);
+    const Item it = g.items[item];
+    if (item >= *g.num_items) return;
     const int lane = lane_id(), wave = (int)threadIdx.x >> 6;
     const int r16 = lane & 15, rho = lane >> 4;
-    const int n0 = ((int)blockIdx.y * kWaves + wave) * 64;
-    if (n0 >= g.N) return;
-    const int col = n0 + 16 * rho;
-    u32x4_t y[TT][2];
-    int64_t token[TT];
+    int n0 = (int)(blockIdx.x - (uint32_t)item * g.col_blocks) * g.chunks * (64 * kWaves) + wave * 64;
+    if (n0 >= g.N || (it.adapter < 0 && g.out == g.y)) return;
+    const int segs = g.r / 8;
     bool ok[TT];
+    const unsigned char* yr[TT];
+    unsigned char* outr[TT];
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
+        // (a token past the item's repeats its last one, unwritten)
         ok[t] = 16 * t + r16 < it.rows;
-        token[t] = g.order[it.first + min(16 * t + r16, it.rows - 1)];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            y[t][h] = ok[t] && col + 8 * h < g.N
-                          ? *reinterpret_cast<const u32x4_t*>(g.y + (token[t] * g.ldy + col + 8 * h) * 2) : u32x4_t{};
+        const int64_t token = g.order[it.first + min(16 * t + r16, it.rows - 1)];
+        yr[t] = g.y + token * g.ldy * 2;
+        outr[t] = g.out + token * g.ldo * 2;
     }
-    if (it.adapter >= 0) {
-        const int segs = g.r / 8;
+    u32x4_t fv[KS][TT];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        const int s = 4 * ks + rho;
+        const int at = s >= 2 * segs ? 0 : (s >= segs ? s - segs : s) * 8;
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+            f32x4_t v[2] = {};
+            if (it.adapter >= 0) {
+                const float* p = g.v + (it.first + min(16 * t + r16, it.rows - 1)) * (int64_t)g.r + at;
+                v[0] = *reinterpret_cast<const f32x4_t*>(p);
+                v[1] = *reinterpret_cast<const f32x4_t*>(p + 4);
+                for (int sp = 1; sp < g.splits; ++sp) {
+                    p += g.T * g.r;
+                    v[0] += *reinterpret_cast<const f32x4_t*>(p);
+                    v[1] += *reinterpret_cast<const f32x4_t*>(p + 4);
+                }
+            }
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float a = v[w >> 1][2 * (w & 1)], b = v[w >> 1][2 * (w & 1) + 1];
+                const uint32_t hi = pack_bf16x2(a, b);
+                fv[ks][t][w] = s >= 2 * segs ? 0u : s >= segs ? pack_bf16x2(a - bf16lo(hi), b - bf16hi(hi)) : hi;
+            }
+        }
+    }
+    const int64_t first_row = max(it.adapter, 0) * (int64_t)g.N;
+    u32x4_t y[TT][2];
+    const auto load_y = [&](u32x4_t (&to)[TT][2], int n) {
+#pragma unroll
+        for (int t = 0; t < TT; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                to[t][h] = *reinterpret_cast<const u32x4_t*>(yr[t] + 2 * min(n + 8 * rho + 32 * h, g.N - 8));
+    };
+    load_y(y, n0);
+    for (int c = 0; c < g.chunks; ++c, n0 += 64 * kWaves) {
+        if (n0 >= g.N) break;
+        const __amdgpu_buffer_rsrc_t bres = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<unsigned char*>(g.b + (first_row + n0) * g.r * 2), (short)0,
+            it.adapter >= 0 ? min(64, g.N - n0) * g.r * 2 : 0, kBufDword3);
         f32x4_t acc[TT][4];
 #pragma unroll
         for (int t = 0; t < TT; ++t)
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[t][j] = f32x4_t{};
+        u32x4_t next[TT][2];
+        load_y(next, n0 + 64 * kWaves);
+        // (EVEN: rank a multiple of 32, the second half of the k-steps has the first
+        // half's columns of b)
+        constexpr int STEPS = EVEN ? KS / 2 : KS;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
+        for (int ks = 0; ks < STEPS; ++ks) {
             const int s = 4 * ks + rho;
-            const bool in = s < 2 * segs, low = s >= segs;
-            const int at = (low ? s - segs : s) * 8;
+            const int at = (!EVEN && s >= segs ? s - segs : s) * 8;
             u32x4_t fb[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int n = n0 + 16 * (r16 >> 2) + 4 * j + (r16 & 3);
-                fb[j] = in && n < g.N ? *reinterpret_cast<const u32x4_t*>(g.b + (((int64_t)it.adapter * g.N + n) * g.r + at) * 2)
-                                      : u32x4_t{};
-            }
+            for (int j = 0; j < 4; ++j)
+                fb[j] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                    bres, s < 2 * segs ? (uint32_t)((32 * (j >> 1) + 8 * (r16 >> 2) + 4 * (j & 1) + (r16 & 3)) * g.r + at) * 2u
+                                       : kOOR, 0, 0));
 #pragma unroll
-            for (int t = 0; t < TT; ++t) {
-                float v[8];
+            for (int half = 0; half < (EVEN ? 2 : 1); ++half)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-                if (in && ok[t]) {
-                    const float* p = g.v + (it.first + 16 * t + r16) * (int64_t)g.r + at;
-                    for (int sp = 0; sp < g.splits; ++sp, p += g.T * g.r) {
-                        const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(p), hi = *reinterpret_cast<const f32x4_t*>(p + 4);
+                for (int t = 0; t < TT; ++t)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            v[e] += lo[e];
-                            v[4 + e] += hi[e];
-                        }
-                    }
+                    for (int j = 0; j < 4; ++j)
+                        acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            __builtin_bit_cast(bf16x8_t, fb[j]), __builtin_bit_cast(bf16x8_t, fv[ks + half * STEPS][t]), acc[t][j], 0, 0, 0);
+        }
+        const int col = n0 + 8 * rho;
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                u32x4_t q = y[t][h];
+                if (it.adapter >= 0) {
+#pragma unroll
+                    for (int w = 0; w < 4; ++w)
+                        q[w] = pack_bf16x2(bf16lo(q[w]) + acc[t][2 * h + (w >> 1)][2 * (w & 1)],
+                                           bf16hi(q[w]) + acc[t][2 * h + (w >> 1)][2 * (w & 1) + 1]);
                 }
-                u32x4_t fv;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const uint32_t hi = pack_bf16x2(v[2 * w], v[2 * w + 1]);
-                    fv[w] = low ? pack_bf16x2(v[2 * w] - bf16lo(hi), v[2 * w + 1] - bf16hi(hi)) : hi;
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, fb[j]),
-                                                                        __builtin_bit_cast(bf16x8_t, fv), acc[t][j], 0, 0, 0);
+                if (ok[t] && col + 32 * h < g.N) *reinterpret_cast<u32x4_t*>(outr[t] + 2 * (col + 32 * h)) = q;
+                y[t][h] = next[t][h];
             }
         }
-#pragma unroll
-        for (int t = 0; t < TT; ++t)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                u32x4_t& q = y[t][j >> 1];
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    const uint32_t w = q[2 * (j & 1) + p];
-                    q[2 * (j & 1) + p] = pack_bf16x2(bf16lo(w) + acc[t][j][2 * p], bf16hi(w) + acc[t][j][2 * p + 1]);
-                }
-            }
-    } else if (g.out == g.y) {
-        return;
     }
-#pragma unroll
-    for (int t = 0; t < TT; ++t)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            if (ok[t] && col + 8 * h < g.N)
-                *reinterpret_cast<u32x4_t*>(g.out + (token[t] * g.ldo + col + 8 * h) * 2) = y[t][h];
 }
 
 // --------------------------------------------------------------------------
@@ -295,30 +318,37 @@ int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 int refuse(const char* fn, const char* what) { return fail(ET_ERR_INVALID_ARGUMENT, std::string(fn) + ": " + what); }
 
-// Tokens of an item: 16 up to 2048 tokens, 32 above, where an adapter's matrices
-// are read from the caches once for twice as many tokens.
-int tile_of(int64_t T) { return T <= 2048 ? 16 : 32; }
+// Tokens of an item: 16 up to 2048 tokens, 64 above, where an adapter's matrices
+// are read from the caches once for four times as many tokens.
+int tile_of(int64_t T) { return T <= 2048 ? 16 : 64; }
 
 int64_t most_items(int64_t T, int64_t n) { return up(T, tile_of(T)) + std::min(T, n + 1); }
 
-// Splits of the sum over K: blocks for all CUs, 256 k a split at least.
+// Splits of the sum over K: blocks for all CUs, a chunk for each wave at least.
 int splits_of(int64_t items, int64_t K)
 {
-    return (int)std::max<int64_t>(1, std::min<int64_t>({8, 512 / std::max<int64_t>(1, items), K / 256}));
+    return (int)std::max<int64_t>(1, std::min<int64_t>({4, 256 / std::max<int64_t>(1, items), K / (64 * kShrinkWaves)}));
 }
 
 template <int RT>
 void launch_shrink(const AdapterArgs& g, int tile, dim3 grid, hipStream_t s)
 {
-    if (tile == 16) adapter_shrink_kernel<RT, 1><<<grid, dim3(kThreads), 0, s>>>(g);
-    else adapter_shrink_kernel<RT, 2><<<grid, dim3(kThreads), 0, s>>>(g);
+    constexpr int U = RT <= 2 ? 2 : 1, W = RT == 8 ? kShrinkWaves / 2 : kShrinkWaves;
+    if (tile == 16) adapter_shrink_kernel<RT, 1, U, kShrinkWaves><<<grid, dim3(kShrinkWaves * kWave), 0, s>>>(g);
+    else adapter_shrink_kernel<RT, 4, 1, W><<<grid, dim3(W * kWave), 0, s>>>(g);
 }
 
 template <int KS>
 void launch_expand(const AdapterArgs& g, int tile, dim3 grid, hipStream_t s)
 {
-    if (tile == 16) adapter_expand_kernel<KS, 1><<<grid, dim3(kThreads), 0, s>>>(g);
-    else adapter_expand_kernel<KS, 2><<<grid, dim3(kThreads), 0, s>>>(g);
+    const dim3 block(kThreads);
+    if (KS > 1 && g.r == 16 * KS) {
+        if (tile == 16) adapter_expand_kernel<KS, 1, true><<<grid, block, 0, s>>>(g);
+        else adapter_expand_kernel<KS, 4, true><<<grid, block, 0, s>>>(g);
+    } else {
+        if (tile == 16) adapter_expand_kernel<KS, 1, false><<<grid, block, 0, s>>>(g);
+        else adapter_expand_kernel<KS, 4, false><<<grid, block, 0, s>>>(g);
+    }
 }
 
 }  // namespace
@@ -400,9 +430,15 @@ extern "C" int et_adapter_add(const void* y, int64_t y_stride, const void* x, in
     g.splits = splits_of(most, K);
     g.step = (int)(up(up(K, g.splits), 64) * 64);
     g.splits = (int)up(K, g.step);
+    // (several chunks a wave where there are many blocks all the same)
+    g.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(4, most * up(N, 64 * kWaves) / 2048));
+    g.col_blocks = (int)up(N, 64 * kWaves * g.chunks);
+    // (a launch has less than 2^32 threads)
+    if (most * g.col_blocks >= (int64_t)1 << 24 || most * kShrinkWaves * kWave >= (int64_t)1 << 32)
+        return refuse(fn, "num_tokens * N is too large");
     const int tile = tile_of(num_tokens);
     hipStream_t s = (hipStream_t)stream;
-    const dim3 shrink((unsigned)most, (unsigned)g.splits), expand((unsigned)most, (unsigned)up(N, 64 * kWaves));
+    const dim3 shrink((unsigned)most, (unsigned)g.splits), expand((unsigned)(most * g.col_blocks));
     if (rank <= 16) launch_shrink<1>(g, tile, shrink, s);
     else if (rank <= 32) launch_shrink<2>(g, tile, shrink, s);
     else if (rank <= 64) launch_shrink<4>(g, tile, shrink, s);

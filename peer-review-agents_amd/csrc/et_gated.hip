@@ -20,6 +20,8 @@
 namespace et {
 namespace {
 
+int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
 constexpr float kRootHalf = 0.70710678118654752f, kInvRoot2Pi = 0.39894228040143268f;
 
 // act(g) and, for the backward, act'(g).
@@ -137,52 +139,84 @@ struct GatedPolicy {
     }
 };
 
-// The forward of up to 64 tokens, where reading the weight is the work: no LDS
-// stages, a wave's loads go straight into the operands.  A block owns 8 hidden
-// units, whose gate and up rows fill one MFMA tile of 16 rows, and TT tiles of 16
-// tokens; its 8 waves take K's chunks of 64 in turn (128 contiguous bytes of each
-// row), U at a time, and their sums meet in LDS.  F = 2048 then makes a block for
-// each CU, with the whole of a block's weights (128 KB at K = 4096) in flight at
-// once.  Chunks past K read 0 through the descriptors' range check.
+// The forward of few tokens, where reading the weight is the work.  A block
+// owns 8 hidden units, whose gate and up rows fill one MFMA tile of 16 rows, and
+// TT tiles of 16 tokens; its 8 waves take K's chunks of 64 in turn, each through a
+// ring of D stages of LDS of its own (no barriers), and their sums meet in LDS.
+// F = 2048 then makes a block for each CU.  A direct load fills 8 rows x 128
+// bytes: whole cache lines.  (Loads straight into the operands' registers take 16
+// rows x 64 bytes, which move 14 bytes a cycle and CU: 64 tokens took 23 us at
+// K = 4096, F = 2048.)  What lies past K and the tokens reads 0, without traffic.
 constexpr int kSkinnyWaves = 8;
-constexpr int kSkinnyTokens = 64;
 
-template <int TT, int U, int ACT>
+template <int TT, int D, int ACT>
 __global__ __launch_bounds__(kSkinnyWaves * kWave) void gated_skinny_kernel(GatedArgs g)
 {
-    __shared__ f32x4_t part[kSkinnyWaves][TT][kWave];
-    const int lane = lane_id(), wave = (int)threadIdx.x >> 6;
+    constexpr int kStageBytes = (1 + TT) * 2048, NI = 2 * (1 + TT);
+    constexpr int kRing = kSkinnyWaves * D * kStageBytes, kPart = kSkinnyWaves * TT * kWave * 16;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[kRing > kPart ? kRing : kPart];
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int r16 = lane & 15, rho = lane >> 4;
     const int hid0 = (int)blockIdx.x * 8;
-    const int T = (int)g.T, K = g.K, F = g.F;
+    const int m0 = (int)blockIdx.y * (16 * TT);
+    const int T = min(16 * TT, (int)g.T - m0), K = g.K, F = g.F;
     const __amdgpu_buffer_rsrc_t wres = dense_rsrc(g.w, 2 * F * K * 2);
-    const __amdgpu_buffer_rsrc_t xres = dense_rsrc(g.x, ((T - 1) * g.ldx + K) * 2);
-    const uint32_t wrow = (uint32_t)(r16 < 8 ? hid0 + r16 : F + hid0 + r16 - 8) * (uint32_t)K * 2u;
-    uint32_t xrow[TT];
+    const __amdgpu_buffer_rsrc_t xres = dense_rsrc(g.x + (int64_t)m0 * g.ldx * 2, ((T - 1) * g.ldx + K) * 2);
+    unsigned char* const mine = smem + wave * (D * kStageBytes);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_t*)mine;
+    const int seg0 = (lane & 7) ^ (lane >> 3);
+    // chunk j of the wave: k from (8 j + wave) 64 on
+    const auto load = [&](int j, uint32_t lds) {
+        const int k0 = (kSkinnyWaves * j + wave) * 64;
 #pragma unroll
-    for (int t = 0; t < TT; ++t) xrow[t] = (uint32_t)min(16 * t + r16, T - 1) * (uint32_t)g.ldx * 2u;
+        for (int i = 0; i < 2; ++i) {
+            const int k = k0 + (seg0 ^ i) * 8;
+            const uint32_t row = (uint32_t)((i ? F : 0) + hid0 + (lane >> 3));
+            dense_dma(wres, k < K ? (row * (uint32_t)K + (uint32_t)k) * 2u : kOOR, 0u, lds + i * 1024);
+        }
+#pragma unroll
+        for (int t = 0; t < TT; ++t)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int k = k0 + (seg0 ^ i) * 8;
+                const uint32_t row = (uint32_t)(16 * t + 8 * i + (lane >> 3));
+                dense_dma(xres, k < K && (int)row < T ? (row * (uint32_t)g.ldx + (uint32_t)k) * 2u : kOOR, 0u,
+                          lds + (1 + t) * 2048 + i * 1024);
+            }
+    };
     f32x4_t acc[TT];
 #pragma unroll
     for (int t = 0; t < TT; ++t) acc[t] = f32x4_t{};
-    for (int c = wave * 64 + 8 * rho; c - 8 * rho < K; c += kSkinnyWaves * 64 * U) {
-        u32x4_t fw[2 * U], fx[2 * U][TT];
+    const int turns = (K + kSkinnyWaves * 64 - 1) / (kSkinnyWaves * 64);
 #pragma unroll
-        for (int u = 0; u < 2 * U; ++u) {
-            const int k = c + (u >> 1) * (kSkinnyWaves * 64) + (u & 1) * 32;
-            fw[u] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(wres, k < K ? wrow + 2 * k : kOOR, 0, 0));
+    for (int d = 0; d < D; ++d) load(d, lds0 + d * kStageBytes);
+    const int fkey = (lane & 7) ^ ((lane >> 3) & 1);
+    const int frow = (r16 >> 3) * 1024 + (lane & 7) * 128;
+    for (int j = 0, stage = 0; j < turns; ++j) {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * NI) : "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        const unsigned char* const at = mine + stage * kStageBytes;
 #pragma unroll
-            for (int t = 0; t < TT; ++t)
-                fx[u][t] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(xres, k < K ? xrow[t] + 2 * k : kOOR, 0, 0));
+        for (int ks = 0; ks < 2; ++ks) {
+            const auto read = [&](int tile) {
+                return __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const u32x4_t*>(at + tile * 2048 + frow + (((4 * ks + rho) ^ fkey) << 4)));
+            };
+            const bf16x8_t fw = read(0);
+#pragma unroll
+            for (int t = 0; t < TT; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw, read(1 + t), acc[t], 0, 0, 0);
         }
-#pragma unroll
-        for (int u = 0; u < 2 * U; ++u)
-#pragma unroll
-            for (int t = 0; t < TT; ++t)
-                acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, fw[u]),
-                                                                 __builtin_bit_cast(bf16x8_t, fx[u][t]), acc[t], 0, 0, 0);
+        // (the reads above have ended: their results were used.  Chunks past K load
+        // nothing, so that the count of loads in flight is the same)
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(0xC07F);      // lgkmcnt(0)
+        load(j + D, lds0 + stage * kStageBytes);
+        stage = stage + 1 == D ? 0 : stage + 1;
     }
+    dense_wait_barrier<0>();
+    f32x4_t* const part = reinterpret_cast<f32x4_t*>(smem);
 #pragma unroll
-    for (int t = 0; t < TT; ++t) part[wave][t][lane] = acc[t];
+    for (int t = 0; t < TT; ++t) part[(wave * TT + t) * kWave + lane] = acc[t];
     __syncthreads();
     // (row r of the tile, token c: lane 16 (r / 4) + c, element r % 4)
     for (int q = (int)threadIdx.x; q < TT * 128; q += kSkinnyWaves * kWave) {
@@ -190,19 +224,31 @@ __global__ __launch_bounds__(kSkinnyWaves * kWave) void gated_skinny_kernel(Gate
         float gate = 0.0f, up = 0.0f;
 #pragma unroll
         for (int w = 0; w < kSkinnyWaves; ++w) {
-            gate += part[w][token >> 4][16 * (h >> 2) + (token & 15)][h & 3];
-            up += part[w][token >> 4][16 * (2 + (h >> 2)) + (token & 15)][h & 3];
+            const f32x4_t* const p = part + (w * TT + (token >> 4)) * kWave + 16 * (h >> 2) + (token & 15);
+            gate += p[0][h & 3];
+            up += p[32][h & 3];
         }
-        if (token < T) g.out[(int64_t)token * F + hid0 + h] = (uint16_t)f32_to_bf16_bits(gate_value<ACT>(gate) * up);
+        if (token < T) g.out[(int64_t)(m0 + token) * F + hid0 + h] = (uint16_t)f32_to_bf16_bits(gate_value<ACT>(gate) * up);
     }
+}
+
+// us at K = 4096, a call another weight each time: F = 2048, where the weights are
+// 6.8 us at 4.9 TB/s, one token 9.0, 16 tokens 9.7, 32 11.3, 64 14.8, a round of 128 x 128
+// tiles 42 to 45 up to 256 tokens; F = 8192 31 up to 16 tokens, tiles 47 to 51 up to 128.
+// So a round of these blocks (one a CU) is taken for a third of one of tiles.
+bool is_skinny(int64_t T, int64_t F)
+{
+    const int cus = dense_cus();
+    const int64_t rounds = up(F / 8 * up(T, 64), cus), tiled = up(up(T, 128) * up(F, 64), 2 * cus);
+    return T <= 16 || (T <= 256 && rounds <= 3 * tiled);
 }
 
 template <int ACT>
 void launch_skinny(const GatedArgs& g, hipStream_t s)
 {
-    const dim3 grid((unsigned)(g.F / 8)), block(kSkinnyWaves * kWave);
+    const dim3 grid((unsigned)(g.F / 8), (unsigned)up(g.T, 64)), block(kSkinnyWaves * kWave);
     if (g.T <= 16) gated_skinny_kernel<1, 4, ACT><<<grid, block, 0, s>>>(g);
-    else if (g.T <= 32) gated_skinny_kernel<2, 2, ACT><<<grid, block, 0, s>>>(g);
+    else if (g.T <= 32) gated_skinny_kernel<2, 3, ACT><<<grid, block, 0, s>>>(g);
     else gated_skinny_kernel<4, 2, ACT><<<grid, block, 0, s>>>(g);
 }
 
@@ -347,8 +393,6 @@ __global__ __launch_bounds__(kDenseThreads) void gated_zero_kernel(uint32_t* p, 
         p[at] = 0u;
 }
 
-int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 template <template <int> class POLICY, class ARGS>
 int launch_sided(ARGS g, int side, int64_t tiles, hipStream_t s, const char* what)
 {
@@ -393,7 +437,7 @@ int check_pointer(const char* fn, const char* name, const void* p)
 
 int launch_gated(GatedArgs g, int act, bool backward, int side, hipStream_t s)
 {
-    if (side == 0 && !backward && g.T <= kSkinnyTokens) {
+    if (side == 0 && !backward && is_skinny(g.T, g.F)) {
         if (act == ET_GATED_SILU) launch_skinny<ET_GATED_SILU>(g, s);
         else launch_skinny<ET_GATED_GELU>(g, s);
         return check_launch("gated_skinny_kernel");

@@ -68,7 +68,7 @@ def test_adapter_add(et, dev, T, K, N, rank, n):
     assert sum(rows for _, _, rows, _ in items) == T and sorted(first for _, first, _, _ in items)[0] == 0
     sorted_index = index[order].tolist()
     for adapter, first, rows, _ in items:
-        assert 1 <= rows <= 32 and set(sorted_index[first:first + rows]) == {adapter}
+        assert 1 <= rows <= 64 and set(sorted_index[first:first + rows]) == {adapter}
     before = y.clone()
     got = et.adapter_add(y, x, bank, plan)
     assert torch.equal(y, before)

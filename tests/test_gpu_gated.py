@@ -73,7 +73,7 @@ def _close(got, want, name):
     assert worst <= 1.0, (name, worst)
 
 
-SIZES = [(1, 8, 8), (1, 64, 8), (2, 72, 24), (17, 136, 40), (64, 512, 104), (65, 200, 72), (128, 64, 64), (130, 64, 136),
+SIZES = [(1, 8, 8), (1, 64, 8), (2, 72, 24), (17, 136, 40), (33, 1032, 16), (64, 512, 104), (65, 200, 72), (200, 72, 48), (128, 64, 64), (130, 64, 136),
          (257, 1000, 712), (1025, 136, 264)]
 
 
