@@ -10,23 +10,26 @@
 //
 // Tiling.  A block of 2 x 2 waves owns a tile of 32 MI x 32 NJ; a wave owns
 // MI x NJ tiles of v_mfma_f32_16x16x32.  k advances in chunks of 64 through two
-// LDS stages filled by direct-to-LDS buffer loads.  MI = NJ = 8: a 256 x 256
-// tile, one block per CU, 16 fragment reads for 64 MFMAs, so LDS is read for half
-// of the MFMAs' time; MI = NJ = 4: a 128 x 128 tile, two blocks per CU, LDS reads
-// as long as the MFMAs, but four times as many tiles for calls that have few.
+// LDS stages filled by direct-to-LDS buffer loads.  Three shapes (TileKind): big,
+// 256 x 256, one block per CU, 16 fragment reads for 64 MFMAs, so LDS is read for
+// half of the MFMAs' time; small, 128 x 128, two blocks per CU, LDS reads as long as
+// the MFMAs, but four times as many tiles; thin, 64 x 128 or 64 x 64, for calls that
+// have few tiles all the same (dense_kind).
 // A wave holds a whole chunk's fragments in registers, so a stage is free again
 // as soon as every wave has read it and two chunks stream in while one is
 // multiplied; loads and fragment reads are placed between MFMAs in a pinned
 // order.  The grid is persistent and a block's tiles form one stream of chunks:
-// a tile's last two chunks load the next tile's first two.
+// a tile's last two chunks load the next tile's first two.  (Four stages, one block
+// per CU, change little: 128 x 128 at K = 4096 45 to 42 us, at K = 1024 13.3 to 14.5: a
+// chunk of a small tile is its two barriers and LDS reads, not its way from memory.)
 //
 // LDS layout.  k along rows: 128 bytes (64 k) per row, the 16-byte segment s of
 // row R at slot s ^ (R & 7) ^ (R >> 3 & 1).  k down columns: 64 rows (k) of 64 MI
-// bytes, segment s of row r at slot s ^ 4 (r & 3) ^ 2 (r >> 3 & 1).  Either way the
-// fragment reads spread over all banks.
+// bytes, segment s of row r at slot s ^ 4 (r & 3) ^ 2 (r >> 3 & 1) (MI = 2, two rows to 256
+// bytes: s ^ 4 (r >> 1 & 1) ^ 2 (r >> 3 & 1)).  Either way the fragment reads spread over
+// all banks.
 //
-// A policy P has: MI, NJ, kACol, kBCol, kF16, kBlocks (per CU), Args, Tile (with
-// a GemmTile first), tiles(), tile(), b_row() and epilogue().
+// A policy P has: a DenseTile's MI, NJ and kBlocks (per CU); kACol, kBCol, kF16; Args, Tile (with a GemmTile first), tiles(), tile(), b_row() and epilogue().
 #pragma once
 
 #include <type_traits>
@@ -40,6 +43,15 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kDenseThreads = 256;
+
+enum TileKind { kTileThin = 2, kTileSmall = 4, kTileBig = 8 };
+
+// THIN: thin tiles are 64 x 32 THIN.
+template <int KIND, int THIN>
+struct DenseTile {
+    static constexpr int MI = KIND, NJ = KIND == kTileThin ? THIN : KIND;
+    static constexpr int kBlocks = KIND == kTileBig ? 1 : 2;
+};
 
 // Operands of a tile, all wave-uniform.  a and b point at the tile's first row
 // and first k (k along rows) or first k and first column (k down columns).
@@ -178,13 +190,14 @@ __global__ __launch_bounds__(kDenseThreads, P::kBlocks) void dense_gemm_kernel(t
     };
     const auto col_chunk = [&](auto n, const unsigned char* p, int cols, int ld, int k, int c) -> ColChunk {
         constexpr int N = decltype(n)::value, LPR = 4 * N;                        // lanes a row
-        static_assert(N == 8 || N == 4, "tile side");
+        static_assert(N == 8 || N == 4 || N == 2, "tile side");
         ColChunk r;
         r.res = dense_rsrc(p + (int64_t)c * 128 * ld, (min(64, k - c * 64) - 1) * ld * 2 + ((cols + 7) & ~7) * 2);
         const int in = lane / LPR;
 #pragma unroll
         for (int v = 0; v < 4; ++v)
-            r.at[v] = (uint32_t)(in * 2 * ld + ((lane % LPR) ^ (4 * in ^ (N == 8 ? 8 * (v & 1) ^ 2 * (v >> 1) : 2 * (v & 1)))) * 16);
+            r.at[v] = (uint32_t)(in * 2 * ld + ((lane % LPR) ^ (N == 2 ? 4 * (in >> 1 & 1) ^ 2 * (v & 1)
+                                                                : 4 * in ^ (N == 8 ? 8 * (v & 1) ^ 2 * (v >> 1) : 2 * (v & 1)))) * 16);
         return r;
     };
     const auto a_chunk = [&](const typename P::Tile& t, int c) {
@@ -201,7 +214,7 @@ __global__ __launch_bounds__(kDenseThreads, P::kBlocks) void dense_gemm_kernel(t
     };
     const auto load_cols = [&](auto n, const ColChunk& r, int ld, int i, uint32_t lds) {
         constexpr int N = decltype(n)::value, RPI = 16 / N;                       // rows a load
-        const int v = N == 8 ? (i & 1) + 2 * (i >> 2 & 1) : i >> 1 & 1;
+        const int v = N == 8 ? (i & 1) + 2 * (i >> 2 & 1) : N == 4 ? i >> 1 & 1 : i & 1;
         dense_dma(r.res, r.at[v] + (uint32_t)((wave * N + i) * RPI) * (uint32_t)(2 * ld), 0u, lds);
     };
     const auto dma_one = [&](const typename P::Tile& t, const auto& ra, const auto& rb, int c, int par, int q) {
@@ -231,14 +244,14 @@ __global__ __launch_bounds__(kDenseThreads, P::kBlocks) void dense_gemm_kernel(t
     u32x4_t fa[2][MI], fb[2][NJ];
     const int fkey = (lane & 7) ^ ((lane >> 3) & 1);
     const int frow = (r16 >> 3) * 1024 + (lane & 7) * 128;
-    const int tkey = (2 * (r16 >> 2) ^ (rho & 1)) << 5;
+    const int tkey = (2 * (r16 >> 2) ^ (rho & 1)) << 5, tkey2 = (2 * (r16 >> 3) ^ (rho & 1)) << 5;
     const int tin = ((r16 & 3) >> 1) * 16 + (r16 & 1) * 8;
     const auto read_rows = [&](const unsigned char* op, int tile, int ks) -> u32x4_t {
         return *reinterpret_cast<const u32x4_t*>(op + tile * 2048 + frow + (((4 * ks + rho) ^ fkey) << 4));
     };
     const auto read_cols = [&](auto n, const unsigned char* op, int tile, int ks) -> u32x4_t {
         constexpr int RBytes = 64 * decltype(n)::value;
-        const unsigned char* const p = op + (32 * ks + 8 * rho + (r16 >> 2)) * RBytes + ((tile << 5) ^ tkey) + tin;
+        const unsigned char* const p = op + (32 * ks + 8 * rho + (r16 >> 2)) * RBytes + ((tile << 5) ^ (decltype(n)::value == 2 ? tkey2 : tkey)) + tin;
         const uint2 lo = dense_read_tr(p), hi = dense_read_tr(p + 4 * RBytes);
         return u32x4_t{lo.x, lo.y, hi.x, hi.y};
     };
@@ -271,23 +284,23 @@ __global__ __launch_bounds__(kDenseThreads, P::kBlocks) void dense_gemm_kernel(t
     if (!more) return;
     int par = 0;              // stage of chunk c: (c + par) & 1
     int nk = (cur.k + 63) / 64;
-    {
-        const auto a0 = a_chunk(cur, 0);
-        const auto b0 = b_chunk(cur, 0);
+    // A tile's first two chunks: waits for the first.
+    const auto begin = [&](const typename P::Tile& t, int n, int par2) {
 #pragma unroll
-        for (int q = 0; q < NL; ++q) dma_one(cur, a0, b0, 0, par, q);
-        if (nk > 1) {
-            const auto a1 = a_chunk(cur, 1);
-            const auto b1 = b_chunk(cur, 1);
+        for (int c = 0; c < 2; ++c) {
+            if (c < n) {
+                const auto a0 = a_chunk(t, c);
+                const auto b0 = b_chunk(t, c);
 #pragma unroll
-            for (int q = 0; q < NL; ++q) dma_one(cur, a1, b1, 1, par, q);
-            dense_wait_barrier<NL>();
-        } else {
-            dense_wait_barrier<0>();
+                for (int q = 0; q < NL; ++q) dma_one(t, a0, b0, c, par2, q);
+            }
         }
+        if (n > 1) dense_wait_barrier<NL>();
+        else dense_wait_barrier<0>();
+    };
+    begin(cur, nk, par);
 #pragma unroll
-        for (int r = 0; r < RPK; ++r) read_r(0, 0, r);
-    }
+    for (int r = 0; r < RPK; ++r) read_r(0, 0, r);
     // Chunk c, its first k-step's fragments in registers: the second one's are read
     // under the first quarter of the MFMAs; then no wave reads this stage any more
     // and the stream's chunk two ahead is loaded into it under the next half; the
@@ -346,8 +359,7 @@ __global__ __launch_bounds__(kDenseThreads, P::kBlocks) void dense_gemm_kernel(t
         const bool stream = more && nk >= 2 && nk1 >= 2;
         const int nmain = nk - 2;
         for (int c = 0; c < nmain; ++c) step(c, cur, c + 2, par, true, true);
-        for (int c = max(nmain, 0); c < nk; ++c)
-            step(c, nxt, c + 2 - nk, par + nk, stream, c + 1 < nk || stream);
+        for (int c = max(nmain, 0); c < nk; ++c) step(c, nxt, c + 2 - nk, par + nk, stream, c + 1 < nk || stream);
         // (the accumulators stay in the accumulation registers up to here)
 #pragma unroll
         for (int i = 0; i < MI; ++i)
@@ -368,19 +380,7 @@ __global__ __launch_bounds__(kDenseThreads, P::kBlocks) void dense_gemm_kernel(t
         if (!stream) {
             // (every wave has read its last fragments: they were consumed above)
             dense_wait_barrier<0>();
-            const auto a0 = a_chunk(nxt, 0);
-            const auto b0 = b_chunk(nxt, 0);
-#pragma unroll
-            for (int q = 0; q < NL; ++q) dma_one(nxt, a0, b0, 0, par + nk, q);
-            if (nk1 > 1) {
-                const auto a1 = a_chunk(nxt, 1);
-                const auto b1 = b_chunk(nxt, 1);
-#pragma unroll
-                for (int q = 0; q < NL; ++q) dma_one(nxt, a1, b1, 1, par + nk, q);
-                dense_wait_barrier<NL>();
-            } else {
-                dense_wait_barrier<0>();
-            }
+            begin(nxt, nk1, par + nk);
         }
 #pragma unroll
         for (int r = 0; r < RPK; ++r) read_r((par + nk) & 1, 0, r);
@@ -396,6 +396,35 @@ inline unsigned dense_grid(int64_t tiles, int blocks_per_cu, int cus)
 {
     const int64_t held = (int64_t)cus * blocks_per_cu / 8 * 8;
     return (unsigned)std::max<int64_t>(8, std::min<int64_t>(held, (tiles + 7) / 8 * 8));
+}
+
+// The tile's shape for a call of so many tiles of each kind, by what their rounds
+// take.  In 1/100 of a chunk of two small tiles a CU (1.0 us): a big one 134, a small
+// one with a CU of its own 60, thin ones 71 and 48 (64 x 128) or 60 and 40 (64 x 64).
+// Measured at K = 2048 and 4096, SwiGLU forward: 192 small tiles 38 us, as 352 thin ones
+// 40; 96 small 38, 160 thin 32; 512 small 64, 128 big 89, 1024 thin 91; Newton-Schulz,
+// five steps: 512 x 512 138 us small, 100 thin; 8 of them 153 and 126; 24 of 512 x 1024
+// 305 and 403.
+inline int dense_kind(int64_t big, int64_t small, int64_t thin, bool wide, int cus)
+{
+    const auto rounds = [cus](int64_t tiles, int alone, int pair) {
+        const int64_t full = tiles / (2 * cus), rest = tiles - full * 2 * cus;
+        return full * pair + (rest == 0 ? 0 : rest <= cus ? alone : pair);
+    };
+    const int64_t b = (big + cus - 1) / cus * 134, s = rounds(small, 60, 100);
+    const int64_t t = wide ? rounds(thin, 48, 71) : rounds(thin, 40, 60);
+    return b <= s && b <= t ? kTileBig : s <= t ? kTileSmall : kTileThin;
+}
+
+// Launches POLICY<kind> on `tiles` tiles.
+template <template <int> class POLICY, class ARGS>
+int launch_dense(const ARGS& g, int kind, int64_t tiles, int cus, hipStream_t s, const char* what)
+{
+    const dim3 block(kDenseThreads), grid(dense_grid(tiles, kind == kTileBig ? 1 : 2, cus));
+    if (kind == kTileBig) dense_gemm_kernel<POLICY<kTileBig>><<<grid, block, 0, s>>>(g);
+    else if (kind == kTileSmall) dense_gemm_kernel<POLICY<kTileSmall>><<<grid, block, 0, s>>>(g);
+    else dense_gemm_kernel<POLICY<kTileThin>><<<grid, block, 0, s>>>(g);
+    return check_launch(what);
 }
 
 // Compute units of the current device, looked up once per device.

@@ -60,11 +60,11 @@ struct GatedArgs {
 
 // x (rows) times gate and up rows: a wave's first NJ / 2 tiles are gate rows, the
 // others the up rows of the same hidden units.
-template <int SIDE, int ACT, bool BACKWARD>
-struct GatedPolicy {
-    static constexpr int MI = SIDE, NJ = SIDE;
+template <int KIND, int ACT, bool BACKWARD>
+struct GatedPolicy : DenseTile<KIND, 4> {
+    using DenseTile<KIND, 4>::MI;
+    using DenseTile<KIND, 4>::NJ;
     static constexpr bool kACol = false, kBCol = false, kF16 = false;
-    static constexpr int kBlocks = SIDE == 8 ? 1 : 2;
     static constexpr int BM = 32 * MI, BH = 16 * NJ;      // rows and hidden units of a tile
     using Args = GatedArgs;
     struct Tile : GemmTile {
@@ -240,7 +240,7 @@ bool is_skinny(int64_t T, int64_t F)
 {
     const int cus = dense_cus();
     const int64_t rounds = up(F / 8 * up(T, 64), cus), tiled = up(up(T, 128) * up(F, 64), 2 * cus);
-    return T <= 16 || (T <= 256 && rounds <= 3 * tiled);
+    return T <= 16 || rounds <= 3 * tiled;
 }
 
 template <int ACT>
@@ -262,11 +262,11 @@ struct InputGradArgs {
     int nm, nn;
 };
 
-template <int SIDE>
-struct InputGradPolicy {
-    static constexpr int MI = SIDE, NJ = SIDE;
+template <int KIND>
+struct InputGradPolicy : DenseTile<KIND, 4> {
+    using DenseTile<KIND, 4>::MI;
+    using DenseTile<KIND, 4>::NJ;
     static constexpr bool kACol = false, kBCol = true, kF16 = false;
-    static constexpr int kBlocks = SIDE == 8 ? 1 : 2;
     static constexpr int BM = 32 * MI, BN = 32 * NJ;
     using Args = InputGradArgs;
     struct Tile : GemmTile {
@@ -318,11 +318,11 @@ struct WeightGradArgs {
     bool f32;
 };
 
-template <int SIDE>
-struct WeightGradPolicy {
-    static constexpr int MI = SIDE, NJ = SIDE;
+template <int KIND>
+struct WeightGradPolicy : DenseTile<KIND, 4> {
+    using DenseTile<KIND, 4>::MI;
+    using DenseTile<KIND, 4>::NJ;
     static constexpr bool kACol = true, kBCol = true, kF16 = false;
-    static constexpr int kBlocks = SIDE == 8 ? 1 : 2;
     static constexpr int BM = 32 * MI, BN = 32 * NJ;
     using Args = WeightGradArgs;
     struct Tile : GemmTile {
@@ -393,26 +393,19 @@ __global__ __launch_bounds__(kDenseThreads) void gated_zero_kernel(uint32_t* p, 
         p[at] = 0u;
 }
 
-template <template <int> class POLICY, class ARGS>
-int launch_sided(ARGS g, int side, int64_t tiles, hipStream_t s, const char* what)
-{
-    const int cus = dense_cus();
-    if (side == 8) dense_gemm_kernel<POLICY<8>><<<dim3(dense_grid(tiles, 1, cus)), dim3(kDenseThreads), 0, s>>>(g);
-    else dense_gemm_kernel<POLICY<4>><<<dim3(dense_grid(tiles, 2, cus)), dim3(kDenseThreads), 0, s>>>(g);
-    return check_launch(what);
-}
+template <int KIND> using SiluFwd = GatedPolicy<KIND, ET_GATED_SILU, false>;
+template <int KIND> using GeluFwd = GatedPolicy<KIND, ET_GATED_GELU, false>;
+template <int KIND> using SiluBwd = GatedPolicy<KIND, ET_GATED_SILU, true>;
+template <int KIND> using GeluBwd = GatedPolicy<KIND, ET_GATED_GELU, true>;
 
-template <int SIDE> using SiluFwd = GatedPolicy<SIDE, ET_GATED_SILU, false>;
-template <int SIDE> using GeluFwd = GatedPolicy<SIDE, ET_GATED_GELU, false>;
-template <int SIDE> using SiluBwd = GatedPolicy<SIDE, ET_GATED_SILU, true>;
-template <int SIDE> using GeluBwd = GatedPolicy<SIDE, ET_GATED_GELU, true>;
+// Rows and columns of a kind's tiles.
+int rows_of(int kind) { return kind == kTileBig ? 256 : kind == kTileSmall ? 128 : 64; }
+int cols_of(int kind) { return kind == kTileBig ? 256 : 128; }
 
-// Tile side of a product of m x n outputs (8: 256 x 256 tiles, 4: 128 x 128).
-int dense_side(int64_t m, int64_t n, int64_t splits = 1)
+// The tiles of a product of m x n outputs.
+int kind_of(int64_t m, int64_t n)
 {
-    const int cus = dense_cus();
-    const int64_t big = up(m, 256) * up(n, 256) * splits, small = up(m, 128) * up(n, 128) * splits;
-    return 4 * up(big, cus) <= 3 * up(small, 2 * cus) ? 8 : 4;
+    return dense_kind(up(m, 256) * up(n, 256), up(m, 128) * up(n, 128), up(m, 64) * up(n, 128), true, dense_cus());
 }
 
 int check_sizes(const char* fn, int64_t T, int64_t K, int64_t F, int64_t ldx, int act)
@@ -435,36 +428,41 @@ int check_pointer(const char* fn, const char* name, const void* p)
     return ET_OK;
 }
 
-int launch_gated(GatedArgs g, int act, bool backward, int side, hipStream_t s)
+// kind: the tiles (0: by size)
+int launch_gated(GatedArgs g, int act, bool backward, int kind, hipStream_t s)
 {
-    if (side == 0 && !backward && is_skinny(g.T, g.F)) {
+    if (kind == 0 && !backward && is_skinny(g.T, g.F)) {
         if (act == ET_GATED_SILU) launch_skinny<ET_GATED_SILU>(g, s);
         else launch_skinny<ET_GATED_GELU>(g, s);
         return check_launch("gated_skinny_kernel");
     }
-    if (side == 0) side = dense_side(g.T, 2 * g.F);
-    g.nm = (int)up(g.T, 32 * side);
-    g.nn = (int)up(g.F, 16 * side);
+    if (kind == 0) kind = kind_of(g.T, 2 * g.F);
+    g.nm = (int)up(g.T, rows_of(kind));
+    g.nn = (int)up(g.F, cols_of(kind) / 2);
     const int64_t tiles = (int64_t)g.nm * g.nn;
+    const int cus = dense_cus();
     if (act == ET_GATED_SILU)
-        return backward ? launch_sided<SiluBwd>(g, side, tiles, s, "gated_backward") : launch_sided<SiluFwd>(g, side, tiles, s, "gated_linear");
-    return backward ? launch_sided<GeluBwd>(g, side, tiles, s, "gated_backward") : launch_sided<GeluFwd>(g, side, tiles, s, "gated_linear");
+        return backward ? launch_dense<SiluBwd>(g, kind, tiles, cus, s, "gated_backward")
+                        : launch_dense<SiluFwd>(g, kind, tiles, cus, s, "gated_linear");
+    return backward ? launch_dense<GeluBwd>(g, kind, tiles, cus, s, "gated_backward")
+                    : launch_dense<GeluFwd>(g, kind, tiles, cus, s, "gated_linear");
 }
 
 // Splits of dW's sum over the tokens: as many blocks as the GPU holds, a split
 // of 512 tokens at least.
 struct Split {
-    int side, splits;
+    int kind, splits;
     int64_t step;
 };
 Split split_tokens(int64_t T, int64_t K, int64_t F)
 {
     const int cus = dense_cus();
-    if (up(2 * F, 256) * up(K, 256) * 4 >= 3 * cus) return {8, 1, T};
+    if (up(2 * F, 256) * up(K, 256) * 4 >= 3 * cus) return {kTileBig, 1, T};
     const int64_t tiles = up(2 * F, 128) * up(K, 128);
     const int64_t most = std::max<int64_t>(1, 2 * cus / tiles);
     const int64_t step = std::max<int64_t>(512, up(up(T, most), 64) * 64);
-    return {4, (int)std::max<int64_t>(1, up(T, step)), step};
+    const int64_t splits = std::max<int64_t>(1, up(T, step));
+    return {kTileSmall, (int)splits, step};
 }
 
 }  // namespace
@@ -473,7 +471,7 @@ Split split_tokens(int64_t T, int64_t K, int64_t F)
 using namespace et;
 
 extern "C" int et_gated_linear_impl(const void* x, int64_t x_stride, const void* w, int64_t rows, int64_t K, int64_t F,
-                                    int activation, void* h, int side, void* stream)
+                                    int activation, void* h, int kind, void* stream)
 {
     const char* fn = "et_gated_linear";
     int rc = check_sizes(fn, rows, K, F, x_stride, activation);
@@ -490,7 +488,7 @@ extern "C" int et_gated_linear_impl(const void* x, int64_t x_stride, const void*
     g.ldx = (int)x_stride;
     g.K = (int)K;
     g.F = (int)F;
-    return launch_gated(g, activation, false, side, (hipStream_t)stream);
+    return launch_gated(g, activation, false, kind, (hipStream_t)stream);
 }
 
 extern "C" int et_gated_linear(const void* x, int64_t x_stride, const void* w, int64_t rows, int64_t K, int64_t F,
@@ -554,10 +552,10 @@ extern "C" int et_gated_linear_bwd(const void* dh, const void* x, int64_t x_stri
         a.T = rows;
         a.K = (int)K;
         a.F = (int)F;
-        const int side = dense_side(rows, K);
-        a.nm = (int)up(rows, 32 * side);
-        a.nn = (int)up(K, 32 * side);
-        rc = launch_sided<InputGradPolicy>(a, side, (int64_t)a.nm * a.nn, s, "gated_input_grad");
+        const int kind = kind_of(rows, K);
+        a.nm = (int)up(rows, rows_of(kind));
+        a.nn = (int)up(K, cols_of(kind));
+        rc = launch_dense<InputGradPolicy>(a, kind, (int64_t)a.nm * a.nn, dense_cus(), s, "gated_input_grad");
         if (rc) return rc;
     }
     if (dw) {
@@ -574,9 +572,9 @@ extern "C" int et_gated_linear_bwd(const void* dh, const void* x, int64_t x_stri
         a.ldx = (int)x_stride;
         a.K = (int)K;
         a.F = (int)F;
-        a.nm = (int)up(2 * F, 32 * sp.side);
-        a.nn = (int)up(K, 32 * sp.side);
-        rc = launch_sided<WeightGradPolicy>(a, sp.side, (int64_t)a.nm * a.nn * sp.splits, s, "gated_weight_grad");
+        a.nm = (int)up(2 * F, rows_of(sp.kind));
+        a.nn = (int)up(K, cols_of(sp.kind));
+        rc = launch_dense<WeightGradPolicy>(a, sp.kind, (int64_t)a.nm * a.nn * sp.splits, dense_cus(), s, "gated_weight_grad");
         if (rc) return rc;
         if (sp.splits > 1) {
             const int64_t n = 2 * F * K;

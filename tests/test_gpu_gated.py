@@ -100,9 +100,9 @@ def test_forward_and_backward(et, dev, T, K, F, activation):
     assert torch.equal(dx, dx2) and torch.equal(dw, dw2)
 
 
-@pytest.mark.parametrize("side", [4, 8])
-@pytest.mark.parametrize("T,K,F", [(1, 8, 8), (5, 64, 24), (300, 72, 136), (513, 256, 520), (1100, 136, 40)])
-def test_both_tiles_of_the_forward(et, dev, T, K, F, side):
+@pytest.mark.parametrize("side", [2, 4, 8])
+@pytest.mark.parametrize("T,K,F", [(1, 8, 8), (5, 64, 24), (300, 72, 136), (513, 256, 520), (1100, 136, 40), (700, 328, 4104), (700, 136, 4104), (300, 64, 8200)])
+def test_all_tiles_of_the_forward(et, dev, T, K, F, side):
     print(f"gated tile {side} T={T} K={K} F={F}", flush=True)
     x, w, _ = _inputs(dev, T, K, F)
     x = x.contiguous()

@@ -65,7 +65,7 @@ def _gradient(dev, E, m, n, seed=0, low_rank=True):
 
 
 SIZES = [(1, 1, 1), (1, 1, 7), (3, 9, 1), (2, 5, 3), (1, 16, 64), (1, 77, 130), (2, 130, 77), (3, 501, 154), (2, 154, 501),
-         (4, 256, 256), (1, 520, 300), (1, 8, 2048), (40, 512, 384), (40, 384, 520)]
+         (4, 256, 256), (1, 520, 300), (1, 8, 2048), (2, 2048, 9), (3, 64, 1024), (2, 1100, 50), (2, 40, 4096), (40, 512, 384), (40, 384, 520)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -237,7 +237,8 @@ def test_refusals(et, dev):
     for bad in (dict(g=g.mT), dict(g=g[0, 0]), dict(g=g.cpu()), dict(steps=0), dict(steps=65), dict(eps=-1.0),
                 dict(coefficients=(3.0, 1.0)), dict(coefficients=(4.0, 0.0, 0.0)), dict(coefficients=(-1.0, 0.0, 0.0)),
                 dict(coefficients=(20.0, -40.0, 20.5)), dict(out=torch.empty(2, 8, 8, device=dev, dtype=torch.bfloat16)),
-                dict(workspace=torch.empty(256, device=dev, dtype=torch.uint8)), dict(g=torch.empty(1, 65536, device=dev))):
+                dict(g=torch.empty(2, 80, 96, device=dev), workspace=torch.empty(256, device=dev, dtype=torch.uint8)),
+                dict(g=torch.empty(1, 65536, device=dev))):
         with pytest.raises(ValueError):
             et.orthogonalize(**{**dict(g=g), **bad})
     p, m = torch.zeros(2, 8, 16, device=dev), torch.zeros(2, 8, 16, device=dev)
