@@ -7,17 +7,15 @@
 // to 16 or 32 tokens of one adapter, so that every item is a pair of small matrix
 // products.  Two launches a projection:
 //   shrink  v = scale_i A_i x of an item's tokens: the sum over K split over the
-//           waves of a block, and over blocks where there are few items; A and x go
-//           from memory straight into the matrix units' operands (both have k along
-//           their rows, and each is read once a block);
-//   expand  out = y + B_i v: 64 columns a wave.  v is taken as a sum of two bf16
+//           waves of a block, and over blocks where there are few items;
+//   expand  out = y + B_i v: 64 columns of a wave at a time.  v is taken as a sum of two bf16
 //           numbers (16 bits of it; with rank 16 both fill one MFMA's k of 32), so
 //           the one rounding that counts is that of the result.
 // The bytes of x, y, out and the adapters in use bound both.  Which tokens share an item
 // changes no result: every sum runs within a token.
 #include <algorithm>
 
-#include "et_gemm_common.hpp"
+#include "et_dense_gemm.hpp"
 #include "etmoe_dense.h"
 
 namespace et {
@@ -26,7 +24,6 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
-constexpr int kShrinkWaves = 8;
 
 struct Item {
     int adapter, first, rows, unused;
@@ -111,79 +108,142 @@ struct AdapterArgs {
     const int32_t* order;
     const Item* items;
     const int32_t* num_items;
-    float* v;                    // [splits, T, r], by place in the order
+    float* v;                    // by place in the order: [splits, T, r], or (large items) bf16 hi and lo [2, T, r]
     unsigned char* out;
     int64_t ldx, ldy, ldo, T;
     int K, N, r, splits, step;   // step: the k of a split
     int col_blocks, chunks;      // of an item, and of a wave, in the expand kernel
 };
 
-// RT: tiles of 16 rows of A; TT: tiles of 16 tokens; U: chunks of a wave in flight; 64
-// tokens of rank 128 leave room in LDS for the sums of 4 WAVES.
+// RT: tiles of 16 rows of A; TT: tiles of 16 tokens.  A wave brings its chunks of 64
+// k through a ring of D stages of LDS of its own: a direct load fills 8 rows x 128
+// bytes, whole cache lines.  (Loads of an operand's 16 rows x 64 bytes into
+// registers move 14 bytes a cycle and CU: 8192 tokens, K = 4096, rank 32 22 us.)
 // (items has room for every block: it is read beside their number)
-template <int RT, int TT, int U, int WAVES>
-__global__ __launch_bounds__(WAVES * kWave) void adapter_shrink_kernel(AdapterArgs g)
+template <int RT, int TT>
+struct ShrinkShape {
+    static constexpr int kStageBytes = (RT + TT) * 2048;
+    static constexpr int kWaves = RT + TT <= 3 ? 8 : 4;
+    // (tiles of 32 tokens: two blocks a CU)
+    static constexpr int kFit = (TT == 2 && RT <= 4 ? 72 : 144) * 1024 / (kWaves * kStageBytes), D = kFit > 4 ? 4 : kFit;
+    static_assert(D >= 1, "LDS");
+};
+
+// The same direct load from an address of each lane's own.
+__device__ __forceinline__ void dma_global(const unsigned char* p, uint32_t lds)
 {
-    __shared__ f32x4_t part[WAVES][TT * RT][kWave];
-    const Item it = g.items[blockIdx.x];
-    if ((int)blockIdx.x >= *g.num_items || it.adapter < 0) return;
-    const int lane = lane_id(), wave = (int)threadIdx.x >> 6;
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "{m0}"(lds) : "memory");
+}
+
+// SUBS: blocks of 16 TT tokens an item.  SPLIT: partial sums of v in f32 (of splits of
+// K); otherwise v as two bf16 numbers, as the other kernel takes it.
+template <int RT, int TT, int SUBS, bool SPLIT>
+__global__ __launch_bounds__((ShrinkShape<RT, TT>::kWaves * kWave)) void adapter_shrink_kernel(AdapterArgs g)
+{
+    using Shape = ShrinkShape<RT, TT>;
+    constexpr int W = Shape::kWaves, D = Shape::D, kStageBytes = Shape::kStageBytes, NI = 2 * (RT + TT);
+    constexpr int kRing = W * D * kStageBytes, kPart = W * RT * TT * kWave * 16;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[kRing > kPart ? kRing : kPart];
+    const int item = (int)blockIdx.x / SUBS;
+    Item it = g.items[item];
+    it.first += (int)blockIdx.x % SUBS * (16 * TT);
+    it.rows -= (int)blockIdx.x % SUBS * (16 * TT);
+    if (item >= *g.num_items || it.adapter < 0 || it.rows <= 0) return;
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int r16 = lane & 15, rho = lane >> 4;
     const int split = (int)blockIdx.y;
     const int k0 = split * g.step, k1 = min(g.K, k0 + g.step);
-    const __amdgpu_buffer_rsrc_t ares = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<unsigned char*>(g.a + (int64_t)it.adapter * g.r * g.K * 2), (short)0, g.r * g.K * 2, kBufDword3);
-    const unsigned char* xr[TT];
+    const __amdgpu_buffer_rsrc_t ares = dense_rsrc(g.a + (int64_t)it.adapter * g.r * g.K * 2, g.r * g.K * 2);
+    // (tokens past the item's repeat its last one: their columns are not used)
+    const unsigned char* xr[TT][2];
 #pragma unroll
-    for (int t = 0; t < TT; ++t) {
-        // (tokens past the item's repeat its last one: their columns are not used)
-        const int64_t token = g.order[it.first + min(16 * t + r16, it.rows - 1)];
-        xr[t] = g.x + token * g.ldx * 2;
-    }
+    for (int t = 0; t < TT; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int64_t token = g.order[it.first + min(16 * t + 8 * i + (lane >> 3), it.rows - 1)];
+            xr[t][i] = g.x + token * g.ldx * 2;
+        }
+    unsigned char* const mine = smem + wave * (D * kStageBytes);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_t*)mine;
+    const int seg0 = (lane & 7) ^ (lane >> 3);
+    // Chunk j of the wave.  Past the end A is 0 (and x any of the row's own values: one
+    // that is not finite makes the token's sum so anyway).
+    const auto load = [&](int j, uint32_t lds) {
+        const int c = k0 + (W * j + wave) * 64;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int k = c + (seg0 ^ i) * 8;
+#pragma unroll
+            for (int a = 0; a < RT; ++a) {
+                const int row = 16 * a + 8 * i + (lane >> 3);
+                dense_dma(ares, k < k1 && row < g.r ? (uint32_t)(row * g.K + k) * 2u : kOOR, 0u, lds + a * 2048 + i * 1024);
+            }
+#pragma unroll
+            for (int t = 0; t < TT; ++t) dma_global(xr[t][i] + 2 * (int64_t)min(k, g.K - 8), lds + (RT + t) * 2048 + i * 1024);
+        }
+    };
     f32x4_t acc[RT][TT];
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
         for (int t = 0; t < TT; ++t) acc[i][t] = f32x4_t{};
-    // Chunks of 64 k, dealt to the waves in turn: a row's 128 bytes in two loads of
-    // one wave.  Past the end A is 0 (and x any of the row's own values: one that is
-    // not finite makes the token's sum so anyway).
-    const int chunks = (k1 - k0 + 63) / 64;
-    for (int c = wave; c < chunks; c += WAVES * U) {
-        u32x4_t fa[2 * U][RT], fx[2 * U][TT];
+    const int turns = (k1 - k0 + W * 64 - 1) / (W * 64);
 #pragma unroll
-        for (int u = 0; u < 2 * U; ++u) {
-            const int k = k0 + 64 * (c + (u >> 1) * WAVES) + 32 * (u & 1) + 8 * rho;
+    for (int d = 0; d < D; ++d) load(d, lds0 + d * kStageBytes);
+    const int fkey = (lane & 7) ^ ((lane >> 3) & 1);
+    const int frow = (r16 >> 3) * 1024 + (lane & 7) * 128;
+    for (int j = 0, stage = 0; j < turns; ++j) {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * NI) : "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        const unsigned char* const at = mine + stage * kStageBytes;
 #pragma unroll
-            for (int i = 0; i < RT; ++i)
-                fa[u][i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
-                    ares, k < k1 ? (uint32_t)(min(16 * i + r16, g.r - 1) * g.K + k) * 2u : kOOR, 0, 0));
+        for (int ks = 0; ks < 2; ++ks) {
+            const auto read = [&](int tile) {
+                return __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const u32x4_t*>(at + tile * 2048 + frow + (((4 * ks + rho) ^ fkey) << 4)));
+            };
+            bf16x8_t fa[RT];
 #pragma unroll
-            for (int t = 0; t < TT; ++t) fx[u][t] = *reinterpret_cast<const u32x4_t*>(xr[t] + 2 * (int64_t)min(k, g.K - 8));
+            for (int i = 0; i < RT; ++i) fa[i] = read(i);
+#pragma unroll
+            for (int t = 0; t < TT; ++t) {
+                const bf16x8_t fx = read(RT + t);
+#pragma unroll
+                for (int i = 0; i < RT; ++i) acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i], fx, acc[i][t], 0, 0, 0);
+            }
         }
-#pragma unroll
-        for (int u = 0; u < 2 * U; ++u)
-#pragma unroll
-            for (int i = 0; i < RT; ++i)
-#pragma unroll
-                for (int t = 0; t < TT; ++t)
-                    acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, fa[u][i]),
-                                                                        __builtin_bit_cast(bf16x8_t, fx[u][t]), acc[i][t], 0, 0, 0);
+        // (the reads above have ended; chunks past the end keep the count of loads)
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(0xC07F);      // lgkmcnt(0)
+        load(j + D, lds0 + stage * kStageBytes);
+        stage = stage + 1 == D ? 0 : stage + 1;
     }
+    dense_wait_barrier<0>();
+    f32x4_t* const part = reinterpret_cast<f32x4_t*>(smem);
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int t = 0; t < TT; ++t) part[wave][i * TT + t][lane] = acc[i][t];
+        for (int t = 0; t < TT; ++t) part[(wave * RT * TT + i * TT + t) * kWave + lane] = acc[i][t];
     __syncthreads();
     const float scale = g.scale[it.adapter];
-    for (int q = (int)threadIdx.x; q < RT * TT * kWave; q += WAVES * kWave) {
+    for (int q = (int)threadIdx.x; q < RT * TT * kWave; q += W * kWave) {
         const int tile = q >> 6, l = q & 63;
-        f32x4_t sum = part[0][tile][l];
+        f32x4_t sum = part[q];
 #pragma unroll
-        for (int w = 1; w < WAVES; ++w) sum += part[w][tile][l];
+        for (int w = 1; w < W; ++w) sum += part[w * RT * TT * kWave + q];
         const int row = 16 * (tile / TT) + 4 * (l >> 4), token = 16 * (tile % TT) + (l & 15);
-        if (row < g.r && token < it.rows)
-            *reinterpret_cast<f32x4_t*>(g.v + ((int64_t)split * g.T + it.first + token) * g.r + row) = sum * scale;
+        if (row >= g.r || token >= it.rows) continue;
+        sum *= scale;
+        const int64_t to = (int64_t)(it.first + token) * g.r + row;
+        if constexpr (SPLIT) {
+            *reinterpret_cast<f32x4_t*>(g.v + (int64_t)split * g.T * g.r + to) = sum;
+        } else {
+            const u32x2_t hi = {pack_bf16x2(sum[0], sum[1]), pack_bf16x2(sum[2], sum[3])};
+            uint16_t* const v = (uint16_t*)g.v;
+            *reinterpret_cast<u32x2_t*>(v + to) = hi;
+            *reinterpret_cast<u32x2_t*>(v + g.T * g.r + to) =
+                u32x2_t{pack_bf16x2(sum[0] - bf16lo(hi[0]), sum[1] - bf16hi(hi[0])), pack_bf16x2(sum[2] - bf16lo(hi[1]), sum[3] - bf16hi(hi[1]))};
+        }
     }
 }
 
@@ -191,17 +251,16 @@ __global__ __launch_bounds__(WAVES * kWave) void adapter_shrink_kernel(AdapterAr
 // expand
 // --------------------------------------------------------------------------
 
-// KS: k-steps of 32 over v's two parts (2 r / 32, rounded up).  A wave's 64 columns
-// are dealt to four MFMA tiles so that a lane holds 8 consecutive ones of a token
-// twice and four lanes 64 contiguous bytes: row i of tile j is column
-// 32 (j / 2) + 8 (i / 4) + 4 (j % 2) + i % 4.
-// A wave goes through g.chunks chunks of columns with its tokens' v in registers (v
-// is as many bytes as a chunk of y at rank 32), the next chunk's y on its way.
-// Blocks take an item's columns in turn, so that those that run together cover
-// whole rows of y.
-template <int KS, int TT, bool EVEN>
+// KS: k-steps of 32 over v's two parts (2 r / 32, rounded up).  A wave goes through
+// g.chunks chunks of 64 columns with its tokens' v in registers.  The products go
+// through LDS so that y and out move in whole cache lines, 8 rows x 128 bytes a load;
+// a chunk's y is on its way while its products are made.  Blocks take an item's
+// columns in turn, so that those that run together cover whole rows of y.
+template <int KS, int TT, bool EVEN, bool SPLIT>
 __global__ __launch_bounds__(kThreads) void adapter_expand_kernel(AdapterArgs g)
 {
+    constexpr int kRow = 64 + 4;      // floats from a token's products to the next's
+    __shared__ __attribute__((aligned(16))) float smem[kWaves * 16 * kRow];
     const int item = (int)(blockIdx.x / (uint32_t)g.col_blocks);
     const Item it = g.items[item];
     if (item >= *g.num_items) return;
@@ -210,17 +269,11 @@ __global__ __launch_bounds__(kThreads) void adapter_expand_kernel(AdapterArgs g)
     int n0 = (int)(blockIdx.x - (uint32_t)item * g.col_blocks) * g.chunks * (64 * kWaves) + wave * 64;
     if (n0 >= g.N || (it.adapter < 0 && g.out == g.y)) return;
     const int segs = g.r / 8;
-    bool ok[TT];
-    const unsigned char* yr[TT];
-    unsigned char* outr[TT];
+    // this lane's rows of y (8 q + lane / 8), and its 8 columns
+    const int line = 8 * (lane & 7);
+    int64_t token[2 * TT];
 #pragma unroll
-    for (int t = 0; t < TT; ++t) {
-        // (a token past the item's repeats its last one, unwritten)
-        ok[t] = 16 * t + r16 < it.rows;
-        const int64_t token = g.order[it.first + min(16 * t + r16, it.rows - 1)];
-        yr[t] = g.y + token * g.ldy * 2;
-        outr[t] = g.out + token * g.ldo * 2;
-    }
+    for (int q = 0; q < 2 * TT; ++q) token[q] = g.order[it.first + min(8 * q + (lane >> 3), it.rows - 1)];
     u32x4_t fv[KS][TT];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -228,85 +281,91 @@ __global__ __launch_bounds__(kThreads) void adapter_expand_kernel(AdapterArgs g)
         const int at = s >= 2 * segs ? 0 : (s >= segs ? s - segs : s) * 8;
 #pragma unroll
         for (int t = 0; t < TT; ++t) {
-            f32x4_t v[2] = {};
-            if (it.adapter >= 0) {
-                const float* p = g.v + (it.first + min(16 * t + r16, it.rows - 1)) * (int64_t)g.r + at;
-                v[0] = *reinterpret_cast<const f32x4_t*>(p);
-                v[1] = *reinterpret_cast<const f32x4_t*>(p + 4);
-                for (int sp = 1; sp < g.splits; ++sp) {
-                    p += g.T * g.r;
-                    v[0] += *reinterpret_cast<const f32x4_t*>(p);
-                    v[1] += *reinterpret_cast<const f32x4_t*>(p + 4);
+            // (a token past the item's repeats its last one, unwritten)
+            const int64_t from = (it.first + min(16 * t + r16, it.rows - 1)) * (int64_t)g.r + at;
+            const bool low = s >= segs;
+            u32x4_t w = {};
+            if constexpr (SPLIT) {
+                f32x4_t v[2] = {};
+                if (it.adapter >= 0) {
+                    const float* p = g.v + from;
+                    v[0] = *reinterpret_cast<const f32x4_t*>(p);
+                    v[1] = *reinterpret_cast<const f32x4_t*>(p + 4);
+                    for (int sp = 1; sp < g.splits; ++sp) {
+                        p += g.T * g.r;
+                        v[0] += *reinterpret_cast<const f32x4_t*>(p);
+                        v[1] += *reinterpret_cast<const f32x4_t*>(p + 4);
+                    }
                 }
-            }
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float a = v[w >> 1][2 * (w & 1)], b = v[w >> 1][2 * (w & 1) + 1];
-                const uint32_t hi = pack_bf16x2(a, b);
-                fv[ks][t][w] = s >= 2 * segs ? 0u : s >= segs ? pack_bf16x2(a - bf16lo(hi), b - bf16hi(hi)) : hi;
+                for (int i = 0; i < 4; ++i) {
+                    const float a = v[i >> 1][2 * (i & 1)], b = v[i >> 1][2 * (i & 1) + 1];
+                    const uint32_t hi = pack_bf16x2(a, b);
+                    w[i] = low ? pack_bf16x2(a - bf16lo(hi), b - bf16hi(hi)) : hi;
+                }
+            } else if (it.adapter >= 0) {
+                w = *reinterpret_cast<const u32x4_t*>((const uint16_t*)g.v + (low ? g.T * g.r : 0) + from);
             }
+            fv[ks][t] = s >= 2 * segs ? u32x4_t{} : w;
         }
     }
     const int64_t first_row = max(it.adapter, 0) * (int64_t)g.N;
-    u32x4_t y[TT][2];
-    const auto load_y = [&](u32x4_t (&to)[TT][2], int n) {
+    float* const mine = smem + wave * (16 * kRow);
+    for (int c = 0; c < g.chunks && n0 < g.N; ++c, n0 += 64 * kWaves) {
+        const int col = n0 + line;
+        u32x4_t y[2 * TT];
 #pragma unroll
-        for (int t = 0; t < TT; ++t)
+        for (int q = 0; q < 2 * TT; ++q)
+            y[q] = *reinterpret_cast<const u32x4_t*>(g.y + (token[q] * g.ldy + min(col, g.N - 8)) * 2);
+        if (it.adapter >= 0) {
+            const __amdgpu_buffer_rsrc_t bres = dense_rsrc(g.b + (first_row + n0) * g.r * 2, min(64, g.N - n0) * g.r * 2);
+            f32x4_t acc[TT][4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                to[t][h] = *reinterpret_cast<const u32x4_t*>(yr[t] + 2 * min(n + 8 * rho + 32 * h, g.N - 8));
-    };
-    load_y(y, n0);
-    for (int c = 0; c < g.chunks; ++c, n0 += 64 * kWaves) {
-        if (n0 >= g.N) break;
-        const __amdgpu_buffer_rsrc_t bres = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<unsigned char*>(g.b + (first_row + n0) * g.r * 2), (short)0,
-            it.adapter >= 0 ? min(64, g.N - n0) * g.r * 2 : 0, kBufDword3);
-        f32x4_t acc[TT][4];
+            for (int t = 0; t < TT; ++t)
 #pragma unroll
-        for (int t = 0; t < TT; ++t)
+                for (int j = 0; j < 4; ++j) acc[t][j] = f32x4_t{};
+            // (EVEN: rank a multiple of 32, the second half of the k-steps has the first
+            // half's columns of b)
+            constexpr int STEPS = EVEN ? KS / 2 : KS;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[t][j] = f32x4_t{};
-        u32x4_t next[TT][2];
-        load_y(next, n0 + 64 * kWaves);
-        // (EVEN: rank a multiple of 32, the second half of the k-steps has the first
-        // half's columns of b)
-        constexpr int STEPS = EVEN ? KS / 2 : KS;
+            for (int ks = 0; ks < STEPS; ++ks) {
+                const int s = 4 * ks + rho;
+                const int at = (!EVEN && s >= segs ? s - segs : s) * 8;
+                u32x4_t fb[4];
 #pragma unroll
-        for (int ks = 0; ks < STEPS; ++ks) {
-            const int s = 4 * ks + rho;
-            const int at = (!EVEN && s >= segs ? s - segs : s) * 8;
-            u32x4_t fb[4];
+                for (int j = 0; j < 4; ++j)
+                    fb[j] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                        bres, s < 2 * segs ? (uint32_t)((16 * j + r16) * g.r + at) * 2u : kOOR, 0, 0));
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                fb[j] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
-                    bres, s < 2 * segs ? (uint32_t)((32 * (j >> 1) + 8 * (r16 >> 2) + 4 * (j & 1) + (r16 & 3)) * g.r + at) * 2u
-                                       : kOOR, 0, 0));
+                for (int half = 0; half < (EVEN ? 2 : 1); ++half)
 #pragma unroll
-            for (int half = 0; half < (EVEN ? 2 : 1); ++half)
+                    for (int t = 0; t < TT; ++t)
 #pragma unroll
-                for (int t = 0; t < TT; ++t)
+                        for (int j = 0; j < 4; ++j)
+                            acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                __builtin_bit_cast(bf16x8_t, fb[j]), __builtin_bit_cast(bf16x8_t, fv[ks + half * STEPS][t]), acc[t][j], 0, 0, 0);
+            }
+            // (one wave's own part of LDS: its operations stay in order)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                            __builtin_bit_cast(bf16x8_t, fb[j]), __builtin_bit_cast(bf16x8_t, fv[ks + half * STEPS][t]), acc[t][j], 0, 0, 0);
-        }
-        const int col = n0 + 8 * rho;
+            for (int t = 0; t < TT; ++t) {
 #pragma unroll
-        for (int t = 0; t < TT; ++t) {
+                for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4_t*>(mine + r16 * kRow + 16 * j + 4 * rho) = acc[t][j];
+                __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                u32x4_t q = y[t][h];
-                if (it.adapter >= 0) {
+                for (int q = 2 * t; q < 2 * t + 2; ++q) {
+                    const float* const p = mine + (8 * (q & 1) + (lane >> 3)) * kRow + line;
+                    const f32x4_t d[2] = {*reinterpret_cast<const f32x4_t*>(p), *reinterpret_cast<const f32x4_t*>(p + 4)};
 #pragma unroll
                     for (int w = 0; w < 4; ++w)
-                        q[w] = pack_bf16x2(bf16lo(q[w]) + acc[t][2 * h + (w >> 1)][2 * (w & 1)],
-                                           bf16hi(q[w]) + acc[t][2 * h + (w >> 1)][2 * (w & 1) + 1]);
+                        y[q][w] = pack_bf16x2(bf16lo(y[q][w]) + d[w >> 1][2 * (w & 1)], bf16hi(y[q][w]) + d[w >> 1][2 * (w & 1) + 1]);
                 }
-                if (ok[t] && col + 32 * h < g.N) *reinterpret_cast<u32x4_t*>(outr[t] + 2 * (col + 32 * h)) = q;
-                y[t][h] = next[t][h];
+                __builtin_amdgcn_wave_barrier();
             }
         }
+#pragma unroll
+        for (int q = 0; q < 2 * TT; ++q)
+            if (8 * q + (lane >> 3) < it.rows && col < g.N)
+                *reinterpret_cast<u32x4_t*>(g.out + (token[q] * g.ldo + col) * 2) = y[q];
     }
 }
 
@@ -324,18 +383,26 @@ int tile_of(int64_t T) { return T <= 2048 ? 16 : 64; }
 
 int64_t most_items(int64_t T, int64_t n) { return up(T, tile_of(T)) + std::min(T, n + 1); }
 
-// Splits of the sum over K: blocks for all CUs, a chunk for each wave at least.
-int splits_of(int64_t items, int64_t K)
+// Splits of the sum over K, where the items leave CUs idle: the fewest rounds of
+// blocks for the work of each, a chunk for each of 8 waves at least.
+int splits_of(int64_t T, int64_t items, int64_t K)
 {
-    return (int)std::max<int64_t>(1, std::min<int64_t>({4, 256 / std::max<int64_t>(1, items), K / (64 * kShrinkWaves)}));
+    const int64_t cus = dense_cus(), most = tile_of(T) == 16 ? std::min<int64_t>(4, K / 512) : 1;
+    int best = 1;
+    for (int s = 2; s <= most; ++s)
+        if (up(items * s, cus) * best < up(items * best, cus) * s) best = s;
+    return best;
 }
 
 template <int RT>
 void launch_shrink(const AdapterArgs& g, int tile, dim3 grid, hipStream_t s)
 {
-    constexpr int U = RT <= 2 ? 2 : 1, W = RT == 8 ? kShrinkWaves / 2 : kShrinkWaves;
-    if (tile == 16) adapter_shrink_kernel<RT, 1, U, kShrinkWaves><<<grid, dim3(kShrinkWaves * kWave), 0, s>>>(g);
-    else adapter_shrink_kernel<RT, 4, 1, W><<<grid, dim3(W * kWave), 0, s>>>(g);
+    if (tile == 16) {
+        adapter_shrink_kernel<RT, 1, 1, true><<<grid, dim3(ShrinkShape<RT, 1>::kWaves * kWave), 0, s>>>(g);
+    } else {
+        grid.x *= 2;
+        adapter_shrink_kernel<RT, 2, 2, false><<<grid, dim3(ShrinkShape<RT, 2>::kWaves * kWave), 0, s>>>(g);
+    }
 }
 
 template <int KS>
@@ -343,11 +410,11 @@ void launch_expand(const AdapterArgs& g, int tile, dim3 grid, hipStream_t s)
 {
     const dim3 block(kThreads);
     if (KS > 1 && g.r == 16 * KS) {
-        if (tile == 16) adapter_expand_kernel<KS, 1, true><<<grid, block, 0, s>>>(g);
-        else adapter_expand_kernel<KS, 4, true><<<grid, block, 0, s>>>(g);
+        if (tile == 16) adapter_expand_kernel<KS, 1, true, true><<<grid, block, 0, s>>>(g);
+        else adapter_expand_kernel<KS, 4, true, false><<<grid, block, 0, s>>>(g);
     } else {
-        if (tile == 16) adapter_expand_kernel<KS, 1, false><<<grid, block, 0, s>>>(g);
-        else adapter_expand_kernel<KS, 4, false><<<grid, block, 0, s>>>(g);
+        if (tile == 16) adapter_expand_kernel<KS, 1, false, true><<<grid, block, 0, s>>>(g);
+        else adapter_expand_kernel<KS, 4, false, false><<<grid, block, 0, s>>>(g);
     }
 }
 
@@ -381,7 +448,7 @@ extern "C" size_t et_adapter_add_workspace_bytes(int64_t num_tokens, int64_t num
 {
     const int64_t items = et_adapter_plan_items(num_tokens, num_adapters);
     if (items < 0 || K < 8 || rank < 8 || rank > ET_MAX_ADAPTER_RANK) return 0;
-    return (size_t)splits_of(items, K) * num_tokens * rank * 4;
+    return (size_t)splits_of(num_tokens, items, K) * num_tokens * rank * 4;
 }
 
 extern "C" int et_adapter_add(const void* y, int64_t y_stride, const void* x, int64_t x_stride, const void* a, const void* b,
@@ -427,14 +494,14 @@ extern "C" int et_adapter_add(const void* y, int64_t y_stride, const void* x, in
     g.K = (int)K;
     g.N = (int)N;
     g.r = (int)rank;
-    g.splits = splits_of(most, K);
+    g.splits = splits_of(num_tokens, most, K);
     g.step = (int)(up(up(K, g.splits), 64) * 64);
     g.splits = (int)up(K, g.step);
     // (several chunks a wave where there are many blocks all the same)
     g.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(4, most * up(N, 64 * kWaves) / 2048));
     g.col_blocks = (int)up(N, 64 * kWaves * g.chunks);
     // (a launch has less than 2^32 threads)
-    if (most * g.col_blocks >= (int64_t)1 << 24 || most * kShrinkWaves * kWave >= (int64_t)1 << 32)
+    if (most * g.col_blocks >= (int64_t)1 << 24 || most >= 1 << 23)
         return refuse(fn, "num_tokens * N is too large");
     const int tile = tile_of(num_tokens);
     hipStream_t s = (hipStream_t)stream;
