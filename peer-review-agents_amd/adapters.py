@@ -5,6 +5,7 @@ include/etmoe_dense.h; there is no CPU fallback."""
 from __future__ import annotations
 
 from dataclasses import dataclass
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -90,17 +91,25 @@ def adapter_plan(index: torch.Tensor, num_adapters: int) -> AdapterPlan:
     return AdapterPlan(order, items, count, T, num_adapters)
 
 
+@lru_cache(maxsize=1024)
+def _workspace_bytes(num_tokens: int, n: int, K: int, rank: int, device: int) -> int:
+    # (the splits that it has room for go by the device's CUs)
+    with torch.cuda.device(device):
+        return int(lib().et_adapter_add_workspace_bytes(num_tokens, n, K, rank))
+
+
 def adapter_add_workspace_bytes(num_tokens: int, bank: AdapterBank) -> int:
     n, rank, K = bank.a.shape
-    return int(lib().et_adapter_add_workspace_bytes(num_tokens, n, K, rank))
+    return _workspace_bytes(num_tokens, n, K, rank, bank.a.get_device())
 
 
-def _rows(t: torch.Tensor, name: str, shape, dev) -> int:
-    if (isinstance(t, torch.Tensor) and t.dtype == torch.bfloat16 and t.shape == shape and t.device == dev
+def _rows(t: torch.Tensor, name: str, rows: int, width: int, dev) -> int:
+    """The row stride of a checked bf16 [rows, width]."""
+    if (isinstance(t, torch.Tensor) and t.dtype == torch.bfloat16 and t.device == dev and t.shape == (rows, width)
             and t.is_contiguous()):
-        stride = shape[1]
+        stride = width
     else:
-        stride = _require_rows(t, name, torch.bfloat16, torch.Size(shape), dev)
+        stride = _require_rows(t, name, torch.bfloat16, torch.Size((rows, width)), dev)
     if stride % 8 or t.data_ptr() % 16:
         raise ValueError(f"{name} must be 16-byte aligned and its rows a multiple of 8 elements apart")
     return stride
@@ -125,12 +134,12 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, bank: AdapterBank, plan: Adapt
         raise ValueError(f"the plan is of {plan.num_adapters} adapters, the bank has {n}")
     if order.device != dev:
         raise ValueError(f"the plan is on {order.device}, the bank on {dev}")
-    ldy, ldx = _rows(y, "y", (T, N), dev), _rows(x, "x", (T, K), dev)
+    ldy, ldx = _rows(y, "y", T, N, dev), _rows(x, "x", T, K, dev)
     if out is None:
         out, ldo = y.new_empty((T, N)), N
     else:
-        ldo = _rows(out, "out", (T, N), dev)
-    wsb = lib().et_adapter_add_workspace_bytes(T, n, K, rank)
+        ldo = _rows(out, "out", T, N, dev)
+    wsb = _workspace_bytes(T, n, K, rank, a.get_device())
     if workspace is None:
         workspace = y.new_empty(wsb >> 1)       # (bf16 elements)
     else:

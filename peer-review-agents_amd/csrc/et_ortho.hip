@@ -285,7 +285,7 @@ __global__ __launch_bounds__(kDenseThreads) void ortho_finish_kernel(OrthoList l
 // (three layers' routers and 8 experts of 512 x 64 and 32 x 512: 227 us).
 constexpr int kFusedThreads = 512, kFusedWaves = kFusedThreads / kWave;
 constexpr int kFusedSide = 64;
-constexpr int kFusedSmall = 40 * 1024, kFusedLarge = 152 * 1024;     // bytes of LDS: four blocks a CU, or one
+constexpr int kFusedSmall = 30 * 1024, kFusedLarge = 150 * 1024;     // bytes of LDS: four blocks a CU, or one
 
 __host__ __device__ inline int64_t round_to(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
@@ -313,6 +313,7 @@ __global__ __launch_bounds__(kFusedThreads) void ortho_fused_kernel(OrthoList l,
 {
     __shared__ __attribute__((aligned(16))) unsigned char smem[LDS_BYTES];
     __shared__ double part[kFusedWaves];
+    __shared__ f32x4_t sums[kFusedWaves][kWave];
     const OrthoTensor& t = l.t[tensor_of(l, blockIdx.x)];
     const int m = (int)t.m, n = (int)t.n, size = m * n;
     const bool tall = m > n;
@@ -329,28 +330,70 @@ __global__ __launch_bounds__(kFusedThreads) void ortho_fused_kernel(OrthoList l,
     uint16_t* const X = (uint16_t*)smem;
     uint16_t* const A = X + f.r16 * f.ldx;
     uint16_t* const S = A + f.r16 * f.lds;
-    // momentum and norm; the places between and behind the values are 0
-    for (int64_t i = tid; i < f.bytes / 16; i += kFusedThreads) reinterpret_cast<u32x4_t*>(smem)[i] = u32x4_t{};
-    constexpr int U = 16;
-    double sum = 0.0;
-    for (int at0 = tid; at0 < size; at0 += U * kFusedThreads) {
-        float v[U], w[U];
+    // Elements go by groups of four, group tid + 512 i to a thread.
+    const auto load4 = [&](const void* p, auto type, int at, float (&v)[4]) {
+        using T = decltype(type);
+        if (t.wide) {
+            if constexpr (sizeof(T) == 4) {
+                const f32x4_t w = *reinterpret_cast<const f32x4_t*>((const float*)p + base + min(at, size - 4));
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int at = min(at0 + u * kFusedThreads, size - 1);
-            v[u] = read1<G>(t.g, base + at);
-            if constexpr (MOM) w[u] = t.mom[base + at];
-        }
+                for (int e = 0; e < 4; ++e) v[e] = w[e];
+            } else {
+                const u32x2_t w = *reinterpret_cast<const u32x2_t*>((const uint16_t*)p + base + min(at, size - 4));
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int at = at0 + u * kFusedThreads;
-            if (at >= size) break;
-            if constexpr (MOM) {
-                v[u] = direction(l, v[u] * gs, w[u]);
-                t.mom[base + at] = w[u];
+                for (int e = 0; e < 4; ++e) v[e] = e & 1 ? bf16hi(w[e >> 1]) : bf16lo(w[e >> 1]);
             }
-            sum += (double)v[u] * (double)v[u];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = read1<T>(p, base + min(at + e, size - 1));
         }
+    };
+    const auto store4 = [&](float* p, int at, const float (&v)[4]) {
+        if (t.wide) {
+            *reinterpret_cast<f32x4_t*>(p + base + at) = f32x4_t{v[0], v[1], v[2], v[3]};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (at + e < size) p[base + at + e] = v[e];
+        }
+    };
+    const auto first_of = [&](int group) { return (group * kFusedThreads + tid) * 4; };
+    // Momentum and norm; the first NG groups' U stay in registers.  (The places between
+    // and behind X's values are 0.)
+    for (int64_t i = tid; i < f.bytes / 16; i += kFusedThreads) reinterpret_cast<u32x4_t*>(smem)[i] = u32x4_t{};
+    constexpr int NG = LDS_BYTES == kFusedSmall ? 8 : 16;
+    float u[NG][4];
+    double sum = 0.0;
+    const auto take = [&](int at, float (&v)[4], float (&w)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (MOM) v[e] = direction(l, v[e] * gs, w[e]);
+            if (at + e >= size) v[e] = 0.0f;
+            sum += (double)v[e] * (double)v[e];
+        }
+        if constexpr (MOM) {
+            if (at < size) store4(t.mom, at, w);
+        }
+    };
+    {
+        float w[NG][4];
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            if (i * kFusedThreads * 4 >= size) break;
+            load4(t.g, G{}, first_of(i), u[i]);
+            if constexpr (MOM) load4(t.mom, float{}, first_of(i), w[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            if (i * kFusedThreads * 4 >= size) break;
+            take(first_of(i), u[i], w[i]);
+        }
+    }
+    for (int i = NG; i * kFusedThreads * 4 < size; ++i) {
+        float v[4], w[4];
+        load4(t.g, G{}, first_of(i), v);
+        if constexpr (MOM) load4(t.mom, float{}, first_of(i), w);
+        take(first_of(i), v, w);
     }
     sum = wave_sum_dpp_f64(sum);
     if (lane == 0) part[wave] = sum;
@@ -359,32 +402,36 @@ __global__ __launch_bounds__(kFusedThreads) void ortho_fused_kernel(OrthoList l,
 #pragma unroll
     for (int w = 0; w < kFusedWaves; ++w) sum += part[w];
     const double inv = (double)(1 << kScaleX) / (sqrt(sum) + (double)l.eps);
-    // (this thread's own values of the momentum, as it wrote them; row and column go
-    // on by kFusedThreads elements at a time)
-    const int rows_on = kFusedThreads / n, cols_on = kFusedThreads - rows_on * n;
-    {
-        int i = tid / n, j = tid - i * n;
-        for (int at0 = tid; at0 < size; at0 += U * kFusedThreads) {
-            float v[U], w[U];
+    // the place in X of element `at` of the matrix, and the step to the next
+    const auto walk = [&](int at, auto f4) {
+        int i = at / n, j = at - i * n;
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int at = min(at0 + u * kFusedThreads, size - 1);
-                v[u] = read1<G>(t.g, base + at);
-                if constexpr (MOM) w[u] = t.mom[base + at];
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (at0 + u * kFusedThreads >= size) break;
-                if constexpr (MOM) v[u] = l.nesterov ? l.one_minus_beta * (v[u] * gs) + l.beta * w[u] : w[u];
-                X[tall ? j * f.ldx + i : i * f.ldx + j] = __builtin_bit_cast(uint16_t, (_Float16)(float)(v[u] * inv));
-                i += rows_on;
-                j += cols_on;
-                if (j >= n) {
-                    j -= n;
-                    ++i;
-                }
+        for (int e = 0; e < 4; ++e) {
+            if (at + e < size) f4(e, X + (tall ? j * f.ldx + i : i * f.ldx + j));
+            if (++j == n) {
+                j = 0;
+                ++i;
             }
         }
+    };
+    const auto scale4 = [&](int at, const float (&v)[4]) {
+        walk(at, [&](int e, uint16_t* x) { *x = __builtin_bit_cast(uint16_t, (_Float16)(float)(v[e] * inv)); });
+    };
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+        if (i * kFusedThreads * 4 >= size) break;
+        scale4(first_of(i), u[i]);
+    }
+    for (int i = NG; i * kFusedThreads * 4 < size; ++i) {
+        float v[4], w[4];
+        load4(t.g, G{}, first_of(i), v);
+        if constexpr (MOM) {
+            // (as this thread wrote it)
+            load4(t.mom, float{}, first_of(i), w);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = l.nesterov ? l.one_minus_beta * (v[e] * gs) + l.beta * w[e] : w[e];
+        }
+        scale4(first_of(i), v);
     }
     __syncthreads();
     const auto frag = [&](const uint16_t* p) {
@@ -396,21 +443,49 @@ __global__ __launch_bounds__(kFusedThreads) void ortho_fused_kernel(OrthoList l,
         *reinterpret_cast<u32x2_t*>(p) = u32x2_t{pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3])};
     };
     for (int it = 0; it < q.iterations; ++it) {
-        for (int tile = wave; tile < tiles; tile += kFusedWaves) {
+        // A: up to two tiles of a row of tiles to a wave (their sums share fragments); with
+        // one or four tiles in all the waves share the sum over c instead
+        if (RT <= 2) {
+            const int tile = wave % tiles, share = kFusedWaves / tiles;
             const int ti = tile / RT, tj = tile - ti * RT;
             const uint16_t* const pa = X + (16 * ti + r16) * f.ldx + 8 * rho;
             const uint16_t* const pb = X + (16 * tj + r16) * f.ldx + 8 * rho;
-            f32x4_t acc[2] = {};
-            int k = 0;
-            for (; k + 64 < f.ldx; k += 64) {
-                acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(frag(pb + k), frag(pa + k), acc[0], 0, 0, 0);
-                acc[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(frag(pb + k + 32), frag(pa + k + 32), acc[1], 0, 0, 0);
-            }
-            if (k + 32 < f.ldx) acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(frag(pb + k), frag(pa + k), acc[0], 0, 0, 0);
-            float v[4];
+            f32x4_t acc = {};
+#pragma unroll 4
+            for (int k = wave / tiles * 32; k + 32 < f.ldx; k += 32 * share)
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(frag(pb + k), frag(pa + k), acc, 0, 0, 0);
+            sums[wave][lane] = acc;
+            __syncthreads();
+            if (wave < tiles) {
+                float v[4];
+                for (int w = wave + tiles; w < kFusedWaves; w += tiles) acc += sums[w][lane];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = (acc[0][e] + acc[1][e]) * q.alpha_a;
-            put(A + (16 * ti + r16) * f.lds + 16 * tj + 4 * rho, v);
+                for (int e = 0; e < 4; ++e) v[e] = acc[e] * q.alpha_a;
+                put(A + (16 * ti + r16) * f.lds + 16 * tj + 4 * rho, v);
+            }
+        } else {
+            // (3 x 3 or 4 x 4 tiles: 6 or 8 pairs, the third row's second tile left out)
+            const int ti = wave >> 1, tj = 2 * (wave & 1);
+            if (ti < RT) {
+                const bool two = tj + 1 < RT;
+                const uint16_t* const pa = X + (16 * ti + r16) * f.ldx + 8 * rho;
+                const uint16_t* const pb = X + (16 * tj + r16) * f.ldx + 8 * rho;
+                const uint16_t* const pc = two ? pb + 16 * f.ldx : pb;
+                f32x4_t acc[2] = {};
+#pragma unroll 4
+                for (int k = 0; k + 32 < f.ldx; k += 32) {
+                    const f16x8_t fa = frag(pa + k);
+                    acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(frag(pb + k), fa, acc[0], 0, 0, 0);
+                    acc[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(frag(pc + k), fa, acc[1], 0, 0, 0);
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = acc[h][e] * q.alpha_a;
+                    if (h == 0 || two) put(A + (16 * ti + r16) * f.lds + 16 * (tj + h) + 4 * rho, v);
+                }
+            }
         }
         __syncthreads();
         for (int tile = wave; tile < tiles; tile += kFusedWaves) {
@@ -432,10 +507,20 @@ __global__ __launch_bounds__(kFusedThreads) void ortho_fused_kernel(OrthoList l,
             put(S + i * f.lds + j, v);
         }
         __syncthreads();
-        // (rows past r16 are read as the last one's: S is 0 there)
+        // (S's fragments stay in registers; rows past r16 are read as the last one's: S is
+        // 0 there)
+        f16x8_t fs[2][kFusedSide / 16];
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int ti = 0; ti < kFusedSide / 16; ++ti)
+                if (ti < RT && ks < ks_s) fs[ks][ti] = frag(S + (16 * ti + r16) * f.lds + 32 * ks + 8 * rho);
+#pragma unroll 2
         for (int jb = wave; 16 * jb < c; jb += kFusedWaves) {
             f32x4_t acc[kFusedSide / 16] = {};
-            for (int ks = 0; ks < ks_s; ++ks) {
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                if (ks >= ks_s) break;
                 uint2 half[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -446,9 +531,7 @@ __global__ __launch_bounds__(kFusedThreads) void ortho_fused_kernel(OrthoList l,
                 const f16x8_t fb = __builtin_bit_cast(f16x8_t, w);
 #pragma unroll
                 for (int ti = 0; ti < kFusedSide / 16; ++ti)
-                    if (ti < RT)
-                        acc[ti] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb, frag(S + (16 * ti + r16) * f.lds + 32 * ks + 8 * rho),
-                                                                         acc[ti], 0, 0, 0);
+                    if (ti < RT) acc[ti] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb, fs[ks][ti], acc[ti], 0, 0, 0);
             }
 #pragma unroll
             for (int ti = 0; ti < kFusedSide / 16; ++ti) {
@@ -464,31 +547,48 @@ __global__ __launch_bounds__(kFusedThreads) void ortho_fused_kernel(OrthoList l,
     }
     const float unit = 1.0f / (1 << kScaleX), step = t.step * unit;
     float* const p = OUT == kOutMaster ? t.master : (float*)t.out;
-    int i = tid / n, j = tid - i * n;
-    for (int at0 = tid; at0 < size; at0 += U * kFusedThreads) {
-        float w[U] = {};
+    const auto give = [&](int at, float (&w)[4]) {
+        float x[4] = {};
+        walk(at, [&](int e, uint16_t* from) { x[e] = (float)__builtin_bit_cast(_Float16, *from); });
+        if (at >= size) return;
+        if constexpr (OUT == kOutBf16) {
+            uint16_t* const o = (uint16_t*)t.out + base + at;
+            if (t.wide) {
+                *reinterpret_cast<u32x2_t*>(o) = u32x2_t{pack_bf16x2(x[0] * unit, x[1] * unit), pack_bf16x2(x[2] * unit, x[3] * unit)};
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (at + e < size) o[e] = (uint16_t)f32_to_bf16_bits(x[e] * unit);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = __builtin_fmaf(-step, x[e], l.decay * w[e]);
+            store4(p, at, w);
+            if constexpr (OUT == kOutMaster) {
+                uint16_t* const o = (uint16_t*)t.out + base + at;
+                if (t.wide) {
+                    *reinterpret_cast<u32x2_t*>(o) = u32x2_t{pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3])};
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (at + e < size) o[e] = (uint16_t)f32_to_bf16_bits(w[e]);
+                }
+            }
+        }
+    };
+    for (int i0 = 0; i0 * kFusedThreads * 4 < size; i0 += NG) {
+        float w[NG][4];
         if constexpr (OUT != kOutBf16) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) w[u] = p[base + min(at0 + u * kFusedThreads, size - 1)];
+            for (int i = 0; i < NG; ++i) {
+                if ((i0 + i) * kFusedThreads * 4 >= size) break;
+                load4(p, float{}, first_of(i0 + i), w[i]);
+            }
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int at = at0 + u * kFusedThreads;
-            if (at >= size) break;
-            const float x = (float)__builtin_bit_cast(_Float16, X[tall ? j * f.ldx + i : i * f.ldx + j]);
-            if constexpr (OUT == kOutBf16) {
-                ((uint16_t*)t.out)[base + at] = (uint16_t)f32_to_bf16_bits(x * unit);
-            } else {
-                const float v = __builtin_fmaf(-step, x, l.decay * w[u]);
-                p[base + at] = v;
-                if constexpr (OUT == kOutMaster) ((uint16_t*)t.out)[base + at] = (uint16_t)f32_to_bf16_bits(v);
-            }
-            i += rows_on;
-            j += cols_on;
-            if (j >= n) {
-                j -= n;
-                ++i;
-            }
+        for (int i = 0; i < NG; ++i) {
+            if ((i0 + i) * kFusedThreads * 4 >= size) break;
+            give(first_of(i0 + i), w[i]);
         }
     }
 }
