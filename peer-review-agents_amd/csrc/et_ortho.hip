@@ -401,10 +401,28 @@ __global__ __launch_bounds__(kFusedThreads) void ortho_fused_kernel(OrthoList l,
     sum = 0.0;
 #pragma unroll
     for (int w = 0; w < kFusedWaves; ++w) sum += part[w];
+    // 2^14 / (|U| + eps) as the product of two binary32 factors, each of half its
+    // exponent: its own may pass their range
     const double inv = (double)(1 << kScaleX) / (sqrt(sum) + (double)l.eps);
-    // the place in X of element `at` of the matrix, and the step to the next
+    const double half_inv = sqrt(inv);
+    const float inv0 = (float)half_inv, inv1 = (float)(inv / (double)inv0);
+    // row and column of element `at` of the matrix
+    const float per_n = 1.0f / (float)n;
+    const auto place = [&](int at, int& i, int& j) {
+        i = (int)((float)at * per_n);         // (at < 2^17: one off at most)
+        j = at - i * n;
+        if (j < 0) {
+            j += n;
+            --i;
+        } else if (j >= n) {
+            j -= n;
+            ++i;
+        }
+    };
+    // f4(e, X's place) for the four elements from `at` on
     const auto walk = [&](int at, auto f4) {
-        int i = at / n, j = at - i * n;
+        int i, j;
+        place(at, i, j);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             if (at + e < size) f4(e, X + (tall ? j * f.ldx + i : i * f.ldx + j));
@@ -414,8 +432,17 @@ __global__ __launch_bounds__(kFusedThreads) void ortho_fused_kernel(OrthoList l,
             }
         }
     };
+    const bool lines = t.wide && !tall;       // four elements lie in one row of X
     const auto scale4 = [&](int at, const float (&v)[4]) {
-        walk(at, [&](int e, uint16_t* x) { *x = __builtin_bit_cast(uint16_t, (_Float16)(float)(v[e] * inv)); });
+        if (lines) {
+            if (at >= size) return;
+            int i, j;
+            place(at, i, j);
+            *reinterpret_cast<u32x2_t*>(X + i * f.ldx + j) =
+                u32x2_t{pack_f16x2(v[0] * inv0 * inv1, v[1] * inv0 * inv1), pack_f16x2(v[2] * inv0 * inv1, v[3] * inv0 * inv1)};
+        } else {
+            walk(at, [&](int e, uint16_t* x) { *x = __builtin_bit_cast(uint16_t, (_Float16)(v[e] * inv0 * inv1)); });
+        }
     };
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
@@ -549,8 +576,17 @@ __global__ __launch_bounds__(kFusedThreads) void ortho_fused_kernel(OrthoList l,
     float* const p = OUT == kOutMaster ? t.master : (float*)t.out;
     const auto give = [&](int at, float (&w)[4]) {
         float x[4] = {};
-        walk(at, [&](int e, uint16_t* from) { x[e] = (float)__builtin_bit_cast(_Float16, *from); });
         if (at >= size) return;
+        if (lines) {
+            int i, j;
+            place(at, i, j);
+            const u32x2_t d = *reinterpret_cast<const u32x2_t*>(X + i * f.ldx + j);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                x[e] = (float)__builtin_bit_cast(_Float16, (uint16_t)(e & 1 ? d[e >> 1] >> 16 : d[e >> 1] & 0xffffu));
+        } else {
+            walk(at, [&](int e, uint16_t* from) { x[e] = (float)__builtin_bit_cast(_Float16, *from); });
+        }
         if constexpr (OUT == kOutBf16) {
             uint16_t* const o = (uint16_t*)t.out + base + at;
             if (t.wide) {
