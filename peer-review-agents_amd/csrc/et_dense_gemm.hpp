@@ -29,7 +29,8 @@
 // bytes: s ^ 4 (r >> 1 & 1) ^ 2 (r >> 3 & 1)).  Either way the fragment reads spread over
 // all banks.
 //
-// A policy P has: a DenseTile's MI, NJ and kBlocks (per CU); kACol, kBCol, kF16; Args, Tile (with a GemmTile first), tiles(), tile(), b_row() and epilogue().
+// A policy P has: a DenseTile's MI, NJ and kBlocks (per CU); kACol, kBCol, kF16; kScratch, the
+// bytes of LDS that its epilogue has for a wave; Args, Tile (with a GemmTile first), tiles(), tile(), b_row() and epilogue().
 #pragma once
 
 #include <type_traits>
@@ -147,7 +148,7 @@ __global__ __launch_bounds__(kDenseThreads, P::kBlocks) void dense_gemm_kernel(t
     constexpr int NM = MI * NJ, NL = MI + NJ;                          // MFMAs a k-step, loads a wave and chunk
     constexpr int RPK = MI + NJ;                                       // fragments a k-step
     constexpr int Q1 = NM / 2;
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * kStage];
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * kStage + 4 * P::kScratch];
 
     const int lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -365,7 +366,7 @@ __global__ __launch_bounds__(kDenseThreads, P::kBlocks) void dense_gemm_kernel(t
         for (int i = 0; i < MI; ++i)
 #pragma unroll
             for (int j = 0; j < NJ; ++j) asm volatile("" : "+a"(acc[i][j]));
-        P::epilogue(g, cur, acc, wm, wn, r16, rho);
+        P::epilogue(g, cur, acc, wm, wn, r16, rho, smem + 2 * kStage + wave * P::kScratch);
         if (!more) break;
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll

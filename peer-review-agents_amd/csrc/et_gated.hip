@@ -65,6 +65,7 @@ struct GatedPolicy : DenseTile<KIND, 4> {
     using DenseTile<KIND, 4>::MI;
     using DenseTile<KIND, 4>::NJ;
     static constexpr bool kACol = false, kBCol = false, kF16 = false;
+    static constexpr int kScratch = 0;
     static constexpr int BM = 32 * MI, BH = 16 * NJ;      // rows and hidden units of a tile
     using Args = GatedArgs;
     struct Tile : GemmTile {
@@ -92,7 +93,7 @@ struct GatedPolicy : DenseTile<KIND, 4> {
         const int hid = t.n0 + R / (16 * NJ) * (8 * NJ) + tt % (NJ / 2) * 16 + (R & 15);
         return hid < g.F ? (tt >= NJ / 2 ? g.F + hid : hid) : -1;
     }
-    __device__ static void epilogue(const Args& g, const Tile& t, f32x4_t (&acc)[MI][NJ], int wm, int wn, int r16, int rho)
+    __device__ static void epilogue(const Args& g, const Tile& t, f32x4_t (&acc)[MI][NJ], int wm, int wn, int r16, int rho, unsigned char*)
     {
         const int F = g.F;
         const int width = BACKWARD ? 2 * F : F;
@@ -267,6 +268,7 @@ struct InputGradPolicy : DenseTile<KIND, 4> {
     using DenseTile<KIND, 4>::MI;
     using DenseTile<KIND, 4>::NJ;
     static constexpr bool kACol = false, kBCol = true, kF16 = false;
+    static constexpr int kScratch = 0;
     static constexpr int BM = 32 * MI, BN = 32 * NJ;
     using Args = InputGradArgs;
     struct Tile : GemmTile {
@@ -288,7 +290,7 @@ struct InputGradPolicy : DenseTile<KIND, 4> {
         t.k = 2 * g.F;
     }
     __device__ static int b_row(const Args&, const Tile&, int) { return -1; }
-    __device__ static void epilogue(const Args& g, const Tile& t, f32x4_t (&acc)[MI][NJ], int wm, int wn, int r16, int rho)
+    __device__ static void epilogue(const Args& g, const Tile& t, f32x4_t (&acc)[MI][NJ], int wm, int wn, int r16, int rho, unsigned char*)
     {
         const __amdgpu_buffer_rsrc_t res = dense_rsrc(g.dx + t.m0 * g.K, t.a_rows * g.K * 2);
 #pragma unroll
@@ -323,6 +325,7 @@ struct WeightGradPolicy : DenseTile<KIND, 4> {
     using DenseTile<KIND, 4>::MI;
     using DenseTile<KIND, 4>::NJ;
     static constexpr bool kACol = true, kBCol = true, kF16 = false;
+    static constexpr int kScratch = 0;
     static constexpr int BM = 32 * MI, BN = 32 * NJ;
     using Args = WeightGradArgs;
     struct Tile : GemmTile {
@@ -345,7 +348,7 @@ struct WeightGradPolicy : DenseTile<KIND, 4> {
         t.k = (int)min<int64_t>(g.step, g.T - k0);
     }
     __device__ static int b_row(const Args&, const Tile&, int) { return -1; }
-    __device__ static void epilogue(const Args& g, const Tile& t, f32x4_t (&acc)[MI][NJ], int wm, int wn, int r16, int rho)
+    __device__ static void epilogue(const Args& g, const Tile& t, f32x4_t (&acc)[MI][NJ], int wm, int wn, int r16, int rho, unsigned char*)
     {
         const int es = g.f32 ? 4 : 2;
         const int64_t first = ((int64_t)t.split * 2 * g.F + t.m0) * g.K;

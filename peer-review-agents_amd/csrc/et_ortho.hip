@@ -661,12 +661,16 @@ struct OrthoArgs {
 };
 static_assert(sizeof(OrthoArgs) <= 4096, "kernel arguments");
 
-template <int KIND, bool ACOL, bool BCOL, bool POLY>
+// SYM: A B^T is symmetric (X X^T, A A): the tiles on and above the diagonal are
+// computed and those above it written a second time, across it, by way of LDS.
+template <int KIND, bool ACOL, bool BCOL, bool POLY, bool SYM>
 struct OrthoPolicy : DenseTile<KIND, 2> {
     using DenseTile<KIND, 2>::MI;
     using DenseTile<KIND, 2>::NJ;
     static constexpr bool kACol = ACOL, kBCol = BCOL, kF16 = true;
     static constexpr int BM = 32 * MI, BN = 32 * NJ;
+    static constexpr int kLine = 16 * MI + 16;          // bytes of half of a wave's rows of a column, and 16
+    static constexpr int kScratch = SYM ? 32 * kLine : 0;
     using Args = OrthoArgs;
     struct Tile : GemmTile {
         int at, e, m0, n0;
@@ -677,9 +681,16 @@ struct OrthoPolicy : DenseTile<KIND, 2> {
         int i = 0;
         while (i + 1 < g.count && g.t[i + 1].first <= q) ++i;
         const OrthoGemm& p = g.t[i];
-        const int each = p.nm * p.nn;
+        const int each = SYM ? p.nm * (p.nm + 1) / 2 : p.nm * p.nn;
         const int e = (q - p.first) / each;
-        const TileAt at = tile_at(q - p.first - e * each, p.nm, p.nn, 8);
+        TileAt at;
+        if constexpr (SYM) {
+            at = {0, q - p.first - e * each};
+            for (; at.n >= p.nm - at.m; ++at.m) at.n -= p.nm - at.m;
+            at.n += at.m;
+        } else {
+            at = tile_at(q - p.first - e * each, p.nm, p.nn, 8);
+        }
         t.at = i;
         t.e = e;
         t.m0 = at.m * BM;
@@ -693,7 +704,8 @@ struct OrthoPolicy : DenseTile<KIND, 2> {
         t.k = p.K;
     }
     __device__ static int b_row(const Args&, const Tile&, int R) { return R; }
-    __device__ static void epilogue(const Args& g, const Tile& t, f32x4_t (&acc)[MI][NJ], int wm, int wn, int r16, int rho)
+    __device__ static void epilogue(const Args& g, const Tile& t, f32x4_t (&acc)[MI][NJ], int wm, int wn, int r16, int rho,
+                                    unsigned char* scratch)
     {
         const OrthoGemm& p = g.t[t.at];
         const int ldc = p.ldc;
@@ -701,37 +713,73 @@ struct OrthoPolicy : DenseTile<KIND, 2> {
         const __amdgpu_buffer_rsrc_t res = dense_rsrc(p.c + first, t.a_rows * ldc * 2);
         const __amdgpu_buffer_rsrc_t dres = dense_rsrc(POLY ? p.d + first : nullptr, t.a_rows * ldc * 2);
         const float alpha = g.alpha;
+        // the values of two tiles side by side, rows of tile i
+        const auto values = [&](int i, int j, const u32x2_t (&d)[2], float (&v)[8]) {
 #pragma unroll
-        for (int i = 0; i < MI; ++i) {
-            __builtin_amdgcn_sched_barrier(0);
-            const int row = (wm * MI + i) * 16 + r16;
-            u32x2_t d[NJ];
-            if constexpr (POLY) {
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) {
-                    const int col = t.n0 + (wn * NJ + j) * 16 + 4 * rho;
-                    d[j] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(
-                        dres, row < t.a_rows && col < ldc ? (uint32_t)(row * ldc + col) * 2u : kOOR, 0, 0));
+            for (int e = 0; e < 8; ++e) {
+                const int jj = j + (e >> 2);
+                v[e] = acc[i][jj][e & 3] * alpha;
+                if constexpr (POLY) {
+                    // (halves by a shift: as elements of a pair, hipcc 7.2 takes both words of the
+                    // load for the first)
+                    const uint32_t word = d[e >> 2][(e & 3) >> 1];
+                    const _Float16 w = __builtin_bit_cast(_Float16, (uint16_t)(e & 1 ? word >> 16 : word & 0xffffu));
+                    v[e] = __builtin_fmaf(g.beta, (float)w, v[e]);
+                    if (t.m0 + (wm * MI + i) * 16 + r16 == t.n0 + (wn * NJ + jj) * 16 + 4 * rho + (e & 3)) v[e] += g.gamma;
                 }
             }
+        };
+        const auto load_d = [&](int i, int j, u32x2_t (&d)[2]) {
+            const int row = (wm * MI + i) * 16 + r16;
 #pragma unroll
-            for (int j = 0; j < NJ; j += 2) {
+            for (int h = 0; h < 2; ++h) {
+                const int col = t.n0 + (wn * NJ + j + h) * 16 + 4 * rho;
+                d[h] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(
+                    dres, row < t.a_rows && col < ldc ? (uint32_t)(row * ldc + col) * 2u : kOOR, 0, 0));
+            }
+        };
+        // SYM, above the diagonal: 32 columns x half of the wave's rows also go through LDS, and
+        // from there to c as rows n0 + j, columns m0 .. (which are all there)
+        const __amdgpu_buffer_rsrc_t cres = dense_rsrc(SYM ? p.c + t.e * p.sc + (int64_t)t.n0 * ldc : nullptr, t.b_rows * ldc * 2);
+        const bool both = SYM && t.m0 != t.n0;
+        constexpr int HI = SYM ? MI / 2 : MI;
+#pragma unroll
+        for (int j = 0; j < NJ; j += 2) {
+#pragma unroll
+            for (int i0 = 0; i0 < MI; i0 += HI) {
                 __builtin_amdgcn_sched_barrier(0);
-                float v[8];
+                u32x2_t d[HI][2];
+                if constexpr (POLY) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int jj = j + (e >> 2);
-                    v[e] = acc[i][jj][e & 3] * alpha;
-                    if constexpr (POLY) {
-                        // (halves by a shift: as elements of a pair, hipcc 7.2 takes both words of the
-                        // load for the first)
-                        const uint32_t word = d[jj][(e & 3) >> 1];
-                        const _Float16 w = __builtin_bit_cast(_Float16, (uint16_t)(e & 1 ? word >> 16 : word & 0xffffu));
-                        v[e] = __builtin_fmaf(g.beta, (float)w, v[e]);
-                        if (t.m0 + row == t.n0 + (wn * NJ + jj) * 16 + 4 * rho + (e & 3)) v[e] += g.gamma;
+                    for (int i = 0; i < HI; ++i) load_d(i0 + i, j, d[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < HI; ++i) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    const int row = (wm * MI + i0 + i) * 16 + r16;
+                    float v[8];
+                    values(i0 + i, j, d[i], v);
+                    store_pair<true>(v, res, row < t.a_rows, (uint32_t)(row * ldc), t.n0 + (wn * NJ + j) * 16, ldc, rho);
+                    if (SYM && both) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            *reinterpret_cast<_Float16*>(scratch + (16 * (e >> 2) + 4 * rho + (e & 3)) * kLine + (16 * i + r16) * 2) = (_Float16)v[e];
                     }
                 }
-                store_pair<true>(v, res, row < t.a_rows, (uint32_t)(row * ldc), t.n0 + (wn * NJ + j) * 16, ldc, rho);
+                if (SYM && both) {
+                    constexpr int kSegs = 2 * HI, kLines = 64 / kSegs;      // 16-byte pieces of a line, lines a store
+                    const int lane = 16 * rho + r16;
+                    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                    for (int h = 0; h < 32 / kLines; ++h) {
+                        const int line = h * kLines + lane / kSegs, seg = lane % kSegs;
+                        const u32x4_t w = *reinterpret_cast<const u32x4_t*>(scratch + line * kLine + seg * 16);
+                        const int to = (wn * NJ + j) * 16 + line;
+                        __builtin_amdgcn_raw_buffer_store_b128(
+                            w, cres, to < t.b_rows ? (uint32_t)(to * ldc + t.m0 + (wm * MI + i0) * 16 + seg * 8) * 2u : kOOR, 0, 0);
+                    }
+                    __builtin_amdgcn_wave_barrier();
+                }
             }
         }
     }
@@ -740,22 +788,26 @@ struct OrthoPolicy : DenseTile<KIND, 2> {
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t round8(int64_t n) { return up(n, 8) * 8; }
 
-template <bool ACOL, bool BCOL, bool POLY>
+template <bool ACOL, bool BCOL, bool POLY, bool SYM>
 struct Products {
-    template <int KIND> using Policy = OrthoPolicy<KIND, ACOL, BCOL, POLY>;
+    template <int KIND> using Policy = OrthoPolicy<KIND, ACOL, BCOL, POLY, SYM>;
 };
 
 // Launches the products in `args` (nm, nn, first and tiles are set here).
-template <bool ACOL, bool BCOL, bool POLY>
+template <bool ACOL, bool BCOL, bool POLY, bool SYM>
 int launch_products(OrthoArgs& args, const int64_t* batch, hipStream_t s)
 {
     const int cus = dense_cus();
     int64_t big = 0, small = 0, thin = 0;
+    const auto tiles = [](const OrthoGemm& p, int64_t side) {
+        const int64_t m = up(p.M, side), n = up(p.N, side);
+        return SYM ? m * (m + 1) / 2 : m * n;
+    };
     for (int i = 0; i < args.count; ++i) {
         const OrthoGemm& p = args.t[i];
-        big += batch[i] * up(p.M, 256) * up(p.N, 256);
-        small += batch[i] * up(p.M, 128) * up(p.N, 128);
-        thin += batch[i] * up(p.M, 64) * up(p.N, 64);
+        big += batch[i] * tiles(p, 256);
+        small += batch[i] * tiles(p, 128);
+        thin += batch[i] * tiles(p, 64);
     }
     const int kind = dense_kind(big, small, thin, false, cus), side = kind == kTileBig ? 256 : kind == kTileSmall ? 128 : 64;
     args.tiles = 0;
@@ -764,9 +816,9 @@ int launch_products(OrthoArgs& args, const int64_t* batch, hipStream_t s)
         p.nm = (int)up(p.M, side);
         p.nn = (int)up(p.N, side);
         p.first = args.tiles;
-        args.tiles += (int)batch[i] * p.nm * p.nn;
+        args.tiles += (int)(batch[i] * tiles(p, side));
     }
-    return launch_dense<Products<ACOL, BCOL, POLY>::template Policy>(args, kind, args.tiles, cus, s, "ortho_products");
+    return launch_dense<Products<ACOL, BCOL, POLY, SYM>::template Policy>(args, kind, args.tiles, cus, s, "ortho_products");
 }
 
 // --------------------------------------------------------------------------
@@ -914,7 +966,7 @@ int run_set(const OrthoCall& call, OrthoList list, const int64_t* index, unsigne
             p.ldc = ldr;
         });
         args.alpha = alpha_a;
-        int rc = tall ? launch_products<true, true, false>(args, batch, s) : launch_products<false, false, false>(args, batch, s);
+        int rc = tall ? launch_products<true, true, false, true>(args, batch, s) : launch_products<false, false, false, true>(args, batch, s);
         if (rc) return rc;
         fill([&](OrthoGemm& p, int i, const Shape&, int r, int ldr, int) {
             p.a = p.b = p.d = ga[i];
@@ -926,7 +978,7 @@ int run_set(const OrthoCall& call, OrthoList list, const int64_t* index, unsigne
         args.alpha = alpha_s;
         args.beta = beta_s;
         args.gamma = gamma_s;
-        rc = launch_products<false, false, true>(args, batch, s);
+        rc = launch_products<false, false, true, true>(args, batch, s);
         if (rc) return rc;
         fill([&](OrthoGemm& p, int i, const Shape& sh, int r, int ldr, int ldx) {
             // wide: S X, X read down its columns; tall: X S, S symmetric
@@ -944,7 +996,7 @@ int run_set(const OrthoCall& call, OrthoList list, const int64_t* index, unsigne
             p.ldc = ldx;
         });
         args.alpha = alpha_x;
-        rc = tall ? launch_products<false, false, false>(args, batch, s) : launch_products<false, true, false>(args, batch, s);
+        rc = tall ? launch_products<false, false, false, false>(args, batch, s) : launch_products<false, true, false, false>(args, batch, s);
         if (rc) return rc;
         for (int i = 0; i < count; ++i) std::swap(x[i], y[i]);
     }
