@@ -141,21 +141,23 @@ __device__ __forceinline__ TileAt tile_at(int q, int nm, int nn, int gm)
 }
 
 template <class P>
-__global__ __launch_bounds__(kDenseThreads, P::kBlocks) void dense_gemm_kernel(typename P::Args g)
+constexpr int kDenseLds = 2 * (P::MI + P::NJ) * 4096 + 4 * P::kScratch;
+
+// Block `block` of `blocks` (a multiple of 8) goes through its tiles.
+template <class P>
+__device__ __forceinline__ void dense_tiles(const typename P::Args& g, unsigned char* smem, int block, int blocks)
 {
     constexpr int MI = P::MI, NJ = P::NJ;
     constexpr int kA = MI * 4096, kB = NJ * 4096, kStage = kA + kB;    // a chunk's bytes
     constexpr int NM = MI * NJ, NL = MI + NJ;                          // MFMAs a k-step, loads a wave and chunk
     constexpr int RPK = MI + NJ;                                       // fragments a k-step
     constexpr int Q1 = NM / 2;
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * kStage + 4 * P::kScratch];
-
     const int lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int r16 = lane & 15, rho = lane >> 4;
     const int wm = wave >> 1, wn = wave & 1;
     const int Q = P::tiles(g), per = (Q + 7) / 8;
-    const int nloc = (int)(gridDim.x / 8), xcd = (int)(blockIdx.x & 7);
+    const int nloc = blocks / 8, xcd = block & 7;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_t*)smem;
     const int seg0 = (lane & 7) ^ (lane >> 3);
 
@@ -280,7 +282,7 @@ __global__ __launch_bounds__(kDenseThreads, P::kBlocks) void dense_gemm_kernel(t
     };
     const auto pin = [&]() { __builtin_amdgcn_sched_barrier(0); };
 
-    int l = (int)(blockIdx.x >> 3);
+    int l = block >> 3;
     bool more = setup(l, cur);
     if (!more) return;
     int par = 0;              // stage of chunk c: (c + par) & 1
@@ -389,6 +391,23 @@ __global__ __launch_bounds__(kDenseThreads, P::kBlocks) void dense_gemm_kernel(t
         cur = nxt;
         nk = nk1;
     }
+}
+
+template <class P>
+__global__ __launch_bounds__(kDenseThreads, P::kBlocks) void dense_gemm_kernel(typename P::Args g)
+{
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[kDenseLds<P>];
+    dense_tiles<P>(g, smem, (int)blockIdx.x, (int)gridDim.x);
+}
+
+// Two calls' tiles in one launch: the first `blocks` blocks have the first's.
+template <class P, class Q>
+__global__ __launch_bounds__(kDenseThreads, P::kBlocks) void dense_pair_kernel(typename P::Args p, typename Q::Args q, int blocks)
+{
+    static_assert(P::kBlocks == Q::kBlocks, "one shape");
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[kDenseLds<P> > kDenseLds<Q> ? kDenseLds<P> : kDenseLds<Q>];
+    if ((int)blockIdx.x < blocks) dense_tiles<P>(p, smem, (int)blockIdx.x, blocks);
+    else dense_tiles<Q>(q, smem, (int)blockIdx.x - blocks, (int)gridDim.x - blocks);
 }
 
 // Blocks of a launch: a multiple of 8 (the XCDs take them in turn), no more than

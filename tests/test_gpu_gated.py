@@ -181,6 +181,26 @@ def test_large_values_saturate_as_the_formula(et, dev):
         assert bool((dx[1] == 0).all()) and bool((dx[3] == 0).all())
 
 
+def test_gelu_over_its_range(et, dev):
+    """g Phi(g) of every bf16 g in [-13, 40], against erfc in float64: 2^-20 of the value and the
+    rounding to bf16 (below -13 the value is under 2^-120)."""
+    bits = torch.arange(1 << 16, device=dev, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    g = bits[torch.isfinite(bits.float()) & (bits.float() >= -13) & (bits.float() <= 40)]
+    x = torch.zeros(len(g), 8, device=dev, dtype=torch.bfloat16)
+    x[:, 0], x[:, 1] = g, 1
+    w = torch.zeros(16, 8, device=dev, dtype=torch.bfloat16)
+    w[:8, 0] = 1                    # the gates: g
+    w[8:, 1] = 1                    # up: 1
+    h = et.gated_linear(x, w, activation="gelu").double()
+    want = _act(g.double(), "gelu")[0][:, None]
+    off = (h - want).abs()
+    assert bool((off <= (HALF + 2.0 ** -20) * want.abs() + 2.0 ** -133).all()), (off / want.abs()).max().item()
+    # the slope: dx[:, 0] is the sum of 8 units' slopes, each rounded to bf16 (they are equal)
+    dx, _ = et.gated_linear_backward(torch.ones(len(g), 8, device=dev, dtype=torch.bfloat16), x, w, activation="gelu")
+    slope = _act(g.double(), "gelu")[1] * 8
+    assert bool(((dx[:, 0].double() - slope).abs() <= 2 * (HALF + 2.0 ** -20) * slope.abs() + 8 * 2.0 ** -22).all())
+
+
 @pytest.mark.parametrize("activation", ["silu", "gelu"])
 def test_gradients_against_differences(et, dev, activation):
     """The loss sum(h c) along a direction: the float64 formula's central difference against <dx, v> + <dw, z>."""
