@@ -29,8 +29,8 @@ constexpr float kRootHalf = 0.70710678118654752f, kInvRoot2Pi = 0.39894228040143
 // log2(erfc(x) exp(x^2) / u) for x in [0, 10], 5e-8 of erfc off (3e-7 in binary32), and
 // exp(-87) and below are 0.  The exponent's rounding error is taken out by an fma, so
 // the relative error is the same far out on the left, where 1 + erf would cancel.
-// (erfcf and expf, with a branch for each range, cost the 128 x 128 tiles of a forward 2.5
-// us of 24 and those of a backward 5 of 28 at 3001 x 1000 x 712.)
+// (Instead of erfcf and expf with their branches for each range: the backward's kernel of
+// projections 27.6 to 25.6 us at 3001 x 1000 x 712, the forward 24.2 to 24.0.)
 __device__ __forceinline__ float normal_distribution(float g, float& e)
 {
     const float a = __builtin_fminf(__builtin_fabsf(g), 16.0f);
@@ -480,8 +480,8 @@ int launch_gated(GatedArgs g, int act, bool backward, int kind, hipStream_t s)
                     : launch_dense<GeluFwd>(g, kind, tiles, cus, s, "gated_linear");
 }
 
-// Splits of dW's sum over the tokens: as many blocks as the GPU holds beside
-// `others`, a split of 512 tokens at least.
+// Splits of dW's sum over the tokens: a block takes its share of the chunks of 64 that
+// the launch has, of dW and of `others`, 8 chunks at least.
 struct Split {
     int kind, splits;
     int64_t step;
@@ -490,11 +490,10 @@ Split split_tokens(int64_t T, int64_t K, int64_t F, int64_t others = 0)
 {
     const int cus = dense_cus();
     if (up(2 * F, 256) * up(K, 256) * 4 >= 3 * cus) return {kTileBig, 1, T};
-    const int64_t tiles = up(2 * F, 128) * up(K, 128);
-    const int64_t most = std::max<int64_t>(1, (2 * cus - others) / tiles);
-    const int64_t step = std::max<int64_t>(512, up(up(T, most), 64) * 64);
-    const int64_t splits = std::max<int64_t>(1, up(T, step));
-    return {kTileSmall, (int)splits, step};
+    const int64_t tiles = up(2 * F, 128) * up(K, 128), chunks = std::max<int64_t>(1, up(T, 64));
+    const int64_t share = std::max<int64_t>(8, up(tiles * chunks + others, 2 * cus));
+    const int64_t step = up(chunks, std::max<int64_t>(1, up(chunks, share))) * 64;
+    return {kTileSmall, (int)std::max<int64_t>(1, up(T, step)), step};
 }
 
 }  // namespace
@@ -578,7 +577,7 @@ extern "C" int et_gated_linear_bwd(const void* dh, const void* x, int64_t x_stri
     if (rc) return rc;
     const int cus = dense_cus();
     const int kind = kind_of(rows, K);
-    const Split sp = split_tokens(rows, K, F, dx && kind != kTileBig ? up(rows, 128) * up(K, 128) : 0);
+    const Split sp = split_tokens(rows, K, F, dx && kind != kTileBig ? up(rows, 128) * up(K, 128) * up(2 * F, 64) : 0);
     InputGradArgs a = {};
     a.dp = dp;
     a.w = (const unsigned char*)w;
@@ -605,17 +604,23 @@ extern "C" int et_gated_linear_bwd(const void* dh, const void* x, int64_t x_stri
     };
     if (dx && dw && kind != kTileBig && sp.kind == kTileSmall) {
         // In one launch, where neither has tiles for the whole GPU: its tail is the other's
-        // work (3001 x 1000 x 712: 28 us for 18 and 19).
+        // work (3001 x 1000 x 712: 28 us for 18 and 19).  dW's blocks, which may be the
+        // longer ones, come first.
         const int64_t ta = lay_out(a, rows, K, kTileSmall), tb = lay_out(b, 2 * F, K, kTileSmall) * sp.splits;
-        const unsigned first = dense_grid(ta, 2, cus), second = dense_grid(tb, 2, cus);
-        dense_pair_kernel<InputGradPolicy<kTileSmall>, WeightGradPolicy<kTileSmall>>
-            <<<dim3(first + second), dim3(kDenseThreads), 0, s>>>(a, b, (int)first);
+        const unsigned first = dense_grid(tb, 2, cus), second = dense_grid(ta, 2, cus);
+        dense_pair_kernel<WeightGradPolicy<kTileSmall>, InputGradPolicy<kTileSmall>>
+            <<<dim3(first + second), dim3(kDenseThreads), 0, s>>>(b, a, (int)first);
         rc = check_launch("gated_gradients");
         if (rc) return rc;
     } else {
         if (dx) rc = launch_dense<InputGradPolicy>(a, kind, lay_out(a, rows, K, kind), cus, s, "gated_input_grad");
-        if (!rc && dw)
-            rc = launch_dense<WeightGradPolicy>(b, sp.kind, lay_out(b, 2 * F, K, sp.kind) * sp.splits, cus, s, "gated_weight_grad");
+        if (!rc && dw) {
+            const int64_t tiles = lay_out(b, 2 * F, K, sp.kind) * sp.splits;
+            const dim3 block(kDenseThreads), grid(dense_grid(tiles, sp.kind == kTileBig ? 1 : 2, cus));
+            if (sp.kind == kTileBig) dense_gemm_kernel<WeightGradPolicy<kTileBig>><<<grid, block, 0, s>>>(b);
+            else dense_gemm_kernel<WeightGradPolicy<kTileSmall>><<<grid, block, 0, s>>>(b);
+            rc = check_launch("gated_weight_grad");
+        }
         if (rc) return rc;
     }
     if (dw) {
