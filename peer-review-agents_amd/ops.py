@@ -30,12 +30,15 @@ Every eager kernel calls the C ABI of libetmoe.so through the functions of
     torch.ops.etmoe.layer_norm(x, weight, bias, eps)            -> (Y, mean, rstd)
     torch.ops.etmoe.add_layer_norm(x, residual, weight, bias, eps) -> (Y, sum, mean, rstd)
     torch.ops.etmoe.layer_norm_backward(dy, h, weight, mean, rstd, dsum) -> (dX, dweight, dbias)
+    torch.ops.etmoe.gated_linear(x, w, activation)              -> H [T, F]
+    torch.ops.etmoe.gated_linear_backward(dh, x, w, activation, need_dx, need_dw) -> (dX, dW)
 
 Gradients: dispatch -> dispatch_backward; combine -> combine_backward, with
 respect to yp, to the router logits (through the gates, which are the
 sigmoid scores at the routed pairs: dlogits) and to slot_gate (dgate);
 layer_norm and add_layer_norm -> layer_norm_backward, with respect to the rows,
-the weight and the bias (mean and rstd are marked as not differentiable).  The routing
+the weight and the bias (mean and rstd are marked as not differentiable);
+gated_linear -> gated_linear_backward, with respect to x and w.  The routing
 itself is piecewise constant and has no gradient.
 """
 from typing import Optional, Tuple
@@ -44,6 +47,7 @@ import torch
 from torch import Tensor
 
 from . import expert_threshold as _et
+from . import gated as _gated
 from . import norm as _norm
 
 Plan = Tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]
@@ -286,3 +290,46 @@ def _add_layer_norm_grad(ctx, dy, dsum, _dmean, _drstd):
 
 
 torch.library.register_autograd("etmoe::add_layer_norm", _add_layer_norm_grad, setup_context=_add_layer_norm_setup)
+
+
+# --------------------------------------------------------------------------- #
+# gated projection
+# --------------------------------------------------------------------------- #
+
+@torch.library.custom_op("etmoe::gated_linear", mutates_args=())
+def gated_linear(x: Tensor, w: Tensor, activation: str) -> Tensor:
+    """H = act(x Wg^T) * (x Wu^T)."""
+    return _gated.gated_linear(x, w, activation=activation)
+
+
+@gated_linear.register_fake
+def _gated_linear_fake(x, w, activation):
+    return x.new_empty(x.shape[0], w.shape[0] // 2)
+
+
+@torch.library.custom_op("etmoe::gated_linear_backward", mutates_args=())
+def gated_linear_backward(dh: Tensor, x: Tensor, w: Tensor, activation: str, need_dx: bool,
+                          need_dw: bool) -> Tuple[Tensor, Tensor]:
+    """(dX, dW), one that is not needed without rows."""
+    dx, dw = _gated.gated_linear_backward(dh, x, w, activation=activation, need_dx=need_dx, need_dw=need_dw)
+    return x.new_empty(0, x.shape[1]) if dx is None else dx, w.new_empty(0, w.shape[1]) if dw is None else dw
+
+
+@gated_linear_backward.register_fake
+def _gated_linear_backward_fake(dh, x, w, activation, need_dx, need_dw):
+    return x.new_empty(x.shape[0] if need_dx else 0, x.shape[1]), w.new_empty(w.shape[0] if need_dw else 0, w.shape[1])
+
+
+def _gated_setup(ctx, inputs, output):
+    x, w, ctx.activation = inputs
+    ctx.save_for_backward(x, w)
+
+
+def _gated_grad(ctx, dh):
+    x, w = ctx.saved_tensors
+    need_dx, need_dw, _ = ctx.needs_input_grad
+    dx, dw = torch.ops.etmoe.gated_linear_backward(dh.contiguous(), x, w, ctx.activation, need_dx, need_dw)
+    return dx if need_dx else None, dw if need_dw else None, None
+
+
+torch.library.register_autograd("etmoe::gated_linear", _gated_grad, setup_context=_gated_setup)

@@ -125,6 +125,20 @@ def test_large_tiles_of_the_backward(et, dev, T, K, F):
     _close(dw, want["dw"], "dw")
 
 
+@pytest.mark.parametrize("T,K,F", [(20001, 264, 72), (40000, 64, 16), (9000, 72, 200)])
+def test_long_sums_of_the_weight_gradient(et, dev, T, K, F):
+    """Many tokens for few weights: dW's sum split beside dx, which alone fills the GPU; and alone, whose
+    splits differ."""
+    print(f"gated long T={T} K={K} F={F}", flush=True)
+    x, w, dh = _inputs(dev, T, K, F)
+    want = _want(x, w, "silu", dh)
+    for need_dx in (True, False):
+        dx, dw = et.gated_linear_backward(dh, x, w, need_dx=need_dx)
+        _close(dw, want["dw"], "dw")
+        if need_dx:
+            _close(dx, want["dx"], "dx")
+
+
 def test_no_rows_and_wide_strides(et, dev):
     w = torch.randn(48, 64, device=dev).bfloat16()
     x = torch.empty(0, 64, device=dev, dtype=torch.bfloat16)
@@ -272,6 +286,26 @@ def test_streams_and_graph(et, dev):
         for a, b in zip((gh, gdx, gdw), want):
             assert torch.equal(a, b), rep
     del graph
+
+
+def test_operators(et, dev):
+    x, w, dh = (t.contiguous() for t in _inputs(dev, 20, 72, 40))
+    ops = torch.ops.etmoe
+    tests = ("test_schema", "test_faketensor", "test_autograd_registration")
+    torch.library.opcheck(ops.gated_linear.default, (x.clone().requires_grad_(), w.clone().requires_grad_(), "gelu"),
+                          test_utils=tests)
+    for need in ((True, True), (False, True), (True, False)):
+        torch.library.opcheck(ops.gated_linear_backward.default, (dh, x, w, "silu", *need),
+                              test_utils=("test_schema", "test_faketensor"))
+    a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+
+    def f(a, b):
+        return ops.gated_linear(a, b, "silu").float().square().sum()
+
+    f(a, b).backward()
+    c, d = x.clone().requires_grad_(), w.clone().requires_grad_()
+    torch.compile(f, fullgraph=True, backend="aot_eager")(c, d).backward()
+    assert torch.equal(a.grad, c.grad) and torch.equal(b.grad, d.grad)
 
 
 def test_refusals(et, dev):
