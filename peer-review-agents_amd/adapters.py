@@ -15,7 +15,7 @@ from .expert_threshold import _call, _require, _require_workspace
 from .norm import _require_rows
 
 
-@dataclass
+@dataclass(frozen=True)
 class AdapterBank:
     """The adapters of one projection: a bf16 [n, rank, K], b bf16 [n, N, rank] and
     a float32 scale [n] (alpha / rank); adapter i adds scale[i] * b[i] @ (a[i] @ x).
@@ -55,7 +55,7 @@ class AdapterBank:
         return self.a.device
 
 
-@dataclass
+@dataclass(frozen=True)
 class AdapterPlan:
     """A batch's tokens sorted by adapter (:func:`adapter_plan`): ``order`` [T], and
     ``items``, of which the first ``num_items`` [1] are valid."""
@@ -65,6 +65,18 @@ class AdapterPlan:
     num_items: torch.Tensor
     num_tokens: int
     num_adapters: int
+
+    def __post_init__(self) -> None:
+        most = int(lib().et_adapter_plan_items(self.num_tokens, self.num_adapters))
+        if most < 0:
+            raise ValueError(f"no plan of {self.num_tokens} tokens and {self.num_adapters} adapters")
+        _require(self.order, "order", torch.int32, 1)
+        _require(self.items, "items", torch.int32, 2, self.order.device)
+        _require(self.num_items, "num_items", torch.int32, 1, self.order.device)
+        if (self.order.shape[0] != self.num_tokens or self.items.shape[0] < most or self.items.shape[1] != 4
+                or self.num_items.shape[0] != 1 or self.items.data_ptr() % 16):
+            raise ValueError(f"a plan of {self.num_tokens} tokens and {self.num_adapters} adapters needs order "
+                             f"[{self.num_tokens}], 16-byte aligned items [{most}, 4] and num_items [1]")
 
     @property
     def device(self) -> torch.device:

@@ -4,7 +4,7 @@
 //   out[t] = y[t] + scale[i] B_i (A_i x[t]),   i = index[t]   (no adapter: out = y)
 //
 // A plan sorts the tokens by adapter once for all projections of a step: items of up
-// to 16 or 32 tokens of one adapter, so that every item is a pair of small matrix
+// to 16 or 64 tokens of one adapter, so that every item is a pair of small matrix
 // products.  Two launches a projection:
 //   shrink  v = scale_i A_i x of an item's tokens: the sum over K split over the
 //           waves of a block, and over blocks where there are few items;
@@ -267,7 +267,7 @@ __global__ __launch_bounds__(kThreads) void adapter_expand_kernel(AdapterArgs g)
     const int lane = lane_id(), wave = (int)threadIdx.x >> 6;
     const int r16 = lane & 15, rho = lane >> 4;
     int n0 = (int)(blockIdx.x - (uint32_t)item * g.col_blocks) * g.chunks * (64 * kWaves) + wave * 64;
-    if (n0 >= g.N || (it.adapter < 0 && g.out == g.y)) return;
+    if (n0 >= g.N || (it.adapter < 0 && g.out == g.y && g.ldo == g.ldy)) return;
     const int segs = g.r / 8;
     // this lane's rows of y (8 q + lane / 8), and its 8 columns
     const int line = 8 * (lane & 7);

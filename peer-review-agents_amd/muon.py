@@ -99,7 +99,7 @@ def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients=MUON_COEFFICI
         X = g / (|g| + eps);  ``steps`` times  A = X X^T,  X = (a + b A + c A A) X
 
     (over the shorter side), which leaves g's singular vectors and brings its
-    singular values near 1.  bf16, of g's shape.  Held in f16 between the
+    singular values near 1.  bf16, of g's shape; ``out`` may be a bf16 g itself.  Held in f16 between the
     products, with binary32 sums: 0.1 to 0.2% off in norm.  A zero matrix gives
     zero, a matrix with a value that is not finite NaN.
     """
@@ -150,15 +150,18 @@ def _check_update(update_rms) -> None:
 
 def _step(dev, params, grads, momenta, masters, shapes, step_sizes, scalars, grad_scale, workspace) -> None:
     """The library calls of one step, its lists checked."""
-    for at in _kinds(params, grads):
-        def take(ts):
-            return ts if at is None else [ts[i] for i in at]
-        p, g = take(params), take(grads)
-        sh = take(shapes)
-        ws = _workspace(sh, workspace, dev)
+    kinds = list(_kinds(params, grads))
+
+    def take(ts, at):
+        return ts if at is None else [ts[i] for i in at]
+
+    # (all workspaces before the first call, which a refusal would leave half a step behind)
+    spaces = [_workspace(take(shapes, at), workspace, dev) for at in kinds]
+    for at, ws in zip(kinds, spaces):
+        p, g, sh = take(params, at), take(grads, at), take(shapes, at)
         low = p[0].dtype == torch.bfloat16
-        _call("et_muon", dev, _pointers(p), _pointers(g), _pointers(take(momenta)), _pointers(take(masters)) if low else None,
-              (ctypes.c_float * len(p))(*take(step_sizes)), _shape_array(sh), len(p), _DTYPES[p[0].dtype],
+        _call("et_muon", dev, _pointers(p), _pointers(g), _pointers(take(momenta, at)), _pointers(take(masters, at)) if low else None,
+              (ctypes.c_float * len(p))(*take(step_sizes, at)), _shape_array(sh), len(p), _DTYPES[p[0].dtype],
               _DTYPES[g[0].dtype], scalars, _vp(grad_scale), _vp(ws), ws.numel() * ws.element_size())
 
 

@@ -175,6 +175,25 @@ def test_beside_a_shared_4_bit_projection(et, dev):
     assert torch.equal(other[1], out)
 
 
+def test_a_plan_of_other_tensors(et, dev):
+    """What a plan is made of is checked where it is made, and neither it nor a bank can be changed after that."""
+    index = torch.zeros(5, dtype=torch.int32, device=dev)
+    plan = et.adapter_plan(index, 3)
+    good = dict(order=plan.order, items=plan.items, num_items=plan.num_items, num_tokens=5, num_adapters=3)
+    et.AdapterPlan(**good)
+    for bad in (dict(order=plan.order[:4]), dict(items=plan.items[:1]), dict(items=plan.items.view(-1, 2)), dict(num_tokens=500),
+                dict(items=torch.zeros(9, 5, dtype=torch.int32, device=dev)), dict(num_adapters=4000, num_tokens=6),
+                dict(num_items=plan.order), dict(num_items=plan.num_items.cpu())):
+        with pytest.raises(ValueError):
+            et.AdapterPlan(**{**good, **bad})
+    with pytest.raises(TypeError):
+        et.AdapterPlan(**{**good, "order": plan.order.long()})
+    bank = _bank(et, dev, 3, 16, 64, 72)
+    for thing, name in ((plan, "order"), (bank, "a")):
+        with pytest.raises(AttributeError):
+            setattr(thing, name, getattr(thing, name)[:1])
+
+
 def test_refusals(et, dev):
     bank = _bank(et, dev, 3, 16, 64, 72)
     x, y, index = _batch(dev, 5, 64, 72, 3)

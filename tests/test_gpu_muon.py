@@ -229,6 +229,25 @@ def test_graph_and_stream(et, dev):
     del graph
 
 
+@pytest.mark.parametrize("E,m,n", [(3, 16, 200), (2, 130, 264), (1, 300, 72)])
+def test_in_place(et, dev, E, m, n):
+    g = torch.randn(E, m, n, device=dev).bfloat16()
+    want = et.orthogonalize(g)
+    assert et.orthogonalize(g, out=g) is g and torch.equal(g, want)
+
+
+def test_a_refused_workspace_leaves_every_kind_as_it_was(et, dev):
+    """float32 and bfloat16 tensors are two calls: a workspace that is too small for the second one is
+    refused before the first."""
+    p = [torch.randn(16, 64, device=dev), torch.randn(200, 264, device=dev).bfloat16()]
+    masters, momenta = [None, p[1].float()], [torch.zeros_like(t, dtype=torch.float32) for t in p]
+    before = [t.clone() for t in p]
+    with pytest.raises(ValueError, match="workspace"):
+        et.muon_step_(p, [torch.ones_like(t) for t in p], momenta, lr=0.1, masters=masters,
+                      workspace=torch.empty(256, dtype=torch.uint8, device=dev))
+    assert all(torch.equal(a, b) for a, b in zip(p, before)) and not any(m.any() for m in momenta)
+
+
 def test_refusals(et, dev):
     g = torch.randn(2, 8, 16, device=dev)
     for bad in (dict(g=g.double()), dict(out=torch.empty(2, 8, 16, device=dev))):
