@@ -10,11 +10,11 @@
 //
 // Tiling.  A block of 2 x 2 waves owns a tile of 32 MI x 32 NJ; a wave owns
 // MI x NJ tiles of v_mfma_f32_16x16x32.  k advances in chunks of 64 through two
-// LDS stages filled by direct-to-LDS buffer loads.  Three shapes (TileKind): big,
+// LDS stages filled by direct-to-LDS buffer loads.  The shapes (TileKind): big,
 // 256 x 256, one block per CU, 16 fragment reads for 64 MFMAs, so LDS is read for
 // half of the MFMAs' time; small, 128 x 128, two blocks per CU, LDS reads as long as
-// the MFMAs, but four times as many tiles; thin, 64 x 128 or 64 x 64, for calls that
-// have few tiles all the same (dense_kind).
+// the MFMAs, but four times as many tiles; mid, 192 x 128, between them (for A along its
+// rows); thin, 64 x 128 or 64 x 64, for calls that have few tiles all the same (dense_kind).
 // A wave holds a whole chunk's fragments in registers, so a stage is free again
 // as soon as every wave has read it and two chunks stream in while one is
 // multiplied; loads and fragment reads are placed between MFMAs in a pinned
@@ -29,7 +29,7 @@
 // bytes: s ^ 4 (r >> 1 & 1) ^ 2 (r >> 3 & 1)).  Either way the fragment reads spread over
 // all banks.
 //
-// A policy P has: a DenseTile's MI, NJ and kBlocks (per CU); kACol, kBCol, kF16; kScratch, the
+// A policy P has: a DenseTile's MI, NJ and kBlocks (per CU); kACol, kBCol, kF16; kMid, whether it has mid tiles; kScratch, the
 // bytes of LDS that its epilogue has for a wave; Args, Tile (with a GemmTile first), tiles(), tile(), b_row() and epilogue().
 #pragma once
 
@@ -45,12 +45,12 @@ typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 
 constexpr int kDenseThreads = 256;
 
-enum TileKind { kTileThin = 2, kTileSmall = 4, kTileBig = 8 };
+enum TileKind { kTileThin = 2, kTileSmall = 4, kTileMid = 6, kTileBig = 8 };
 
 // THIN: thin tiles are 64 x 32 THIN.
 template <int KIND, int THIN>
 struct DenseTile {
-    static constexpr int MI = KIND, NJ = KIND == kTileThin ? THIN : KIND;
+    static constexpr int MI = KIND, NJ = KIND == kTileThin ? THIN : KIND == kTileMid ? 4 : KIND;
     static constexpr int kBlocks = KIND == kTileBig ? 1 : 2;
 };
 
@@ -418,22 +418,28 @@ inline unsigned dense_grid(int64_t tiles, int blocks_per_cu, int cus)
     return (unsigned)std::max<int64_t>(8, std::min<int64_t>(held, (tiles + 7) / 8 * 8));
 }
 
-// The tile's shape for a call of so many tiles of each kind, by what their rounds
-// take.  In 1/100 of a chunk of two small tiles a CU (1.0 us): a big one 134, a small
-// one with a CU of its own 60, thin ones 71 and 48 (64 x 128) or 60 and 40 (64 x 64).
-// Measured at K = 2048 and 4096, SwiGLU forward: 192 small tiles 38 us, as 352 thin ones
-// 40; 96 small 38, 160 thin 32; 512 small 64, 128 big 89, 1024 thin 91; Newton-Schulz,
+// The tile's shape for a call of so many tiles of each kind (mid 0: a product without
+// them), by what their rounds take.  In 1/100 of a chunk of two small tiles a CU (1.0 us):
+// a big one 134, two mid ones 122 and one 74, a small one 60, thin ones 71 and 48 (64 x
+// 128) or 60 and 40 (64 x 64).  Measured at K = 2048 and 4096, SwiGLU forward: 192 small tiles
+// 40 us, as 128 mid ones 49, as 352 thin ones 41; 96 small 38, 160 thin 30; 512 small 68, 352
+// mid 79, 128 big 88, 1024 thin 91; 1056 small 79, 704 mid 69, 264 big 104.  Newton-Schulz,
 // five steps: 512 x 512 138 us small, 100 thin; 8 of them 153 and 126; 24 of 512 x 1024
 // 305 and 403.
-inline int dense_kind(int64_t big, int64_t small, int64_t thin, bool wide, int cus)
+inline int dense_kind(int64_t big, int64_t mid, int64_t small, int64_t thin, bool wide, int cus)
 {
     const auto rounds = [cus](int64_t tiles, int alone, int pair) {
         const int64_t full = tiles / (2 * cus), rest = tiles - full * 2 * cus;
         return full * pair + (rest == 0 ? 0 : rest <= cus ? alone : pair);
     };
-    const int64_t b = (big + cus - 1) / cus * 134, s = rounds(small, 60, 100);
-    const int64_t t = wide ? rounds(thin, 48, 71) : rounds(thin, 40, 60);
-    return b <= s && b <= t ? kTileBig : s <= t ? kTileSmall : kTileThin;
+    struct { int kind; int64_t cost; } best = {kTileBig, (big + cus - 1) / cus * 134};
+    const auto other = [&best](int kind, int64_t cost) {
+        if (cost < best.cost) best = {kind, cost};
+    };
+    if (mid) other(kTileMid, rounds(mid, 74, 122));
+    other(kTileSmall, rounds(small, 60, 100));
+    other(kTileThin, wide ? rounds(thin, 48, 71) : rounds(thin, 40, 60));
+    return best.kind;
 }
 
 // Launches POLICY<kind> on `tiles` tiles.
@@ -442,7 +448,9 @@ int launch_dense(const ARGS& g, int kind, int64_t tiles, int cus, hipStream_t s,
 {
     const dim3 block(kDenseThreads), grid(dense_grid(tiles, kind == kTileBig ? 1 : 2, cus));
     if (kind == kTileBig) dense_gemm_kernel<POLICY<kTileBig>><<<grid, block, 0, s>>>(g);
-    else if (kind == kTileSmall) dense_gemm_kernel<POLICY<kTileSmall>><<<grid, block, 0, s>>>(g);
+    else if (kind == kTileMid) {
+        if constexpr (POLICY<kTileMid>::kMid) dense_gemm_kernel<POLICY<kTileMid>><<<grid, block, 0, s>>>(g);
+    } else if (kind == kTileSmall) dense_gemm_kernel<POLICY<kTileSmall>><<<grid, block, 0, s>>>(g);
     else dense_gemm_kernel<POLICY<kTileThin>><<<grid, block, 0, s>>>(g);
     return check_launch(what);
 }

@@ -93,7 +93,7 @@ template <int KIND, int ACT, bool BACKWARD>
 struct GatedPolicy : DenseTile<KIND, 4> {
     using DenseTile<KIND, 4>::MI;
     using DenseTile<KIND, 4>::NJ;
-    static constexpr bool kACol = false, kBCol = false, kF16 = false;
+    static constexpr bool kACol = false, kBCol = false, kF16 = false, kMid = true;
     static constexpr int kScratch = 0;
     static constexpr int BM = 32 * MI, BH = 16 * NJ;      // rows and hidden units of a tile
     using Args = GatedArgs;
@@ -296,7 +296,7 @@ template <int KIND>
 struct InputGradPolicy : DenseTile<KIND, 4> {
     using DenseTile<KIND, 4>::MI;
     using DenseTile<KIND, 4>::NJ;
-    static constexpr bool kACol = false, kBCol = true, kF16 = false;
+    static constexpr bool kACol = false, kBCol = true, kF16 = false, kMid = true;
     static constexpr int kScratch = 0;
     static constexpr int BM = 32 * MI, BN = 32 * NJ;
     using Args = InputGradArgs;
@@ -353,7 +353,7 @@ template <int KIND>
 struct WeightGradPolicy : DenseTile<KIND, 4> {
     using DenseTile<KIND, 4>::MI;
     using DenseTile<KIND, 4>::NJ;
-    static constexpr bool kACol = true, kBCol = true, kF16 = false;
+    static constexpr bool kACol = true, kBCol = true, kF16 = false, kMid = false;
     static constexpr int kScratch = 0;
     static constexpr int BM = 32 * MI, BN = 32 * NJ;
     using Args = WeightGradArgs;
@@ -431,13 +431,14 @@ template <int KIND> using SiluBwd = GatedPolicy<KIND, ET_GATED_SILU, true>;
 template <int KIND> using GeluBwd = GatedPolicy<KIND, ET_GATED_GELU, true>;
 
 // Rows and columns of a kind's tiles.
-int rows_of(int kind) { return kind == kTileBig ? 256 : kind == kTileSmall ? 128 : 64; }
+int rows_of(int kind) { return kind == kTileBig ? 256 : kind == kTileMid ? 192 : kind == kTileSmall ? 128 : 64; }
 int cols_of(int kind) { return kind == kTileBig ? 256 : 128; }
 
 // The tiles of a product of m x n outputs.
 int kind_of(int64_t m, int64_t n)
 {
-    return dense_kind(up(m, 256) * up(n, 256), up(m, 128) * up(n, 128), up(m, 64) * up(n, 128), true, dense_cus());
+    return dense_kind(up(m, 256) * up(n, 256), up(m, 192) * up(n, 128), up(m, 128) * up(n, 128), up(m, 64) * up(n, 128), true,
+                      dense_cus());
 }
 
 int check_sizes(const char* fn, int64_t T, int64_t K, int64_t F, int64_t ldx, int act)

@@ -670,6 +670,7 @@ struct OrthoPolicy : DenseTile<KIND, 2> {
     static constexpr bool kACol = ACOL, kBCol = BCOL, kF16 = true;
     static constexpr int BM = 32 * MI, BN = 32 * NJ;
     static constexpr int kLine = 16 * MI + 16;          // bytes of half of a wave's rows of a column, and 16
+    static constexpr bool kMid = false;
     static constexpr int kScratch = SYM ? 32 * kLine : 0;
     using Args = OrthoArgs;
     struct Tile : GemmTile {
@@ -809,7 +810,7 @@ int launch_products(OrthoArgs& args, const int64_t* batch, hipStream_t s)
         small += batch[i] * tiles(p, 128);
         thin += batch[i] * tiles(p, 64);
     }
-    const int kind = dense_kind(big, small, thin, false, cus), side = kind == kTileBig ? 256 : kind == kTileSmall ? 128 : 64;
+    const int kind = dense_kind(big, 0, small, thin, false, cus), side = kind == kTileBig ? 256 : kind == kTileSmall ? 128 : 64;
     args.tiles = 0;
     for (int i = 0; i < args.count; ++i) {
         OrthoGemm& p = args.t[i];

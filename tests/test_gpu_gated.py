@@ -100,7 +100,7 @@ def test_forward_and_backward(et, dev, T, K, F, activation):
     assert torch.equal(dx, dx2) and torch.equal(dw, dw2)
 
 
-@pytest.mark.parametrize("side", [2, 4, 8])
+@pytest.mark.parametrize("side", [2, 4, 6, 8])
 @pytest.mark.parametrize("T,K,F", [(1, 8, 8), (5, 64, 24), (300, 72, 136), (513, 256, 520), (1100, 136, 40), (700, 328, 4104), (700, 136, 4104), (300, 64, 8200)])
 def test_all_tiles_of_the_forward(et, dev, T, K, F, side):
     print(f"gated tile {side} T={T} K={K} F={F}", flush=True)
@@ -113,9 +113,10 @@ def test_all_tiles_of_the_forward(et, dev, T, K, F, side):
     _close(h, _want(x, w, "silu")["h"], "h")
 
 
-@pytest.mark.parametrize("T,K,F", [(8200, 1088, 600), (150, 3584, 1800), (5000, 520, 2200)])
+@pytest.mark.parametrize("T,K,F", [(8200, 1088, 600), (150, 3584, 1800), (5000, 520, 2200), (3001, 72, 712), (3001, 1400, 72), (3003, 2824, 1408)])
 def test_large_tiles_of_the_backward(et, dev, T, K, F):
-    """Enough tiles for 256 x 256 ones in the recomputation, dx or dw, and a block that walks several."""
+    """Enough tiles for 192 x 128 or 256 x 256 ones in the recomputation, dx (alone too) or dw, and a block that
+    walks several."""
     print(f"gated large T={T} K={K} F={F}", flush=True)
     x, w, dh = _inputs(dev, T, K, F)
     want = _want(x, w, "silu", dh)
@@ -123,6 +124,7 @@ def test_large_tiles_of_the_backward(et, dev, T, K, F):
     dx, dw = et.gated_linear_backward(dh, x, w)
     _close(dx, want["dx"], "dx")
     _close(dw, want["dw"], "dw")
+    _close(et.gated_linear_backward(dh, x, w, need_dw=False)[0], want["dx"], "dx")
 
 
 @pytest.mark.parametrize("T,K,F", [(20001, 264, 72), (40000, 64, 16), (9000, 72, 200)])
