@@ -142,16 +142,24 @@ __global__ __launch_bounds__(kDenseThreads) void ortho_norm_kernel(OrthoList l)
             for (int j = 0; j < 8; ++j) sum += (double)v[j] * (double)v[j];
         }
     } else {
-        for (int i = 0; i < kChunk / kDenseThreads; ++i) {
+        // (all loads before the first sum, as above)
+        constexpr int N = kChunk / kDenseThreads;
+        float v[N], w[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int64_t at = base + min(at0 + i * kDenseThreads + (int)threadIdx.x, size - 1);
+            v[i] = read1<G>(t.g, at);
+            if constexpr (MOM) w[i] = t.mom[at];
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
             const int64_t at = at0 + i * kDenseThreads + (int)threadIdx.x;
             if (at >= size) break;
-            float v = read1<G>(t.g, base + at);
             if constexpr (MOM) {
-                float w = t.mom[base + at];
-                v = direction(l, v * scale, w);
-                t.mom[base + at] = w;
+                v[i] = direction(l, v[i] * scale, w[i]);
+                t.mom[base + at] = w[i];
             }
-            sum += (double)v * (double)v;
+            sum += (double)v[i] * (double)v[i];
         }
     }
     sum = block_sum(sum);
@@ -172,44 +180,52 @@ __global__ __launch_bounds__(kDenseThreads) void ortho_scale_kernel(OrthoList l)
         gs = *l.grad_scale;
         if (!(__builtin_fabsf(gs) < __builtin_inff())) return;
     }
+    // (With a momentum all of U is loaded first, on its way while the norm is summed: 64 x 512
+    // x 2048 f32, this and the last kernel 20 us less of 676 each.  A bf16 gradient alone is
+    // better taken piece by piece: 64 x 1024 x 2048 90 us, 112 at once.)
+    constexpr int N = kChunk / (8 * kDenseThreads);
+    const uint32_t row_segs = t.ldx / 8, segs = t.m * row_segs;
+    float v[N][8];
+    const auto load = [&](int i) {
+        const uint32_t seg = min(c * (kChunk / 8) + i * kDenseThreads + threadIdx.x, segs - 1);
+        const uint32_t row = seg / row_segs, col = (seg - row * row_segs) * 8;
+        const int64_t at = base + (int64_t)row * t.n + col;
+        float m[8];
+        if (t.wide) {
+            read8<G>(t.g, at, v[i]);
+            if constexpr (MOM) read8<float>(t.mom, at, m);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int64_t from = base + (int64_t)row * t.n + min(col + j, t.n - 1);
+                v[i][j] = read1<G>(t.g, from);
+                if constexpr (MOM) m[j] = t.mom[from];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if constexpr (MOM) v[i][j] = l.nesterov ? l.one_minus_beta * (v[i][j] * gs) + l.beta * m[j] : m[j];
+            if (col + j >= t.n) v[i][j] = 0.0f;
+        }
+    };
+    if constexpr (MOM) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) load(i);
+    }
     double sum = 0.0;
     for (uint32_t i = threadIdx.x; i < t.sums; i += kDenseThreads) sum += t.partial[(int64_t)e * t.sums + i];
     sum = block_sum(sum);
     // (in binary64: the norm of values near binary32's smallest or largest is in its range)
     const double inv = (double)(1 << kScaleX) / (sqrt(sum) + (double)l.eps);
-    const uint32_t row_segs = t.ldx / 8, segs = t.m * row_segs;
     uint16_t* const x = t.x + (int64_t)e * t.m * t.ldx;
 #pragma unroll
-    for (int i = 0; i < kChunk / (8 * kDenseThreads); ++i) {
+    for (int i = 0; i < N; ++i) {
         const uint32_t seg = c * (kChunk / 8) + i * kDenseThreads + threadIdx.x;
         if (seg >= segs) break;
-        const uint32_t row = seg / row_segs, col = (seg - row * row_segs) * 8;
-        const int64_t at = base + (int64_t)row * t.n + col;
-        float v[8];
-        if (t.wide) {
-            read8<G>(t.g, at, v);
-            if constexpr (MOM) {
-                float m[8];
-                read8<float>(t.mom, at, m);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = l.nesterov ? l.one_minus_beta * (v[j] * gs) + l.beta * m[j] : m[j];
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[j] = 0.0f;
-                if (col + j < t.n) {
-                    v[j] = read1<G>(t.g, at + j);
-                    if constexpr (MOM) {
-                        const float m = t.mom[at + j];
-                        v[j] = l.nesterov ? l.one_minus_beta * (v[j] * gs) + l.beta * m : m;
-                    }
-                }
-            }
-        }
+        if constexpr (!MOM) load(i);
         u32x4_t w;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = pack_f16x2((float)(v[2 * j] * inv), (float)(v[2 * j + 1] * inv));
+        for (int j = 0; j < 4; ++j) w[j] = pack_f16x2((float)(v[i][2 * j] * inv), (float)(v[i][2 * j + 1] * inv));
         *reinterpret_cast<u32x4_t*>(x + (int64_t)seg * 8) = w;
     }
 }
@@ -228,47 +244,58 @@ __global__ __launch_bounds__(kDenseThreads) void ortho_finish_kernel(OrthoList l
     const uint32_t row_segs = t.ldx / 8, segs = t.m * row_segs;
     const uint16_t* const x = t.x + (int64_t)e * t.m * t.ldx;
     const float unit = 1.0f / (1 << kScaleX), step = t.step * unit;
-#pragma unroll
-    for (int i = 0; i < kChunk / (8 * kDenseThreads); ++i) {
-        const uint32_t seg = c * (kChunk / 8) + i * kDenseThreads + threadIdx.x;
-        if (seg >= segs) break;
-        const uint32_t row = seg / row_segs, col = (seg - row * row_segs) * 8;
-        const int64_t at = base + (int64_t)row * t.n + col;
-        const f16x8_t v = *reinterpret_cast<const f16x8_t*>(x + (int64_t)seg * 8);
-        if constexpr (OUT == kOutBf16) {
+    float* const w = OUT == kOutMaster ? t.master : (float*)t.out;
+    constexpr int N = kChunk / (8 * kDenseThreads);
+    f16x8_t v[N];
+    float p[N][8];
+    int64_t at[N];
+    uint32_t cols[N];         // that there are; 0: none of the block's
+    const auto load = [&](int i) {
+        const uint32_t seg = c * (kChunk / 8) + i * kDenseThreads + threadIdx.x, held = min(seg, segs - 1);
+        const uint32_t row = held / row_segs, col = (held - row * row_segs) * 8;
+        cols[i] = seg < segs ? min(t.n - col, 8u) : 0u;
+        at[i] = base + (int64_t)row * t.n + col;
+        v[i] = *reinterpret_cast<const f16x8_t*>(x + (int64_t)held * 8);
+        if constexpr (OUT != kOutBf16) {
             if (t.wide) {
-                u32x4_t w;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = pack_bf16x2((float)v[2 * j] * unit, (float)v[2 * j + 1] * unit);
-                *reinterpret_cast<u32x4_t*>((uint16_t*)t.out + at) = w;
+                read8<float>(w, at[i], p[i]);
             } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (col + j < t.n) ((uint16_t*)t.out)[at + j] = (uint16_t)f32_to_bf16_bits((float)v[j] * unit);
+                for (int j = 0; j < 8; ++j) p[i][j] = w[at[i] + min((uint32_t)j, t.n - 1 - col)];
+            }
+        }
+    };
+    // (the loads of a parameter first, as in ortho_scale_kernel)
+    if constexpr (OUT != kOutBf16) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) load(i);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if constexpr (OUT == kOutBf16) load(i);
+        if (cols[i] == 0) break;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            p[i][j] = OUT == kOutBf16 ? (float)v[i][j] * unit : __builtin_fmaf(-step, (float)v[i][j], l.decay * p[i][j]);
+        if (t.wide) {
+            if constexpr (OUT != kOutBf16) {
+                f32x4_t* const q = reinterpret_cast<f32x4_t*>(w + at[i]);
+                q[0] = f32x4_t{p[i][0], p[i][1], p[i][2], p[i][3]};
+                q[1] = f32x4_t{p[i][4], p[i][5], p[i][6], p[i][7]};
+            }
+            if constexpr (OUT != kOutParam) {
+                u32x4_t o;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] = pack_bf16x2(p[i][2 * j], p[i][2 * j + 1]);
+                *reinterpret_cast<u32x4_t*>((uint16_t*)t.out + at[i]) = o;
             }
         } else {
-            float* const w = OUT == kOutMaster ? t.master : (float*)t.out;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (t.wide) {
-                    f32x4_t* const q = reinterpret_cast<f32x4_t*>(w + at) + h;
-                    f32x4_t p = *q;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) p[j] = __builtin_fmaf(-step, (float)v[4 * h + j], l.decay * p[j]);
-                    *q = p;
-                    if constexpr (OUT == kOutMaster)
-                        reinterpret_cast<u32x2_t*>((uint16_t*)t.out + at)[h] =
-                            u32x2_t{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3])};
-                } else {
-#pragma unroll
-                    for (int j = 4 * h; j < 4 * h + 4; ++j)
-                        if (col + j < t.n) {
-                            const float p = __builtin_fmaf(-step, (float)v[j], l.decay * w[at + j]);
-                            w[at + j] = p;
-                            if constexpr (OUT == kOutMaster) ((uint16_t*)t.out)[at + j] = (uint16_t)f32_to_bf16_bits(p);
-                        }
+            for (int j = 0; j < 8; ++j)
+                if ((uint32_t)j < cols[i]) {
+                    if constexpr (OUT != kOutBf16) w[at[i] + j] = p[i][j];
+                    if constexpr (OUT != kOutParam) ((uint16_t*)t.out)[at[i] + j] = (uint16_t)f32_to_bf16_bits(p[i][j]);
                 }
-            }
         }
     }
 }
@@ -786,6 +813,145 @@ struct OrthoPolicy : DenseTile<KIND, 2> {
     }
 };
 
+// The same products where there are few tiles, so that a call is its way from memory: a
+// block owns 32 x 32, its 8 waves take k's chunks of 64 in turn, each through a
+// ring of D stages of LDS of its own (no barriers), and their sums meet in LDS.  With k
+// up to 512 all of it is on its way at once: 512 x 512 4.2 us a product, 6.7 with 64 x 64 tiles.
+constexpr int kShortWaves = 8, kShortThreads = kShortWaves * kWave;
+
+template <bool ACOL, bool BCOL, bool POLY, bool SYM, int D>
+__global__ __launch_bounds__(kShortThreads) void ortho_short_kernel(OrthoArgs g)
+{
+    using P = OrthoPolicy<1, ACOL, BCOL, POLY, SYM>;
+    constexpr int kStageBytes = 8192, NI = 8, kLine = 40;      // f16 from a line of the result to the next
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[kShortWaves * D * kStageBytes];
+    const int per = (g.tiles + 7) / 8;
+    const int q = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3);
+    if (q >= g.tiles) return;
+    typename P::Tile t = {};
+    P::tile(g, q, t);
+    const OrthoGemm& p = g.t[t.at];
+    const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r16 = lane & 15, rho = lane >> 4;
+    // this thread's two values of the result: row, col and col + 1
+    const int part_of = tid >> 7, place = (tid >> 1) & 63;
+    const int row = 16 * (part_of >> 1) + (place & 15), col = 16 * (part_of & 1) + 4 * (place >> 4) + 2 * (tid & 1);
+    const int ldc = p.ldc;
+    const int64_t first = t.e * p.sc + (int64_t)t.m0 * ldc;
+    uint32_t d = 0;
+    if constexpr (POLY) {
+        if (row < t.a_rows && t.n0 + col < ldc) d = *reinterpret_cast<const uint32_t*>(p.d + first + (int64_t)row * ldc + t.n0 + col);
+    }
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_t*)smem + wave * (D * kStageBytes);
+    const int seg0 = (lane & 7) ^ (lane >> 3);
+    // a chunk of an operand in 4 KB: k along rows 32 lines of 128 bytes, swizzled as
+    // the large tiles'; k down columns 64 lines of 64 bytes, piece s of line r at slot
+    // s ^ 2 (r >> 3 & 1)
+    const auto load = [&](auto down, const unsigned char* from, int rows, int ld, int c, uint32_t lds) {
+        const int left = t.k - c * 64;
+        if constexpr (decltype(down)::value) {
+            const __amdgpu_buffer_rsrc_t res =
+                dense_rsrc(from + (int64_t)c * 128 * ld, left > 0 ? (min(64, left) - 1) * ld * 2 + ((rows + 7) & ~7) * 2 : 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                dense_dma(res, (uint32_t)((16 * i + (lane >> 2)) * 2 * ld + (((lane & 3) ^ (lane >> 4 & 2)) << 4)), 0u, lds + i * 1024);
+        } else {
+            const __amdgpu_buffer_rsrc_t res = dense_rsrc(from, (rows - 1) * ld * 2 + ((t.k + 7) & ~7) * 2);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int seg = seg0 ^ (i & 1);
+                dense_dma(res, seg * 8 < left ? (uint32_t)((8 * i + (lane >> 3)) * 2 * ld + c * 128 + seg * 16) : kOOR, 0u, lds + i * 1024);
+            }
+        }
+    };
+    const auto load_both = [&](int j, uint32_t lds) {
+        const int c = kShortWaves * j + wave;
+        load(std::bool_constant<ACOL>{}, t.a, t.a_rows, t.lda, c, lds);
+        load(std::bool_constant<BCOL>{}, t.b, t.b_rows, t.ldb, c, lds + 4096);
+    };
+    const int fkey = (lane & 7) ^ ((lane >> 3) & 1);
+    const int frow = (r16 >> 3) * 1024 + (lane & 7) * 128;
+    const int tin = (r16 >> 2) * 64 + ((r16 & 3) >> 1) * 16 + (r16 & 1) * 8;
+    const auto read = [&](auto down, const unsigned char* op, int tile, int ks) -> f16x8_t {
+        if constexpr (decltype(down)::value) {
+            const unsigned char* const at = op + (32 * ks + 8 * rho) * 64 + ((tile ^ (rho & 1)) << 5) + tin;
+            const uint2 lo = dense_read_tr(at), hi = dense_read_tr(at + 256);
+            return __builtin_bit_cast(f16x8_t, u32x4_t{lo.x, lo.y, hi.x, hi.y});
+        } else {
+            return __builtin_bit_cast(f16x8_t, *reinterpret_cast<const u32x4_t*>(op + tile * 2048 + frow + (((4 * ks + rho) ^ fkey) << 4)));
+        }
+    };
+    f32x4_t acc[2][2] = {};
+    const int turns = (t.k + kShortWaves * 64 - 1) / (kShortWaves * 64);
+#pragma unroll
+    for (int i = 0; i < D; ++i) load_both(i, lds0 + i * kStageBytes);
+    for (int j = 0, stage = 0; j < turns; ++j) {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * NI) : "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        const unsigned char* const at = smem + (wave * D + stage) * kStageBytes;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            f16x8_t fa[2], fb[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                fa[i] = read(std::bool_constant<ACOL>{}, at, i, ks);
+                fb[i] = read(std::bool_constant<BCOL>{}, at + 4096, i, ks);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) acc[i][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb[h], fa[i], acc[i][h], 0, 0, 0);
+        }
+        // (the reads above have ended; chunks past the end load nothing and keep the count)
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(0xC07F);      // lgkmcnt(0)
+        if (j + 1 < turns) load_both(j + D, lds0 + stage * kStageBytes);
+        stage = stage + 1 == D ? 0 : stage + 1;
+    }
+    dense_wait_barrier<0>();
+    f32x4_t* const part = reinterpret_cast<f32x4_t*>(smem);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) part[(wave * 4 + 2 * i + h) * kWave + lane] = acc[i][h];
+    __syncthreads();
+    float v[2] = {};
+#pragma unroll
+    for (int w = 0; w < kShortWaves; ++w) {
+        const float* const from = reinterpret_cast<const float*>(part) + ((w * 4 + part_of) * kWave + place) * 4 + 2 * (tid & 1);
+        v[0] += from[0];
+        v[1] += from[1];
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        v[e] *= g.alpha;
+        if constexpr (POLY) {
+            v[e] = __builtin_fmaf(g.beta, (float)__builtin_bit_cast(_Float16, (uint16_t)(e ? d >> 16 : d & 0xffffu)), v[e]);
+            if (t.m0 + row == t.n0 + col + e) v[e] += g.gamma;
+        }
+    }
+    // The result's lines, and those across the diagonal, by way of LDS (behind the sums).
+    const bool both = SYM && t.m0 != t.n0;
+    uint16_t* const line = reinterpret_cast<uint16_t*>(smem + kShortWaves * 4096);
+    const uint32_t pair = pack_f16x2(v[0], v[1]);
+    *reinterpret_cast<uint32_t*>(line + row * kLine + col) = pair;
+    if (both) {
+        line[(32 + col) * kLine + row] = (uint16_t)pair;
+        line[(33 + col) * kLine + row] = (uint16_t)(pair >> 16);
+    }
+    __syncthreads();
+    if (tid < (both ? 256 : 128)) {
+        const int to = tid >> 2, seg = (tid & 3) * 8;      // line 0 .. 63
+        const u32x4_t w = *reinterpret_cast<const u32x4_t*>(line + to * kLine + seg);
+        if (to < 32) {
+            if (to < t.a_rows && t.n0 + seg < ldc) *reinterpret_cast<u32x4_t*>(p.c + first + (int64_t)to * ldc + t.n0 + seg) = w;
+        } else if (to - 32 < t.b_rows) {
+            *reinterpret_cast<u32x4_t*>(p.c + t.e * p.sc + (int64_t)(t.n0 + to - 32) * ldc + t.m0 + seg) = w;
+        }
+    }
+}
+
 int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int64_t round8(int64_t n) { return up(n, 8) * 8; }
 
@@ -799,7 +965,7 @@ template <bool ACOL, bool BCOL, bool POLY, bool SYM>
 int launch_products(OrthoArgs& args, const int64_t* batch, hipStream_t s)
 {
     const int cus = dense_cus();
-    int64_t big = 0, small = 0, thin = 0;
+    int64_t big = 0, small = 0, thin = 0, few = 0, k = 0;
     const auto tiles = [](const OrthoGemm& p, int64_t side) {
         const int64_t m = up(p.M, side), n = up(p.N, side);
         return SYM ? m * (m + 1) / 2 : m * n;
@@ -809,16 +975,31 @@ int launch_products(OrthoArgs& args, const int64_t* batch, hipStream_t s)
         big += batch[i] * tiles(p, 256);
         small += batch[i] * tiles(p, 128);
         thin += batch[i] * tiles(p, 64);
+        few += batch[i] * tiles(p, 32);
+        k = std::max<int64_t>(k, p.K);
+    }
+    const auto lay_out = [&](int64_t side) {
+        args.tiles = 0;
+        for (int i = 0; i < args.count; ++i) {
+            OrthoGemm& p = args.t[i];
+            p.nm = (int)up(p.M, side);
+            p.nn = (int)up(p.N, side);
+            p.first = args.tiles;
+            args.tiles += (int)(batch[i] * tiles(p, side));
+        }
+    };
+    // One round of the short kernel's blocks.  Five steps, with it and without: 512 x 512 72
+    // and 102 us, 300 x 4000 127 and 194, 8 of 80 x 1000 64 and 83; two or four rounds would
+    // take 512 x 1024 89 to 84, but 2 of 128 x 2048 77 to 80 and 16 of 256 x 256 79 to 109.
+    if (few <= cus) {
+        lay_out(32);
+        const dim3 grid((unsigned)(up(args.tiles, 8) * 8)), block(kShortThreads);
+        if (k <= kShortWaves * 64) ortho_short_kernel<ACOL, BCOL, POLY, SYM, 1><<<grid, block, 0, s>>>(args);
+        else ortho_short_kernel<ACOL, BCOL, POLY, SYM, 2><<<grid, block, 0, s>>>(args);
+        return check_launch("ortho_short_kernel");
     }
     const int kind = dense_kind(big, 0, small, thin, false, cus), side = kind == kTileBig ? 256 : kind == kTileSmall ? 128 : 64;
-    args.tiles = 0;
-    for (int i = 0; i < args.count; ++i) {
-        OrthoGemm& p = args.t[i];
-        p.nm = (int)up(p.M, side);
-        p.nn = (int)up(p.N, side);
-        p.first = args.tiles;
-        args.tiles += (int)(batch[i] * tiles(p, side));
-    }
+    lay_out(side);
     return launch_dense<Products<ACOL, BCOL, POLY, SYM>::template Policy>(args, kind, args.tiles, cus, s, "ortho_products");
 }
 

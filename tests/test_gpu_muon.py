@@ -82,6 +82,22 @@ def test_orthogonalize(et, dev, E, m, n, dtype):
     assert torch.equal(et.orthogonalize(g[E - 1].contiguous()), got[E - 1]) or min(m, n) > 128
 
 
+@pytest.mark.parametrize("E,m,n", [(1, 65, 65), (1, 66, 512), (3, 72, 520), (1, 300, 1300), (1, 1300, 200), (1, 90, 4104), (2, 1031, 97), (1, 512, 512)])
+def test_products_of_few_tiles(et, dev, E, m, n):
+    """Tiles of 32 x 32: sums of one chunk, of a chunk for each wave, of several turns, and lines that end inside a tile.
+    The same bits again, beside other tensors."""
+    u = _gradient(dev, E, m, n, seed=3)
+    got = et.orthogonalize(u)
+    _check(got, u, "few")
+    assert torch.equal(got, et.orthogonalize(u))
+    p = [torch.zeros_like(u), torch.zeros(70, 330, device=dev)]
+    et.muon_step_(p, [u, torch.randn(70, 330, device=dev)], [torch.zeros_like(t) for t in p], lr=1.0, momentum=0.0, update_rms=None,
+                  nesterov=False)
+    size = max(1.0, m / n) ** 0.5
+    assert bool((torch.isfinite(p[0])).all())
+    _check(-p[0] / size, u, "beside others")
+
+
 @pytest.mark.parametrize("steps,abc", [(1, ABC), (3, ABC), (8, ABC), (10, (1.875, -1.25, 0.375)), (5, (1.5, -0.5, 0.0))])
 def test_other_polynomials(et, dev, steps, abc):
     g = _gradient(dev, 2, 96, 200, low_rank=False)
