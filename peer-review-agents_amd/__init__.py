@@ -3,9 +3,10 @@
 Import with ``importlib.import_module("peer-review-agents_amd")`` (the
 directory name is not a Python identifier).  Kernels live in csrc/ and are
 built into libetmoe.so by build.py; the host API is in expert_threshold.py (the
-dispatch path), norm.py (layer norm), optimizer.py (AdamW, the gradient norm)
-and w4.py (products with 4-bit weights), and ops.py registers
-the path as PyTorch operators (torch.ops.etmoe.*).
+dispatch path), norm.py (layer norm), optimizer.py (AdamW, the gradient norm),
+w4.py (products with 4-bit weights), gated.py (the gated projection of a dense
+expert), muon.py (orthogonalised steps of matrices) and adapters.py (low-rank
+adapters), and ops.py registers the path as PyTorch operators (torch.ops.etmoe.*).
 """
 from ._lib import BLOCK_HEADER_PATH, DENSE_HEADER_PATH, ETMoEError, LIB_PATH, header_symbols, lib  # noqa: F401
 from . import ops  # noqa: F401  (registers torch.ops.etmoe.*)

@@ -12,7 +12,9 @@
 //           numbers (16 bits of it; with rank 16 both fill one MFMA's k of 32), so
 //           the one rounding that counts is that of the result.
 // The bytes of x, y, out and the adapters in use bound both.  Which tokens share an item
-// changes no result: every sum runs within a token.
+// changes no result: every sum runs within a token.  Measured: 48 tokens, K = N = 4096, rank
+// 16, 64 adapters 4.3 + 4.2 us (two launches' latency; 8.7 MB); 8192 tokens, K = 4096, N =
+// 7168, rank 32, 24 adapters 14.9 + 48.4 us (4.6 and 4.9 TB/s of x, y and out).
 #include <algorithm>
 
 #include "et_dense_gemm.hpp"

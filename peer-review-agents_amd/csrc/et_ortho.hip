@@ -5,7 +5,8 @@
 //
 // (X X^T over the shorter side: for more rows than columns A = X^T X and X = X S.)
 // The matrices of many tensors go through one launch a product, each tile finding
-// its matrix in a table.
+// its matrix in a table.  64 matrices of 1024 x 2048: X X^T 172 us, S 129 (the tiles on and above
+// the diagonal alone), S X 268, 1.0, 0.67 and 1.03 PFLOP/s of what is computed.
 //
 // Number format.  X, A and S are held in f16 times fixed powers of two and
 // multiplied on the matrix units with binary32 sums.  The largest singular value
@@ -309,7 +310,7 @@ __global__ __launch_bounds__(kDenseThreads) void ortho_finish_kernel(OrthoList l
 // rows 16 bytes apart from a multiple of 64, so that 16 rows' segments fall on
 // all banks.  X = S X goes column by column: a wave replaces 16 columns of X by
 // their own product, in place.  The products above launch 17 kernels for the same
-// (three layers' routers and 8 experts of 512 x 64 and 32 x 512: 227 us).
+// (three layers' routers and 8 experts of 64 x 512 and 512 x 32: 227 us, here 41).
 constexpr int kFusedThreads = 512, kFusedWaves = kFusedThreads / kWave;
 constexpr int kFusedSide = 64;
 constexpr int kFusedSmall = 30 * 1024, kFusedLarge = 150 * 1024;     // bytes of LDS: four blocks a CU, or one
