@@ -26,6 +26,7 @@ namespace {
 
 constexpr int kScaleX = 14;                  // X and A are held times 2^14
 constexpr int kChunk = 4096;                 // elements a block of the elementwise kernels takes
+constexpr int64_t kSums = 1024;              // partial sums of a matrix's norm, which every block of the next kernel adds
 constexpr int kTensors = 20;                 // tensors of one launch
 
 float pow2(int e) { return std::ldexp(1.0f, e); }
@@ -119,48 +120,49 @@ __global__ __launch_bounds__(kDenseThreads) void ortho_norm_kernel(OrthoList l)
         if (!(__builtin_fabsf(scale) < __builtin_inff())) return;
     }
     double sum = 0.0;
-    const int64_t at0 = (int64_t)c * kChunk;
-    if (t.wide) {
+    for (int64_t at0 = (int64_t)c * kChunk; at0 < size; at0 += (int64_t)t.sums * kChunk) {
+        if (t.wide) {
 #pragma unroll
-        for (int i = 0; i < kChunk / (8 * kDenseThreads); ++i) {
-            const int64_t at = at0 + (i * kDenseThreads + (int)threadIdx.x) * 8;
-            if (at >= size) break;
-            float v[8];
-            read8<G>(t.g, base + at, v);
-            if constexpr (MOM) {
-                f32x4_t* const q = reinterpret_cast<f32x4_t*>(t.mom + base + at);
-                f32x4_t m[2] = {q[0], q[1]};
+            for (int i = 0; i < kChunk / (8 * kDenseThreads); ++i) {
+                const int64_t at = at0 + (i * kDenseThreads + (int)threadIdx.x) * 8;
+                if (at >= size) break;
+                float v[8];
+                read8<G>(t.g, base + at, v);
+                if constexpr (MOM) {
+                    f32x4_t* const q = reinterpret_cast<f32x4_t*>(t.mom + base + at);
+                    f32x4_t m[2] = {q[0], q[1]};
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    float w = m[j >> 2][j & 3];
-                    v[j] = direction(l, v[j] * scale, w);
-                    m[j >> 2][j & 3] = w;
+                    for (int j = 0; j < 8; ++j) {
+                        float w = m[j >> 2][j & 3];
+                        v[j] = direction(l, v[j] * scale, w);
+                        m[j >> 2][j & 3] = w;
+                    }
+                    q[0] = m[0];
+                    q[1] = m[1];
                 }
-                q[0] = m[0];
-                q[1] = m[1];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum += (double)v[j] * (double)v[j];
+            }
+        } else {
+            // (all loads before the first sum)
+            constexpr int N = kChunk / kDenseThreads;
+            float v[N], w[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int64_t at = base + min(at0 + i * kDenseThreads + (int)threadIdx.x, size - 1);
+                v[i] = read1<G>(t.g, at);
+                if constexpr (MOM) w[i] = t.mom[at];
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum += (double)v[j] * (double)v[j];
-        }
-    } else {
-        // (all loads before the first sum, as above)
-        constexpr int N = kChunk / kDenseThreads;
-        float v[N], w[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int64_t at = base + min(at0 + i * kDenseThreads + (int)threadIdx.x, size - 1);
-            v[i] = read1<G>(t.g, at);
-            if constexpr (MOM) w[i] = t.mom[at];
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int64_t at = at0 + i * kDenseThreads + (int)threadIdx.x;
-            if (at >= size) break;
-            if constexpr (MOM) {
-                v[i] = direction(l, v[i] * scale, w[i]);
-                t.mom[base + at] = w[i];
+            for (int i = 0; i < N; ++i) {
+                const int64_t at = at0 + i * kDenseThreads + (int)threadIdx.x;
+                if (at >= size) break;
+                if constexpr (MOM) {
+                    v[i] = direction(l, v[i] * scale, w[i]);
+                    t.mom[base + at] = w[i];
+                }
+                sum += (double)v[i] * (double)v[i];
             }
-            sum += (double)v[i] * (double)v[i];
         }
     }
     sum = block_sum(sum);
@@ -1014,8 +1016,8 @@ struct Shape {
     int64_t r() const { return std::min(m, n); }
     int64_t ldx() const { return round8(n); }
     int64_t ldr() const { return round8(r()); }
-    int64_t sums() const { return up(m * n, kChunk); }
-    int64_t blocks() const { return std::max(sums(), up(m * ldx(), kChunk)); }
+    int64_t sums() const { return std::min(up(m * n, kChunk), kSums); }
+    int64_t blocks() const { return up(m * ldx(), kChunk); }
     int64_t x_bytes() const { return up(E * m * ldx() * 2, 256) * 256; }
     int64_t a_bytes() const { return up(E * r() * ldr() * 2, 256) * 256; }
     int64_t sum_bytes() const { return up(E * sums() * 8, 256) * 256; }

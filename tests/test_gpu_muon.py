@@ -98,6 +98,17 @@ def test_products_of_few_tiles(et, dev, E, m, n):
     _check(-p[0] / size, u, "beside others")
 
 
+@pytest.mark.parametrize("m,n", [(2100, 2200), (1500, 5001)])
+def test_norm_of_many_elements(et, dev, m, n):
+    """More elements than the blocks of a norm take at once, whole rows of 16 bytes and not."""
+    u = _gradient(dev, 1, m, n, seed=4)
+    _check(et.orthogonalize(u), u, "large")
+    p, mom = torch.zeros_like(u), torch.zeros_like(u)
+    et.muon_step_([p], [u], [mom], lr=1.0, momentum=0.5, update_rms=None, nesterov=False)
+    assert torch.equal(mom, 0.5 * u)
+    _check(-p / max(1.0, m / n) ** 0.5, 0.5 * u, "large step")
+
+
 @pytest.mark.parametrize("steps,abc", [(1, ABC), (3, ABC), (8, ABC), (10, (1.875, -1.25, 0.375)), (5, (1.5, -0.5, 0.0))])
 def test_other_polynomials(et, dev, steps, abc):
     g = _gradient(dev, 2, 96, 200, low_rank=False)
