@@ -494,15 +494,16 @@ __global__ __launch_bounds__(kFusedThreads) void ortho_fused_kernel(OrthoList l,
     const auto frag = [&](const uint16_t* p) {
         return __builtin_bit_cast(f16x8_t, *reinterpret_cast<const u32x4_t*>(p));
     };
-    const int RT = f.r16 / 16, tiles = RT * RT, ks_s = (f.lds - 8) / 32;
     // four values of row i from column j on, rounded to f16
     const auto put = [&](uint16_t* p, const float (&v)[4]) {
         *reinterpret_cast<u32x2_t*>(p) = u32x2_t{pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3])};
     };
-    for (int it = 0; it < q.iterations; ++it) {
+    // One step, for matrices of RT tiles of 16 rows
+    const auto iterate = [&](auto rows) {
+        constexpr int RT = decltype(rows)::value, tiles = RT * RT, KS = (RT + 1) / 2;
         // A: up to two tiles of a row of tiles to a wave (their sums share fragments); with
         // one or four tiles in all the waves share the sum over c instead
-        if (RT <= 2) {
+        if constexpr (RT <= 2) {
             const int tile = wave % tiles, share = kFusedWaves / tiles;
             const int ti = tile / RT, tj = tile - ti * RT;
             const uint16_t* const pa = X + (16 * ti + r16) * f.ldx + 8 * rho;
@@ -548,7 +549,7 @@ __global__ __launch_bounds__(kFusedThreads) void ortho_fused_kernel(OrthoList l,
         for (int tile = wave; tile < tiles; tile += kFusedWaves) {
             const int ti = tile / RT, tj = tile - ti * RT;
             f32x4_t acc = {};
-            for (int ks = 0; ks < ks_s; ++ks)
+            for (int ks = 0; ks < KS; ++ks)
                 acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(frag(A + (16 * tj + r16) * f.lds + 32 * ks + 8 * rho),
                                                              frag(A + (16 * ti + r16) * f.lds + 32 * ks + 8 * rho), acc, 0, 0, 0);
             const int i = 16 * ti + r16, j = 16 * tj + 4 * rho;
@@ -566,18 +567,16 @@ __global__ __launch_bounds__(kFusedThreads) void ortho_fused_kernel(OrthoList l,
         __syncthreads();
         // (S's fragments stay in registers; rows past r16 are read as the last one's: S is
         // 0 there)
-        f16x8_t fs[2][kFusedSide / 16];
+        f16x8_t fs[KS][RT];
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-            for (int ti = 0; ti < kFusedSide / 16; ++ti)
-                if (ti < RT && ks < ks_s) fs[ks][ti] = frag(S + (16 * ti + r16) * f.lds + 32 * ks + 8 * rho);
+            for (int ti = 0; ti < RT; ++ti) fs[ks][ti] = frag(S + (16 * ti + r16) * f.lds + 32 * ks + 8 * rho);
 #pragma unroll 2
         for (int jb = wave; 16 * jb < c; jb += kFusedWaves) {
-            f32x4_t acc[kFusedSide / 16] = {};
+            f32x4_t acc[RT] = {};
 #pragma unroll
-            for (int ks = 0; ks < 2; ++ks) {
-                if (ks >= ks_s) break;
+            for (int ks = 0; ks < KS; ++ks) {
                 uint2 half[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -587,20 +586,24 @@ __global__ __launch_bounds__(kFusedThreads) void ortho_fused_kernel(OrthoList l,
                 const u32x4_t w = {half[0].x, half[0].y, half[1].x, half[1].y};
                 const f16x8_t fb = __builtin_bit_cast(f16x8_t, w);
 #pragma unroll
-                for (int ti = 0; ti < kFusedSide / 16; ++ti)
-                    if (ti < RT) acc[ti] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb, fs[ks][ti], acc[ti], 0, 0, 0);
+                for (int ti = 0; ti < RT; ++ti)
+                    acc[ti] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb, fs[ks][ti], acc[ti], 0, 0, 0);
             }
 #pragma unroll
-            for (int ti = 0; ti < kFusedSide / 16; ++ti) {
-                if (ti < RT) {
-                    float v[4];
+            for (int ti = 0; ti < RT; ++ti) {
+                float v[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = acc[ti][e] * q.alpha_x;
-                    put(X + (16 * ti + r16) * f.ldx + 16 * jb + 4 * rho, v);
-                }
+                for (int e = 0; e < 4; ++e) v[e] = acc[ti][e] * q.alpha_x;
+                put(X + (16 * ti + r16) * f.ldx + 16 * jb + 4 * rho, v);
             }
         }
         __syncthreads();
+    };
+    for (int it = 0; it < q.iterations; ++it) {
+        if (f.r16 == 16) iterate(std::integral_constant<int, 1>{});
+        else if (f.r16 == 32) iterate(std::integral_constant<int, 2>{});
+        else if (f.r16 == 48) iterate(std::integral_constant<int, 3>{});
+        else iterate(std::integral_constant<int, 4>{});
     }
     const float unit = 1.0f / (1 << kScaleX), step = t.step * unit;
     float* const p = OUT == kOutMaster ? t.master : (float*)t.out;
