@@ -338,6 +338,9 @@ struct FusedScalars {
     int iterations;
 };
 
+// How a matrix's elements go by fours: in a row of X, down a column of it, one by one.
+enum { kLines = 0, kTall = 1, kOdd = 2 };
+
 template <typename G, bool MOM, int OUT, int LDS_BYTES>
 __global__ __launch_bounds__(kFusedThreads) void ortho_fused_kernel(OrthoList l, FusedScalars q)
 {
@@ -361,9 +364,9 @@ __global__ __launch_bounds__(kFusedThreads) void ortho_fused_kernel(OrthoList l,
     uint16_t* const A = X + f.r16 * f.ldx;
     uint16_t* const S = A + f.r16 * f.lds;
     // Elements go by groups of four, group tid + 512 i to a thread.
-    const auto load4 = [&](const void* p, auto type, int at, float (&v)[4]) {
+    const auto load4 = [&](auto mode, const void* p, auto type, int at, float (&v)[4]) {
         using T = decltype(type);
-        if (t.wide) {
+        if constexpr (decltype(mode)::value != kOdd) {
             if constexpr (sizeof(T) == 4) {
                 const f32x4_t w = *reinterpret_cast<const f32x4_t*>((const float*)p + base + min(at, size - 4));
 #pragma unroll
@@ -378,8 +381,8 @@ __global__ __launch_bounds__(kFusedThreads) void ortho_fused_kernel(OrthoList l,
             for (int e = 0; e < 4; ++e) v[e] = read1<T>(p, base + min(at + e, size - 1));
         }
     };
-    const auto store4 = [&](float* p, int at, const float (&v)[4]) {
-        if (t.wide) {
+    const auto store4 = [&](auto mode, float* p, int at, const float (&v)[4]) {
+        if constexpr (decltype(mode)::value != kOdd) {
             *reinterpret_cast<f32x4_t*>(p + base + at) = f32x4_t{v[0], v[1], v[2], v[3]};
         } else {
 #pragma unroll
@@ -388,54 +391,6 @@ __global__ __launch_bounds__(kFusedThreads) void ortho_fused_kernel(OrthoList l,
         }
     };
     const auto first_of = [&](int group) { return (group * kFusedThreads + tid) * 4; };
-    // Momentum and norm; the first NG groups' U stay in registers.  (The places between
-    // and behind X's values are 0.)
-    for (int64_t i = tid; i < f.bytes / 16; i += kFusedThreads) reinterpret_cast<u32x4_t*>(smem)[i] = u32x4_t{};
-    constexpr int NG = LDS_BYTES == kFusedSmall ? 8 : 16;
-    float u[NG][4];
-    double sum = 0.0;
-    const auto take = [&](int at, float (&v)[4], float (&w)[4]) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if constexpr (MOM) v[e] = direction(l, v[e] * gs, w[e]);
-            if (at + e >= size) v[e] = 0.0f;
-            sum += (double)v[e] * (double)v[e];
-        }
-        if constexpr (MOM) {
-            if (at < size) store4(t.mom, at, w);
-        }
-    };
-    {
-        float w[NG][4];
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
-            if (i * kFusedThreads * 4 >= size) break;
-            load4(t.g, G{}, first_of(i), u[i]);
-            if constexpr (MOM) load4(t.mom, float{}, first_of(i), w[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
-            if (i * kFusedThreads * 4 >= size) break;
-            take(first_of(i), u[i], w[i]);
-        }
-    }
-    for (int i = NG; i * kFusedThreads * 4 < size; ++i) {
-        float v[4], w[4];
-        load4(t.g, G{}, first_of(i), v);
-        if constexpr (MOM) load4(t.mom, float{}, first_of(i), w);
-        take(first_of(i), v, w);
-    }
-    sum = wave_sum_dpp_f64(sum);
-    if (lane == 0) part[wave] = sum;
-    __syncthreads();
-    sum = 0.0;
-#pragma unroll
-    for (int w = 0; w < kFusedWaves; ++w) sum += part[w];
-    // 2^14 / (|U| + eps) as the product of two binary32 factors, each of half its
-    // exponent: its own may pass their range
-    const double inv = (double)(1 << kScaleX) / (sqrt(sum) + (double)l.eps);
-    const double half_inv = sqrt(inv);
-    const float inv0 = (float)half_inv, inv1 = (float)(inv / (double)inv0);
     // row and column of element `at` of the matrix
     const float per_n = 1.0f / (float)n;
     const auto place = [&](int at, int& i, int& j) {
@@ -462,34 +417,88 @@ __global__ __launch_bounds__(kFusedThreads) void ortho_fused_kernel(OrthoList l,
             }
         }
     };
-    const bool lines = t.wide && !tall;       // four elements lie in one row of X
-    const auto scale4 = [&](int at, const float (&v)[4]) {
-        if (lines) {
-            if (at >= size) return;
-            int i, j;
-            place(at, i, j);
-            *reinterpret_cast<u32x2_t*>(X + i * f.ldx + j) =
-                u32x2_t{pack_f16x2(v[0] * inv0 * inv1, v[1] * inv0 * inv1), pack_f16x2(v[2] * inv0 * inv1, v[3] * inv0 * inv1)};
-        } else {
-            walk(at, [&](int e, uint16_t* x) { *x = __builtin_bit_cast(uint16_t, (_Float16)(v[e] * inv0 * inv1)); });
+    constexpr int NG = LDS_BYTES == kFusedSmall ? 8 : 16;
+    const auto enter = [&](auto mode) {
+        // Momentum and norm; the first NG groups' U stay in registers.  (The places between
+        // and behind X's values are 0.)
+        for (int64_t i = tid; i < f.bytes / 16; i += kFusedThreads) reinterpret_cast<u32x4_t*>(smem)[i] = u32x4_t{};
+        float u[NG][4];
+        double sum = 0.0;
+        const auto take = [&](int at, float (&v)[4], float (&w)[4]) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (MOM) v[e] = direction(l, v[e] * gs, w[e]);
+                if (at + e >= size) v[e] = 0.0f;
+                sum += (double)v[e] * (double)v[e];
+            }
+            if constexpr (MOM) {
+                if (at < size) store4(mode, t.mom, at, w);
+            }
+        };
+        {
+            float w[NG][4];
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                if (i * kFusedThreads * 4 >= size) break;
+                load4(mode, t.g, G{}, first_of(i), u[i]);
+                if constexpr (MOM) load4(mode, t.mom, float{}, first_of(i), w[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                if (i * kFusedThreads * 4 >= size) break;
+                take(first_of(i), u[i], w[i]);
+            }
+        }
+        for (int i = NG; i * kFusedThreads * 4 < size; ++i) {
+            float v[4], w[4];
+            load4(mode, t.g, G{}, first_of(i), v);
+            if constexpr (MOM) load4(mode, t.mom, float{}, first_of(i), w);
+            take(first_of(i), v, w);
+        }
+        sum = wave_sum_dpp_f64(sum);
+        if (lane == 0) part[wave] = sum;
+        __syncthreads();
+        sum = 0.0;
+#pragma unroll
+        for (int w = 0; w < kFusedWaves; ++w) sum += part[w];
+        // 2^14 / (|U| + eps) as the product of two binary32 factors, each of half its
+        // exponent: its own may pass their range
+        const double inv = (double)(1 << kScaleX) / (sqrt(sum) + (double)l.eps);
+        const double half_inv = sqrt(inv);
+        const float inv0 = (float)half_inv, inv1 = (float)(inv / (double)inv0);
+        const auto scale4 = [&](int at, const float (&v)[4]) {
+            if constexpr (decltype(mode)::value == kLines) {
+                if (at >= size) return;
+                int i, j;
+                place(at, i, j);
+                *reinterpret_cast<u32x2_t*>(X + i * f.ldx + j) =
+                    u32x2_t{pack_f16x2(v[0] * inv0 * inv1, v[1] * inv0 * inv1), pack_f16x2(v[2] * inv0 * inv1, v[3] * inv0 * inv1)};
+            } else {
+                walk(at, [&](int e, uint16_t* x) { *x = __builtin_bit_cast(uint16_t, (_Float16)(v[e] * inv0 * inv1)); });
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            if (i * kFusedThreads * 4 >= size) break;
+            scale4(first_of(i), u[i]);
+        }
+        for (int i = NG; i * kFusedThreads * 4 < size; ++i) {
+            float v[4], w[4];
+            load4(mode, t.g, G{}, first_of(i), v);
+            if constexpr (MOM) {
+                // (as this thread wrote it)
+                load4(mode, t.mom, float{}, first_of(i), w);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = l.nesterov ? l.one_minus_beta * (v[e] * gs) + l.beta * w[e] : w[e];
+            }
+            scale4(first_of(i), v);
         }
     };
-#pragma unroll
-    for (int i = 0; i < NG; ++i) {
-        if (i * kFusedThreads * 4 >= size) break;
-        scale4(first_of(i), u[i]);
-    }
-    for (int i = NG; i * kFusedThreads * 4 < size; ++i) {
-        float v[4], w[4];
-        load4(t.g, G{}, first_of(i), v);
-        if constexpr (MOM) {
-            // (as this thread wrote it)
-            load4(t.mom, float{}, first_of(i), w);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = l.nesterov ? l.one_minus_beta * (v[e] * gs) + l.beta * w[e] : w[e];
-        }
-        scale4(first_of(i), v);
-    }
+    // (a kind of matrix's code lies together: it runs once, and is read from memory)
+    const int kind = !t.wide ? kOdd : tall ? kTall : kLines;
+    if (kind == kLines) enter(std::integral_constant<int, kLines>{});
+    else if (kind == kTall) enter(std::integral_constant<int, kTall>{});
+    else enter(std::integral_constant<int, kOdd>{});
     __syncthreads();
     const auto frag = [&](const uint16_t* p) {
         return __builtin_bit_cast(f16x8_t, *reinterpret_cast<const u32x4_t*>(p));
@@ -605,61 +614,66 @@ __global__ __launch_bounds__(kFusedThreads) void ortho_fused_kernel(OrthoList l,
         else if (f.r16 == 48) iterate(std::integral_constant<int, 3>{});
         else iterate(std::integral_constant<int, 4>{});
     }
-    const float unit = 1.0f / (1 << kScaleX), step = t.step * unit;
-    float* const p = OUT == kOutMaster ? t.master : (float*)t.out;
-    const auto give = [&](int at, float (&w)[4]) {
-        float x[4] = {};
-        if (at >= size) return;
-        if (lines) {
-            int i, j;
-            place(at, i, j);
-            const u32x2_t d = *reinterpret_cast<const u32x2_t*>(X + i * f.ldx + j);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                x[e] = (float)__builtin_bit_cast(_Float16, (uint16_t)(e & 1 ? d[e >> 1] >> 16 : d[e >> 1] & 0xffffu));
-        } else {
-            walk(at, [&](int e, uint16_t* from) { x[e] = (float)__builtin_bit_cast(_Float16, *from); });
-        }
-        if constexpr (OUT == kOutBf16) {
-            uint16_t* const o = (uint16_t*)t.out + base + at;
-            if (t.wide) {
-                *reinterpret_cast<u32x2_t*>(o) = u32x2_t{pack_bf16x2(x[0] * unit, x[1] * unit), pack_bf16x2(x[2] * unit, x[3] * unit)};
-            } else {
+    const auto leave = [&](auto mode) {
+        const float unit = 1.0f / (1 << kScaleX), step = t.step * unit;
+        float* const p = OUT == kOutMaster ? t.master : (float*)t.out;
+        const auto give = [&](int at, float (&w)[4]) {
+            float x[4] = {};
+            if (at >= size) return;
+            if constexpr (decltype(mode)::value == kLines) {
+                int i, j;
+                place(at, i, j);
+                const u32x2_t d = *reinterpret_cast<const u32x2_t*>(X + i * f.ldx + j);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (at + e < size) o[e] = (uint16_t)f32_to_bf16_bits(x[e] * unit);
+                    x[e] = (float)__builtin_bit_cast(_Float16, (uint16_t)(e & 1 ? d[e >> 1] >> 16 : d[e >> 1] & 0xffffu));
+            } else {
+                walk(at, [&](int e, uint16_t* from) { x[e] = (float)__builtin_bit_cast(_Float16, *from); });
             }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = __builtin_fmaf(-step, x[e], l.decay * w[e]);
-            store4(p, at, w);
-            if constexpr (OUT == kOutMaster) {
+            if constexpr (OUT == kOutBf16) {
                 uint16_t* const o = (uint16_t*)t.out + base + at;
-                if (t.wide) {
-                    *reinterpret_cast<u32x2_t*>(o) = u32x2_t{pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3])};
+                if constexpr (decltype(mode)::value != kOdd) {
+                    *reinterpret_cast<u32x2_t*>(o) = u32x2_t{pack_bf16x2(x[0] * unit, x[1] * unit), pack_bf16x2(x[2] * unit, x[3] * unit)};
                 } else {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (at + e < size) o[e] = (uint16_t)f32_to_bf16_bits(w[e]);
+                        if (at + e < size) o[e] = (uint16_t)f32_to_bf16_bits(x[e] * unit);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = __builtin_fmaf(-step, x[e], l.decay * w[e]);
+                store4(mode, p, at, w);
+                if constexpr (OUT == kOutMaster) {
+                    uint16_t* const o = (uint16_t*)t.out + base + at;
+                    if constexpr (decltype(mode)::value != kOdd) {
+                        *reinterpret_cast<u32x2_t*>(o) = u32x2_t{pack_bf16x2(w[0], w[1]), pack_bf16x2(w[2], w[3])};
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (at + e < size) o[e] = (uint16_t)f32_to_bf16_bits(w[e]);
+                    }
                 }
             }
-        }
-    };
-    for (int i0 = 0; i0 * kFusedThreads * 4 < size; i0 += NG) {
-        float w[NG][4];
-        if constexpr (OUT != kOutBf16) {
+        };
+        for (int i0 = 0; i0 * kFusedThreads * 4 < size; i0 += NG) {
+            float w[NG][4];
+            if constexpr (OUT != kOutBf16) {
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    if ((i0 + i) * kFusedThreads * 4 >= size) break;
+                    load4(mode, p, float{}, first_of(i0 + i), w[i]);
+                }
+            }
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
                 if ((i0 + i) * kFusedThreads * 4 >= size) break;
-                load4(p, float{}, first_of(i0 + i), w[i]);
+                give(first_of(i0 + i), w[i]);
             }
         }
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
-            if ((i0 + i) * kFusedThreads * 4 >= size) break;
-            give(first_of(i0 + i), w[i]);
-        }
-    }
+    };
+    if (kind == kLines) leave(std::integral_constant<int, kLines>{});
+    else if (kind == kTall) leave(std::integral_constant<int, kTall>{});
+    else leave(std::integral_constant<int, kOdd>{});
 }
 
 template <typename G, int LDS_BYTES>
