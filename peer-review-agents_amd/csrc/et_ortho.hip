@@ -312,7 +312,7 @@ __global__ __launch_bounds__(kDenseThreads) void ortho_finish_kernel(OrthoList l
 // rows 16 bytes apart from a multiple of 64, so that 16 rows' segments fall on
 // all banks.  X = S X goes column by column: a wave replaces 16 columns of X by
 // their own product, in place.  The products above launch 17 kernels for the same
-// (three layers' routers and 8 experts of 64 x 512 and 512 x 32: 227 us, here 41).
+// (three layers' routers and 8 experts of 64 x 512 and 512 x 32: 227 us, here 35).
 constexpr int kFusedThreads = 512, kFusedWaves = kFusedThreads / kWave;
 constexpr int kFusedSide = 64;
 constexpr int kFusedSmall = 30 * 1024, kFusedLarge = 150 * 1024;     // bytes of LDS: four blocks a CU, or one
@@ -1254,7 +1254,8 @@ int check_call(const char* fn, const int64_t* shapes, int64_t count, int dtype, 
 int run_call(const OrthoCall& call, const OrthoList& scalars, unsigned char* workspace, hipStream_t s)
 {
     // Blocks of both sizes of LDS that find a CU each go in one launch, beside one another
-    // (3 x 8 of 512 x 64 and 32 x 512, and three routers: 57 to 41 us).
+    // (three routers and 3 x 8 matrices of 64 x 512 and of 512 x 32, in one or the other: 57 us
+    // in two launches, 41 in one, before other steps).
     int64_t small = 0, large = 0;
     for (int64_t i = 0; i < call.count; ++i) {
         const Shape sh = shape_at(call.shapes, i);
