@@ -116,6 +116,23 @@ def test_slices_of_wider_rows(et, dev):
     assert torch.equal(far[:, K:K + N], want)
 
 
+@pytest.mark.parametrize("T", [40, 2100])
+def test_a_bank_beyond_32_bits(et, dev, T):
+    """The last of 4096 adapters lies more than 4 GiB into a and b."""
+    n, rank, K, N = 4096, 128, 4120, 4128
+    few = _bank(et, dev, 2, rank, K, N)
+    a = torch.zeros(n, rank, K, device=dev, dtype=torch.bfloat16)
+    b = torch.zeros(n, N, rank, device=dev, dtype=torch.bfloat16)
+    assert (n - 1) * rank * K * 2 > 2 ** 32
+    scale = torch.zeros(n, device=dev)
+    for at, i in ((0, 0), (n - 1, 1)):
+        a[at], b[at], scale[at] = few.a[i], few.b[i], few.scale[i]
+    bank = et.AdapterBank(a, b, scale)
+    x, y, index = _batch(dev, T, K, N, 2)
+    got = et.adapter_add(y, x, bank, et.adapter_plan(torch.where(index == 1, n - 1, index), n))
+    _check(got, y, x, few, index)
+
+
 def test_a_bad_token_stays_a_token(et, dev):
     T, K, N, n = 60, 72, 64, 3
     bank = _bank(et, dev, n, 16, K, N)

@@ -164,6 +164,24 @@ def test_no_rows_and_wide_strides(et, dev):
     _close(dw, want["dw"], "dw")
 
 
+def test_rows_beyond_32_bits(et, dev):
+    """h, dh and the projections' gradient of more than 4 GiB: the last rows' results."""
+    T, K, F, n = (1 << 20) + 77, 64, 2056, 70
+    last, w, dlast = _inputs(dev, n, K, F)
+    x = torch.zeros(T, K, device=dev, dtype=torch.bfloat16)
+    dh = torch.zeros(T, F, device=dev, dtype=torch.bfloat16)
+    x[-n:], dh[-n:] = last, dlast
+    want = _want(last, w, "silu", dlast)
+    h = et.gated_linear(x, w)
+    _close(h[-n:], want["h"], "h")
+    assert not h[:-n].any()
+    del h
+    dx, dw = et.gated_linear_backward(dh, x, w)
+    _close(dx[-n:], want["dx"], "dx")
+    _close(dw, want["dw"], "dw")
+    assert not dx[:-n].any()
+
+
 def test_a_bad_row_stays_a_row(et, dev):
     x, w, dh = _inputs(dev, 70, 72, 40)
     x = x.contiguous()

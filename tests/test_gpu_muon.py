@@ -98,6 +98,18 @@ def test_products_of_few_tiles(et, dev, E, m, n):
     _check(-p[0] / size, u, "beside others")
 
 
+@pytest.mark.parametrize("m,n", [(1024, 2048), (64, 1024)])
+def test_tensors_beyond_32_bits(et, dev, m, n):
+    """The last matrices of a tensor of more than 4 GiB, through every way that takes many."""
+    E = 2 ** 31 // (m * n) + 20
+    g = torch.zeros(E, m, n, device=dev, dtype=torch.bfloat16)
+    last = _gradient(dev, 3, m, n, seed=6).bfloat16()
+    g[-3:] = last
+    got = et.orthogonalize(g)
+    _check(got[-3:], last.float(), "last")
+    assert not got[:-3].any()
+
+
 @pytest.mark.parametrize("m,n", [(2100, 2200), (1500, 5001)])
 def test_norm_of_many_elements(et, dev, m, n):
     """More elements than the blocks of a norm take at once, whole rows of 16 bytes and not."""
