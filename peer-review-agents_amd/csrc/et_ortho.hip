@@ -10,9 +10,10 @@
 //
 // Number format.  X, A and S are held in f16 times fixed powers of two and
 // multiplied on the matrix units with binary32 sums.  The largest singular value
-// of X stays below 1.21 and that of S below a, for the coefficients that the host
-// accepts, so no entry is larger: X and A times 2^14 and S times 2^kScaleS stay
-// below f16's largest number, and entries down to 2^-28 keep all 11 bits.  A bf16
+// of X stays below 1.9 and that of S below 1.01 a, for the coefficients that the host
+// accepts, so no entry of X, A or S is larger than 1.9, 3.61 or 1.01 a: X and A times 2^14 and S
+// times the largest power of two that keeps a below 60000 stay below f16's largest
+// number, 65504, and entries down to 2^-28 keep all 11 bits.  A bf16
 // number has 8 bits, and rounding errors of X grow by a in each step where a
 // singular value is still small: with bf16 operands the result is 1 to 2% off, with
 // f16 0.1 to 0.2%, about the rounding of a bf16 result (measured on gradients of
@@ -1233,19 +1234,22 @@ int check_call(const char* fn, const int64_t* shapes, int64_t count, int dtype, 
     if (iterations < 1 || iterations > 64) return fail_at(fn, "iterations must be in [1, 64]");
     if (!abc) return fail_at(fn, "null coefficients");
     if (!(eps >= 0.0f) || !(eps < __builtin_inff())) return fail_at(fn, "eps must be finite and >= 0");
-    // the scaled f16 numbers hold X's singular values up to 3.9 and S's up to a
+    // the scaled f16 numbers hold X's singular values up to 1.9 (A's up to 3.61, 59146 times
+    // 2^-14) and S's up to 1.01 a
     const double a = abc[0], b = abc[1], c = abc[2];
     bool ok = a > 0.0 && a < 16.0 && __builtin_fabs(b) < 64.0 && __builtin_fabs(c) < 64.0;
     double most = 1.0;        // the largest singular value that a step can start from
-    for (int it = 0; ok && it < iterations && it < 8; ++it) {
+    for (int it = 0; ok && it < iterations; ++it) {
         double next = 0.0;
         for (int k = 0; k <= 256; ++k) {
             const double s = most * k / 256.0, f = a + b * s * s + c * s * s * s * s;
             ok = ok && __builtin_fabs(f) <= 1.01 * a;
             next = std::max(next, __builtin_fabs(f * s));
         }
+        const double before = most;
         most = std::max(most, 1.01 * next);
         ok = ok && most < 1.9;
+        if (most == before) break;      // (all further steps are alike)
     }
     if (!ok) return fail_at(fn, "coefficients must keep singular values in [0, 1] below 1.9 and |a + b s^2 + c s^4| at most a (below 16)");
     return ET_OK;

@@ -50,12 +50,13 @@ def _coefficients(coefficients, steps: int, eps: float):
     a, b, c = map(float, coefficients)
     # (as the library checks it: f16 holds the numbers in between)
     most, fine = 1.0, 0.0 < a < 16.0 and abs(b) < 64.0 and abs(c) < 64.0
-    for _ in range(min(steps, 8) if fine else 0):
+    for _ in range(steps if fine else 0):
         values = [most * k / 256.0 for k in range(257)]
         slopes = [abs(a + b * s * s + c * s ** 4) for s in values]
-        fine = fine and max(slopes) <= 1.01 * a
-        most = max(most, 1.01 * max(s * f for s, f in zip(values, slopes)))
-        fine = fine and most < 1.9
+        before, most = most, max(most, 1.01 * max(s * f for s, f in zip(values, slopes)))
+        fine = max(slopes) <= 1.01 * a and most < 1.9
+        if not fine or most == before:      # (refused, or all further steps are alike)
+            break
     if not fine:
         raise ValueError("coefficients must keep singular values from [0, 1] below 1.9 and |a + b s^2 + c s^4| at most a "
                          f"(below 16), got {tuple(coefficients)}")
