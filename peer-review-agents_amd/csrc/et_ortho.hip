@@ -220,7 +220,8 @@ __global__ __launch_bounds__(kDenseThreads) void ortho_scale_kernel(OrthoList l)
     for (uint32_t i = threadIdx.x; i < t.sums; i += kDenseThreads) sum += t.partial[(int64_t)e * t.sums + i];
     sum = block_sum(sum);
     // (in binary64: the norm of values near binary32's smallest or largest is in its range)
-    const double inv = (double)(1 << kScaleX) / (sqrt(sum) + (double)l.eps);
+    // (a matrix of zeros stays one, without eps too)
+    const double inv = sum == 0.0 ? 0.0 : (double)(1 << kScaleX) / (sqrt(sum) + (double)l.eps);
     uint16_t* const x = t.x + (int64_t)e * t.m * t.ldx;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -463,8 +464,8 @@ __global__ __launch_bounds__(kFusedThreads) void ortho_fused_kernel(OrthoList l,
 #pragma unroll
         for (int w = 0; w < kFusedWaves; ++w) sum += part[w];
         // 2^14 / (|U| + eps) as the product of two binary32 factors, each of half its
-        // exponent: its own may pass their range
-        const double inv = (double)(1 << kScaleX) / (sqrt(sum) + (double)l.eps);
+        // exponent: its own may pass their range (a matrix of zeros is taken times 1, without eps too)
+        const double inv = sum == 0.0 ? 1.0 : (double)(1 << kScaleX) / (sqrt(sum) + (double)l.eps);
         const double half_inv = sqrt(inv);
         const float inv0 = (float)half_inv, inv1 = (float)(inv / (double)inv0);
         const auto scale4 = [&](int at, const float (&v)[4]) {

@@ -17,3 +17,36 @@ def test_polynomials_near_the_largest_singular_value(et, dev, m, n):
     want = u.double() / u.double().flatten(1).norm(dim=1)[:, None, None] * 1.07 ** 6
     off = ((got - want).flatten(1).norm(dim=1) / 1.07 ** 6).max().item()
     assert off <= 13 * 2.0 ** -11 + HALF, off
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-60])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("E,m,n", [(3, 8, 16), (3, 64, 1024), (3, 500, 40), (3, 130, 77), (40, 384, 520)])
+def test_a_zero_matrix_gives_zero_without_eps(et, dev, E, m, n, dtype, eps):
+    """By every way that a matrix can go; a bad matrix and others beside it (eps 1e-60 is 0 in binary32)."""
+    g = torch.randn(E, m, n, generator=torch.Generator(device=dev).manual_seed(m), device=dev).to(dtype)
+    want = et.orthogonalize(g, eps=eps)
+    assert torch.isfinite(want.float()).all() and want.any()
+    g[1] = 0
+    got = et.orthogonalize(g, eps=eps)
+    assert not got[1].any()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[2:], want[2:])
+    for bad in (float("nan"), float("inf")):
+        g[2, m // 2, n // 3] = bad
+        got = et.orthogonalize(g, eps=eps)
+        assert not got[1].any() and bool(torch.isnan(got[2]).all()) and torch.equal(got[0], want[0])
+
+
+@pytest.mark.parametrize("m,n", [(16, 64), (96, 264)])
+@pytest.mark.parametrize("low", [False, True])
+def test_an_expert_without_tokens_keeps_its_weights(et, dev, m, n, low):
+    """A step without eps, the second expert's gradient and momentum zero: its weights decay and stay."""
+    g = torch.randn(3, m, n, generator=torch.Generator(device=dev).manual_seed(n), device=dev)
+    g[1] = 0
+    w = torch.ones_like(g)
+    params = [w.bfloat16() if low else w]
+    masters = [w] if low else None
+    momenta = [torch.zeros_like(g)]
+    et.muon_step_(params, [g], momenta, lr=0.5, weight_decay=0.5, eps=0.0, masters=masters)
+    assert bool((w[1] == 0.75).all()) and bool((params[0][1] == 0.75).all()) and not momenta[0][1].any()
+    assert torch.isfinite(w).all() and bool((w[0] != 0.75).any())
