@@ -80,7 +80,8 @@ size_t et_orthogonalize_workspace_bytes(const int64_t* shapes, int64_t count);
  * X, A and the polynomial are held in f16 with 11 bits: the result is 0.1 to 0.2%
  * off in norm.  Fixed order: repeated calls give identical bits.  A matrix
  * that is all zero gives zero; one with a value that is not finite gives NaN,
- * and no other matrix does.  Sides below 65536.  workspace 256-byte aligned.
+ * and no other matrix does.  Sides below 65536, a tensor below 2^23 matrices and 2^36
+ * elements.  workspace 256-byte aligned.
  */
 int et_orthogonalize(const void* const* g, void* const* out, const int64_t* shapes, int64_t count, int dtype,
                      int iterations, const float* coefficients, float eps, void* workspace, size_t workspace_bytes,
@@ -142,7 +143,8 @@ size_t et_adapter_add_workspace_bytes(int64_t num_tokens, int64_t num_adapters, 
  * be y; bf16 a [num_adapters, rank, K] and b [num_adapters, N, rank], f32 scale
  * [num_adapters].  K, N and rank multiples of 8, rank at most
  * ET_MAX_ADAPTER_RANK.  order, items and num_items are those of et_adapter_plan for the
- * same num_tokens and num_adapters.  Binary32 sums in a fixed order, the inner one
+ * same num_tokens and num_adapters; num_tokens is below 2^27, and the plan's items times
+ * N / 1024 (rounded up) below 2^24.  Binary32 sums in a fixed order, the inner one
  * kept to 16 bits, one rounding of out: repeated calls give identical bits.  An
  * inner sum that is not finite gives NaN in its token's row.
  * Pointers 16-byte aligned (scale, order and num_items 4).

@@ -502,8 +502,8 @@ extern "C" int et_adapter_add(const void* y, int64_t y_stride, const void* x, in
     // (several chunks a wave where there are many blocks all the same)
     g.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(4, most * up(N, 64 * kWaves) / 2048));
     g.col_blocks = (int)up(N, 64 * kWaves * g.chunks);
-    // (a launch has less than 2^32 threads)
-    if (most * g.col_blocks >= (int64_t)1 << 24 || most >= 1 << 23)
+    // (a launch has less than 2^32 threads: the first kernel's has two blocks of up to 512 an item)
+    if (most * g.col_blocks >= (int64_t)1 << 24 || most >= 1 << 22)
         return refuse(fn, "num_tokens * N is too large");
     const int tile = tile_of(num_tokens);
     hipStream_t s = (hipStream_t)stream;

@@ -1049,17 +1049,22 @@ struct Shape {
         }
         return tall() ? 1 : 0;
     }
+    // of all its matrices, in blocks of kDenseThreads threads
+    int64_t launch_blocks() const { return E * (way() >= 2 ? kFusedThreads / kDenseThreads : blocks()); }
     int64_t bytes() const { return way() >= 2 ? 0 : 2 * x_bytes() + 2 * a_bytes() + sum_bytes(); }
 };
 constexpr int kWays = 4;
 
 constexpr int64_t kMostSide = 1 << 16;
+// A launch has less than 2^32 threads: 2^24 blocks of the elementwise kernels, 2^23 of the one
+// that takes a matrix in one block.
+constexpr int64_t kMostBlocks = 1 << 24, kMostMatrices = 1 << 23;
+static_assert(kMostBlocks * kDenseThreads <= (int64_t)1 << 32 && kMostMatrices * kFusedThreads <= (int64_t)1 << 32, "threads");
 
 bool shape_ok(const Shape& s)
 {
-    // (a launch has less than 2^32 threads)
-    if (s.E < 0 || s.m < 0 || s.n < 0 || s.m >= kMostSide || s.n >= kMostSide || s.E >= 1 << 24) return false;
-    return s.E * s.m * s.n == 0 || s.E * s.blocks() < 1 << 24;
+    if (s.E < 0 || s.m < 0 || s.n < 0 || s.m >= kMostSide || s.n >= kMostSide || s.E >= kMostMatrices) return false;
+    return s.E * s.m * s.n == 0 || s.launch_blocks() < kMostBlocks;
 }
 
 struct OrthoCall {
@@ -1230,7 +1235,7 @@ int check_call(const char* fn, const int64_t* shapes, int64_t count, int dtype, 
     if (count < 0) return fail_at(fn, "count must be >= 0");
     if (count > 0 && !shapes) return fail_at(fn, "null shapes");
     for (int64_t i = 0; i < count; ++i)
-        if (!shape_ok(shape_at(shapes, i))) return fail_at(fn, "sides must be in [0, 65536), and a tensor below 2^24 matrices and 2^36 elements");
+        if (!shape_ok(shape_at(shapes, i))) return fail_at(fn, "sides must be in [0, 65536), and a tensor below 2^23 matrices and 2^36 elements");
     if (dtype != ET_DTYPE_F32 && dtype != ET_DTYPE_BF16) return fail_at(fn, "dtype must be ET_DTYPE_F32 or ET_DTYPE_BF16");
     if (iterations < 1 || iterations > 64) return fail_at(fn, "iterations must be in [1, 64]");
     if (!abc) return fail_at(fn, "null coefficients");
@@ -1292,12 +1297,12 @@ int run_call(const OrthoCall& call, const OrthoList& scalars, unsigned char* wor
             if (sh.E * sh.m * sh.n == 0) continue;
             at += sh.bytes();
             if (way_of(sh) != way) continue;
-            if (list.count == kTensors || blocks + sh.E * sh.blocks() >= 1 << 24) {
+            if (list.count == kTensors || blocks + sh.launch_blocks() >= kMostBlocks) {
                 if (const int rc = flush()) return rc;
             }
             index[list.count] = i;
             place[list.count++] = here;
-            blocks += sh.E * sh.blocks();
+            blocks += sh.launch_blocks();
         }
         if (const int rc = flush()) return rc;
     }

@@ -41,3 +41,19 @@ def test_polynomials_that_stay_are_taken(et, abc, steps):
     muon = importlib.import_module("peer-review-agents_amd.muon")
     assert muon._coefficients(abc, steps, 1e-7) == abc
     assert _polynomial(et, abc, steps) == 0
+
+
+def test_launches_stay_below_2_32_threads(et):
+    """A matrix that goes one block has 512 threads; an item of the adapters' first kernel two blocks of up to 512."""
+    lib, P = et.lib(), ctypes.c_void_p(0x1000)
+    one, abc, step = (ctypes.c_void_p * 1)(0x1000), (ctypes.c_float * 3)(3.4445, -4.775, 2.0315), (ctypes.c_float * 1)(0.1)
+    scalars = importlib.import_module("peer-review-agents_amd._lib").MuonScalars(0.95, 0.05, 1.0, 1e-7, 3.4445, -4.775, 2.0315, 5, 1)
+    for E, m, n in ((1 << 23, 2, 2), (1 << 23, 1, 1), ((1 << 24) - 1, 8, 8)):
+        shape = _shapes((E, m, n))
+        assert lib.et_orthogonalize(one, one, shape, 1, 0, 5, abc, 1e-7, P, 1 << 40, None) == ET_ERR_INVALID_ARGUMENT
+        assert "2^23" in _err(et)
+        assert lib.et_muon(one, one, one, None, step, shape, 1, 0, 0, scalars, None, P, 1 << 40, None) == ET_ERR_INVALID_ARGUMENT
+        assert lib.et_orthogonalize_workspace_bytes(shape, 1) == 0
+    for T, rank in ((1 << 28, 8), ((1 << 28) + 64, 32), ((1 << 29) - 64, 8)):
+        rc = lib.et_adapter_add(P, 8, P, 8, P, P, P, P, P, P, T, 4, 8, 8, rank, P, 8, P, 1 << 62, None)
+        assert rc == ET_ERR_INVALID_ARGUMENT and "too large" in _err(et), T

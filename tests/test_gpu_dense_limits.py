@@ -50,3 +50,21 @@ def test_an_expert_without_tokens_keeps_its_weights(et, dev, m, n, low):
     et.muon_step_(params, [g], momenta, lr=0.5, weight_decay=0.5, eps=0.0, masters=masters)
     assert bool((w[1] == 0.75).all()) and bool((params[0][1] == 0.75).all()) and not momenta[0][1].any()
     assert torch.isfinite(w).all() and bool((w[0] != 0.75).any())
+
+
+def test_more_small_matrices_than_a_launch_takes(et, dev):
+    """Two tensors of 2^22 + 5 matrices of one row, a block each: more than 2^23 blocks in all.  A row's singular
+    value is 1 and follows the polynomial; X and S are rounded to f16 in 5 steps (a factor of up to 3.45 in the first, below
+    1 in size behind it: 5 products of 3 roundings each, times 3.45), and to bf16 once in one of the calls."""
+    E = (1 << 22) + 5
+    g = torch.Generator(device=dev).manual_seed(8)
+    us = [torch.randn(E, 1, n, generator=g, device=dev) + 3.0 for n in (1, 2)]
+    ps, moms = [torch.zeros_like(u) for u in us], [torch.zeros_like(u) for u in us]
+    et.muon_step_(ps, us, moms, lr=1.0, momentum=0.0, nesterov=False, update_rms=None)
+    s = 1.0
+    for _ in range(5):
+        s = s * (3.4445 - 4.7750 * s ** 2 + 2.0315 * s ** 4)
+    for u, p, m in zip(us, ps, moms):
+        assert torch.equal(m, u)
+        want = u.double() / u.double().flatten(1).norm(dim=1)[:, None, None] * s
+        assert ((-p.double() - want).abs().amax() <= 15 * 3.45 * 2.0 ** -11).item()
