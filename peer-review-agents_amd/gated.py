@@ -62,6 +62,13 @@ def gated_linear(x: torch.Tensor, w: torch.Tensor, *, activation: str = "silu",
     return h
 
 
+def _own_place(dh: torch.Tensor) -> torch.Tensor:
+    """A gradient as the library reads it: autograd may hand over a view of another tensor, from
+    any element on."""
+    dh = dh.contiguous()
+    return dh if dh.data_ptr() % 16 == 0 else dh.clone()
+
+
 def gated_linear_backward_workspace_bytes(rows: int, K: int, F: int) -> int:
     return int(lib().et_gated_linear_bwd_workspace_bytes(rows, K, F))
 
@@ -112,7 +119,7 @@ class _GatedLinearFn(torch.autograd.Function):
     def backward(ctx, dh):
         x, w = ctx.saved_tensors
         need_dx, need_dw, _ = ctx.needs_input_grad
-        dx, dw = gated_linear_backward(dh.contiguous(), x, w, activation=ctx.activation, need_dx=need_dx, need_dw=need_dw)
+        dx, dw = gated_linear_backward(_own_place(dh), x, w, activation=ctx.activation, need_dx=need_dx, need_dw=need_dw)
         return dx, dw, None
 
 

@@ -311,7 +311,8 @@ def _gated_linear_fake(x, w, activation):
 def gated_linear_backward(dh: Tensor, x: Tensor, w: Tensor, activation: str, need_dx: bool,
                           need_dw: bool) -> Tuple[Tensor, Tensor]:
     """(dX, dW), one that is not needed without rows."""
-    dx, dw = _gated.gated_linear_backward(dh, x, w, activation=activation, need_dx=need_dx, need_dw=need_dw)
+    # (the gradient's place is known here only, not where a compiled backward is traced)
+    dx, dw = _gated.gated_linear_backward(_gated._own_place(dh), x, w, activation=activation, need_dx=need_dx, need_dw=need_dw)
     return x.new_empty(0, x.shape[1]) if dx is None else dx, w.new_empty(0, w.shape[1]) if dw is None else dw
 
 
