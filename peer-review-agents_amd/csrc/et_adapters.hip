@@ -385,6 +385,17 @@ int tile_of(int64_t T) { return T <= 2048 ? 16 : 64; }
 
 int64_t most_items(int64_t T, int64_t n) { return up(T, tile_of(T)) + std::min(T, n + 1); }
 
+// What is wrong with the sizes of adapter_add (N apart), or null; its plan has `items`.
+const char* size_error(int64_t items, int64_t K, int64_t rank)
+{
+    if (items < 0) return "num_tokens must be in [0, 2^30) and num_adapters in [1, ET_MAX_ADAPTERS]";
+    // (a launch has less than 2^32 threads: the first kernel's has two blocks of up to 512 an item)
+    if (items >= 1 << 22) return "num_tokens is too large";
+    if (K < 8 || K % 8 || K >= 1 << 22) return "K must be a positive multiple of 8 below 2^22";
+    if (rank < 8 || rank % 8 || rank > ET_MAX_ADAPTER_RANK) return "rank must be a positive multiple of 8, at most ET_MAX_ADAPTER_RANK";
+    return nullptr;
+}
+
 // Splits of the sum over K, where the items leave CUs idle: the fewest rounds of
 // blocks for the work of each, a chunk for each of 8 waves at least.
 int splits_of(int64_t T, int64_t items, int64_t K)
@@ -449,7 +460,7 @@ extern "C" int et_adapter_plan(const int32_t* index, int64_t num_tokens, int64_t
 extern "C" size_t et_adapter_add_workspace_bytes(int64_t num_tokens, int64_t num_adapters, int64_t K, int64_t rank)
 {
     const int64_t items = et_adapter_plan_items(num_tokens, num_adapters);
-    if (items < 0 || K < 8 || rank < 8 || rank > ET_MAX_ADAPTER_RANK) return 0;
+    if (size_error(items, K, rank)) return 0;
     return (size_t)splits_of(num_tokens, items, K) * num_tokens * rank * 4;
 }
 
@@ -460,11 +471,8 @@ extern "C" int et_adapter_add(const void* y, int64_t y_stride, const void* x, in
 {
     const char* fn = "et_adapter_add";
     const int64_t most = et_adapter_plan_items(num_tokens, num_adapters);
-    if (most < 0) return refuse(fn, "num_tokens must be in [0, 2^30) and num_adapters in [1, ET_MAX_ADAPTERS]");
-    if (K < 8 || K % 8 || K >= 1 << 22) return refuse(fn, "K must be a positive multiple of 8 below 2^22");
+    if (const char* const error = size_error(most, K, rank)) return refuse(fn, error);
     if (N < 8 || N % 8 || N >= 1 << 22) return refuse(fn, "N must be a positive multiple of 8 below 2^22");
-    if (rank < 8 || rank % 8 || rank > ET_MAX_ADAPTER_RANK)
-        return refuse(fn, "rank must be a positive multiple of 8, at most ET_MAX_ADAPTER_RANK");
     for (const auto& [ld, least] : {std::pair<int64_t, int64_t>{x_stride, K}, {y_stride, N}, {out_stride, N}})
         if (ld < least || ld % 8 || ld >= (int64_t)1 << 40) return refuse(fn, "row strides must be multiples of 8 and at least a row");
     if (num_tokens == 0) return ET_OK;
@@ -502,8 +510,8 @@ extern "C" int et_adapter_add(const void* y, int64_t y_stride, const void* x, in
     // (several chunks a wave where there are many blocks all the same)
     g.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(4, most * up(N, 64 * kWaves) / 2048));
     g.col_blocks = (int)up(N, 64 * kWaves * g.chunks);
-    // (a launch has less than 2^32 threads: the first kernel's has two blocks of up to 512 an item)
-    if (most * g.col_blocks >= (int64_t)1 << 24 || most >= 1 << 22)
+    // (a launch has less than 2^32 threads)
+    if (most * g.col_blocks >= (int64_t)1 << 24)
         return refuse(fn, "num_tokens * N is too large");
     const int tile = tile_of(num_tokens);
     hipStream_t s = (hipStream_t)stream;

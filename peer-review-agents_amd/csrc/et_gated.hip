@@ -445,16 +445,23 @@ int kind_of(int64_t m, int64_t n)
                       dense_cus());
 }
 
+// What is wrong with the sizes, or null.
+const char* size_error(int64_t T, int64_t K, int64_t F)
+{
+    if (T < 0 || T >= (int64_t)1 << 31) return "rows must be in [0, 2^31)";
+    if (K < 8 || K % 8 || K >= 1 << 21) return "K must be a positive multiple of 8 below 2^21";
+    if (F < 8 || F % 8 || F >= 1 << 20) return "F must be a positive multiple of 8 below 2^20";
+    if (2 * F * K * 2 >= (int64_t)1 << 31) return "the weight must be below 2 GiB";
+    return nullptr;
+}
+
 int check_sizes(const char* fn, int64_t T, int64_t K, int64_t F, int64_t ldx, int act)
 {
-    const std::string at = fn;
-    if (T < 0 || T >= (int64_t)1 << 31) return fail(ET_ERR_INVALID_ARGUMENT, at + ": rows must be in [0, 2^31)");
-    if (K < 8 || K % 8 || K >= 1 << 21) return fail(ET_ERR_INVALID_ARGUMENT, at + ": K must be a positive multiple of 8 below 2^21");
-    if (F < 8 || F % 8 || F >= 1 << 20) return fail(ET_ERR_INVALID_ARGUMENT, at + ": F must be a positive multiple of 8 below 2^20");
-    if (2 * F * K * 2 >= (int64_t)1 << 31) return fail(ET_ERR_INVALID_ARGUMENT, at + ": the weight must be below 2 GiB");
+    const std::string at = std::string(fn) + ": ";
+    if (const char* const error = size_error(T, K, F)) return fail(ET_ERR_INVALID_ARGUMENT, at + error);
     if (ldx < K || ldx % 8 || ldx >= 1 << 22)
-        return fail(ET_ERR_INVALID_ARGUMENT, at + ": the row stride of x must be a multiple of 8, at least K and below 2^22");
-    if (act != ET_GATED_SILU && act != ET_GATED_GELU) return fail(ET_ERR_INVALID_ARGUMENT, at + ": unknown activation");
+        return fail(ET_ERR_INVALID_ARGUMENT, at + "the row stride of x must be a multiple of 8, at least K and below 2^22");
+    if (act != ET_GATED_SILU && act != ET_GATED_GELU) return fail(ET_ERR_INVALID_ARGUMENT, at + "unknown activation");
     return ET_OK;
 }
 
@@ -535,7 +542,7 @@ extern "C" int et_gated_linear(const void* x, int64_t x_stride, const void* w, i
 
 extern "C" size_t et_gated_linear_bwd_workspace_bytes(int64_t rows, int64_t K, int64_t F)
 {
-    if (rows < 0 || K < 8 || F < 8) return 0;
+    if (size_error(rows, K, F)) return 0;
     const Split sp = split_tokens(rows, K, F);
     const size_t dp = (size_t)up(rows * 2 * F * 2, 256) * 256;
     return dp + (sp.splits > 1 ? (size_t)sp.splits * 2 * F * K * 4 : 0);

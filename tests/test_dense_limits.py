@@ -57,3 +57,16 @@ def test_launches_stay_below_2_32_threads(et):
     for T, rank in ((1 << 28, 8), ((1 << 28) + 64, 32), ((1 << 29) - 64, 8)):
         rc = lib.et_adapter_add(P, 8, P, 8, P, P, P, P, P, P, T, 4, 8, 8, rank, P, 8, P, 1 << 62, None)
         assert rc == ET_ERR_INVALID_ARGUMENT and "too large" in _err(et), T
+
+
+def test_workspace_sizes_of_sizes_that_are_refused(et):
+    """0, as the header says, for whatever the call itself refuses."""
+    lib = et.lib()
+    gated, adapters = lib.et_gated_linear_bwd_workspace_bytes, lib.et_adapter_add_workspace_bytes
+    assert gated(100, 64, 16) > 0 and adapters(100, 4, 64, 16) > 0
+    for T, K, F in ((-1, 64, 16), (1 << 31, 64, 16), (1 << 62, 64, 16), (100, 60, 16), (100, 0, 16), (100, 1 << 21, 8), (100, 64, 12),
+                    (100, 64, 0), (100, 8, 1 << 20), (100, 1 << 20, 1 << 10), (100, 1 << 62, 16), (100, 64, 1 << 62)):
+        assert gated(T, K, F) == 0, (T, K, F)
+    for T, n, K, r in ((-1, 4, 64, 16), (1 << 30, 4, 64, 16), (8, 0, 64, 16), (8, 4097, 64, 16), (8, 4, 60, 16), (8, 4, 0, 16),
+                       (8, 4, 1 << 22, 16), (8, 4, 64, 12), (8, 4, 64, 0), (8, 4, 64, 136), (1 << 28, 4, 64, 16)):
+        assert adapters(T, n, K, r) == 0, (T, n, K, r)
