@@ -426,20 +426,29 @@ inline unsigned dense_grid(int64_t tiles, int blocks_per_cu, int cus)
 // mid 79, 128 big 88, 1024 thin 91; 1056 small 79, 704 mid 69, 264 big 104.  Newton-Schulz,
 // five steps: 512 x 512 138 us small, 100 thin; 8 of them 153 and 126; 24 of 512 x 1024
 // 305 and 403.
-inline int dense_kind(int64_t big, int64_t mid, int64_t small, int64_t thin, bool wide, int cus)
+struct DenseChoice {
+    int kind;
+    int64_t cost;
+};
+inline DenseChoice dense_choice(int64_t big, int64_t mid, int64_t small, int64_t thin, bool wide, int cus)
 {
     const auto rounds = [cus](int64_t tiles, int alone, int pair) {
         const int64_t full = tiles / (2 * cus), rest = tiles - full * 2 * cus;
         return full * pair + (rest == 0 ? 0 : rest <= cus ? alone : pair);
     };
-    struct { int kind; int64_t cost; } best = {kTileBig, (big + cus - 1) / cus * 134};
+    DenseChoice best = {kTileBig, (big + cus - 1) / cus * 134};
     const auto other = [&best](int kind, int64_t cost) {
         if (cost < best.cost) best = {kind, cost};
     };
     if (mid) other(kTileMid, rounds(mid, 74, 122));
     other(kTileSmall, rounds(small, 60, 100));
     other(kTileThin, wide ? rounds(thin, 48, 71) : rounds(thin, 40, 60));
-    return best.kind;
+    return best;
+}
+
+inline int dense_kind(int64_t big, int64_t mid, int64_t small, int64_t thin, bool wide, int cus)
+{
+    return dense_choice(big, mid, small, thin, wide, cus).kind;
 }
 
 // Launches POLICY<kind> on `tiles` tiles.

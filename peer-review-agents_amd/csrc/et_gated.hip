@@ -266,17 +266,6 @@ __global__ __launch_bounds__(kSkinnyWaves * kWave) void gated_skinny_kernel(Gate
     }
 }
 
-// us at K = 4096, a call another weight each time: F = 2048, where the weights are
-// 6.8 us at 4.9 TB/s, one token 9.0, 16 tokens 9.7, 32 11.3, 64 14.8, a round of 128 x 128
-// tiles 42 to 45 up to 256 tokens; F = 8192 31 up to 16 tokens, tiles 47 to 51 up to 128.
-// So a round of these blocks (one a CU) is taken for a third of one of tiles.
-bool is_skinny(int64_t T, int64_t F)
-{
-    const int cus = dense_cus();
-    const int64_t rounds = up(F / 8 * up(T, 64), cus), tiled = up(up(T, 128) * up(F, 64), 2 * cus);
-    return T <= 16 || rounds <= 3 * tiled;
-}
-
 template <int ACT>
 void launch_skinny(const GatedArgs& g, hipStream_t s)
 {
@@ -439,10 +428,29 @@ int rows_of(int kind) { return kind == kTileBig ? 256 : kind == kTileMid ? 192 :
 int cols_of(int kind) { return kind == kTileBig ? 256 : 128; }
 
 // The tiles of a product of m x n outputs.
-int kind_of(int64_t m, int64_t n)
+DenseChoice choice_of(int64_t m, int64_t n)
 {
-    return dense_kind(up(m, 256) * up(n, 256), up(m, 192) * up(n, 128), up(m, 128) * up(n, 128), up(m, 64) * up(n, 128), true,
-                      dense_cus());
+    return dense_choice(up(m, 256) * up(n, 256), up(m, 192) * up(n, 128), up(m, 128) * up(n, 128), up(m, 64) * up(n, 128), true,
+                        dense_cus());
+}
+int kind_of(int64_t m, int64_t n) { return choice_of(m, n).kind; }
+
+// Few tokens or tiles: what their rounds take.  A round of few tokens' blocks (one a CU) is 2 us
+// and, for each 512 of K, 0.7, 0.9 or 1.0 us with 16, 32 or 64 tokens a block; tiles take
+// dense_choice's cost for each chunk of 64, 10% more beside the epilogue, and 7 chunks besides.
+// Measured in us, few tokens' blocks / tiles, another weight each call: K = 512, F = 2048, 64
+// tokens 5.0 / 7.6, 128 8.0 / 7.6, 192 11.0 / 7.7; F = 8192, 8 tokens 11.7 / 8.8; K = 2048, F =
+// 256, 1024 tokens 13.0 / 16.9, 1536 18.4 / 17.0; K = 4096, F = 2048, 8 tokens 9.4 / 35.9, 64
+// 14.5 / 38.3, 192 32.6 / 38.4, 256 41.5 / 38.1; K = 7168, F = 8192, 17 tokens 53 / 69.  Over 900
+// sizes (K 512 to 7168, F 64 to 8192, up to 6000 tokens) the choice is 8% from the faster one at
+// most.  Above 2048 tokens the XCDs' readings of x, each of all of it, take longer than the tiles
+// do (K = 7168, F = 64: 2048 tokens 34 / 48, 4096 65 / 48).
+bool is_skinny(int64_t T, int64_t K, int64_t F)
+{
+    if (T > 2048) return false;
+    const int64_t rounds = up(F / 8 * up(T, 64), dense_cus());
+    const int64_t skinny = rounds * (200 + (T <= 16 ? 70 : T <= 32 ? 90 : 100) * up(K, 512));
+    return skinny * 10 <= choice_of(T, 2 * F).cost * (11 * up(K, 64) + 70);
 }
 
 // What is wrong with the sizes, or null.
@@ -475,7 +483,7 @@ int check_pointer(const char* fn, const char* name, const void* p)
 // kind: the tiles (0: by size)
 int launch_gated(GatedArgs g, int act, bool backward, int kind, hipStream_t s)
 {
-    if (kind == 0 && !backward && is_skinny(g.T, g.F)) {
+    if (kind == 0 && !backward && is_skinny(g.T, g.K, g.F)) {
         if (act == ET_GATED_SILU) launch_skinny<ET_GATED_SILU>(g, s);
         else launch_skinny<ET_GATED_GELU>(g, s);
         return check_launch("gated_skinny_kernel");
