@@ -4,6 +4,7 @@ Python, each call is one library call on torch's current stream
 (include/etmoe_dense.h has the formulas); there is no CPU fallback."""
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -69,8 +70,21 @@ def _own_place(dh: torch.Tensor) -> torch.Tensor:
     return dh if dh.data_ptr() % 16 == 0 else dh.clone()
 
 
-def gated_linear_backward_workspace_bytes(rows: int, K: int, F: int) -> int:
-    return int(lib().et_gated_linear_bwd_workspace_bytes(rows, K, F))
+@lru_cache(maxsize=1024)
+def _workspace_bytes(rows: int, K: int, F: int, device: int) -> int:
+    # (the splits that it has room for go by the device's CUs)
+    with torch.cuda.device(device):
+        return int(lib().et_gated_linear_bwd_workspace_bytes(rows, K, F))
+
+
+def gated_linear_backward_workspace_bytes(rows: int, K: int, F: int, device=None) -> int:
+    """Bytes that :func:`gated_linear_backward` works in on ``device`` (the current one by default)."""
+    if device is None:
+        return int(lib().et_gated_linear_bwd_workspace_bytes(rows, K, F))
+    index = torch.device(device).index
+    if index is None:
+        raise ValueError(f"device must name one of the devices, got {device!r}")
+    return _workspace_bytes(rows, K, F, index)
 
 
 def gated_linear_backward(dh: torch.Tensor, x: torch.Tensor, w: torch.Tensor, *, activation: str = "silu",
@@ -95,7 +109,7 @@ def gated_linear_backward(dh: torch.Tensor, x: torch.Tensor, w: torch.Tensor, *,
     if need_dw or out_dw is not None:
         kind = torch.float32 if isinstance(out_dw, torch.Tensor) and out_dw.dtype == torch.float32 else torch.bfloat16
         dw = _out_or_new(out_dw, (2 * F, K), kind, dev, "out_dw")
-    wsb = gated_linear_backward_workspace_bytes(rows, K, F)
+    wsb = _workspace_bytes(rows, K, F, x.get_device())
     if workspace is None:
         workspace = torch.empty(wsb, dtype=torch.uint8, device=dev)
     else:

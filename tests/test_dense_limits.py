@@ -70,3 +70,33 @@ def test_workspace_sizes_of_sizes_that_are_refused(et):
     for T, n, K, r in ((-1, 4, 64, 16), (1 << 30, 4, 64, 16), (8, 0, 64, 16), (8, 4097, 64, 16), (8, 4, 60, 16), (8, 4, 0, 16),
                        (8, 4, 1 << 22, 16), (8, 4, 64, 12), (8, 4, 64, 0), (8, 4, 64, 136), (1 << 28, 4, 64, 16)):
         assert adapters(T, n, K, r) == 0, (T, n, K, r)
+
+
+def test_the_backwards_workspace_goes_by_the_tensors_device(et, monkeypatch):
+    """Its splits go by a device's CUs: those of the device that the call runs on, not of the current one."""
+    gated = importlib.import_module("peer-review-agents_amd.gated")
+    current = [0]
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            current.append(self.index)
+
+        def __exit__(self, *_):
+            current.pop()
+
+    class Library:
+        @staticmethod
+        def et_gated_linear_bwd_workspace_bytes(rows, K, F):
+            return 1000 * rows + current[-1]
+
+    monkeypatch.setattr(gated.torch.cuda, "device", Device)
+    monkeypatch.setattr(gated, "lib", lambda: Library)
+    try:
+        assert gated.gated_linear_backward_workspace_bytes(5, 64, 16) == 5000
+        assert gated.gated_linear_backward_workspace_bytes(5, 64, 16, device=3) == 5003
+        assert gated.gated_linear_backward_workspace_bytes(5, 64, 16, device=gated.torch.device("cuda:2")) == 5002
+    finally:
+        gated._workspace_bytes.cache_clear()
