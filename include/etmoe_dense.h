@@ -66,7 +66,7 @@ int et_gated_linear_bwd(const void* dh, const void* x, int64_t x_stride, const v
 
 /* Bytes of device workspace et_orthogonalize and et_muon need for `count` tensors
  * of shapes[3 i] matrices of shapes[3 i + 1] rows and shapes[3 i + 2] columns (HOST
- * array).  0 for invalid shapes. */
+ * array), or for some of them.  0 for invalid shapes, and where no tensor needs any. */
 size_t et_orthogonalize_workspace_bytes(const int64_t* shapes, int64_t count);
 
 /*

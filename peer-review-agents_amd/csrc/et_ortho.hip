@@ -1261,6 +1261,31 @@ int check_call(const char* fn, const int64_t* shapes, int64_t count, int dtype, 
     return ET_OK;
 }
 
+// The tensors that go one way, in sets of one launch a kernel: f(index, offset, count), with each
+// tensor's place in the workspace.  The sets run one behind the other on a stream, so they share it.
+template <typename W, typename F>
+int each_set(const int64_t* shapes, int64_t count, int way, const W& way_of, const F& f)
+{
+    int64_t index[kTensors], offset[kTensors], blocks = 0, bytes = 0;
+    int n = 0;
+    for (int64_t i = 0; i < count; ++i) {
+        const Shape sh = shape_at(shapes, i);
+        if (sh.E * sh.m * sh.n == 0 || way_of(sh) != way) continue;
+        if (n == kTensors || blocks + sh.launch_blocks() >= kMostBlocks) {
+            if (n) {
+                if (const int rc = f(index, offset, n)) return rc;
+            }
+            n = 0;
+            blocks = bytes = 0;
+        }
+        index[n] = i;
+        offset[n++] = bytes;
+        blocks += sh.launch_blocks();
+        bytes += sh.bytes();
+    }
+    return n ? f(index, offset, n) : ET_OK;
+}
+
 int run_call(const OrthoCall& call, const OrthoList& scalars, unsigned char* workspace, hipStream_t s)
 {
     // Blocks of both sizes of LDS that find a CU each go in one launch, beside one another
@@ -1278,33 +1303,14 @@ int run_call(const OrthoCall& call, const OrthoList& scalars, unsigned char* wor
         return together && way == 2 ? 3 : way;
     };
     for (int way = 0; way < kWays; ++way) {
-        OrthoList list = scalars;
-        list.count = 0;
-        int64_t index[kTensors];
-        unsigned char* place[kTensors];
-        unsigned char* at = workspace;
-        int64_t blocks = 0;
-        const auto flush = [&]() -> int {
-            if (!list.count) return ET_OK;
-            const int rc = run_set(call, list, way, index, place, s);
-            list.count = 0;
-            blocks = 0;
-            return rc;
-        };
-        for (int64_t i = 0; i < call.count; ++i) {
-            const Shape sh = shape_at(call.shapes, i);
-            unsigned char* const here = at;
-            if (sh.E * sh.m * sh.n == 0) continue;
-            at += sh.bytes();
-            if (way_of(sh) != way) continue;
-            if (list.count == kTensors || blocks + sh.launch_blocks() >= kMostBlocks) {
-                if (const int rc = flush()) return rc;
-            }
-            index[list.count] = i;
-            place[list.count++] = here;
-            blocks += sh.launch_blocks();
-        }
-        if (const int rc = flush()) return rc;
+        const int rc = each_set(call.shapes, call.count, way, way_of, [&](const int64_t* index, const int64_t* offset, int count) {
+            OrthoList list = scalars;
+            list.count = count;
+            unsigned char* place[kTensors];
+            for (int i = 0; i < count; ++i) place[i] = workspace + offset[i];
+            return run_set(call, list, way, index, place, s);
+        });
+        if (rc) return rc;
     }
     return ET_OK;
 }
@@ -1317,13 +1323,25 @@ using namespace et;
 extern "C" size_t et_orthogonalize_workspace_bytes(const int64_t* shapes, int64_t count)
 {
     if (count < 0 || (count > 0 && !shapes)) return 0;
-    int64_t n = 0;
-    for (int64_t i = 0; i < count; ++i) {
-        const Shape s = shape_at(shapes, i);
-        if (!shape_ok(s)) return 0;
-        if (s.E * s.m * s.n) n += s.bytes();
+    for (int64_t i = 0; i < count; ++i)
+        if (!shape_ok(shape_at(shapes, i))) return 0;
+    // The largest kTensors of a way: whatever set they come in, so that the space for a list is
+    // enough for any part of it.  (Matrices that one block takes need none.)
+    int64_t most = 0;
+    for (const int way : {0, 1}) {
+        int64_t bytes[kTensors] = {};           // falling
+        for (int64_t i = 0; i < count; ++i) {
+            const Shape s = shape_at(shapes, i);
+            if (s.E * s.m * s.n == 0 || s.way() != way || s.bytes() <= bytes[kTensors - 1]) continue;
+            int at = kTensors - 1;
+            for (; at > 0 && bytes[at - 1] < s.bytes(); --at) bytes[at] = bytes[at - 1];
+            bytes[at] = s.bytes();
+        }
+        int64_t sum = 0;
+        for (const int64_t n : bytes) sum += n;
+        most = std::max(most, sum);
     }
-    return (size_t)n;
+    return (size_t)most;
 }
 
 namespace {

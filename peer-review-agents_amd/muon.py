@@ -89,8 +89,12 @@ def _check_coefficients(coefficients, steps: int, eps: float):
     return _checked[key]
 
 
+def _workspace_bytes(shapes) -> int:
+    return int(lib().et_orthogonalize_workspace_bytes(_shape_array(shapes), len(shapes)))
+
+
 def _workspace(shapes, workspace, dev):
-    nbytes = int(lib().et_orthogonalize_workspace_bytes(_shape_array(shapes), len(shapes)))
+    nbytes = _workspace_bytes(shapes)
     if workspace is None:
         return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=dev)
     _require_workspace(workspace, nbytes, dev, "workspace")
@@ -100,9 +104,8 @@ def _workspace(shapes, workspace, dev):
 
 
 def orthogonalize_workspace_bytes(shapes: Sequence[Sequence[int]]) -> int:
-    """Bytes that :func:`orthogonalize` and :func:`muon_step_` work in, for tensors of these shapes."""
-    shapes = [_matrices(s, "shape") for s in shapes]
-    return int(lib().et_orthogonalize_workspace_bytes(_shape_array(shapes), len(shapes)))
+    """Bytes that :func:`orthogonalize` and :func:`muon_step_` work in, for tensors of these shapes or some of them."""
+    return _workspace_bytes([_matrices(s, "shape") for s in shapes])
 
 
 def orthogonalize(g: torch.Tensor, *, steps: int = 5, coefficients=MUON_COEFFICIENTS, eps: float = 1e-7,
@@ -169,9 +172,14 @@ def _step(dev, params, grads, momenta, masters, shapes, step_sizes, scalars, gra
     def take(ts, at):
         return ts if at is None else [ts[i] for i in at]
 
-    # (all workspaces before the first call, which a refusal would leave half a step behind)
-    spaces = [_workspace(take(shapes, at), workspace, dev) for at in kinds]
-    for at, ws in zip(kinds, spaces):
+    # (the calls, one behind the other, share a workspace: what the largest needs, and refused before the first
+    # call, which a later refusal would leave half a step behind)
+    if len(kinds) == 1:
+        ws = _workspace(shapes, workspace, dev)
+    else:
+        most = max((take(shapes, at) for at in kinds), key=_workspace_bytes)
+        ws = _workspace(most, workspace, dev)
+    for at in kinds:
         p, g, sh = take(params, at), take(grads, at), take(shapes, at)
         low = p[0].dtype == torch.bfloat16
         _call("et_muon", dev, _pointers(p), _pointers(g), _pointers(take(momenta, at)), _pointers(take(masters, at)) if low else None,
@@ -226,8 +234,9 @@ class Muon:
     of one allocation for each kind, ``flat[name]``, each tensor from a multiple
     of 256 elements on.  ``step(grads)`` takes one gradient for each parameter,
     or None for one that has none this time: it and its momentum stay as they
-    are.  The workspace (about four bytes an element, and eight for an element of a
-    matrix's shorter side squared) is allocated for each step.
+    are.  The workspace is allocated for each step: for the up to 20 tensors that run at a time
+    about four bytes an element, and four for an element of a matrix's shorter side squared; none
+    for matrices that one block takes (a shorter side of at most 64, some 75000 elements).
     """
 
     def __init__(self, params: Sequence[torch.Tensor], *, lr: float = 1e-3, momentum: float = 0.95,

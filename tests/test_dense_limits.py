@@ -100,3 +100,19 @@ def test_the_backwards_workspace_goes_by_the_tensors_device(et, monkeypatch):
         assert gated.gated_linear_backward_workspace_bytes(5, 64, 16, device=gated.torch.device("cuda:2")) == 5002
     finally:
         gated._workspace_bytes.cache_clear()
+
+
+def test_sets_of_tensors_share_the_workspace(et):
+    """At most 20 tensors run at a time, wide ones and tall ones apart: a step needs what the largest of these needs."""
+    size = lambda *s: et.lib().et_orthogonalize_workspace_bytes(_shapes(*s), len(s))  # noqa: E731
+    one, tall = size((4, 200, 520)), size((2, 900, 136))
+    assert 4 * 4 * 200 * 520 < one < 4 * 4 * (200 * 520 + 200 * 200) * 1.1 and tall > 0
+    assert size(*[(4, 200, 520)] * 20) == 20 * one
+    assert size(*[(4, 200, 520)] * 100) == 20 * one
+    assert size(*[(4, 200, 520), (2, 900, 136)] * 5) == max(5 * one, 5 * tall)
+    assert size((4, 200, 520), *[(8, 64, 512)] * 50) == one and size(*[(8, 64, 512)] * 50) == 0
+    assert size((0, 200, 520), (3, 0, 200)) == 0
+    # whatever the order, and enough for a part of the list (the tensors of one pair of types)
+    mixed = [(4, 200, 520), (1, 100, 100)] * 20
+    assert size(*mixed) == size(*mixed[::2]) == 20 * one == size(*mixed[::-1])
+    assert size(*mixed[:10]) < size(*mixed[:30]) < size(*mixed)

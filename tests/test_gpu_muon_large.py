@@ -54,3 +54,18 @@ def test_more_tensors_than_a_set(et, dev):
     et.muon_step_(params, grads, momenta, lr=0.01, momentum=0.9, weight_decay=0.1, masters=masters)
     _check_step(old, list(zip(fp, momenta)), grads, 1.0, 0.9, True, 0.01, 0.1, 0.2)
     assert all(torch.equal(p, m.bfloat16()) for p, m in zip(params, masters) if m is not None)
+
+
+def test_a_callers_workspace_of_the_stated_size(et, dev):
+    """Of all shapes at once, for a step of two kinds of types whose tensors alternate: the bits of the step with its own."""
+    shapes = [(128, 200), (70, 66), (300, 90)] * 16
+    a, b = (_lists(dev, shapes, torch.float32, torch.float32)[0::2] for _ in range(2))
+    grads = [g.bfloat16() if i % 2 else g for i, g in enumerate(_lists(dev, shapes, torch.float32, torch.float32)[3])]
+    et.muon_step_(a[0], grads, a[1], lr=0.01)
+    n = et.orthogonalize_workspace_bytes(shapes)
+    ws = torch.full((n + 4096,), 0x7f, device=dev, dtype=torch.uint8)        # (NaN as f16; as f32 and binary64 large)
+    et.muon_step_(b[0], grads, b[1], lr=0.01, workspace=ws[:n])
+    assert all(torch.equal(x, y) for x, y in zip(a[0] + a[1], b[0] + b[1]))
+    assert bool((ws[n:] == 0x7f).all())
+    with pytest.raises(ValueError, match="workspace"):
+        et.muon_step_(b[0], grads, b[1], lr=0.01, workspace=ws[:1 << 20])
