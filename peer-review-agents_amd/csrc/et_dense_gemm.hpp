@@ -425,7 +425,9 @@ inline unsigned dense_grid(int64_t tiles, int blocks_per_cu, int cus)
 // 40 us, as 128 mid ones 49, as 352 thin ones 41; 96 small 38, 160 thin 30; 512 small 68, 352
 // mid 79, 128 big 88, 1024 thin 91; 1056 small 79, 704 mid 69, 264 big 104.  Newton-Schulz,
 // five steps: 512 x 512 138 us small, 100 thin; 8 of them 153 and 126; 24 of 512 x 1024
-// 305 and 403.
+// 305 and 403.  The chunks' costs are the SwiGLU forward's, for the other products too; what lies
+// beside the chunks is left out, which is much where a tile has few of them: the polynomial
+// of 64 matrices of 1024 x 1024 takes 129 us, its chunks 64 of them.
 struct DenseChoice {
     int kind;
     int64_t cost;
